@@ -150,6 +150,67 @@ int wv_topk_sample_dev(const float* d_logits, int n, int top_k, float temperatur
 int wv_topk_sample(const float* d_logits, int n, int top_k, float temperature, int deterministic, double u01,
                    int* index_host, void* stream);
 
+/* Batched serving: many sequences at once, each with some new tokens, over a key/value cache in pages. No counterpart in
+ * the reference, whose cache is one float32 row per position of one sequence (layers/mha/cpu.go:184-207).
+ *
+ * WvKvPages is the cache of one block (layer). `pool` holds num_pages pages; a page holds, for each kv head in turn, one
+ * block of wv_kv_block_bytes(): page_size tokens' worth of
+ *     K codes | V codes | K scales | V scales [| K sub-scales | V sub-scales]
+ * each part token after token. A token's row of head_dim values is stored in `bits` bits a value:
+ *   16  f16 codes, value = scale * code, scale = 2^(floor(log2 max|x|) - 14)
+ *    8  int8 codes, value = scale * code, scale = max|x| / 127
+ *    4  codes + 8 in nibbles (value 2i in the low one of byte i), value = scale * (sub * code); scale = max|x| / 1785, and a
+ *       byte sub for each 16 values, ceil(max|x of the 16| / 7 / scale), at least 1, so that |code| <= 7
+ * with the scale (float32, at least 2^-126) of a row and codes rounded to nearest even. A row with a value that is not
+ * finite gets the scale NaN and codes of zero: who may see that token gets NaN, and nobody else does. page_size is a multiple of
+ * 16, head_dim a multiple of 16 up to 256, pool 16-byte aligned.
+ *
+ * WvKvBatch is the batch of a step, arrays on the device, so that a captured graph can be replayed with new contents:
+ * q_start[num_seqs + 1] rising rows of the sequences' new tokens in q / k / v / out (q_start[num_seqs] <= total_q; rows past
+ * it are not touched), kv_len[num_seqs] tokens of each sequence in the cache, its new ones included, pages[num_seqs][table_stride] the
+ * page that holds tokens i * page_size and on. A sequence may have no new tokens, or none at all. max_q and max_kv bound the
+ * lengths. A length, row or page number beyond these bounds is cut to them on the device, its page is not read or
+ * written, and wv_device_status() then reports WV_ESHAPE. A sequence must not hold a page twice, nor two sequences a page that
+ * either of them writes.
+ *
+ * Row strides (ld*) count floats, 0 stands for rows without a gap; they are multiples of 4 and the vectors 16-byte
+ * aligned. All calls are asynchronous on `stream`. */
+typedef struct WvKvPages {
+  void* pool;
+  int bits, num_pages, page_size, num_kv_heads, head_dim;
+} WvKvPages;
+typedef struct WvKvBatch {
+  const int* q_start;
+  const int* kv_len;
+  const int* pages;
+  int num_seqs, table_stride, total_q, max_q, max_kv;
+} WvKvBatch;
+int wv_kv_block_bytes(int bits, int page_size, int head_dim, uint64_t* bytes);
+/* New token i of a sequence stands at position kv_len - (its new tokens) + i (one before position 0 is left out). The call
+ * rotates K, and Q if dq is given, as wv_rope_cache_dev does (theta <= 0: not at all), writes Q [rows, num_heads * head_dim]
+ * to dq_out (which may be dq) and K and V [rows, num_kv_heads * head_dim], rounded, to the tokens' places in the pages. */
+int wv_kv_write_dev(const WvKvPages* kv, const WvKvBatch* batch, const float* dk, int ldk, const float* dv, int ldv,
+                    const float* dq, int ldq, float* dq_out, int ldqo, int num_heads, double theta, void* stream);
+/* The same tokens' K and V out of the pages, as float32 (rows of tokens before position 0 or in pages out of bounds: zeros). */
+int wv_kv_read_dev(const WvKvPages* kv, const WvKvBatch* batch, float* dk, int ldk, float* dv, int ldv, void* stream);
+/* Attention of the new tokens over the cached ones (mha/attn.go:15-120 for a chunk): the token at position p sees positions
+ * max(0, p - window + 1) .. p (window <= 0: from 0), out = sum of softmax(scale q.k) v over them, zeros where it sees
+ * none, NaN for a query that is not finite; query head h reads kv head h / (num_heads / num_kv_heads). max_q == 1 is a decode step. Scratch for the results of
+ * splits belongs to the stream (or to the graph, in a capture): the first call for a larger shape allocates it. */
+int wv_attn_paged_dev(const WvKvPages* kv, const WvKvBatch* batch, const float* dq, int ldq, float* dout, int ldo, int num_heads,
+                      float scale, int window, void* stream);
+
+/* The next token of each of `rows` rows of n logits (row r at d_logits + r * ld, ld 0: n). Parameters are device arrays, one
+ * value a row: temperature T, top_k, top_p, min_p and the draw u in [0, 1]. Candidates are the logits that are neither NaN nor
+ * -inf, ordered by logit / T from the largest down, equal ones by rising index. Kept are the first top_k (all for
+ * top_k <= 0); of those, with w = exp((logit - max) / T), the ones whose preceding w add up to less than top_p of the sum, the first
+ * one in any case; of those the ones with w >= min_p, again the first one in any case. The token is the first whose running sum of w reaches u times the sum of the
+ * kept ones. T <= 0 or top_k == 1: the first candidate. d_index[r] is the token, d_prob[r] (may be NULL) its share of the kept
+ * weight; -1 and 0 for a row without a candidate. Sums are integers in units of 2^-(62 - ceil(log2 n)), so the result does not
+ * depend on the order of summation. */
+int wv_sample_rows_dev(const float* d_logits, int rows, int n, int64_t ld, const float* d_temperature, const int* d_top_k,
+                       const float* d_top_p, const float* d_min_p, const double* d_u, int* d_index, float* d_prob, void* stream);
+
 /* Dequantise the resident blob to f32 on the device and copy rows*cols floats out —
  * quant.Unpack (quant/unpack.go:4-34); results are bit-identical to it. */
 int wv_unpack(uint64_t key, float* out_host);
@@ -242,7 +303,8 @@ int wv_gather_sync(unsigned* const* flags_all, int world, int rank, void* stream
 int wv_gather_read(const void* dptr, size_t offset_bytes, void* host, size_t bytes, void* stream);
 
 /* After the caller has synchronised its stream: 0, or WV_ETIMEOUT when a bounded device wait
- * of an asynchronous call (wv_matvec_dev) ran out since the last query. The reference reports
+ * of an asynchronous call (wv_matvec_dev) ran out since the last query, or WV_ESHAPE when a paged call met a length or a page
+ * number outside its bounds. The reference reports
  * device failures through the error of the synchronous call (webgpu/affine_cache.go:439-443). */
 int wv_device_status(void);
 

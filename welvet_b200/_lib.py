@@ -23,6 +23,7 @@ SYMBOLS = [
     "wv_matvec_dev_swiglu", "wv_matvec_dev_add", "wv_matvec_dev_group_gather", "wv_matvec_dev_fused", "wv_rmsnorm_dev", "wv_rope_cache_dev",
     "wv_attn_decode_dev", "wv_silu_mul_dev", "wv_residual_add_dev",
     "wv_topk_sample_dev", "wv_topk_sample", "wv_decode_row", "wv_decode_row_dev",
+    "wv_kv_block_bytes", "wv_kv_write_dev", "wv_kv_read_dev", "wv_attn_paged_dev", "wv_sample_rows_dev",
 ]
 
 # Development hooks (csrc/wv_dev_hooks.h): only in a library built with -DWV_DEV_HOOKS (libwelvet_cuda_dev.so),
@@ -41,6 +42,18 @@ class WvFusedCall(C.Structure):
                 ("world", C.c_int), ("rank", C.c_int), ("row_offset", C.POINTER(C.c_int)), ("in_", C.c_int),
                 ("out_local", C.POINTER(C.c_int)), ("mode", C.c_int), ("dresidual", C.c_void_p), ("dnorm_gamma", C.c_void_p),
                 ("norm_eps", C.c_double)]
+
+
+class WvKvPages(C.Structure):
+    """WvKvPages of include/welvet_cuda.h."""
+    _fields_ = [("pool", C.c_void_p), ("bits", C.c_int), ("num_pages", C.c_int), ("page_size", C.c_int), ("num_kv_heads", C.c_int),
+                ("head_dim", C.c_int)]
+
+
+class WvKvBatch(C.Structure):
+    """WvKvBatch of include/welvet_cuda.h."""
+    _fields_ = [("q_start", C.c_void_p), ("kv_len", C.c_void_p), ("pages", C.c_void_p), ("num_seqs", C.c_int), ("table_stride", C.c_int),
+                ("total_q", C.c_int), ("max_q", C.c_int), ("max_kv", C.c_int)]
 
 
 class WelvetError(RuntimeError):
@@ -110,6 +123,11 @@ def lib() -> C.CDLL:
         L.wv_residual_add_dev.argtypes = [vp, vp, i, vp]
         L.wv_topk_sample_dev.argtypes = [vp, i, i, C.c_float, i, C.c_double, vp, vp]
         L.wv_topk_sample.argtypes = [vp, i, i, C.c_float, i, C.c_double, C.POINTER(i), vp]
+        L.wv_kv_block_bytes.argtypes = [i, i, i, C.POINTER(u64)]
+        L.wv_kv_write_dev.argtypes = [C.POINTER(WvKvPages), C.POINTER(WvKvBatch), vp, i, vp, i, vp, i, vp, i, i, C.c_double, vp]
+        L.wv_kv_read_dev.argtypes = [C.POINTER(WvKvPages), C.POINTER(WvKvBatch), vp, i, vp, i, vp]
+        L.wv_attn_paged_dev.argtypes = [C.POINTER(WvKvPages), C.POINTER(WvKvBatch), vp, i, vp, i, i, C.c_float, i, vp]
+        L.wv_sample_rows_dev.argtypes = [vp, i, i, C.c_int64, vp, vp, vp, vp, vp, vp, vp, vp]
         L.wv_decode_row.argtypes = [u64, i, vp, i]
         L.wv_decode_row_dev.argtypes = [u64, i, vp, vp]
         L.wv_unpack.argtypes = [u64, vp]

@@ -38,6 +38,9 @@ SOURCES = {
     "wv_gemv_ragged.cu": [],
     "wv_gemv_rows.cu": [],
     "wv_decode.cu": [],
+    "wv_kv_cache.cu": [],
+    "wv_attn_paged.cu": [],
+    "wv_sample.cu": [],
     "wv_gemv_tc.cu": [],
     "wv_gemm_tcgen05.cu": [],
     "wv_api.cu": [],

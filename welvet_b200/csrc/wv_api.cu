@@ -35,6 +35,7 @@ int wv_gemv_scratch_init(size_t bytes);  // wv_gemv.cu
 void wv_scratch_own(void* p, size_t bytes);
 int wv_tma_init();                       // wv_gemv_tma.cu
 int wv_tma_take_error();
+int wv_paged_take_error();
 struct Entry {
   WvDevBlob blob;
   void* mem = nullptr;
@@ -1025,6 +1026,10 @@ extern "C" int wv_matvec_bias_act(uint64_t key, const float* x, const double* bi
 
 extern "C" int wv_device_status(void) {
   if (int te = wv_tma_take_error()) { wv_set_error("a bounded device wait ran out (code %d)", te); return WV_ETIMEOUT; }
+  if (int pe = wv_paged_take_error()) {
+    wv_set_error("paged call: %s", pe == 1 ? "a q_start or kv_len is outside its bounds" : "a page number is outside the pool");
+    return WV_ESHAPE;
+  }
   return WV_OK;
 }
 

@@ -892,10 +892,18 @@ int wv_tma_take_error() {
   return v;
 }
 int* wv_tma_err_ptr() { return g_err_dev; }
+// The word behind it is the paged calls': what they met outside its bounds (wv_paged.cuh), not a wait that ran out.
+int* wv_paged_err_ptr() { return g_err_dev ? g_err_dev + 1 : nullptr; }
+int wv_paged_take_error() {
+  if (!g_err_host) return 0;
+  const int v = ((volatile int*)g_err_host)[1];
+  if (v) ((volatile int*)g_err_host)[1] = 0;
+  return v;
+}
 int wv_tma_init() {
   if (g_err_host) return WV_OK;
-  if (cudaHostAlloc(&g_err_host, sizeof(int), cudaHostAllocMapped) != cudaSuccess) { cudaGetLastError(); return WV_ENOMEM; }
-  *g_err_host = 0;
+  if (cudaHostAlloc(&g_err_host, 2 * sizeof(int), cudaHostAllocMapped) != cudaSuccess) { cudaGetLastError(); return WV_ENOMEM; }
+  g_err_host[0] = g_err_host[1] = 0;
   if (cudaHostGetDevicePointer(&g_err_dev, g_err_host, 0) != cudaSuccess) { cudaGetLastError(); return WV_ECUDA; }
   return WV_OK;
 }

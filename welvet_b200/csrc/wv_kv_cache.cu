@@ -1,0 +1,335 @@
+// The paged key/value cache: rows rounded to 16, 8 or 4 bits as they are written, with the rotary embedding of Q and K in the same
+// pass, and read back. include/welvet_cuda.h (WvKvPages) defines layout and arithmetic.
+//
+// Bound: HBM for prompts, latency for single tokens. A CTA takes one token (its angles are the same for all heads), a warp a row
+// of head_dim values at a time, a lane four consecutive values of it (and four more beyond 128): float4 in, 8 / 4 / 2 bytes of
+// codes out, and the row's maximum is five shuffles away.
+#include "wv_paged.cuh"
+#include <float.h>
+#include <math.h>
+#include <string.h>
+
+#define KVC_WARPS 8
+
+// theta^(2 d / head_dim) for every pair, computed on the host once per (theta, head_dim) and passed by value.
+struct WvRopeFreq { double p[128]; };
+
+// A token's place: its sequence's page table says which page and slot; no page (block < 0) before position 0 or on a page number
+// outside the pool.
+struct KvPlace { int pos; long long page; int slot; };
+__device__ __forceinline__ KvPlace kv_place(const WvKvGeom& g, const WvKvBatch& b, int row, int* err) {
+  KvPlace p{0, -1, 0};
+  const int s = wv_seq_of_row(b, row);
+  if (s >= b.num_seqs) { p.pos = INT_MIN; return p; }
+  const WvSeq q = wv_seq(b, g.page, s, err);
+  if (row < q.q0 || row >= q.q1) { p.pos = INT_MIN; return p; }
+  p.pos = q.kv - (q.q1 - q.q0) + (row - q.q0);
+  if (p.pos < 0) return p;
+  const int i = p.pos / g.page, id = b.pages[(size_t)s * b.table_stride + i];
+  p.slot = p.pos - i * g.page;
+  if (id < 0 || id >= g.num_pages) wv_paged_report(err, WV_PAGED_PAGE);
+  else p.page = id;
+  return p;
+}
+
+// a * c - b * s with c and s in two float32 pieces each: the products' errors by fma, the sum's by Knuth's two-sum, so that the
+// result is the float64 expression's, rounded, but for one in some 10^7. (float64 itself issues at half the float32 rate here and its
+// conversions at a sixteenth.) What is not finite goes through float64.
+__device__ __forceinline__ float rot(float a, float b, float ch, float cl, float sh, float sl) {
+  const float p = a * ch, q = b * sh;
+  const float t = fmaf(a, cl, fmaf(a, ch, -p)) - fmaf(b, sl, fmaf(b, sh, -q));
+  const float s = __fsub_rn(p, q), z = __fsub_rn(s, p);
+  const float e = __fadd_rn(__fsub_rn(p, __fsub_rn(s, z)), __fsub_rn(-q, z));
+  const float r = s + (e + t);
+  if (fabsf(r) <= FLT_MAX) return r;
+  return (float)((double)a * ((double)ch + (double)cl) - (double)b * ((double)sh + (double)sl));
+}
+
+// One row of V4 x 4 x 32 values at most: lane l holds 4 l .. 4 l + 3 (and 128 + those), lanes past head_dim hold zeros.
+template <int BITS, int V4>
+__device__ __forceinline__ void kv_store_row(const WvKvGeom& g, unsigned char* block, bool is_v, int slot, const float (&x)[V4][4], int lane) {
+  unsigned m = 0;                  // the largest magnitude's bits; infinities and NaN are above all others
+#pragma unroll
+  for (int i = 0; i < V4; i++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) m = max(m, __float_as_uint(x[i][e]) & 0x7fffffffu);
+  unsigned mg[V4];                 // 4 bits: of the four lanes that share a group of 16
+#pragma unroll
+  for (int i = 0; i < V4; i++) {
+    mg[i] = 0;
+    if (BITS == 4) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) mg[i] = max(mg[i], __float_as_uint(x[i][e]) & 0x7fffffffu);
+      mg[i] = max(mg[i], __shfl_xor_sync(0xffffffffu, mg[i], 1));
+      mg[i] = max(mg[i], __shfl_xor_sync(0xffffffffu, mg[i], 2));
+    }
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  const bool fine = m < 0x7f800000u;
+  const float a = __uint_as_float(m);
+  float s;
+  if (BITS == 16) s = __uint_as_float((unsigned)max((int)(m >> 23) - 14, 1) << 23);   // a subnormal has exponent 0: the smallest scale
+  else s = fmaxf(__fdiv_rn(a, BITS == 8 ? 127.f : 1785.f), FLT_MIN);
+  unsigned char* codes = block + (is_v ? g.page * g.code : 0) + slot * g.code;
+#pragma unroll
+  for (int i = 0; i < V4; i++) {
+    const int d = 4 * (lane + 32 * i);
+    if (d >= g.hd) break;
+    if (BITS == 16) {
+      const float inv = __fdiv_rn(1.f, s);                       // a power of two (s <= 2^113): exact
+      __half2 h[2] = {__floats2half2_rn(fine ? x[i][0] * inv : 0.f, fine ? x[i][1] * inv : 0.f),
+                      __floats2half2_rn(fine ? x[i][2] * inv : 0.f, fine ? x[i][3] * inv : 0.f)};
+      *reinterpret_cast<uint2*>(codes + 2 * d) = make_uint2(*reinterpret_cast<unsigned*>(&h[0]), *reinterpret_cast<unsigned*>(&h[1]));
+    } else if (BITS == 8) {
+      unsigned w = 0;
+#pragma unroll
+      for (int e = 0; e < 4; e++) w |= ((unsigned)(fine ? (int)rintf(__fdiv_rn(x[i][e], s)) : 0) & 0xffu) << (8 * e);
+      *reinterpret_cast<unsigned*>(codes + d) = w;
+    } else {
+      const float t = fine ? fminf(fmaxf(ceilf(__fdiv_rn(__fdiv_rn(__uint_as_float(mg[i]), 7.f), s)), 1.f), 255.f) : 1.f;
+      const float st = __fmul_rn(s, t);
+      unsigned w = 0;
+#pragma unroll
+      for (int e = 0; e < 4; e++) w |= (unsigned)(fine ? (int)fminf(fmaxf(rintf(__fdiv_rn(x[i][e], st)), -7.f), 7.f) + 8 : 8) << (4 * e);
+      *reinterpret_cast<unsigned short*>(codes + d / 2) = (unsigned short)w;
+      if ((lane & 3) == 0) block[(is_v ? g.vsub : g.ksub) + slot * (g.hd / 16) + d / 16] = (unsigned char)t;
+    }
+  }
+  if (lane == 0) *reinterpret_cast<float*>(block + (is_v ? g.vscale : g.kscale) + 4 * slot) = fine ? s : __uint_as_float(0x7fc00000u);
+}
+
+// grid (tokens, pieces of a token's rows): rows of K, then V, then Q
+template <int BITS, int V4>
+__global__ void __launch_bounds__(32 * KVC_WARPS) kv_write_kernel(const WvKvGeom g, const WvKvBatch b, const float* __restrict__ k, int ldk,
+                                                                  const float* __restrict__ v, int ldv, const float* q, int ldq, float* q_out,
+                                                                  int ldqo, int heads, int rotate, const __grid_constant__ WvRopeFreq freq,
+                                                                  int* __restrict__ err) {
+  __shared__ float4 s_cs[128];      // cos and sin of a pair, in two pieces each
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = g.hd >> 1;
+  const KvPlace at = kv_place(g, b, row, err);
+  if (at.pos == INT_MIN) return;    // a row that no sequence owns
+  if (rotate) {
+    for (int d = threadIdx.x; d < half; d += 32 * KVC_WARPS) {
+      double c, s;
+      sincos((double)at.pos / freq.p[d], &s, &c);
+      s_cs[d] = make_float4((float)c, (float)(c - (double)(float)c), (float)s, (float)(s - (double)(float)s));
+    }
+    __syncthreads();
+  }
+  const int nr = 2 * g.kvh + heads;
+  for (int r = blockIdx.y * KVC_WARPS + warp; r < nr; r += gridDim.y * KVC_WARPS) {
+    const bool is_q = r >= 2 * g.kvh, is_v = !is_q && r >= g.kvh;
+    const int h = is_q ? r - 2 * g.kvh : (is_v ? r - g.kvh : r);
+    if (!is_q && at.page < 0) continue;
+    const float* src = (is_q ? q + (size_t)row * ldq : is_v ? v + (size_t)row * ldv : k + (size_t)row * ldk) + (size_t)h * g.hd;
+    float x[V4][4];
+#pragma unroll
+    for (int i = 0; i < V4; i++) {
+      const int d = 4 * (lane + 32 * i);
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f), w = o;
+      if (d < g.hd) {
+        o = *reinterpret_cast<const float4*>(src + d);
+        if (rotate && !is_v) w = *reinterpret_cast<const float4*>(src + (d < half ? d + half : d - half));
+      }
+      x[i][0] = o.x; x[i][1] = o.y; x[i][2] = o.z; x[i][3] = o.w;
+      if (rotate && !is_v && d < g.hd) {
+        const float p[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int e = 0; e < 4; e++) {          // first half: a c - b s; second half, with b the first one's value: b s + a c
+          const float4 cs = s_cs[(d < half ? d : d - half) + e];
+          const float sg = d < half ? 1.f : -1.f;
+          x[i][e] = rot(x[i][e], p[e], cs.x, cs.y, sg * cs.z, sg * cs.w);
+        }
+      }
+    }
+    if (is_q) {
+      if (q == q_out) __syncwarp();            // in place: every lane has its partner's value
+      float* dst = q_out + (size_t)row * ldqo + (size_t)h * g.hd;
+#pragma unroll
+      for (int i = 0; i < V4; i++) {
+        const int d = 4 * (lane + 32 * i);
+        if (d < g.hd) *reinterpret_cast<float4*>(dst + d) = make_float4(x[i][0], x[i][1], x[i][2], x[i][3]);
+      }
+    } else {
+      kv_store_row<BITS, V4>(g, g.pool + ((size_t)at.page * g.kvh + h) * g.block, is_v, at.slot, x, lane);
+    }
+  }
+}
+
+template <int BITS, int V4>
+__global__ void __launch_bounds__(32 * KVC_WARPS) kv_read_kernel(const WvKvGeom g, const WvKvBatch b, float* __restrict__ k, int ldk,
+                                                                 float* __restrict__ v, int ldv, int* __restrict__ err) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const KvPlace at = kv_place(g, b, row, err);
+  if (at.pos == INT_MIN) return;
+  for (int r = blockIdx.y * KVC_WARPS + warp; r < 2 * g.kvh; r += gridDim.y * KVC_WARPS) {
+    const bool is_v = r >= g.kvh;
+    const int h = is_v ? r - g.kvh : r;
+    float* dst = (is_v ? v + (size_t)row * ldv : k + (size_t)row * ldk) + (size_t)h * g.hd;
+    const unsigned char* block = g.pool + ((size_t)max(at.page, 0LL) * g.kvh + h) * g.block;
+    const unsigned char* codes = block + (is_v ? g.page * g.code : 0) + at.slot * g.code;
+    const float s = at.page < 0 ? 0.f : *reinterpret_cast<const float*>(block + (is_v ? g.vscale : g.kscale) + 4 * at.slot);
+#pragma unroll
+    for (int i = 0; i < V4; i++) {
+      const int d = 4 * (lane + 32 * i);
+      if (d >= g.hd) break;
+      float c[4] = {0.f, 0.f, 0.f, 0.f};
+      if (at.page >= 0) {
+        if (BITS == 16) {
+          const uint2 w = *reinterpret_cast<const uint2*>(codes + 2 * d);
+          const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), hi = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
+          c[0] = lo.x; c[1] = lo.y; c[2] = hi.x; c[3] = hi.y;
+        } else if (BITS == 8) {
+          const unsigned w = *reinterpret_cast<const unsigned*>(codes + d);
+#pragma unroll
+          for (int e = 0; e < 4; e++) c[e] = (float)(int)(signed char)(w >> (8 * e));
+        } else {
+          const unsigned w = *reinterpret_cast<const unsigned short*>(codes + d / 2);
+          const int t = block[(is_v ? g.vsub : g.ksub) + at.slot * (g.hd / 16) + d / 16];
+#pragma unroll
+          for (int e = 0; e < 4; e++) c[e] = (float)(((int)((w >> (4 * e)) & 15u) - 8) * t);
+        }
+      }
+      *reinterpret_cast<float4*>(dst + d) = make_float4(s * c[0], s * c[1], s * c[2], s * c[3]);
+    }
+  }
+}
+
+static cudaError_t kvc_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* at, int tokens, int rows, cudaStream_t st) {
+  // Enough CTAs for the chip where there are few tokens; with many, a CTA per token, which computes its angles once.
+  const int most = (rows + KVC_WARPS - 1) / KVC_WARPS, want = 592 / tokens;
+  cfg.gridDim = dim3(tokens, want < 1 ? 1 : (want > most ? most : want));
+  cfg.blockDim = dim3(32 * KVC_WARPS); cfg.stream = st;
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at; cfg.numAttrs = 1;
+  return cudaSuccess;
+}
+
+int wv_launch_kv_write(const WvKvPages& kv, const WvKvBatch& b, const float* dk, int ldk, const float* dv, int ldv, const float* dq, int ldq,
+                       float* dq_out, int ldqo, int heads, double theta, cudaStream_t st) {
+  const WvKvGeom g = wv_kv_geom(kv);
+  static thread_local WvRopeFreq freq;
+  static thread_local double freq_theta = 0.0;
+  static thread_local int freq_hd = 0;
+  if (theta > 0.0 && (freq_theta != theta || freq_hd != g.hd)) {
+    for (int d = 0; d < g.hd / 2; d++) freq.p[d] = pow(theta, (double)(2 * d) / (double)g.hd);
+    freq_theta = theta; freq_hd = g.hd;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  kvc_config(cfg, at, b.total_q, 2 * g.kvh + heads, st);
+  auto go = [&](auto kern) { return cudaLaunchKernelEx(&cfg, kern, g, b, dk, ldk, dv, ldv, dq, ldq, dq_out, ldqo, heads, theta > 0.0 ? 1 : 0, freq, wv_paged_err_ptr()); };
+  cudaError_t e;
+  if (g.hd > 128) e = kv.bits == 16 ? go(kv_write_kernel<16, 2>) : kv.bits == 8 ? go(kv_write_kernel<8, 2>) : go(kv_write_kernel<4, 2>);
+  else e = kv.bits == 16 ? go(kv_write_kernel<16, 1>) : kv.bits == 8 ? go(kv_write_kernel<8, 1>) : go(kv_write_kernel<4, 1>);
+  if (e != cudaSuccess) { wv_set_error("wv_kv_write_dev: launch: %s", cudaGetErrorString(cudaGetLastError())); return WV_ECUDA; }
+  return WV_OK;
+}
+
+int wv_launch_kv_read(const WvKvPages& kv, const WvKvBatch& b, float* dk, int ldk, float* dv, int ldv, cudaStream_t st) {
+  const WvKvGeom g = wv_kv_geom(kv);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute at[1];
+  kvc_config(cfg, at, b.total_q, 2 * g.kvh, st);
+  auto go = [&](auto kern) { return cudaLaunchKernelEx(&cfg, kern, g, b, dk, ldk, dv, ldv, wv_paged_err_ptr()); };
+  cudaError_t e;
+  if (g.hd > 128) e = kv.bits == 16 ? go(kv_read_kernel<16, 2>) : kv.bits == 8 ? go(kv_read_kernel<8, 2>) : go(kv_read_kernel<4, 2>);
+  else e = kv.bits == 16 ? go(kv_read_kernel<16, 1>) : kv.bits == 8 ? go(kv_read_kernel<8, 1>) : go(kv_read_kernel<4, 1>);
+  if (e != cudaSuccess) { wv_set_error("wv_kv_read_dev: launch: %s", cudaGetErrorString(cudaGetLastError())); return WV_ECUDA; }
+  return WV_OK;
+}
+
+// ------------------------------------------------------------------ C ABI: the calls' checks
+int wv_api_bind_device();
+int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* dq, int ldq, float* dout, int ldo, int heads, float scale,
+                         int window, cudaStream_t st);
+
+static bool kv_shape_ok(int bits, int page_size, int head_dim) {
+  return (bits == 16 || bits == 8 || bits == 4) && page_size >= 16 && page_size % 16 == 0 && page_size <= 65536 && head_dim >= 16 && head_dim % 16 == 0 && head_dim <= 256;
+}
+extern "C" int wv_kv_block_bytes(int bits, int page_size, int head_dim, uint64_t* bytes) {
+  if (!bytes) { wv_set_error("wv_kv_block_bytes: null pointer"); return WV_EARG; }
+  if (bits != 16 && bits != 8 && bits != 4) { wv_set_error("wv_kv_block_bytes: %d bits (16, 8 or 4)", bits); return WV_EFORMAT; }
+  if (!kv_shape_ok(bits, page_size, head_dim)) { wv_set_error("wv_kv_block_bytes: page_size %d, head_dim %d (multiples of 16, head_dim at most 256)", page_size, head_dim); return WV_ESHAPE; }
+  WvKvPages p = {nullptr, bits, 1, page_size, 1, head_dim};
+  *bytes = (uint64_t)wv_kv_geom(p).block;
+  return WV_OK;
+}
+
+// What the three calls check alike. 1: nothing to do (no rows).
+static int kv_check(const char* who, const WvKvPages* kv, const WvKvBatch* b) {
+  if (!kv || !b || !kv->pool || !b->q_start || !b->kv_len || !b->pages) { wv_set_error("%s: null pointer", who); return WV_EARG; }
+  if (kv->bits != 16 && kv->bits != 8 && kv->bits != 4) { wv_set_error("%s: %d bits (16, 8 or 4)", who, kv->bits); return WV_EFORMAT; }
+  if (!kv_shape_ok(kv->bits, kv->page_size, kv->head_dim) || kv->num_pages < 1 || kv->num_kv_heads < 1) {
+    wv_set_error("%s: %d pages of %d, %d kv heads of %d (page_size and head_dim are multiples of 16, head_dim at most 256)", who, kv->num_pages, kv->page_size,
+                 kv->num_kv_heads, kv->head_dim);
+    return WV_ESHAPE;
+  }
+  if (reinterpret_cast<uintptr_t>(kv->pool) & 15) { wv_set_error("%s: the pool is not 16-byte aligned", who); return WV_EARG; }
+  if (b->num_seqs < 1 || b->table_stride < 0 || b->total_q < 0 || b->max_q < 0 || b->max_kv < 0) { wv_set_error("%s: a negative or zero count in the batch", who); return WV_EARG; }
+  if ((long long)b->max_kv > (long long)b->table_stride * kv->page_size) {
+    wv_set_error("%s: max_kv %d does not fit %d pages of %d", who, b->max_kv, b->table_stride, kv->page_size); return WV_ESHAPE;
+  }
+  return b->total_q == 0 || b->max_q == 0 ? 1 : WV_OK;
+}
+static int kv_rows(const char* who, const char* name, const void* p, int* ld, long long width) {
+  if (!p) { wv_set_error("%s: %s is null", who, name); return WV_EARG; }
+  if (width > INT_MAX) { wv_set_error("%s: rows of %lld values", who, width); return WV_ESHAPE; }
+  if (*ld == 0) *ld = (int)width;
+  if (*ld < width || (*ld & 3)) { wv_set_error("%s: the row stride of %s is %d for %lld values (a multiple of 4)", who, name, *ld, width); return WV_ESHAPE; }
+  if (reinterpret_cast<uintptr_t>(p) & 15) { wv_set_error("%s: %s is not 16-byte aligned", who, name); return WV_EARG; }
+  return WV_OK;
+}
+
+extern "C" int wv_kv_write_dev(const WvKvPages* kv, const WvKvBatch* batch, const float* dk, int ldk, const float* dv, int ldv,
+                               const float* dq, int ldq, float* dq_out, int ldqo, int num_heads, double theta, void* stream) {
+  const char* who = "wv_kv_write_dev";
+  int rc = wv_api_bind_device();
+  if (rc < 0) return rc;
+  if ((rc = kv_check(who, kv, batch)) < 0) return rc;
+  const bool none = rc == 1;
+  const long long kw = (long long)kv->num_kv_heads * kv->head_dim, qw = (long long)num_heads * kv->head_dim;
+  if ((rc = kv_rows(who, "k", dk, &ldk, kw)) || (rc = kv_rows(who, "v", dv, &ldv, kw))) return rc;
+  if (dq || dq_out) {
+    if (num_heads < 1) { wv_set_error("%s: %d heads", who, num_heads); return WV_ESHAPE; }
+    if ((rc = kv_rows(who, "q", dq, &ldq, qw)) || (rc = kv_rows(who, "q_out", dq_out, &ldqo, qw))) return rc;
+    if (dq == dq_out && ldq != ldqo) { wv_set_error("%s: q in place with two strides", who); return WV_EARG; }
+  } else {
+    num_heads = 0;
+  }
+  if (!(theta == theta)) { wv_set_error("%s: theta is NaN", who); return WV_EARG; }
+  if (none) return WV_OK;
+  return wv_launch_kv_write(*kv, *batch, dk, ldk, dv, ldv, dq, ldq, dq_out, ldqo, num_heads, theta, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int wv_kv_read_dev(const WvKvPages* kv, const WvKvBatch* batch, float* dk, int ldk, float* dv, int ldv, void* stream) {
+  const char* who = "wv_kv_read_dev";
+  int rc = wv_api_bind_device();
+  if (rc < 0) return rc;
+  if ((rc = kv_check(who, kv, batch)) < 0) return rc;
+  const bool none = rc == 1;
+  const long long kw = (long long)kv->num_kv_heads * kv->head_dim;
+  if ((rc = kv_rows(who, "k", dk, &ldk, kw)) || (rc = kv_rows(who, "v", dv, &ldv, kw))) return rc;
+  if (none) return WV_OK;
+  return wv_launch_kv_read(*kv, *batch, dk, ldk, dv, ldv, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int wv_attn_paged_dev(const WvKvPages* kv, const WvKvBatch* batch, const float* dq, int ldq, float* dout, int ldo, int num_heads,
+                                 float scale, int window, void* stream) {
+  const char* who = "wv_attn_paged_dev";
+  int rc = wv_api_bind_device();
+  if (rc < 0) return rc;
+  if ((rc = kv_check(who, kv, batch)) < 0) return rc;
+  const bool none = rc == 1;
+  if (num_heads < 1 || num_heads % kv->num_kv_heads) { wv_set_error("%s: %d heads over %d kv heads", who, num_heads, kv->num_kv_heads); return WV_ESHAPE; }
+  if (!(scale == scale) || scale - scale != 0.f) { wv_set_error("%s: the scale is not finite", who); return WV_EARG; }
+  const long long qw = (long long)num_heads * kv->head_dim;
+  if ((rc = kv_rows(who, "q", dq, &ldq, qw)) || (rc = kv_rows(who, "out", dout, &ldo, qw))) return rc;
+  if (none) return WV_OK;
+  return wv_launch_attn_paged(*kv, *batch, dq, ldq, dout, ldo, num_heads, scale, window > 0 ? window : 0, static_cast<cudaStream_t>(stream));
+}

@@ -24,3 +24,11 @@ def SampleTopKCUDA(d_logits: int, n: int, topK: int, temperature: float, determi
         u = random.random()
     check(lib().wv_topk_sample(d_logits, n, topK, temperature, 1 if deterministic else 0, u, C.byref(idx), stream))
     return idx.value
+
+
+def SampleRowsCUDA(d_logits: int, rows: int, n: int, d_temperature: int, d_top_k: int, d_top_p: int, d_min_p: int, d_u: int, d_index: int,
+                   d_prob: int = 0, ld: int = 0, stream: int = 0) -> None:
+    """The next token of every row: temperature, top-k, top-p and min-p of its own from device arrays (float32, int32, float32,
+    float32), the draw from d_u (float64); the index (int32; -1 where nothing can be drawn) and its probability (float32) are left in
+    device memory. wv_sample_rows_dev; no counterpart in the reference, which samples one row by top-k on the host."""
+    check(lib().wv_sample_rows_dev(d_logits, rows, n, ld, d_temperature, d_top_k, d_top_p, d_min_p, d_u, d_index, d_prob or None, stream))
