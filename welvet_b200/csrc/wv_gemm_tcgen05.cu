@@ -33,6 +33,7 @@
 // again) before the TMEM columns and the shared memory are given back.
 #include "wv_gemv_common.cuh"
 #include "wv_tma_common.cuh"
+#include "wv_lease.h"
 #include "wv_dev_hooks.h"
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -614,7 +615,7 @@ static PFN_cuTensorMapEncodeTiled_v12000 tcg_encode_fn() {
   return fn;
 }
 
-// Buffers for the rounded activations. A call's buffer may not be written by another call before its GEMM has read it, and a
+// Buffers for the rounded activations (and for the split results of the paged attention, wv_lease.h). A call's buffer may not be written by another call before its GEMM has read it, and a
 // captured call's may not be freed or used by anything else while a graph holds it:
 //   * a stream has a buffer of its own, which grows with what it is asked for (set-up time); calls on one stream are ordered,
 //     and its lock is held over both launches, so that two threads on one stream do not interleave them;
@@ -652,10 +653,9 @@ struct TcgRelaxed {
   TcgRelaxed() { cudaThreadExchangeStreamCaptureMode(&m); }
   ~TcgRelaxed() { cudaThreadExchangeStreamCaptureMode(&m); }
 };
-struct TcgLease { float* p = nullptr; bool free_after = false; std::unique_lock<std::mutex> lock; };
 
-static int tcg_lease(TcgLease& out, size_t floats, cudaStream_t st) {
-  auto fail = [&]() { cudaGetLastError(); wv_set_error("batched matvec: %zu bytes for the rounded activations unavailable", floats * 4); return WV_ENOMEM; };
+int wv_lease(WvLease& out, size_t floats, cudaStream_t st, const char* what) {
+  auto fail = [&]() { cudaGetLastError(); wv_set_error("%s: %zu bytes unavailable", what, floats * 4); return WV_ENOMEM; };
   TcgBufs& bufs = tcg_bufs();
   unsigned long long id = 0, cap = 0;
   cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
@@ -692,7 +692,7 @@ static int tcg_lease(TcgLease& out, size_t floats, cudaStream_t st) {
   }
   if (!sb) {
     if (cudaMallocAsync(&out.p, floats * 4, st) != cudaSuccess) return fail();
-    out.free_after = true;
+    out.free_on = st; out.free_after = true;
     return WV_OK;
   }
   out.lock = std::unique_lock<std::mutex>(sb->mu);
@@ -781,10 +781,9 @@ static int launch_tcg(const WvDevBlob& b, const float* dx, float* dy, int batch,
   const size_t smem = (size_t)g.rounds * TCG_GROUPS * g.b_bytes + 1024;
   // X rounded to TF32 once, by a small kernel in front (each of the row tiles would otherwise round it again), into a
   // buffer of the library; the main kernel fetches it through a tensor map encoded per call.
-  TcgLease lease;
-  if (const int rc = tcg_lease(lease, (size_t)batch * b.cols, st)) return rc;
+  WvLease lease;
+  if (const int rc = wv_lease(lease, (size_t)batch * b.cols, st, "batched matvec: the rounded activations")) return rc;
   float* xr = lease.p;
-  struct FreeAfter { TcgLease& l; cudaStream_t st; ~FreeAfter() { if (l.free_after) cudaFreeAsync(l.p, st); } } free_after{lease, st};
   CUtensorMap xmap;
   {
     cuuint64_t dims[2] = {(cuuint64_t)b.cols, (cuuint64_t)batch};

@@ -30,7 +30,7 @@ __host__ __device__ inline WvKvGeom wv_kv_geom(const WvKvPages& p) {
 // Codes in the sticky status word of paged calls.
 #define WV_PAGED_LENGTH 1        // q_start or kv_len outside its bounds
 #define WV_PAGED_PAGE 2          // a page number outside the pool
-__device__ __forceinline__ void wv_paged_report(int* err, int code) { atomicCAS_system(err, 0, code); }
+__device__ __forceinline__ void wv_paged_report(int* err, int code) { if (err) atomicCAS_system(err, 0, code); }
 
 // A sequence of the batch, cut to the call's bounds.
 struct WvSeq { int q0, q1, kv; };      // rows q0 .. q1 - 1 of q, kv tokens in the cache
