@@ -40,6 +40,7 @@ SOURCES = {
     "wv_decode.cu": [],
     "wv_kv_cache.cu": [],
     "wv_attn_paged.cu": [],
+    "wv_attn_chunk.cu": [],
     "wv_sample.cu": [],
     "wv_gemv_tc.cu": [],
     "wv_gemm_tcgen05.cu": [],

@@ -49,24 +49,6 @@ __device__ __forceinline__ void pr_mma(float (&d)[4], const uint4& a, unsigned b
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ unsigned pr_sub2(unsigned v, unsigned m) {
-  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&m));
-  return *reinterpret_cast<const unsigned*>(&r);
-}
-__device__ __forceinline__ unsigned pr_mul2(unsigned v, unsigned m) {
-  const __half2 r = __hmul2(*reinterpret_cast<const __half2*>(&v), *reinterpret_cast<const __half2*>(&m));
-  return *reinterpret_cast<const unsigned*>(&r);
-}
-// Integer bytes or nibbles become float16 without a conversion: a byte in the mantissa of 1024, then 1024 + offset is subtracted.
-// The low two (SEL 0x4140) or high two (0x4342) bytes of w, biased by 128, as signed values.
-template <unsigned SEL> __device__ __forceinline__ unsigned pr_bytes(unsigned w) { return pr_sub2(__byte_perm(w, 0x64646464u, SEL), 0x64806480u); }
-// Nibbles j and j + 4 of w, biased by 8, times the sub-scale in both halves of t.
-__device__ __forceinline__ unsigned pr_nibbles(unsigned w, int j, unsigned t) {
-  return pr_mul2(pr_sub2(((w >> (4 * j)) & 0x000f000fu) | 0x64006400u, 0x64086408u), t);
-}
-// Two bytes as a pair of float16.
-__device__ __forceinline__ unsigned pr_pair(unsigned a, unsigned b) { return pr_sub2(0x64006400u | a | (b << 16), 0x64006400u); }
-
 // The value index within a row of element e (0..3: k = 2c, 2c+1, 2c+8, 2c+9 of the fragment) of QK step s in lane column c.
 template <int BITS, int DP> __device__ __forceinline__ int pr_kdim(int s, int c, int e) {
   if constexpr (BITS == 16) return (c + 4 * (s >> 1)) * 8 + 4 * (s & 1) + e;
@@ -119,9 +101,9 @@ __global__ void __launch_bounds__(32 * PR_WARPS, (BITS == 16 && DP == 256) || (D
   int lo, hi;
   pa_range(sq, r0 / c.group, (r0 + rn - 1) / c.group, c.window, lo, hi);
   const int k0 = lo + sp * c.per, k1 = min(hi, k0 + c.per);              // this block's keys; k0 is a multiple of 16
-  auto grow = [&](int r) { return ((size_t)(sq.q0 + (r0 + r) / c.group)) * c.heads + kvh * c.group + (r0 + r) % c.group; };   // of [total_q][heads]
+  auto rec = [&](int r) { return (((size_t)seq * c.g.kvh + kvh) * (tiles * NROW) + r0 + r) * c.nsplit + sp; };      // a row's split result
   if (k0 >= k1) {
-    if (c.nsplit > 1) { if (tid < rn) c.ml[grow(tid) * c.nsplit + sp] = make_float2(-INFINITY, 0.f); }
+    if (c.nsplit > 1) { if (tid < rn) c.ml[rec(tid)] = make_float2(-INFINITY, 0.f); }
     else for (int i = tid; i < rn * c.g.hd; i += 32 * PR_WARPS) {        // rows that see nothing
       const int r = i / c.g.hd, t = sq.q0 + (r0 + r) / c.group, h = kvh * c.group + (r0 + r) % c.group;
       c.out[(size_t)t * c.ldo + (size_t)h * c.g.hd + i % c.g.hd] = 0.f;
@@ -277,9 +259,9 @@ __global__ void __launch_bounds__(32 * PR_WARPS, (BITS == 16 && DP == 256) || (D
       };
       if constexpr (BITS == 4 && DP == 64) {
         const uint2 w = *reinterpret_cast<const uint2*>(st + pr_at<RB>(r, cl >> 1) + 8 * (cl & 1));
-        const unsigned t1 = sc[128 + r * (hd / 16) + min(cl, hd / 16 - 1)], t = pr_pair(t1, t1);
-        step(0, pr_nibbles(w.x, 0, t), pr_nibbles(w.x, 1, t)); step(1, pr_nibbles(w.x, 2, t), pr_nibbles(w.x, 3, t));
-        step(2, pr_nibbles(w.y, 0, t), pr_nibbles(w.y, 1, t)); step(3, pr_nibbles(w.y, 2, t), pr_nibbles(w.y, 3, t));
+        const unsigned t1 = sc[128 + r * (hd / 16) + min(cl, hd / 16 - 1)], t = pa_pair(t1, t1);
+        step(0, pa_nibbles(w.x, 0, t), pa_nibbles(w.x, 1, t)); step(1, pa_nibbles(w.x, 2, t), pa_nibbles(w.x, 3, t));
+        step(2, pa_nibbles(w.y, 0, t), pa_nibbles(w.y, 1, t)); step(3, pa_nibbles(w.y, 2, t), pa_nibbles(w.y, 3, t));
       } else {
 #pragma unroll
         for (int i = 0; i < RB / 64; i++) {
@@ -288,16 +270,16 @@ __global__ void __launch_bounds__(32 * PR_WARPS, (BITS == 16 && DP == 256) || (D
           if constexpr (BITS == 16) { step(2 * i, w[0], w[1]); step(2 * i + 1, w[2], w[3]); }
           if constexpr (BITS == 8) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) { const unsigned x = w[j] ^ 0x80808080u; step(4 * i + j, pr_bytes<0x4140>(x), pr_bytes<0x4342>(x)); }
+            for (int j = 0; j < 4; j++) { const unsigned x = w[j] ^ 0x80808080u; step(4 * i + j, pa_bytes<0x4140>(x), pa_bytes<0x4342>(x)); }
           }
           if constexpr (BITS == 4) {
             const int at = 2 * (cl + 4 * i), n16 = hd / 16;
             const unsigned ta = at < n16 ? sc[128 + r * n16 + at] : 0u, tb = at + 1 < n16 ? sc[128 + r * n16 + at + 1] : 0u;
-            const unsigned t2[2] = {pr_pair(ta, ta), pr_pair(tb, tb)};
+            const unsigned t2[2] = {pa_pair(ta, ta), pa_pair(tb, tb)};
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-              step(8 * i + 2 * j, pr_nibbles(w[j], 0, t2[j >> 1]), pr_nibbles(w[j], 1, t2[j >> 1]));
-              step(8 * i + 2 * j + 1, pr_nibbles(w[j], 2, t2[j >> 1]), pr_nibbles(w[j], 3, t2[j >> 1]));
+              step(8 * i + 2 * j, pa_nibbles(w[j], 0, t2[j >> 1]), pa_nibbles(w[j], 1, t2[j >> 1]));
+              step(8 * i + 2 * j + 1, pa_nibbles(w[j], 2, t2[j >> 1]), pa_nibbles(w[j], 3, t2[j >> 1]));
             }
           }
         }
@@ -439,8 +421,8 @@ __global__ void __launch_bounds__(32 * PR_WARPS, (BITS == 16 && DP == 256) || (D
           const unsigned x0 = __byte_perm(v[0][w], v[1][w], 0x5140) ^ 0x80808080u, x1 = __byte_perm(v[0][w], v[1][w], 0x7362) ^ 0x80808080u;
           const unsigned z0 = __byte_perm(v[2][w], v[3][w], 0x5140) ^ 0x80808080u, z1 = __byte_perm(v[2][w], v[3][w], 0x7362) ^ 0x80808080u;
           const int t = 4 * (NW * i + w);
-          put(t, pr_bytes<0x4140>(x0), pr_bytes<0x4140>(z0)); put(t + 1, pr_bytes<0x4342>(x0), pr_bytes<0x4342>(z0));
-          put(t + 2, pr_bytes<0x4140>(x1), pr_bytes<0x4140>(z1)); put(t + 3, pr_bytes<0x4342>(x1), pr_bytes<0x4342>(z1));
+          put(t, pa_bytes<0x4140>(x0), pa_bytes<0x4140>(z0)); put(t + 1, pa_bytes<0x4342>(x0), pa_bytes<0x4342>(z0));
+          put(t + 2, pa_bytes<0x4140>(x1), pa_bytes<0x4140>(z1)); put(t + 3, pa_bytes<0x4342>(x1), pa_bytes<0x4342>(z1));
         }
       }
     } else {
@@ -464,12 +446,12 @@ __global__ void __launch_bounds__(32 * PR_WARPS, (BITS == 16 && DP == 256) || (D
         unsigned t4[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) t4[j] = sc[128 + S::SUB + rows4[j] * n16 + at];
-        const unsigned ta = pr_pair(t4[0], t4[1]), tb = pr_pair(t4[2], t4[3]);
+        const unsigned ta = pa_pair(t4[0], t4[1]), tb = pa_pair(t4[2], t4[3]);
 #pragma unroll
         for (int hf = 0; hf < 2; hf++) {
           const unsigned x = __byte_perm(v[0][w], v[1][w], hf ? 0x7632 : 0x5410), z = __byte_perm(v[2][w], v[3][w], hf ? 0x7632 : 0x5410);
 #pragma unroll
-          for (int j = 0; j < 4; j++) put(8 * w + 4 * hf + j, pr_nibbles(x, j, ta), pr_nibbles(z, j, tb));
+          for (int j = 0; j < 4; j++) put(8 * w + 4 * hf + j, pa_nibbles(x, j, ta), pa_nibbles(z, j, tb));
         }
       }
     }
@@ -512,8 +494,8 @@ __global__ void __launch_bounds__(32 * PR_WARPS, (BITS == 16 && DP == 256) || (D
       a += sums[(w * NROW + r) * DP + d] * (x.x == -INFINITY ? 1.f : fw);
     }
     if (c.nsplit > 1) {
-      c.acc[(grow(r) * c.nsplit + sp) * hd + d] = a;
-      if (d == 0) c.ml[grow(r) * c.nsplit + sp] = make_float2(M, L);
+      c.acc[rec(r) * hd + d] = a;
+      if (d == 0) c.ml[rec(r)] = make_float2(M, L);
     } else {
       const int t = sq.q0 + (r0 + r) / c.group, h = kvh * c.group + (r0 + r) % c.group;
       c.out[(size_t)t * c.ldo + (size_t)h * hd + d] = L == 0.f ? 0.f : a / L;
@@ -521,26 +503,15 @@ __global__ void __launch_bounds__(32 * PR_WARPS, (BITS == 16 && DP == 256) || (D
   }
 }
 
-// The splits' results of one (token, query head) joined in their order: a block per row, a thread per value. A split without
-// keys left {-inf, 0} and no sums.
-__global__ void __launch_bounds__(256) attn_join_kernel(const PaCall c) {
+// The splits' results joined in their order: a block per (sequence, kv head, row), a thread per value.
+__global__ void __launch_bounds__(256) rows_join_kernel(const __grid_constant__ PaCall c, int per_head) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int row = blockIdx.x / c.heads, h = blockIdx.x % c.heads, d = threadIdx.x;
-  if (row >= min(max(c.b.q_start[c.b.num_seqs], 0), c.b.total_q) || row < c.b.q_start[0] || d >= c.g.hd) return;
-  const size_t at = (size_t)blockIdx.x * c.nsplit;
-  float M = -INFINITY, L = 0.f, a = 0.f;
-  for (int s = 0; s < c.nsplit; s++) M = fmaxf(M, c.ml[at + s].x);
-  const float ref = M == -INFINITY ? 0.f : M;
-#pragma unroll 4
-  for (int s = 0; s < c.nsplit; s++) {
-    const float2 x = c.ml[at + s];
-    if (x.y == 0.f) continue;
-    const float w = x.x == -INFINITY ? 1.f : pa_ex2(x.x - ref);          // -inf with a divisor: NaN, which counts
-    L += x.y * w;
-    a += c.acc[(at + s) * c.g.hd + d] * w;
-  }
-  c.out[(size_t)row * c.ldo + (size_t)h * c.g.hd + d] = L == 0.f ? 0.f : a / L;
+  const int r = blockIdx.x % per_head, kvh = blockIdx.x / per_head % c.g.kvh, seq = blockIdx.x / per_head / c.g.kvh, d = threadIdx.x;
+  const WvSeq sq = wv_seq(c.b, c.g.page, seq, nullptr);
+  const int nrows = (sq.q1 - sq.q0) * c.group;
+  if (r >= nrows || nrows > c.rows_most || d >= c.g.hd) return;
+  pa_join(c, blockIdx.x, sq.q0 + r / c.group, kvh * c.group + r % c.group, d);
 }
 
 template <int BITS, int DP, bool R16>
@@ -582,39 +553,47 @@ int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* d
   c.scale = scale * 1.4426950408889634f;
   c.window = window;
   c.err = wv_paged_err_ptr();
-  c.rows_most = INT_MAX;
-  const long long most = (long long)b.max_q * c.group;                   // rows of a sequence
-  const bool r16 = most > 8;
-  const long long tiles = (most + (r16 ? 15 : 7)) / (r16 ? 16 : 8);
-  // Splits: about four blocks for each of two places an SM, of at least 128 keys each.
+  // Up to 32 rows (tokens x query heads of a kv head) a sequence is taken 8 or 16 rows at a time, beyond in tiles of 128.
+  const long long most = (long long)b.max_q * c.group;
+  c.rows_most = c.g.hd <= 128 ? 32 : INT_MAX;
+  const bool alike = (long long)b.num_seqs * b.max_q == b.total_q;       // every sequence has max_q new tokens
+  const bool chunk = most > c.rows_most, rows = !chunk || !alike;
+  if ((long long)b.total_q * heads > INT_MAX) { wv_set_error("wv_attn_paged_dev: %d rows of %d heads are too many", b.total_q, heads); return WV_ESHAPE; }
+  // what a sequence's new tokens can see together
   const long long keys = window > 0 && (long long)window + b.max_q + 16 < b.max_kv ? (long long)window + b.max_q + 16 : b.max_kv;
-  const long long blocks = (long long)b.num_seqs * tiles * c.g.kvh, want = 2LL * wv_sm_count();
-  if (blocks > INT_MAX || (long long)b.total_q * heads > INT_MAX) { wv_set_error("wv_attn_paged_dev: %d rows of %d heads are too many", b.total_q, heads); return WV_ESHAPE; }
-  long long per = (keys * blocks + want - 1) / want;
-  per = (per + 63) & ~63LL;
-  if (per < 64) per = 64;
-  if (per > 1024) per = 1024;
-  if (per < keys / 8192) per = (keys / 8192 + 63) & ~63LL;
-  long long ns = (keys + per - 1) / per;
-  if (ns < 1) ns = 1;
-  c.per = (int)per; c.nsplit = (int)ns;
-  WvLease lease;
-  if (c.nsplit > 1) {
-    const size_t n = (size_t)b.total_q * heads * c.nsplit;
-    if (const int rc = wv_lease(lease, n * (2 + c.g.hd) + 4, st, "wv_attn_paged_dev: the splits' results")) return rc;
-    c.ml = reinterpret_cast<float2*>(lease.p);
-    c.acc = lease.p + 2 * n;
+  const int sms = wv_sm_count();
+  if (rows) {
+    const long long top = chunk ? c.rows_most : most;
+    const bool r16 = top > 8;
+    const long long tiles = (top + (r16 ? 15 : 7)) / (r16 ? 16 : 8), per_head = tiles * (r16 ? 16 : 8);
+    const long long blocks = (long long)b.num_seqs * tiles * c.g.kvh, want = 2LL * sms;
+    if (blocks * (r16 ? 16 : 8) > INT_MAX) { wv_set_error("wv_attn_paged_dev: %d sequences are too many", b.num_seqs); return WV_ESHAPE; }
+    long long per = (keys * blocks + want - 1) / want;
+    per = (per + 63) & ~63LL;
+    if (per < 64) per = 64;
+    if (per > 1024) per = 1024;
+    if (per < keys / 8192) per = (keys / 8192 + 63) & ~63LL;
+    const long long ns = keys > per ? (keys + per - 1) / per : 1;
+    PaCall r = c;
+    r.per = (int)per; r.nsplit = (int)ns;
+    WvLease lease;
+    if (ns > 1) {
+      const size_t n = (size_t)(b.num_seqs * c.g.kvh) * per_head * ns;
+      if (const int rc = wv_lease(lease, n * (2 + c.g.hd), st, "wv_attn_paged_dev: the splits' results")) return rc;
+      r.ml = reinterpret_cast<float2*>(lease.p);
+      r.acc = lease.p + 2 * n;
+    }
+    cudaError_t e = kv.bits == 16 ? rows_pick<16>(r, r16, (int)tiles, st) : kv.bits == 8 ? rows_pick<8>(r, r16, (int)tiles, st) : rows_pick<4>(r, r16, (int)tiles, st);
+    if (e == cudaSuccess && ns > 1) {
+      cudaLaunchConfig_t cfg = {};
+      cudaLaunchAttribute at[1];
+      cfg.gridDim = dim3((unsigned)(b.num_seqs * c.g.kvh * per_head)); cfg.blockDim = dim3((c.g.hd + 31) & ~31); cfg.stream = st;
+      at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+      at[0].val.programmaticStreamSerializationAllowed = 1;
+      cfg.attrs = at; cfg.numAttrs = 1;
+      e = cudaLaunchKernelEx(&cfg, rows_join_kernel, r, (int)per_head);
+    }
+    if (e != cudaSuccess) { wv_set_error("wv_attn_paged_dev: launch: %s", cudaGetErrorString(cudaGetLastError())); return WV_ECUDA; }
   }
-  cudaError_t e = kv.bits == 16 ? rows_pick<16>(c, r16, (int)tiles, st) : kv.bits == 8 ? rows_pick<8>(c, r16, (int)tiles, st) : rows_pick<4>(c, r16, (int)tiles, st);
-  if (e == cudaSuccess && c.nsplit > 1) {
-    cudaLaunchConfig_t cfg = {};
-    cudaLaunchAttribute at[1];
-    cfg.gridDim = dim3((unsigned)(b.total_q * heads)); cfg.blockDim = dim3((c.g.hd + 31) & ~31); cfg.stream = st;
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = at; cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, attn_join_kernel, c);
-  }
-  if (e != cudaSuccess) { wv_set_error("wv_attn_paged_dev: launch: %s", cudaGetErrorString(cudaGetLastError())); return WV_ECUDA; }
-  return WV_OK;
+  return chunk ? wv_launch_attn_chunk(c, kv.bits, keys, alike, st) : WV_OK;
 }
