@@ -161,7 +161,8 @@ int wv_topk_sample(const float* d_logits, int n, int top_k, float temperature, i
  *    8  int8 codes, value = scale * code, scale = max|x| / 127
  *    4  codes + 8 in nibbles (value 2i in the low one of byte i), value = scale * (sub * code); scale = max|x| / 1785, and a
  *       byte sub for each 16 values, ceil(max|x of the 16| / 7 / scale), at least 1, so that |code| <= 7
- * with the scale (float32, at least 2^-126) of a row and codes rounded to nearest even. A row with a value that is not
+ * with the scale (float32, at least 2^-126) of a row and codes rounded to nearest even; a division by 127, 1785 or 7 is a
+ * product with its float32 reciprocal, one by a scale is a division. A row with a value that is not
  * finite gets the scale NaN and codes of zero: who may see that token gets NaN, and nobody else does. page_size is a multiple of
  * 16, head_dim a multiple of 16 up to 256, pool 16-byte aligned.
  *

@@ -83,11 +83,11 @@ def quantise_finite(x, bits):
         s = np.where(a > 0, s, FLT_MIN)
         return (x / s).astype(np.float16).astype(np.float64) * s
     if bits == 8:
-        s = np.maximum(a / np.float32(127), FLT_MIN)
+        s = np.maximum(a * (np.float32(1) / np.float32(127)), FLT_MIN)
         return np.rint(x / s).astype(np.float64) * s
-    s = np.maximum(a / np.float32(1785), FLT_MIN)
+    s = np.maximum(a * (np.float32(1) / np.float32(1785)), FLT_MIN)
     g = x.reshape(*x.shape[:-1], -1, 16)
-    t = np.clip(np.ceil(np.abs(g).max(-1) / np.float32(7) / s), 1, 255).astype(np.float32)
+    t = np.clip(np.ceil(np.abs(g).max(-1) * (np.float32(1) / np.float32(7)) / s), 1, 255).astype(np.float32)
     c = np.clip(np.rint(g / (s * t)[..., None]), -7, 7).astype(np.float64)
     return (c * t[..., None]).reshape(x.shape) * s
 

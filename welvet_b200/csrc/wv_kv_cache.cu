@@ -69,7 +69,7 @@ __device__ __forceinline__ void kv_store_row(const WvKvGeom& g, unsigned char* b
   const float a = __uint_as_float(m);
   float s;
   if (BITS == 16) s = __uint_as_float((unsigned)max((int)(m >> 23) - 14, 1) << 23);   // a subnormal has exponent 0: the smallest scale
-  else s = fmaxf(__fdiv_rn(a, BITS == 8 ? 127.f : 1785.f), FLT_MIN);
+  else s = fmaxf(__fmul_rn(a, BITS == 8 ? 1.f / 127.f : 1.f / 1785.f), FLT_MIN);
   unsigned char* codes = block + (is_v ? g.page * g.code : 0) + slot * g.code;
 #pragma unroll
   for (int i = 0; i < V4; i++) {
@@ -86,7 +86,7 @@ __device__ __forceinline__ void kv_store_row(const WvKvGeom& g, unsigned char* b
       for (int e = 0; e < 4; e++) w |= ((unsigned)(fine ? (int)rintf(__fdiv_rn(x[i][e], s)) : 0) & 0xffu) << (8 * e);
       *reinterpret_cast<unsigned*>(codes + d) = w;
     } else {
-      const float t = fine ? fminf(fmaxf(ceilf(__fdiv_rn(__fdiv_rn(__uint_as_float(mg[i]), 7.f), s)), 1.f), 255.f) : 1.f;
+      const float t = fine ? fminf(fmaxf(ceilf(__fdiv_rn(__fmul_rn(__uint_as_float(mg[i]), 1.f / 7.f), s)), 1.f), 255.f) : 1.f;
       const float st = __fmul_rn(s, t);
       unsigned w = 0;
 #pragma unroll
