@@ -207,8 +207,8 @@ int wv_attn_paged_dev(const WvKvPages* kv, const WvKvBatch* batch, const float* 
  * top_k <= 0); of those, with w = exp((logit - max) / T), the ones whose preceding w add up to less than top_p of the sum, the first
  * one in any case; of those the ones with w >= min_p, again the first one in any case. The token is the first whose running sum of w reaches u times the sum of the
  * kept ones. T <= 0 or top_k == 1: the first candidate. d_index[r] is the token, d_prob[r] (may be NULL) its share of the kept
- * weight; -1 and 0 for a row without a candidate. Sums are integers in units of 2^-(62 - ceil(log2 n)), so the result does not
- * depend on the order of summation. */
+ * weight; -1 and 0 for a row without a candidate. In the sums a w counts in units of 2^-31, rounded to nearest, as whole
+ * numbers: the result does not depend on the order of summation, and what is below 2^-32 of the largest is never drawn. */
 int wv_sample_rows_dev(const float* d_logits, int rows, int n, int64_t ld, const float* d_temperature, const int* d_top_k,
                        const float* d_top_p, const float* d_min_p, const double* d_u, int* d_index, float* d_prob, void* stream);
 

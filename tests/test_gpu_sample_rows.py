@@ -125,6 +125,39 @@ def test_ties_go_by_index(wv):
     assert abs(prob[3] - 0.1) < 1e-6
 
 
+@pytest.mark.parametrize("n", [9001, 128256, 360448, 360449])
+def test_many_equal_logits(wv, n):
+    """More equal candidates than are sorted together, over one and all of the cluster's parts, and a row that is walked in memory."""
+    x = np.zeros((5, n), np.float32)
+    x[1, 100:n - 100] = -1.0
+    x[2, n - 1] = 1.0
+    x[3, ::3] = 0.25
+    x[4] = np.linspace(0, 1e-4, n, dtype=np.float32)
+    t, k, p, mp = [1.0] * 5, [0, 0, 0, 5000, 0], [1.0, 0.9, 1.0, 0.7, 0.5], [0.0, 0.0, 0.0, 0.9, 0.0]
+    u = [0.7, 0.5, 0.999, 0.9, 0.25]
+    got, prob = run_rows(wv, torch.from_numpy(x).cuda(), t, k, p, mp, u)
+    for r in range(5):
+        want, pw, margin = sample64(x[r], t[r], k[r], p[r], mp[r], u[r])
+        # equal weights: a place is u n of them, rounded up, and the sums are whole numbers; for the slope one place is 1 / n
+        assert abs(got[r] - want) <= (0 if r in (0, 2) else 2), (r, got[r], want)
+        assert abs(prob[r] - pw) <= 1e-6 * pw
+
+
+@pytest.mark.parametrize("n", [200000, 400000])
+def test_long_rows(wv, n):
+    """The token is the definition's for the draw, or for one 2^-20 beside it: with so many candidates the running sums are near one
+    another, and a weight's exponential in float32 is off by 2^-23."""
+    rng = np.random.default_rng(n)
+    x = (rng.normal(0, 1, (10, n)) * 2).astype(np.float32)
+    k, p = [0, 40, 0, 30000, 1, 0, 3000, 0, 1500, n], [1.0, 0.9, 0.95, 0.9, 1.0, 0.4, 1.0, 1.0, 1.0, 0.99]
+    mp, u = [0.0, 0.0, 0.0, 0.0, 0.0, 0.001, 0.0, 0.05, 0.0, 0.0], rng.random(10)
+    got, prob = run_rows(wv, torch.from_numpy(x).cuda(), [0.9] * 10, k, p, mp, u)
+    for r in range(10):
+        want = [sample64(x[r], 0.9, k[r], p[r], mp[r], min(max(u[r] + d, 0.0), 1.0)) for d in (0.0, -2.0 ** -20, 2.0 ** -20)]
+        assert got[r] in [w[0] for w in want], r
+        assert abs(prob[r] - want[0][1]) <= 2.0 ** -18 * want[0][1]
+
+
 def test_ends_of_the_draw(wv):
     """u = 0 takes the first candidate, u = 1 the last one that has weight."""
     rng = np.random.default_rng(0)

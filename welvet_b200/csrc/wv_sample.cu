@@ -1,68 +1,368 @@
 // The next token of each of many rows of logits: temperature, top-k, top-p, min-p and a draw (include/welvet_cuda.h,
 // wv_sample_rows_dev).
 //
-// Candidates are ordered by a 64-bit word (ordered bits of logit / T : ~index), all distinct. Every cut is a prefix of that order,
-// so each step looks for one word: the k-th largest by count, the last one that top-p keeps and the drawn one by weight. Weights
-// are integers in units of 2^-shift, so that no sum depends on its order; each search walks the word's digits from the top with a
-// histogram a digit.
+// Candidates are ordered by a 64-bit word (ordered bits of logit / T : ~index), all distinct. Every cut keeps a prefix of that
+// order, so the kept weight is the smallest of the prefixes' weights, and the token is the first one whose running weight
+// reaches u times that: what has to be found is where the running count reaches k, where the running weight reaches the
+// line of top-p, and where it reaches the draw. Weights count as whole numbers in units of 2^-31, so no sum depends on its order.
+//
+// A row is read once. A cluster of eight CTAs (one up to 8192 logits) holds its logits / T in shared memory and sorts them into 2048
+// bins of 1/64 by their distance from the largest, count and weight of each; the sums over the cluster (distributed shared memory)
+// say in which bin each of the three places lies. Where the bins down to the last of those hold no more than 2048 candidates (any
+// top-k up to there, any nucleus of so many), these are gathered and sorted, and the rest is a scan over them. Otherwise the
+// places are found one after the other, each among the gathered candidates of its own bin; a bin with too many (equal logits) is
+// first cut down by further digits of the word.
+//
+// Bound: HBM for many rows (4 bytes a logit), the cluster's four or five barriers for one. A row that does not fit the cluster's
+// shared memory (more than 360448 logits) is walked digit by digit over global memory by one CTA.
 #include "wv_common.cuh"
+#include <cooperative_groups.h>
 #include <math.h>
 
-#define SMP_THREADS 1024
+namespace cg = cooperative_groups;
+typedef unsigned long long u64;
 
-// exp(d), d <= 0, in units of 2^-shift, rounded to nearest: exp rounds to float32, the rest is integer arithmetic on its bits.
-__device__ __forceinline__ unsigned long long smp_fixed(float w, int shift) {
-  const unsigned u = __float_as_uint(w);
-  const int e = (int)(u >> 23);
-  if (e == 0) return 0ull;                                        // below 2^-126
-  const unsigned long long m = (u & 0x7fffffu) | 0x800000u;
-  const int s = e - 150 + shift;                                  // w = m 2^(e - 150)
-  if (s >= 0) return m << s;
-  return s < -25 ? 0ull : (m + (1ull << (-s - 1))) >> -s;
+__device__ __forceinline__ u64 smp_word(float v, int i) {
+  const unsigned u = __float_as_uint(v == 0.f ? 0.f : v);                // -0 and 0 are equal
+  const unsigned key = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return ((u64)key << 32) | (u64)(0xFFFFFFFFu - (unsigned)i);
 }
+__device__ __forceinline__ float smp_value(u64 w) {
+  const unsigned u = (unsigned)(w >> 32);
+  return __uint_as_float((u & 0x80000000u) ? (u & 0x7FFFFFFFu) : ~u);
+}
+__device__ __forceinline__ int smp_index(u64 w) { return (int)(0xFFFFFFFFu - (unsigned)w); }
+__device__ __forceinline__ float smp_weight(float y, float top) { return y == top ? 1.f : expf(__fsub_rn(y, top)); }
+__device__ __forceinline__ unsigned smp_units(float w) { return __float2uint_rn(w * 2147483648.f); }
+// The smallest whole number that is at least f * total, between 1 and total.
+__device__ __forceinline__ u64 smp_target(double f, u64 total) {
+  const double t = ceil(f * (double)total);
+  if (!(t > 1.0)) return 1ull;
+  return t >= (double)total ? total : (u64)t;
+}
+// logit / T; NaN for what is no candidate. A finite logit may become an infinity by the division: it stays a candidate.
+__device__ __forceinline__ float smp_y(float x, float t, bool greedy) { return !(x > -INFINITY) ? NAN : greedy ? x : __fdiv_rn(x, t); }
 
-struct SmpRow {
-  const float* x; int n; float t; bool greedy; float top; int shift;
-  // logit / T; NaN for what is no candidate. A finite logit may become an infinity by the division: it stays a candidate.
-  __device__ __forceinline__ float y(int i) const { const float v = x[i]; return !(v > -INFINITY) ? NAN : greedy ? v : __fdiv_rn(v, t); }
-  static __device__ __forceinline__ unsigned long long word(float v, int i) {
-    const unsigned u = __float_as_uint(v == 0.f ? 0.f : v);       // -0 and 0 are equal
-    const unsigned key = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
-    return ((unsigned long long)key << 32) | (unsigned long long)(0xFFFFFFFFu - (unsigned)i);
-  }
-  __device__ __forceinline__ float w(float v) const { return v == top ? 1.f : expf(__fsub_rn(v, top)); }
+#define SMP_THREADS 512
+#define SMP_WARPS (SMP_THREADS / 32)
+#define SMP_CLUSTER 8
+#define SMP_SMALL 8192
+#define SMP_BINS 2048
+#define SMP_LIST 2048
+#define SMP_CACHE (44 * 1024)              // logits a CTA holds at most
+
+struct SmpArgs {
+  const float* logits; int n; long long ld;
+  const float* temperature; const int* top_k; const float* top_p; const float* min_p; const double* u;
+  int* index; float* prob;
+};
+// Four neighbouring bins of a thread: counts and weights up to and including each.
+struct SmpScan { unsigned c[4], c0; u64 w[4], w0; };
+struct SmpSel { int bin; unsigned before, count; u64 weight_before; };
+
+struct __align__(16) SmpShared {
+  union {
+    unsigned hist[3][SMP_BINS];            // counts, low and high halves of the weights
+    u64 run[SMP_LIST];                     // afterwards: the list's running weights
+  };
+  u64 list[SMP_LIST];
+  u64 part[SMP_WARPS];
+  unsigned partc[SMP_WARPS];
+  u64 best, least_sum, result_word, result_cum;
+  SmpSel sel;
+  unsigned filled;
 };
 
-// The word where the running total (from the largest word down, over words >= floor) reaches `target`; BY_WEIGHT: of weights
-// w >= least, else of counts.
+__device__ __forceinline__ int smp_bin(float y, float top) {
+  if (y == top) return 0;
+  return min((int)(__fsub_rn(top, y) * 64.f), SMP_BINS - 1);             // rises as y falls: each step rounds monotonously
+}
+
+// Sums of the bins over the cluster and their running totals. Ends with every CTA past its reads of the others' bins.
+__device__ __forceinline__ void smp_scan(cg::cluster_group& cluster, SmpShared& S, SmpScan& r) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ncta = (int)cluster.num_blocks();
+  unsigned c[4] = {0, 0, 0, 0};
+  u64 w[4] = {0, 0, 0, 0};
+  for (int q = 0; q < ncta; q++) {
+    const SmpShared* o = cluster.map_shared_rank(&S, q);
+    const uint4 a = reinterpret_cast<const uint4*>(o->hist[0])[tid], l = reinterpret_cast<const uint4*>(o->hist[1])[tid], h = reinterpret_cast<const uint4*>(o->hist[2])[tid];
+    c[0] += a.x; c[1] += a.y; c[2] += a.z; c[3] += a.w;
+    w[0] += l.x + ((u64)h.x << 16); w[1] += l.y + ((u64)h.y << 16); w[2] += l.z + ((u64)h.z << 16); w[3] += l.w + ((u64)h.w << 16);
+  }
+  unsigned ct = c[0] + c[1] + c[2] + c[3];
+  u64 wt = w[0] + w[1] + w[2] + w[3];
+  const unsigned c_own = ct;
+  const u64 w_own = wt;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const unsigned a = __shfl_up_sync(0xffffffffu, ct, o);
+    const u64 b = __shfl_up_sync(0xffffffffu, wt, o);
+    if (lane >= o) { ct += a; wt += b; }
+  }
+  if (lane == 31) { S.partc[warp] = ct; S.part[warp] = wt; }
+  __syncthreads();
+  for (int q = 0; q < warp; q++) { ct += S.partc[q]; wt += S.part[q]; }
+  r.c0 = ct - c_own; r.w0 = wt - w_own;
+  unsigned a = r.c0;
+  u64 b = r.w0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) { a += c[i]; b += w[i]; r.c[i] = a; r.w[i] = b; }
+  cluster.sync();
+}
+// The bin in which the running count (or weight) reaches target.
+__device__ __forceinline__ SmpSel smp_select(SmpShared& S, const SmpScan& r, bool by_weight, u64 target) {
+  unsigned cb = r.c0;
+  u64 wb = r.w0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if (by_weight ? (wb < target && r.w[i] >= target) : (cb < target && r.c[i] >= target)) S.sel = SmpSel{4 * (int)threadIdx.x + i, cb, r.c[i] - cb, wb};
+    cb = r.c[i]; wb = r.w[i];
+  }
+  __syncthreads();
+  const SmpSel s = S.sel;
+  __syncthreads();
+  return s;
+}
+// The first cnt words of the list from the largest down, and their running weights.
+__device__ __forceinline__ void smp_sort(SmpShared& S, int cnt, float top) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int p2 = 1;
+  while (p2 < cnt) p2 <<= 1;
+  for (int i = cnt + tid; i < p2; i += SMP_THREADS) S.list[i] = 0ull;
+  __syncthreads();
+  for (int size = 2; size <= p2; size <<= 1)
+    for (int stride = size >> 1; stride > 0; stride >>= 1) {
+      for (int i = tid; i < p2 / 2; i += SMP_THREADS) {
+        const int a = 2 * i - (i & (stride - 1)), b = a + stride;
+        const u64 x = S.list[a], y = S.list[b];
+        if (((a & size) == 0) ? (x < y) : (x > y)) { S.list[a] = y; S.list[b] = x; }
+      }
+      // steps of up to 32 stay within the 64 words of a warp
+      const int next = stride > 1 ? stride >> 1 : size;
+      if (stride > 32 || next > 32 || p2 > 2 * SMP_THREADS) __syncthreads(); else __syncwarp();
+    }
+  __syncthreads();
+  constexpr int PER = SMP_LIST / SMP_THREADS;
+  u64 v[PER], t = 0;
+#pragma unroll
+  for (int i = 0; i < PER; i++) { const int q = PER * tid + i; t += q < cnt ? smp_units(smp_weight(smp_value(S.list[q]), top)) : 0u; v[i] = t; }
+  u64 s = t;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) { const u64 b = __shfl_up_sync(0xffffffffu, s, o); if (lane >= o) s += b; }
+  if (lane == 31) S.part[warp] = s;
+  __syncthreads();
+  for (int q = 0; q < warp; q++) s += S.part[q];
+#pragma unroll
+  for (int i = 0; i < PER; i++) S.run[PER * tid + i] = s - t + v[i];
+  __syncthreads();
+}
+// The place in S.run[0 .. cnt) (rising) where the running weight reaches target; the last place if it does not.
+__device__ __forceinline__ int smp_place(const SmpShared& S, int cnt, u64 target) {
+  int lo = 0, hi = cnt - 1;
+  while (lo < hi) { const int m = (lo + hi) >> 1; if (S.run[m] >= target) hi = m; else lo = m + 1; }
+  return lo;
+}
+
+__global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const SmpArgs A, int per) {
+  extern __shared__ __align__(16) unsigned char smp_smem[];
+  SmpShared& S = *reinterpret_cast<SmpShared*>(smp_smem);
+  float* s_y = reinterpret_cast<float*>(smp_smem + sizeof(SmpShared));
+  cg::cluster_group cluster = cg::this_cluster();
+  const int ncta = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), row = blockIdx.x / ncta;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const int i0 = min(A.n, rank * per), mine = min(A.n - i0, per);
+  for (int i = tid; i < 3 * SMP_BINS; i += SMP_THREADS) S.hist[0][i] = 0u;
+  if (tid == 0) { S.best = 0ull; S.least_sum = 0ull; S.filled = 0u; }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const float t = A.temperature[row];
+  const int k = A.top_k[row];
+  const bool greedy = t <= 0.f || k == 1;
+  const float least = A.min_p[row];
+  const double tp = (double)A.top_p[row], u = A.u[row];
+  const float* x = A.logits + (size_t)row * A.ld + i0;
+  __syncthreads();
+  // ---- the row's logits / T into shared memory, and the largest word
+  {
+    float best = -INFINITY;
+    int at = -1;
+    for (int b = tid; b < mine; b += 8 * SMP_THREADS) {
+      float v[8];
+#pragma unroll
+      for (int q = 0; q < 8; q++) v[q] = b + q * SMP_THREADS < mine ? x[b + q * SMP_THREADS] : NAN;
+#pragma unroll
+      for (int q = 0; q < 8; q++) {
+        const int i = b + q * SMP_THREADS;
+        if (i >= mine) break;
+        const float y = smp_y(v[q], t, greedy);
+        s_y[i] = y;
+        if (y > best || (y == best && at < 0)) { best = y; at = i; }     // a thread's places rise: the first of equals
+      }
+    }
+    u64 w = at < 0 ? 0ull : smp_word(best, i0 + at);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) w = max(w, __shfl_xor_sync(0xffffffffu, w, o));
+    if (lane == 0 && w) atomicMax(&S.best, w);
+  }
+  cluster.sync();
+  u64 best = 0ull;
+  for (int q = 0; q < ncta; q++) best = max(best, cluster.map_shared_rank(&S, q)->best);
+  const float top = smp_value(best);
+  if (best == 0ull || greedy) {
+    if (rank == 0 && tid == 0) { A.index[row] = best ? smp_index(best) : -1; if (A.prob) A.prob[row] = best ? 1.f : 0.f; }
+    cluster.sync();                        // nobody leaves while its shared memory may be read
+    return;
+  }
+  // ---- counts and weights of the bins, and the weight that min-p leaves
+  {
+    u64 ms = 0ull;
+    for (int i = tid; i < mine; i += SMP_THREADS) {
+      const float y = s_y[i];
+      if (y != y) continue;
+      const float f = smp_weight(y, top);
+      const unsigned w = smp_units(f);
+      const int b = smp_bin(y, top);
+      atomicAdd(&S.hist[0][b], 1u);
+      if (w) { atomicAdd(&S.hist[1][b], w & 0xffffu); atomicAdd(&S.hist[2][b], w >> 16); }
+      if (f >= least) ms += w;
+    }
+#pragma unroll
+    for (int o = 16; o; o >>= 1) ms += __shfl_xor_sync(0xffffffffu, ms, o);
+    if (lane == 0 && ms) atomicAdd(&S.least_sum, ms);
+  }
+  cluster.sync();
+  u64 wmin = 0ull;
+  for (int q = 0; q < ncta; q++) wmin += cluster.map_shared_rank(&S, q)->least_sum;
+  SmpScan scan;
+  smp_scan(cluster, S, scan);
+  if (tid == SMP_THREADS - 1) { S.partc[0] = scan.c[3]; S.part[0] = scan.w[3]; }
+  __syncthreads();
+  const unsigned count = S.partc[0];
+  const u64 all = S.part[0];
+  __syncthreads();
+  if (!(least <= 1.f)) wmin = 1ull;        // only the first candidate, and the draw finds no other
+  const bool cut_k = k > 0 && (unsigned)k < count, cut_p = !(tp >= 1.0);
+  const SmpSel end = cut_k ? smp_select(S, scan, false, (u64)k) : smp_select(S, scan, true, min(cut_p ? smp_target(tp, all) : all, wmin));
+
+  // words of the logits in bins first .. last whose digits above `himask` are `prefix`, into CTA 0's list
+  auto gather = [&](int first, int last, u64 himask, u64 prefix) {
+    unsigned* filled = &cluster.map_shared_rank(&S, 0)->filled;
+    u64* list = cluster.map_shared_rank(&S, 0)->list;
+    for (int i = tid; i < mine; i += SMP_THREADS) {
+      const float y = s_y[i];
+      if (y != y) continue;
+      const int b = smp_bin(y, top);
+      if (b < first || b > last) continue;
+      const u64 w = smp_word(y, i0 + i);
+      if ((w & himask) != prefix) continue;
+      const unsigned at = atomicAdd(filled, 1u);
+      if (at < SMP_LIST) list[at] = w;
+    }
+    cluster.sync();
+  };
+  auto finish = [&](u64 word, u64 kept) {
+    A.index[row] = smp_index(word);
+    if (A.prob) A.prob[row] = (float)((double)smp_weight(smp_value(word), top) * 2147483648.0 / (double)kept);
+  };
+
+  if (end.before + end.count <= SMP_LIST) {
+    gather(0, end.bin, 0ull, 0ull);
+    if (rank != 0) return;
+    const int cnt = (int)(end.before + end.count);
+    smp_sort(S, cnt, top);
+    if (tid == 0) {
+      const u64 wk = cut_k ? S.run[k - 1] : all;
+      u64 kept = wk;
+      if (cut_p) { const u64 line = smp_target(tp, wk); kept = wmin < line ? wmin : S.run[smp_place(S, cut_k ? k : cnt, line)]; }
+      if (wmin < kept) kept = wmin;
+      if (!(least <= 1.f)) kept = 1ull << 31;
+      finish(S.list[least <= 1.f ? smp_place(S, cnt, smp_target(u, kept)) : 0], kept);
+    }
+    return;
+  }
+
+  // ---- too many to sort together: the three places one after the other
+  auto find = [&](bool by_weight, u64 target, u64& cum) -> u64 {
+    SmpSel s = smp_select(S, scan, by_weight, target);
+    const int bin = s.bin;
+    u64 himask = 0ull, prefix = 0ull, before_w = s.weight_before;
+    u64 left = target - (by_weight ? s.weight_before : (u64)s.before);
+    for (int shift = 64 - 11; s.count > SMP_LIST; shift = max(shift - 11, 0)) {
+      for (int i = tid; i < 3 * SMP_BINS; i += SMP_THREADS) S.hist[0][i] = 0u;
+      __syncthreads();
+      for (int i = tid; i < mine; i += SMP_THREADS) {
+        const float y = s_y[i];
+        if (y != y || smp_bin(y, top) != bin) continue;
+        const u64 w = smp_word(y, i0 + i);
+        if ((w & himask) != prefix) continue;
+        const int d = SMP_BINS - 1 - (int)((w >> shift) & (SMP_BINS - 1));          // the largest digit first
+        const unsigned f = smp_units(smp_weight(y, top));
+        atomicAdd(&S.hist[0][d], 1u);
+        if (f) { atomicAdd(&S.hist[1][d], f & 0xffffu); atomicAdd(&S.hist[2][d], f >> 16); }
+      }
+      cluster.sync();
+      SmpScan fine;
+      smp_scan(cluster, S, fine);
+      s = smp_select(S, fine, by_weight, left);
+      left -= by_weight ? s.weight_before : (u64)s.before;
+      before_w += s.weight_before;
+      himask = shift ? ~0ull << shift : ~0ull;
+      prefix = (prefix & ~((u64)(SMP_BINS - 1) << shift)) | (u64)(SMP_BINS - 1 - s.bin) << shift;
+    }
+    if (rank == 0 && tid == 0) S.filled = 0u;
+    cluster.sync();
+    gather(bin, bin, himask, prefix);
+    if (rank == 0) {
+      const int cnt = (int)s.count;
+      smp_sort(S, cnt, top);
+      if (tid < ncta) {                    // a thread for each CTA tells it
+        const int at = by_weight ? smp_place(S, cnt, left) : (int)left - 1;
+        SmpShared* o = cluster.map_shared_rank(&S, tid);
+        o->result_word = S.list[at]; o->result_cum = before_w + S.run[at];
+      }
+    }
+    cluster.sync();
+    cum = S.result_cum;
+    return S.result_word;
+  };
+  u64 kept = all, cum;
+  if (cut_k) { find(false, (u64)k, cum); kept = cum; }
+  if (cut_p) { const u64 line = smp_target(tp, kept); if (wmin < line) kept = wmin; else { find(true, line, cum); kept = cum; } }
+  if (wmin < kept) kept = wmin;
+  const u64 word = least <= 1.f ? find(true, smp_target(u, kept), cum) : best;
+  if (!(least <= 1.f)) kept = 1ull << 31;
+  if (rank == 0 && tid == 0) finish(word, kept);
+  cluster.sync();
+}
+
+// ------------------------------------------------------------------ a row beyond the cluster's shared memory
+#define SMW_THREADS 1024
+struct SmwRow {
+  const float* x; int n; float t; float top;
+  __device__ __forceinline__ float y(int i) const { return smp_y(x[i], t, false); }
+};
+// The word where the running total from the largest down reaches `target`, and the weight up to it. BY_WEIGHT: of weights, else of counts.
 template <bool BY_WEIGHT>
-__device__ unsigned long long smp_find(const SmpRow& r, unsigned long long floor_word, float least, unsigned long long target) {
-  __shared__ unsigned long long s_hist[256], s_prefix, s_left;
-  unsigned long long prefix = 0ull;
+__device__ u64 smw_find(const SmwRow& r, u64 target) {
+  __shared__ u64 s_hist[256], s_prefix, s_left;
+  u64 prefix = 0ull;
   for (int shift = 56; shift >= 0; shift -= 8) {
-    for (int i = threadIdx.x; i < 256; i += SMP_THREADS) s_hist[i] = 0ull;
+    for (int i = threadIdx.x; i < 256; i += SMW_THREADS) s_hist[i] = 0ull;
     __syncthreads();
-    const unsigned long long himask = shift == 56 ? 0ull : (~0ull << (shift + 8));
-    for (int i = threadIdx.x; i < r.n; i += SMP_THREADS) {
+    const u64 himask = shift == 56 ? 0ull : (~0ull << (shift + 8));
+    for (int i = threadIdx.x; i < r.n; i += SMW_THREADS) {
       const float v = r.y(i);
       if (v != v) continue;
-      const unsigned long long w = SmpRow::word(v, i);
-      if (w < floor_word || (w & himask) != prefix) continue;
-      if (BY_WEIGHT) {
-        const float f = r.w(v);
-        if (f >= least) atomicAdd(&s_hist[(w >> shift) & 255u], smp_fixed(f, r.shift));
-      } else atomicAdd(&s_hist[(w >> shift) & 255u], 1ull);
+      const u64 w = smp_word(v, i);
+      if ((w & himask) != prefix) continue;
+      atomicAdd(&s_hist[(w >> shift) & 255u], BY_WEIGHT ? (u64)smp_units(smp_weight(v, r.top)) : 1ull);
     }
     __syncthreads();
     if (threadIdx.x == 0) {
-      unsigned long long left = target;
-      int d = 255, last = -1;
-      for (; d >= 0; d--) {
-        if (s_hist[d]) last = d;
-        if (s_hist[d] >= left && s_hist[d]) break;
-        left -= s_hist[d];
-      }
-      s_prefix = prefix | ((unsigned long long)(d >= 0 ? d : (last >= 0 ? last : 0)) << shift);
+      u64 left = target;
+      int d = 255;
+      for (; d > 0 && s_hist[d] < left; d--) left -= s_hist[d];
+      s_prefix = prefix | ((u64)d << shift);
       s_left = left;
     }
     __syncthreads();
@@ -71,106 +371,94 @@ __device__ unsigned long long smp_find(const SmpRow& r, unsigned long long floor
   }
   return prefix;
 }
-
-template <typename T> __device__ T smp_sum(T v) {
-  __shared__ T s_part[32];
+template <typename F> __device__ u64 smw_reduce(u64 v, F f) {
+  __shared__ u64 s_part[32];
 #pragma unroll
-  for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  for (int o = 16; o; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
   if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = v;
   __syncthreads();
-  T t = 0;
-  for (int i = 0; i < SMP_THREADS / 32; i++) t += s_part[i];
+  u64 t = s_part[0];
+  for (int i = 1; i < SMW_THREADS / 32; i++) t = f(t, s_part[i]);
   __syncthreads();
   return t;
 }
-__device__ unsigned long long smp_max(unsigned long long v) {
-  __shared__ unsigned long long s_part[32];
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-  if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = v;
-  __syncthreads();
-  unsigned long long t = 0;
-  for (int i = 0; i < SMP_THREADS / 32; i++) t = max(t, s_part[i]);
-  __syncthreads();
-  return t;
-}
-// The smallest whole number that is at least f * total, between 1 and total.
-__device__ __forceinline__ unsigned long long smp_target(double f, unsigned long long total) {
-  const double t = ceil(f * (double)total);
-  if (!(t > 1.0)) return 1ull;
-  return t >= (double)total ? total : (unsigned long long)t;
-}
-
-__global__ void __launch_bounds__(SMP_THREADS, 1) sample_rows_kernel(const float* __restrict__ logits, int n, long long ld, const float* __restrict__ temperature,
-                                                                     const int* __restrict__ top_k, const float* __restrict__ top_p,
-                                                                     const float* __restrict__ min_p, const double* __restrict__ u, int shift,
-                                                                     int* __restrict__ index, float* __restrict__ prob) {
+__global__ void __launch_bounds__(SMW_THREADS, 1) sample_wide_kernel(const SmpArgs A) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int row = blockIdx.x;
-  SmpRow r;
-  r.x = logits + (size_t)row * ld; r.n = n; r.t = temperature[row]; r.shift = shift;
-  const int k = top_k[row];
-  r.greedy = r.t <= 0.f || k == 1;
-  unsigned long long best = 0ull;
-  for (int i = threadIdx.x; i < n; i += SMP_THREADS) { const float v = r.y(i); if (v == v) best = max(best, SmpRow::word(v, i)); }
-  best = smp_max(best);
-  if (best == 0ull || r.greedy) {
-    if (threadIdx.x == 0) { index[row] = best ? (int)(0xFFFFFFFFu - (unsigned)best) : -1; if (prob) prob[row] = best ? 1.f : 0.f; }
+  const int row = blockIdx.x, k = A.top_k[row];
+  SmwRow r;
+  r.x = A.logits + (size_t)row * A.ld; r.n = A.n; r.t = A.temperature[row];
+  const bool greedy = r.t <= 0.f || k == 1;
+  auto add = [](u64 a, u64 b) { return a + b; };
+  u64 best = 0ull, count = 0ull;
+  for (int i = threadIdx.x; i < A.n; i += SMW_THREADS) { const float v = smp_y(r.x[i], r.t, greedy); if (v == v) { best = max(best, smp_word(v, i)); count++; } }
+  best = smw_reduce(best, [](u64 a, u64 b) { return max(a, b); });
+  count = smw_reduce(count, add);
+  if (best == 0ull || greedy) {
+    if (threadIdx.x == 0) { A.index[row] = best ? smp_index(best) : -1; if (A.prob) A.prob[row] = best ? 1.f : 0.f; }
     return;
   }
-  r.top = r.y((int)(0xFFFFFFFFu - (unsigned)best));
-  unsigned long long cut = 0ull;
-  if (k > 0 && k < n) {
-    unsigned long long c = 0;
-    for (int i = threadIdx.x; i < n; i += SMP_THREADS) { const float v = r.y(i); c += v == v ? 1 : 0; }
-    c = smp_sum(c);
-    if (c > (unsigned long long)k) cut = smp_find<false>(r, 0ull, 0.f, (unsigned long long)k);
-  }
-  auto total = [&](unsigned long long from, float least) {
-    unsigned long long t = 0;
-    for (int i = threadIdx.x; i < n; i += SMP_THREADS) {
+  r.top = smp_value(best);
+  // weight of the words from `from` on that are at least `least`
+  auto total = [&](u64 from, float least) {
+    u64 t = 0;
+    for (int i = threadIdx.x; i < A.n; i += SMW_THREADS) {
       const float v = r.y(i);
-      if (v != v || SmpRow::word(v, i) < from) continue;
-      const float f = r.w(v);
-      if (f >= least) t += smp_fixed(f, shift);
+      if (v != v || smp_word(v, i) < from) continue;
+      const float f = smp_weight(v, r.top);
+      if (f >= least) t += smp_units(f);
     }
-    return smp_sum(t);
+    return smw_reduce(t, add);
   };
-  const unsigned long long all = total(cut, 0.f);
-  const double tp = (double)top_p[row];
-  if (!(tp >= 1.0)) cut = smp_find<true>(r, cut, 0.f, smp_target(tp, all));
-  const float least = min_p[row];
-  if (!(least <= 1.f)) cut = best;             // only the first one, whose weight is 1
-  const unsigned long long kept = total(cut, fminf(least, 1.f));
-  const unsigned long long pick = smp_find<true>(r, cut, fminf(least, 1.f), smp_target(u[row], kept));
+  const float least = A.min_p[row];
+  const double tp = (double)A.top_p[row];
+  u64 kept = total(k > 0 && (u64)k < count ? smw_find<false>(r, (u64)k) : 0ull, 0.f);
+  if (!(tp >= 1.0)) kept = total(smw_find<true>(r, smp_target(tp, kept)), 0.f);
+  kept = least <= 1.f ? min(kept, total(0ull, least)) : 1ull << 31;
+  const u64 word = least <= 1.f ? smw_find<true>(r, smp_target(A.u[row], kept)) : best;
   if (threadIdx.x == 0) {
-    const int i = (int)(0xFFFFFFFFu - (unsigned)pick);
-    index[row] = i;
-    if (prob) prob[row] = (float)((double)smp_fixed(r.w(r.y(i)), shift) / (double)kept);
+    A.index[row] = smp_index(word);
+    if (A.prob) A.prob[row] = (float)((double)smp_weight(smp_value(word), r.top) * 2147483648.0 / (double)kept);
   }
 }
 
 int wv_api_bind_device();
 extern "C" int wv_sample_rows_dev(const float* d_logits, int rows, int n, int64_t ld, const float* d_temperature, const int* d_top_k,
                                   const float* d_top_p, const float* d_min_p, const double* d_u, int* d_index, float* d_prob, void* stream) {
-  const int rc = wv_api_bind_device();
-  if (rc < 0) return rc;
+  const int dev = wv_api_bind_device();
+  if (dev < 0) return dev;
   if (!d_logits || !d_temperature || !d_top_k || !d_top_p || !d_min_p || !d_u || !d_index) { wv_set_error("wv_sample_rows_dev: null pointer"); return WV_EARG; }
   if (rows < 0 || n < 1) { wv_set_error("wv_sample_rows_dev: %d rows of %d logits", rows, n); return WV_ESHAPE; }
   if (ld == 0) ld = n;
   if (ld < n) { wv_set_error("wv_sample_rows_dev: the row stride %lld is less than %d", (long long)ld, n); return WV_ESHAPE; }
+  if (rows > INT_MAX / SMP_CLUSTER) { wv_set_error("wv_sample_rows_dev: %d rows are too many", rows); return WV_ESHAPE; }
   if (rows == 0) return WV_OK;
-  int bits = 0;
-  while (bits < 31 && (1ll << bits) < n) bits++;
+  const SmpArgs A = {d_logits, n, (long long)ld, d_temperature, d_top_k, d_top_p, d_min_p, d_u, d_index, d_prob};
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(rows); cfg.blockDim = dim3(SMP_THREADS); cfg.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
+  cfg.stream = static_cast<cudaStream_t>(stream);
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at; cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, sample_rows_kernel, d_logits, n, (long long)ld, d_temperature, d_top_k, d_top_p, d_min_p, d_u, 62 - bits, d_index, d_prob) != cudaSuccess) {
-    wv_set_error("wv_sample_rows_dev: launch: %s", cudaGetErrorString(cudaGetLastError())); return WV_ECUDA;
+  cudaError_t e;
+  if (n > SMP_CLUSTER * SMP_CACHE) {
+    cfg.gridDim = dim3(rows); cfg.blockDim = dim3(SMW_THREADS);
+    e = cudaLaunchKernelEx(&cfg, sample_wide_kernel, A);
+  } else {
+    const int ncta = n <= SMP_SMALL ? 1 : SMP_CLUSTER, per = (n - 1) / ncta + 1;
+    static unsigned long long attr_mask = 0;     // the attribute is set once per device
+    if (dev >= 64 || !(attr_mask & (1ull << dev))) {
+      if (cudaFuncSetAttribute(sample_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(SmpShared) + SMP_CACHE * 4)) != cudaSuccess) {
+        wv_set_error("wv_sample_rows_dev: %s", cudaGetErrorString(cudaGetLastError())); return WV_ECUDA;
+      }
+      if (dev < 64) attr_mask |= 1ull << dev;
+    }
+    cfg.gridDim = dim3((unsigned)(rows * ncta)); cfg.blockDim = dim3(SMP_THREADS); cfg.dynamicSmemBytes = sizeof(SmpShared) + (size_t)per * 4;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = (unsigned)ncta; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+    cfg.numAttrs = 2;
+    e = cudaLaunchKernelEx(&cfg, sample_rows_kernel, A, per);
   }
+  if (e != cudaSuccess) { wv_set_error("wv_sample_rows_dev: launch: %s", cudaGetErrorString(cudaGetLastError())); return WV_ECUDA; }
   return WV_OK;
 }
