@@ -583,7 +583,8 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
 #pragma unroll
                   for (int k = 0; k < 4; k++) { const unsigned b = q[k] ^ 0x80808080u; v[2 * k] = pa_bytes<0x4140>(b); v[2 * k + 1] = pa_bytes<0x4342>(b); }
                 } else {
-                  const unsigned q[2] = {w[u].x, w[u].y}, t2 = pa_pair(t[u], t[u]);
+                  const unsigned q[2] = {w[u].x, w[u].y};
+                  const PaSub t2 = pa_pair(t[u], t[u]);
 #pragma unroll
                   for (int k = 0; k < 8; k++) v[k] = pa_nibbles(q[k >> 2], k & 3, t2);
                 }
@@ -611,6 +612,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
 // The splits' results of a tile's rows joined: a warp per row.
 __global__ void __launch_bounds__(256) chunk_join_kernel(const __grid_constant__ PaCall c) {
   __shared__ int s_at[2];
+  __shared__ float s_w[8][16];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int kvh = blockIdx.x % c.g.kvh, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -626,7 +628,11 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const __grid_constant__
   for (int i = blockIdx.y * 8 + warp; i < 256; i += 8 * gridDim.y) {
     const int r = s_at[1] * 256 + i;
     if (r >= nrows) break;
-    for (int d = lane; d < c.g.hd; d += 32) pa_join(c, (size_t)blockIdx.x * 256 + i, sq.q0 + r / c.group, kvh * c.group + r % c.group, d);
+    const size_t rec = (size_t)blockIdx.x * 256 + i;
+    const float inv = pa_join_weights(c, rec, s_w[warp]);
+    __syncwarp();
+    pa_join_sums(c, rec, sq.q0 + r / c.group, kvh * c.group + r % c.group, s_w[warp], inv, lane, 32);
+    __syncwarp();
   }
 }
 
@@ -664,7 +670,7 @@ int wv_launch_attn_chunk(PaCall c, int bits, long long keys, bool alike, cudaStr
   // tiles and some four more of start and end.
   const long long tiles = (keys + PC_N - 1) / PC_N, sms = wv_sm_count();
   long long best = 1, cost = -1;
-  for (long long ns = 1; ns <= 16 && ns <= tiles; ns++) {
+  for (long long ns = 1; ns <= 16 && ns <= tiles; ns++) {      // 16: chunk_join_kernel's room for weights
     if (ns > 1 && blocks * 256 * ns * (c.g.hd + 2) * 4 > (256LL << 20)) break;
     const long long t = (tiles + ns - 1) / ns, w = (blocks * ns + sms - 1) / sms * (t + 4 + (ns > 1 ? 2 : 0));
     if (cost < 0 || w < cost) { cost = w; best = ns; }

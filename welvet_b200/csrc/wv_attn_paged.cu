@@ -17,21 +17,32 @@
 // another's keys. The keys of a sequence are split over blocks; the splits leave {M, divisor, sums} and a second kernel joins them
 // in order, so results do not depend on who ran first.
 #include "wv_attn_paged.cuh"
+#include "wv_tma_common.cuh"
 #include "wv_lease.h"
-#include <cuda_pipeline.h>
+#include <type_traits>
 
 int wv_sm_count();
 
 #define PR_WARPS 4
+// The running maximum is raised only when a logit is 2^7 above it (the sums, 64 registers a lane, are multiplied each time), so weights
+// reach 2^7 and carry 2^6 instead of 2^13: at most 2^14, and 2^-30 of that is still there.
+#define PR_LIFT 6.f
+#define PR_SLACK 7.f
+#define PR_FAR 10u            // value scales up to 2^10 apart keep 20 bits
 
 template <int BITS, int DP> struct PrShape {
   static constexpr int RB = DP * BITS / 8;                               // bytes of a row in the ring
   static constexpr int SUB = BITS == 4 ? DP : 0;                         // bytes of the sub-scales of 16 keys
   static constexpr int STAGE = 32 * RB + 128 + 2 * SUB;                  // K rows, V rows, 2 x 16 scales, sub-scales
-  static constexpr int FIT = 25 * 1024 / STAGE;
+  static constexpr int NCP = (RB + 31) / 32;                             // copies of 16 bytes that a lane makes for K's 16 rows (and for V's)
+};
+
+// Blocks an SM: three where the registers allow it (up to 8 rows of 128 values), and the stages of a warp's ring in what they leave.
+template <int BITS, int DP, bool R16> struct PrFit {
+  static constexpr int STAGE = PrShape<BITS, DP>::STAGE;
+  static constexpr int BLOCKS = DP == 256 && (BITS == 16 || R16) ? 1 : !R16 && (DP == 64 || (DP == 128 && BITS < 16)) ? 3 : 2;
+  static constexpr int FIT = (BLOCKS == 3 ? 35 * 512 : 25 * 1024) / STAGE;
   static constexpr int NST = FIT < 2 ? 2 : (FIT > 8 ? 8 : FIT);
-  static constexpr int CH = BITS == 4 ? 8 : 16;                          // bytes of a copy: 4-bit rows are multiples of 8
-  static constexpr int NCP = (16 * RB / CH + 31) / 32;                   // copies a lane makes for K (and for V)
 };
 
 // Where the 16-byte piece j of row r lies in a ring of rows of RB bytes.
@@ -45,9 +56,15 @@ template <int RB> __device__ __forceinline__ unsigned pr_at(int r, int j) {
     return (unsigned)(line * 128 + ((((r % PER) * (RB / 16) + j) ^ sw) & 7) * 16);
   }
 }
+__device__ __forceinline__ void pr_copy(unsigned dst, const void* src) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory"); }
+template <int N> __device__ __forceinline__ void pr_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void pr_mma(float (&d)[4], const uint4& a, unsigned b0, unsigned b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void pr_mma0(float (&d)[4], const uint4& a, unsigned b0, unsigned b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1), "f"(0.f));
 }
 // The value index within a row of element e (0..3: k = 2c, 2c+1, 2c+8, 2c+9 of the fragment) of QK step s in lane column c.
 template <int BITS, int DP> __device__ __forceinline__ int pr_kdim(int s, int c, int e) {
@@ -73,10 +90,11 @@ template <int BITS, int DP> __device__ __forceinline__ int pr_vdim(int t, int n)
   return n * (DP / 8) + t;
 }
 
-template <int BITS, int DP, bool R16>
-__global__ void __launch_bounds__(32 * PR_WARPS, (BITS == 16 && DP == 256) || (DP == 256 && R16) ? 1 : 2) attn_rows_kernel(const __grid_constant__ PaCall c) {
+// EXACT: head_dim is DP, known at compile time; otherwise it is smaller and what lies beyond it is zero.
+template <int BITS, int DP, bool R16, bool EXACT>
+__global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) attn_rows_kernel(const __grid_constant__ PaCall c) {
   using S = PrShape<BITS, DP>;
-  constexpr int RB = S::RB, KS = DP / 16, NT = DP / 8, NROW = R16 ? 16 : 8, NST = S::NST;
+  constexpr int RB = S::RB, KS = DP / 16, NT = DP / 8, NROW = R16 ? 16 : 8, NST = PrFit<BITS, DP, R16>::NST;
   constexpr bool QREG = KS * (R16 ? 8 : 4) <= 32;                        // q fragments in registers, or read from shared memory each time
   extern __shared__ __align__(128) unsigned char pr_smem[];
   __shared__ uint4 s_qf[(R16 ? 2 : 1) * KS * 32];
@@ -85,7 +103,8 @@ __global__ void __launch_bounds__(32 * PR_WARPS, (BITS == 16 && DP == 256) || (D
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gl = lane >> 2, cl = lane & 3;
   unsigned char* ring = pr_smem + warp * NST * S::STAGE;
   if (tid == 0) s_qmax = 0;
-  if (c.g.hd < DP) {                                                     // what lies beyond the head stays zero
+  const int hd = EXACT ? DP : c.g.hd, n16 = hd / 16, code = EXACT ? RB : c.g.code;
+  if (!EXACT) {                                                          // what lies beyond the head stays zero
     for (int i = tid * 16; i < PR_WARPS * NST * S::STAGE; i += 32 * PR_WARPS * 16) *reinterpret_cast<uint4*>(pr_smem + i) = make_uint4(0, 0, 0, 0);
     __syncthreads();
   }
@@ -104,81 +123,119 @@ __global__ void __launch_bounds__(32 * PR_WARPS, (BITS == 16 && DP == 256) || (D
   auto rec = [&](int r) { return (((size_t)seq * c.g.kvh + kvh) * (tiles * NROW) + r0 + r) * c.nsplit + sp; };      // a row's split result
   if (k0 >= k1) {
     if (c.nsplit > 1) { if (tid < rn) c.ml[rec(tid)] = make_float2(-INFINITY, 0.f); }
-    else for (int i = tid; i < rn * c.g.hd; i += 32 * PR_WARPS) {        // rows that see nothing
-      const int r = i / c.g.hd, t = sq.q0 + (r0 + r) / c.group, h = kvh * c.group + (r0 + r) % c.group;
-      c.out[(size_t)t * c.ldo + (size_t)h * c.g.hd + i % c.g.hd] = 0.f;
+    else for (int i = tid; i < rn * hd; i += 32 * PR_WARPS) {            // rows that see nothing
+      const int r = i / hd, t = sq.q0 + (r0 + r) / c.group, h = kvh * c.group + (r0 + r) % c.group;
+      c.out[(size_t)t * c.ldo + (size_t)h * hd + i % hd] = 0.f;
     }
     return;
   }
 
   // ---------------------------------------------------------------- the warp's groups of 16 keys: k0 / 16 + warp, + PR_WARPS, ...
   const int g0 = k0 / 16 + warp, ng = ((k1 + 15) / 16 - g0 + PR_WARPS - 1) / PR_WARPS;
-  const int code = c.g.code;
-  // a lane's copies of a group's K (or V) rows: the source is contiguous, the place in the ring the same in every stage
-  const int ncp = 16 * code / S::CH;
+  // A lane's copies of a group's K (or V) rows: the source is contiguous, the place in the ring the same in every stage.
   unsigned dst[S::NCP];
 #pragma unroll
-  for (int i = 0; i < S::NCP; i++) {
-    const int at = (lane + 32 * i) * S::CH, r = at / code, o = at - r * code;
-    dst[i] = lane + 32 * i < ncp ? pr_at<RB>(r, o / 16) + (o & 15) : 0u;
+  for (int i = 0; i < S::NCP; i++) { const int at = (lane + 32 * i) * 16; dst[i] = smem_u32(ring) + pr_at<RB>(at / RB, at % RB / 16); }
+  // Scales (lanes 0-3 of K, 4-7 of V) and sub-scales (the next n16 lanes of K, then of V): offset in the block, bytes a slot, place.
+  int xo = 0, xm = 4;
+  unsigned xd = 0xffffffffu;
+  if (lane < 8) { xo = (lane < 4 ? c.g.kscale : c.g.vscale) + 16 * (lane & 3); xd = smem_u32(ring) + 32 * RB + 16 * lane; }
+  else if (BITS == 4 && DP <= 128 && lane < 8 + 2 * n16) {
+    const int j = lane - 8, v = j >= n16;
+    xo = (v ? c.g.vsub : c.g.ksub) + 16 * (v ? j - n16 : j); xm = n16; xd = smem_u32(ring) + 32 * RB + 128 + (v ? S::SUB : 0) + 16 * (v ? j - n16 : j);
   }
-  int ids = 0;                                                           // page numbers of 32 of the warp's groups, a lane each
-  auto issue = [&](int it) {
-    if ((it & 31) == 0) {
-      const int gi = g0 + (it + lane) * PR_WARPS;
-      int id = it + lane < ng ? c.b.pages[(size_t)seq * c.b.table_stride + gi * 16 / c.g.page] : 0;
-      if (id < 0 || id >= c.g.num_pages) { wv_paged_report(c.err, WV_PAGED_PAGE); id = -1; }
-      ids = id;
-    }
-    const int id = __shfl_sync(0xffffffffu, ids, it & 31);
-    if (it < ng) {
-      unsigned char* st = ring + (it % NST) * S::STAGE;
-      const int key = (g0 + it * PR_WARPS) * 16, slot = key % c.g.page;
-      const int have = id < 0 ? 0 : min(16, k1 - key);                   // keys of the group that exist; the rest is zeros
-      const unsigned char* block = c.g.pool + ((size_t)max(id, 0) * c.g.kvh + kvh) * c.g.block;
-      const unsigned char* ks = block + (size_t)slot * code;
-      const unsigned char* vs = ks + (size_t)c.g.page * code;
-      const int bytes = have * code;
-#pragma unroll
-      for (int i = 0; i < S::NCP; i++) {
-        const int at = (lane + 32 * i) * S::CH;
-        if (at < 16 * code) {
-          const int z = at < bytes ? 0 : S::CH;
-          __pipeline_memcpy_async(st + dst[i], ks + (z ? 0 : at), S::CH, z);
-          __pipeline_memcpy_async(st + 16 * RB + dst[i], vs + (z ? 0 : at), S::CH, z);
-        }
-      }
-      // scales (64 bytes each) and sub-scales
-      unsigned char* sc = st + 32 * RB;
-      if (lane < 8) __pipeline_memcpy_async(sc + 16 * lane, block + (lane < 4 ? c.g.kscale : c.g.vscale) + 4 * slot + 16 * (lane & 3), 16, have ? 0 : 16);
-      if (BITS == 4) {
-        const int n16 = c.g.hd / 16;                                     // 16-byte pieces of the 16 keys' sub-scales
-        for (int i = lane; i < 2 * n16; i += 32) {
-          const bool v = i >= n16;
-          const int j = v ? i - n16 : i;
-          __pipeline_memcpy_async(sc + 128 + (v ? S::SUB : 0) + 16 * j, block + (v ? c.g.vsub : c.g.ksub) + slot * n16 + 16 * j, 16, have ? 0 : 16);
-        }
-      }
-    }
-    __pipeline_commit();
-    return id;
-  };
+  // 32 of the warp's groups at a time, a lane each: where the block is (-1: not in the pool), and the slot in it
+  long long blk = 0;
+  int slots = 0;
   unsigned bad = 0;                                                      // bit it & 31: the group's page is outside the pool
-  auto start = [&](int it) { const int id = issue(it); if (it < ng) bad = (bad & ~(1u << (it & 31))) | (unsigned)(id < 0) << (it & 31); };
+  int stage_in = 0;                                                      // of the next group to be copied
+  auto start = [&](int it) {
+    if ((it & 31) == 0) {
+      const int key = (g0 + (it + lane) * PR_WARPS) * 16, at = key / c.g.page;
+      int id = it + lane < ng ? c.b.pages[(size_t)seq * c.b.table_stride + at] : 0;
+      if (id < 0 || id >= c.g.num_pages) { wv_paged_report(c.err, WV_PAGED_PAGE); id = -1; }
+      blk = id < 0 ? -1LL : ((long long)id * c.g.kvh + kvh) * c.g.block;
+      slots = key - at * c.g.page;
+    }
+    const long long at = __shfl_sync(0xffffffffu, blk, it & 31);
+    const int slot = __shfl_sync(0xffffffffu, slots, it & 31);
+    if (it < ng) {
+      const unsigned so = (unsigned)(stage_in * S::STAGE);
+      const int have = at < 0 ? 0 : min(16, k1 - (g0 + it * PR_WARPS) * 16);      // keys of the group that exist; the rest is zeros
+      bad = (bad & ~(1u << (it & 31))) | (unsigned)(at < 0) << (it & 31);
+      const unsigned char* block = c.g.pool + (at < 0 ? 0 : at);
+      const unsigned char* ks = block + slot * code;
+      const unsigned char* vs = ks + (size_t)c.g.page * code;
+      if (EXACT && have == 16) {
+#pragma unroll
+        for (int i = 0; i < S::NCP; i++) {
+          if (16 * RB / 16 % 32 == 0 || lane + 32 * i < 16 * RB / 16) {
+            pr_copy(dst[i] + so, ks + 16 * lane + 512 * i);
+            pr_copy(dst[i] + so + 16 * RB, vs + 16 * lane + 512 * i);
+          }
+        }
+      } else {
+        constexpr int CH = BITS == 4 ? 8 : 16;                           // 4-bit rows are multiples of 8 bytes
+        for (int a = lane * CH; a < 16 * code; a += 32 * CH) {
+          const int r = a / code, o = a - r * code;
+          const unsigned d = smem_u32(ring) + so + pr_at<RB>(r, o / 16) + (o & 15);
+          const int n = r < have ? CH : 0;
+          if (CH == 16) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(ks + (n ? a : 0)), "r"(n) : "memory");
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d + 16 * RB), "l"(vs + (n ? a : 0)), "r"(n) : "memory");
+          } else {
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(d), "l"(ks + (n ? a : 0)), "r"(n) : "memory");
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(d + 16 * RB), "l"(vs + (n ? a : 0)), "r"(n) : "memory");
+          }
+        }
+      }
+      if (xd != 0xffffffffu) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(xd + so), "l"(block + xo + slot * xm), "r"(have ? 16 : 0) : "memory");
+      if (BITS == 4 && DP == 256)
+        for (int i = lane; i < 2 * n16; i += 32) {
+          const int v = i >= n16, j = v ? i - n16 : i;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(ring) + so + 32 * RB + 128 + (v ? S::SUB : 0) + 16 * j),
+                       "l"(block + (v ? c.g.vsub : c.g.ksub) + slot * n16 + 16 * j), "r"(have ? 16 : 0) : "memory");
+        }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    stage_in = stage_in + 1 == NST ? 0 : stage_in + 1;
+  };
 #pragma unroll
   for (int i = 0; i < NST - 1; i++) start(i);
 
   // ---------------------------------------------------------------- q: a common power of two, then two float16 pieces, as fragments
-  const int hd = c.g.hd;
+  constexpr int NR = R16 ? 2 : 1;
+  const float* qrow[NR];                                                 // of the lane's rows
+  int plast[NR], where[NR];                                              // the last position that they see; token and head as an offset in out
+#pragma unroll
+  for (int i = 0; i < NR; i++) {
+    const int r = r0 + min(gl + 8 * i, rn - 1), tok = r / c.group, h = kvh * c.group + r - tok * c.group;
+    qrow[i] = c.q + (size_t)(sq.q0 + tok) * c.ldq + (size_t)h * hd;
+    plast[i] = sq.kv - (sq.q1 - sq.q0) + tok;
+    where[i] = h * hd;
+  }
+  float qv[NR][KS / PR_WARPS][4];                                        // the lane's fragment values of steps warp, warp + 4, ...
   {
     unsigned m = 0;
-    for (int i = tid; i < rn * hd / 4; i += 32 * PR_WARPS) {
-      const int r = i * 4 / hd, d = i * 4 % hd, t = sq.q0 + (r0 + r) / c.group, h = kvh * c.group + (r0 + r) % c.group;
-      const float4 v = *reinterpret_cast<const float4*>(c.q + (size_t)t * c.ldq + (size_t)h * hd + d);
-      const float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int e = 0; e < 4; e++) { const unsigned u = __float_as_uint(x[e]) & 0x7fffffffu; if (u < 0x7f800000u) m = max(m, u); }
-    }
+    for (int k = 0; k < KS / PR_WARPS; k++)
+#pragma unroll
+      for (int i = 0; i < NR; i++) {
+        const bool on = gl + 8 * i < rn;
+        if constexpr (BITS == 4) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int d = pr_kdim<BITS, DP>(warp + PR_WARPS * k, cl, e);
+            qv[i][k][e] = on && d < hd ? qrow[i][d] : 0.f;
+          }
+        } else {
+          const int d = pr_kdim<BITS, DP>(warp + PR_WARPS * k, cl, 0);   // four neighbours
+          const float4 v = on && d < hd ? *reinterpret_cast<const float4*>(qrow[i] + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+          qv[i][k][0] = v.x; qv[i][k][1] = v.y; qv[i][k][2] = v.z; qv[i][k][3] = v.w;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) { const unsigned u = __float_as_uint(qv[i][k][e]) & 0x7fffffffu; if (u < 0x7f800000u) m = max(m, u); }
+      }
     m = __reduce_max_sync(0xffffffffu, m);
     __syncthreads();
     if (lane == 0) atomicMax(&s_qmax, m);
@@ -187,35 +244,26 @@ __global__ void __launch_bounds__(32 * PR_WARPS, (BITS == 16 && DP == 256) || (D
   const int qe = min(max((int)(s_qmax >> 23) - 127 - 13, -100), 114);    // max |q| 2^-qe in [2^13, 2^14)
   const float qinv = __uint_as_float((unsigned)(127 - qe) << 23);
   const float qf = c.scale * __uint_as_float((unsigned)(127 + qe) << 23);
-  for (int i = tid; i < KS * 32; i += 32 * PR_WARPS) {
-    const int s = i >> 5, g = (i & 31) >> 2, cc = i & 3;
-    unsigned h_[2][2], l_[2][2];                                         // [row g, row g + 8][k half]
 #pragma unroll
-    for (int rr = 0; rr < (R16 ? 2 : 1); rr++) {
-      const int r = g + 8 * rr;
-      float x[4];
+  for (int k = 0; k < KS / PR_WARPS; k++) {
+    unsigned h_[NR][2], l_[NR][2];                                       // [row g, row g + 8][k half]
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const int d = pr_kdim<BITS, DP>(s, cc, e);
-        x[e] = 0.f;
-        if (r < rn && d < hd) {
-          const int t = sq.q0 + (r0 + r) / c.group, h = kvh * c.group + (r0 + r) % c.group;
-          const float v = c.q[(size_t)t * c.ldq + (size_t)h * hd + d];
-          x[e] = v - v == 0.f ? v * qinv : NAN;                          // not finite: the row's sums are NaN
-        }
-      }
+    for (int i = 0; i < NR; i++)
 #pragma unroll
       for (int p = 0; p < 2; p++) {
-        h_[rr][p] = pa_pack(x[2 * p], x[2 * p + 1]);
-        const float2 b = pa_unpack(h_[rr][p]);
-        l_[rr][p] = pa_pack(x[2 * p] - b.x, x[2 * p + 1] - b.y);
+        float x = qv[i][k][2 * p], z = qv[i][k][2 * p + 1];
+        x = x - x == 0.f ? x * qinv : NAN;                               // not finite: the row's sums are NaN
+        z = z - z == 0.f ? z * qinv : NAN;
+        h_[i][p] = pa_pack(x, z);
+        const float2 b = pa_unpack(h_[i][p]);
+        l_[i][p] = pa_pack(x - b.x, z - b.y);
       }
-    }
-    if (R16) {
-      s_qf[i] = make_uint4(h_[0][0], h_[1][0], h_[0][1], h_[1][1]);
-      s_qf[KS * 32 + i] = make_uint4(l_[0][0], l_[1][0], l_[0][1], l_[1][1]);
+    const int at = (warp + PR_WARPS * k) * 32 + lane;
+    if constexpr (R16) {
+      s_qf[at] = make_uint4(h_[0][0], h_[1][0], h_[0][1], h_[1][1]);
+      s_qf[KS * 32 + at] = make_uint4(l_[0][0], l_[1][0], l_[0][1], l_[1][1]);
     } else {
-      s_qf[i] = make_uint4(h_[0][0], l_[0][0], h_[0][1], l_[0][1]);
+      s_qf[at] = make_uint4(h_[0][0], l_[0][0], h_[0][1], l_[0][1]);
     }
   }
   __syncthreads();
@@ -226,11 +274,6 @@ __global__ void __launch_bounds__(32 * PR_WARPS, (BITS == 16 && DP == 256) || (D
   }
   auto qfrag = [&](int i) -> uint4 { if constexpr (QREG) return qr[i]; else return s_qf[i * 32 + lane]; };
 
-  // the last position that a lane's rows see, and how far back
-  constexpr int NR = R16 ? 2 : 1;
-  int plast[NR];
-#pragma unroll
-  for (int i = 0; i < NR; i++) plast[i] = sq.kv - (sq.q1 - sq.q0) + (r0 + min(gl + 8 * i, rn - 1)) / c.group;
   const int pmin = sq.kv - (sq.q1 - sq.q0) + r0 / c.group, pmax = sq.kv - (sq.q1 - sq.q0) + (r0 + rn - 1) / c.group;
 
   float o[NT][4], m[NR], l[NR];
@@ -238,34 +281,41 @@ __global__ void __launch_bounds__(32 * PR_WARPS, (BITS == 16 && DP == 256) || (D
   for (int t = 0; t < NT; t++) o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.f;
 #pragma unroll
   for (int i = 0; i < NR; i++) { m[i] = -INFINITY; l[i] = 0.f; }
+  // where the lane reads K (row gl) and V (rows 2 cl, 2 cl + 1) in a stage; 8 rows further on lie 8 RB bytes further
+  constexpr int NKO = RB >= 64 ? RB / 64 : 1;
+  unsigned kofs[NKO], vofs[2];
+#pragma unroll
+  for (int i = 0; i < NKO; i++) kofs[i] = RB == 32 ? pr_at<RB>(gl, cl >> 1) + 8 * (cl & 1) : pr_at<RB>(gl, cl + 4 * i);
+#pragma unroll
+  for (int i = 0; i < 2; i++)
+    vofs[i] = 16 * RB + (RB >= 128 ? pr_at<RB>(2 * cl + i, gl) : RB == 64 ? pr_at<RB>(2 * cl + i, gl >> 1) + 8 * (gl & 1) : pr_at<RB>(2 * cl + i, gl >> 2) + 4 * (gl & 3));
+  unsigned erun = 37;                                                    // exponent field of the largest value scale so far, at least 2^-90's
+  int stage_out = 0;
 
-  for (int it = 0; it < ng; it++) {
-    __pipeline_wait_prior(NST - 2);
-    __syncwarp();                                                        // every lane has read the stage that is filled next
-    start(it + NST - 1);
-    const unsigned char* st = ring + (it % NST) * S::STAGE;
+  // One group of 16 keys out of a stage of the ring. PLAIN: every row sees all of them, and their value scales are near one another.
+  auto group = [&](auto plain, unsigned sa, const unsigned char* st, int key, const unsigned (&vv)[4], bool far, bool there) {
+    constexpr bool PLAIN = decltype(plain)::value;
     const unsigned char* sc = st + 32 * RB;
-    const int key = (g0 + it * PR_WARPS) * 16;
     // -------------------------------------------------------------- logits of two n-tiles of 8 keys, two chains of sums each
     float s[2][2][4];
 #pragma unroll
     for (int n = 0; n < 2; n++) {
-#pragma unroll
-      for (int ch = 0; ch < 2; ch++) s[n][ch][0] = s[n][ch][1] = s[n][ch][2] = s[n][ch][3] = 0.f;
       const int r = gl + 8 * n;
       auto step = [&](int k, unsigned b0, unsigned b1) {
-        if (R16) pr_mma(s[n][k & 1], qfrag(KS + k), b0, b1);             // the small pieces first
-        pr_mma(s[n][k & 1], qfrag(k), b0, b1);
+        if (k < 2) pr_mma0(s[n][k & 1], qfrag(R16 ? KS + k : k), b0, b1);
+        else pr_mma(s[n][k & 1], qfrag(R16 ? KS + k : k), b0, b1);
+        if (R16) pr_mma(s[n][k & 1], qfrag(k), b0, b1);                  // the small pieces first
       };
       if constexpr (BITS == 4 && DP == 64) {
-        const uint2 w = *reinterpret_cast<const uint2*>(st + pr_at<RB>(r, cl >> 1) + 8 * (cl & 1));
-        const unsigned t1 = sc[128 + r * (hd / 16) + min(cl, hd / 16 - 1)], t = pa_pair(t1, t1);
+        const uint2 w = lds64(sa + kofs[0] + n * 8 * RB);
+        const unsigned t1 = sc[128 + r * n16 + min(cl, n16 - 1)];
+        const PaSub t = pa_pair(t1, t1);
         step(0, pa_nibbles(w.x, 0, t), pa_nibbles(w.x, 1, t)); step(1, pa_nibbles(w.x, 2, t), pa_nibbles(w.x, 3, t));
         step(2, pa_nibbles(w.y, 0, t), pa_nibbles(w.y, 1, t)); step(3, pa_nibbles(w.y, 2, t), pa_nibbles(w.y, 3, t));
       } else {
 #pragma unroll
         for (int i = 0; i < RB / 64; i++) {
-          const uint4 v = *reinterpret_cast<const uint4*>(st + pr_at<RB>(r, cl + 4 * i));
+          const uint4 v = lds128(sa + kofs[i] + n * 8 * RB);
           const unsigned w[4] = {v.x, v.y, v.z, v.w};
           if constexpr (BITS == 16) { step(2 * i, w[0], w[1]); step(2 * i + 1, w[2], w[3]); }
           if constexpr (BITS == 8) {
@@ -273,9 +323,15 @@ __global__ void __launch_bounds__(32 * PR_WARPS, (BITS == 16 && DP == 256) || (D
             for (int j = 0; j < 4; j++) { const unsigned x = w[j] ^ 0x80808080u; step(4 * i + j, pa_bytes<0x4140>(x), pa_bytes<0x4342>(x)); }
           }
           if constexpr (BITS == 4) {
-            const int at = 2 * (cl + 4 * i), n16 = hd / 16;
-            const unsigned ta = at < n16 ? sc[128 + r * n16 + at] : 0u, tb = at + 1 < n16 ? sc[128 + r * n16 + at + 1] : 0u;
-            const unsigned t2[2] = {pa_pair(ta, ta), pa_pair(tb, tb)};
+            const int at = 2 * (cl + 4 * i);
+            unsigned ta, tb;
+            if constexpr (EXACT) {
+              const unsigned both = *reinterpret_cast<const unsigned short*>(sc + 128 + r * n16 + at);
+              ta = both & 255u; tb = both >> 8;
+            } else {
+              ta = at < n16 ? sc[128 + r * n16 + at] : 0u; tb = at + 1 < n16 ? sc[128 + r * n16 + at + 1] : 0u;
+            }
+            const PaSub t2[2] = {pa_pair(ta, ta), pa_pair(tb, tb)};
 #pragma unroll
             for (int j = 0; j < 4; j++) {
               step(8 * i + 2 * j, pa_nibbles(w[j], 0, t2[j >> 1]), pa_nibbles(w[j], 1, t2[j >> 1]));
@@ -286,70 +342,64 @@ __global__ void __launch_bounds__(32 * PR_WARPS, (BITS == 16 && DP == 256) || (D
       }
     }
     // -------------------------------------------------------------- weights of the lane's four keys 2c, 2c + 1, 2c + 8, 2c + 9
-    const bool whole = key >= lo && key + 15 <= pmin && (c.window == 0 || key > pmax - c.window) && !((bad >> (it & 31)) & 1u);
-    float y[NR][4], f[4], inv[4], emin = 1000.f, emax = -1000.f;
+    const float2 k0_ = *reinterpret_cast<const float2*>(sc + 8 * cl), k1_ = *reinterpret_cast<const float2*>(sc + 32 + 8 * cl);
+    const float kk[4] = {k0_.x * qf, k0_.y * qf, k1_.x * qf, k1_.y * qf};
+    const float inv = __uint_as_float((254u - erun) << 23);
+    float y[NR][4], f[4];
+    bool seen[NR][4];
 #pragma unroll
-    for (int n = 0; n < 2; n++) {
-      const float2 ks = *reinterpret_cast<const float2*>(sc + 4 * (8 * n + 2 * cl)), vs = *reinterpret_cast<const float2*>(sc + 64 + 4 * (8 * n + 2 * cl));
-      const float kk[2] = {ks.x * qf, ks.y * qf}, vv[2] = {vs.x, vs.y};
+    for (int j = 0; j < 4; j++) {
+      const int n = j >> 1, e = j & 1;
+      f[j] = __uint_as_float(vv[j]) * inv;
+      if (R16) {
+        y[0][j] = (s[n][0][e] + s[n][1][e]) * kk[j];
+        y[NR - 1][j] = (s[n][0][2 + e] + s[n][1][2 + e]) * kk[j];
+      } else {
+        y[0][j] = ((s[n][0][2 + e] + s[n][1][2 + e]) + (s[n][0][e] + s[n][1][e])) * kk[j];
+      }
+      if (!PLAIN) {
+        const int p = key + 8 * n + 2 * cl + e;
 #pragma unroll
-      for (int j = 0; j < 2; j++) {
-        const float e = pa_split_scale(vv[j], f[2 * n + j], inv[2 * n + j]);
-        if (e > -90.f && vv[j] == vv[j] && key + 8 * n + 2 * cl + j < k1) { emin = fminf(emin, e); emax = fmaxf(emax, e); }
-        if (R16) {
-          y[0][2 * n + j] = fmaf(s[n][0][j] + s[n][1][j], kk[j], e);
-          y[NR - 1][2 * n + j] = fmaf(s[n][0][2 + j] + s[n][1][2 + j], kk[j], e);
-        } else {
-          y[0][2 * n + j] = fmaf((s[n][0][2 + j] + s[n][1][2 + j]) + (s[n][0][j] + s[n][1][j]), kk[j], e);
+        for (int i = 0; i < NR; i++) {
+          seen[i][j] = there && p <= plast[i] && p < k1 && (c.window == 0 || p > plast[i] - c.window);
+          if (!seen[i][j]) y[i][j] = -INFINITY;
         }
       }
     }
-    bool seen[NR][4];
-    if (!whole) {
+    float mx[NR];
+    bool up = false;
 #pragma unroll
-      for (int i = 0; i < NR; i++)
+    for (int i = 0; i < NR; i++) {
+      mx[i] = fmaxf(fmaxf(y[i][0], y[i][1]), fmaxf(y[i][2], y[i][3]));
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+      up |= mx[i] > m[i] + PR_SLACK;
+    }
+    if (__any_sync(0xffffffffu, up)) {
+      float fac[NR];
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const int p = key + 8 * (j >> 1) + 2 * cl + (j & 1);
-          seen[i][j] = p <= plast[i] && p < k1 && (c.window == 0 || p > plast[i] - c.window) && !((bad >> (it & 31)) & 1u);
-          if (!seen[i][j]) y[i][j] = -INFINITY;
-        }
+      for (int i = 0; i < NR; i++) {
+        fac[i] = mx[i] > m[i] ? pa_ex2(m[i] - mx[i]) : 1.f;              // 0 while there was nothing
+        m[i] = fmaxf(m[i], mx[i]);
+        l[i] *= fac[i];
+      }
+#pragma unroll
+      for (int t = 0; t < NT; t++) { o[t][0] *= fac[0]; o[t][1] *= fac[0]; o[t][2] *= fac[NR - 1]; o[t][3] *= fac[NR - 1]; }
     }
     uint4 ph, pl;
     unsigned* hh = reinterpret_cast<unsigned*>(&ph);
     unsigned* ll = reinterpret_cast<unsigned*>(&pl);
-    // The 16 keys' value scales are all within 2^18 of one another, or (rows of zeros apart) the pieces' range may not hold them.
-    const bool far = __any_sync(0xffffffffu, __reduce_max_sync(0xffffffffu, (int)emax + 1000) + __reduce_max_sync(0xffffffffu, 1000 - (int)emin) > 2018);
     float pw[NR][4];
-    bool moved = false;
-    float fac[NR], ref[NR];
-#pragma unroll
-    for (int i = 0; i < NR; i++) {
-      float mx = fmaxf(fmaxf(y[i][0], y[i][1]), fmaxf(y[i][2], y[i][3]));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      mx = fmaxf(mx, m[i]);
-      ref[i] = mx == -INFINITY ? 0.f : mx;
-      fac[i] = pa_ex2(m[i] - ref[i]);
-      moved |= mx != m[i];
-      m[i] = mx;
-    }
-    if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-      for (int i = 0; i < NR; i++) l[i] *= fac[i];
-#pragma unroll
-      for (int t = 0; t < NT; t++) { o[t][0] *= fac[0]; o[t][1] *= fac[0]; o[t][2] *= fac[NR - 1]; o[t][3] *= fac[NR - 1]; }
-    }
 #pragma unroll
     for (int i = 0; i < NR; i++) {
       float (&p)[4] = pw[i];
+      const float off = !PLAIN && m[i] == -INFINITY ? 0.f : PR_LIFT - m[i];
 #pragma unroll
       for (int j = 0; j < 4; j++) {
-        const float e = pa_ex2(y[i][j] - (ref[i] - PA_LIFT));
+        float e = pa_ex2(y[i][j] + off);
         p[j] = e * f[j];
-        const float w = e * inv[j];
-        if (whole) l[i] += w;
-        else { l[i] += seen[i][j] ? w : 0.f; p[j] = seen[i][j] ? p[j] : 0.f; }
+        if (!PLAIN && !seen[i][j]) e = p[j] = 0.f;
+        l[i] += e;
       }
 #pragma unroll
       for (int n = 0; n < 2; n++) {                                      // keys' halves: fragment registers 0, 2 of row g and 1, 3 of row g + 8
@@ -367,7 +417,7 @@ __global__ void __launch_bounds__(32 * PR_WARPS, (BITS == 16 && DP == 256) || (D
       pr_mma(o[t], ph, b0, b1);
     };
     const int rows4[4] = {2 * cl, 2 * cl + 1, 2 * cl + 8, 2 * cl + 9};
-    if (far) {                                                           // value by value in float32
+    if (!PLAIN && far) {                                                 // value by value in float32
 #pragma unroll 1
       for (int j = 0; j < 16; j++) {
         const int mine = 2 * (j >> 3) + (j & 1), from = (lane & ~3) | ((j & 7) >> 1);
@@ -386,14 +436,14 @@ __global__ void __launch_bounds__(32 * PR_WARPS, (BITS == 16 && DP == 256) || (D
             if (R16) o[t][2 + n] += w[NR - 1] * x;
           }
       }
-      continue;
+      return;
     }
     if constexpr (BITS == 16) {
 #pragma unroll
       for (int i = 0; i < NT / 8; i++) {
         uint4 v[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = *reinterpret_cast<const uint4*>(vb + pr_at<RB>(rows4[j], gl + 8 * i));
+        for (int j = 0; j < 4; j++) v[j] = lds128(sa + vofs[j & 1] + (j >> 1) * 8 * RB + 128 * i);
 #pragma unroll
         for (int w = 0; w < 4; w++) {
           const unsigned a = (&v[0].x)[w], b = (&v[1].x)[w], d = (&v[2].x)[w], e = (&v[3].x)[w];
@@ -409,10 +459,10 @@ __global__ void __launch_bounds__(32 * PR_WARPS, (BITS == 16 && DP == 256) || (D
 #pragma unroll
         for (int j = 0; j < 4; j++) {
           if constexpr (NW == 4) {
-            const uint4 x = *reinterpret_cast<const uint4*>(vb + pr_at<RB>(rows4[j], gl + 8 * i));
+            const uint4 x = lds128(sa + vofs[j & 1] + (j >> 1) * 8 * RB + 128 * i);
             v[j][0] = x.x; v[j][1] = x.y; v[j][2] = x.z; v[j][3] = x.w;
           } else {
-            const uint2 x = *reinterpret_cast<const uint2*>(vb + pr_at<RB>(rows4[j], gl >> 1) + 8 * (gl & 1));
+            const uint2 x = lds64(sa + vofs[j & 1] + (j >> 1) * 8 * RB);
             v[j][0] = x.x; v[j][1] = x.y;
           }
         }
@@ -431,22 +481,25 @@ __global__ void __launch_bounds__(32 * PR_WARPS, (BITS == 16 && DP == 256) || (D
 #pragma unroll
       for (int j = 0; j < 4; j++) {
         if constexpr (NW == 4) {
-          const uint4 x = *reinterpret_cast<const uint4*>(vb + pr_at<RB>(rows4[j], gl));
+          const uint4 x = lds128(sa + vofs[j & 1] + (j >> 1) * 8 * RB);
           v[j][0] = x.x; v[j][1] = x.y; v[j][2] = x.z; v[j][3] = x.w;
         } else if constexpr (NW == 2) {
-          const uint2 x = *reinterpret_cast<const uint2*>(vb + pr_at<RB>(rows4[j], gl >> 1) + 8 * (gl & 1));
+          const uint2 x = lds64(sa + vofs[j & 1] + (j >> 1) * 8 * RB);
           v[j][0] = x.x; v[j][1] = x.y;
         } else {
-          v[j][0] = *reinterpret_cast<const unsigned*>(vb + pr_at<RB>(rows4[j], gl >> 2) + 4 * (gl & 3));
+          v[j][0] = lds32(sa + vofs[j & 1] + (j >> 1) * 8 * RB);
         }
       }
+      PaSub ta, tb;
 #pragma unroll
       for (int w = 0; w < NW; w++) {
-        const int n16 = hd / 16, at = min((gl * NW + w) >> 1, n16 - 1);  // beyond the head the codes' columns are dropped
-        unsigned t4[4];
+        if (w % 2 == 0) {                                                // a sub-scale serves two words
+          const int at = EXACT ? (gl * NW + w) >> 1 : min((gl * NW + w) >> 1, n16 - 1);      // beyond the head the codes' columns are dropped
+          unsigned t4[4];
 #pragma unroll
-        for (int j = 0; j < 4; j++) t4[j] = sc[128 + S::SUB + rows4[j] * n16 + at];
-        const unsigned ta = pa_pair(t4[0], t4[1]), tb = pa_pair(t4[2], t4[3]);
+          for (int j = 0; j < 4; j++) t4[j] = sc[128 + S::SUB + rows4[j] * n16 + at];
+          ta = pa_pair(t4[0], t4[1]); tb = pa_pair(t4[2], t4[3]);
+        }
 #pragma unroll
         for (int hf = 0; hf < 2; hf++) {
           const unsigned x = __byte_perm(v[0][w], v[1][w], hf ? 0x7632 : 0x5410), z = __byte_perm(v[2][w], v[3][w], hf ? 0x7632 : 0x5410);
@@ -455,71 +508,126 @@ __global__ void __launch_bounds__(32 * PR_WARPS, (BITS == 16 && DP == 256) || (D
         }
       }
     }
+  };
+  for (int it = 0; it < ng; it++) {
+    pr_wait<NST - 2>();
+    __syncwarp();                                                        // every lane has read the stage that is filled next
+    start(it + NST - 1);
+    const unsigned char* st = ring + stage_out * S::STAGE;
+    const unsigned sa = smem_u32(ring) + stage_out * S::STAGE;
+    stage_out = stage_out + 1 == NST ? 0 : stage_out + 1;
+    const int key = (g0 + it * PR_WARPS) * 16;
+    const bool there = !((bad >> (it & 31)) & 1u);
+    const bool whole = key >= lo && key + 15 <= pmin && key + 16 <= k1 && (c.window == 0 || key > pmax - c.window) && there;
+    const uint2 v0 = *reinterpret_cast<const uint2*>(st + 32 * RB + 64 + 8 * cl), v1 = *reinterpret_cast<const uint2*>(st + 32 * RB + 96 + 8 * cl);
+    unsigned vv[4] = {v0.x, v0.y, v1.x, v1.y};
+    // the largest and smallest exponent among the 16 value scales; a scale of NaN has none, one below 2^-90 is nothing
+    unsigned top = 0u, low = 255u << 23;
+#pragma unroll
+    for (int j = 0; j < 4; j++) {
+      if (!whole && key + 8 * (j >> 1) + 2 * cl + (j & 1) >= k1) vv[j] = 0u;
+      const unsigned u = vv[j] < 0x7f800000u ? vv[j] : 0u;
+      top = max(top, u);
+      low = min(low, u < (37u << 23) ? 255u << 23 : u);
+    }
+    top = __reduce_max_sync(0xffffffffu, top) >> 23;
+    low = __reduce_min_sync(0xffffffffu, low) >> 23;
+    if (top > erun) {
+      const float down = __uint_as_float((unsigned)max(127 - (int)(top - erun), 0) << 23);
+      erun = top;
+#pragma unroll
+      for (int t = 0; t < NT; t++) { o[t][0] *= down; o[t][1] *= down; o[t][2] *= down; o[t][3] *= down; }
+    }
+    const bool far = low + PR_FAR < erun;
+    if (whole && !far) group(std::true_type(), sa, st, key, vv, false, true);
+    else group(std::false_type(), sa, st, key, vv, far, there);
   }
 
   // ---------------------------------------------------------------- the warps' results joined, in the warps' order
-  __pipeline_wait_prior(0);
+  pr_wait<0>();
+  const float beta = __uint_as_float(erun << 23);
 #pragma unroll
   for (int i = 0; i < NR; i++) {
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
     if (cl == 0) s_ml[warp][gl + 8 * i] = make_float2(m[i], l[i]);
   }
-  __syncthreads();                                                       // the rings are free: sums [warp][row][value]
-  float* sums = reinterpret_cast<float*>(pr_smem);
+  __syncthreads();                                                       // the rings are free: sums [warp][row half][n-tile][lane], two values each
+  float2* sums = reinterpret_cast<float2*>(pr_smem);
 #pragma unroll
-  for (int t = 0; t < NT; t++)
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-      const int d = pr_vdim<BITS, DP>(t, 2 * cl + j);
-      if (R16) {
-        sums[(warp * NROW + gl) * DP + d] = o[t][j];
-        sums[(warp * NROW + gl + 8) * DP + d] = o[t][2 + j];
-      } else {
-        sums[(warp * NROW + gl) * DP + d] = o[t][j] + o[t][2 + j];
-      }
+  for (int t = 0; t < NT; t++) {
+    if (R16) {
+      sums[((warp * NR + 0) * NT + t) * 32 + lane] = make_float2(o[t][0] * beta, o[t][1] * beta);
+      sums[((warp * NR + NR - 1) * NT + t) * 32 + lane] = make_float2(o[t][2] * beta, o[t][3] * beta);
+    } else {
+      sums[(warp * NT + t) * 32 + lane] = make_float2((o[t][0] + o[t][2]) * beta, (o[t][1] + o[t][3]) * beta);
     }
+  }
   __syncthreads();
-  for (int i = tid; i < rn * hd; i += 32 * PR_WARPS) {
-    const int r = i / hd, d = i % hd;
-    float M = -INFINITY, L = 0.f, a = 0.f;
+#pragma unroll
+  for (int i = 0; i < NR; i++) {
+    const int r = gl + 8 * i;
+    if (r >= rn) break;
+    float M = -INFINITY, L = 0.f, fw[PR_WARPS];
 #pragma unroll
     for (int w = 0; w < PR_WARPS; w++) M = fmaxf(M, s_ml[w][r].x);
     const float ref = M == -INFINITY ? 0.f : M;
 #pragma unroll
     for (int w = 0; w < PR_WARPS; w++) {
       const float2 x = s_ml[w][r];
-      const float fw = pa_ex2(x.x - ref);
-      L += x.y * (x.x == -INFINITY ? (x.y == x.y ? 0.f : 1.f) : fw);     // a warp that saw nothing has a zero, or a NaN that counts
-      a += sums[(w * NROW + r) * DP + d] * (x.x == -INFINITY ? 1.f : fw);
+      fw[w] = x.x == -INFINITY ? (x.y == x.y ? 0.f : 1.f) : pa_ex2(x.x - ref);      // a warp that saw nothing has zeros, or NaN, which counts
+      L += x.y * fw[w];
     }
+    float* to;
+    float scale = 1.f;
     if (c.nsplit > 1) {
-      c.acc[rec(r) * hd + d] = a;
-      if (d == 0) c.ml[rec(r)] = make_float2(M, L);
+      to = c.acc + rec(r) * hd;
+      if (warp == 0 && cl == 0) c.ml[rec(r)] = make_float2(M, L);
     } else {
-      const int t = sq.q0 + (r0 + r) / c.group, h = kvh * c.group + (r0 + r) % c.group;
-      c.out[(size_t)t * c.ldo + (size_t)h * hd + d] = L == 0.f ? 0.f : a / L;
+      to = c.out + (size_t)(sq.q0 + plast[i] - (sq.kv - (sq.q1 - sq.q0))) * c.ldo + where[i];
+      scale = L == 0.f ? 0.f : 1.f / L;
+    }
+    for (int t4 = warp; t4 < NT / 4; t4 += PR_WARPS) {                   // four neighbouring values at a time, twice
+      float v[2][4];
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        float x = 0.f, z = 0.f;
+#pragma unroll
+        for (int w = 0; w < PR_WARPS; w++) {
+          const float2 s = sums[((w * NR + i) * NT + 4 * t4 + k) * 32 + lane];
+          x += s.x * fw[w]; z += s.y * fw[w];
+        }
+        v[0][k] = x * scale; v[1][k] = z * scale;
+      }
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        const int d = pr_vdim<BITS, DP>(4 * t4, 2 * cl + j);
+        if (d < hd) *reinterpret_cast<float4*>(to + d) = make_float4(v[j][0], v[j][1], v[j][2], v[j][3]);
+      }
     }
   }
 }
 
-// The splits' results joined in their order: a block per (sequence, kv head, row), a thread per value.
-__global__ void __launch_bounds__(256) rows_join_kernel(const __grid_constant__ PaCall c, int per_head) {
+// The splits' results joined in their order: a block per (sequence, kv head, row).
+__global__ void __launch_bounds__(128) rows_join_kernel(const __grid_constant__ PaCall c, int per_head) {
+  extern __shared__ float pr_w[];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int r = blockIdx.x % per_head, kvh = blockIdx.x / per_head % c.g.kvh, seq = blockIdx.x / per_head / c.g.kvh, d = threadIdx.x;
+  const int r = blockIdx.x % per_head, kvh = blockIdx.x / per_head % c.g.kvh, seq = blockIdx.x / per_head / c.g.kvh;
   const WvSeq sq = wv_seq(c.b, c.g.page, seq, nullptr);
   const int nrows = (sq.q1 - sq.q0) * c.group;
-  if (r >= nrows || nrows > c.rows_most || d >= c.g.hd) return;
-  pa_join(c, blockIdx.x, sq.q0 + r / c.group, kvh * c.group + r % c.group, d);
+  if (r >= nrows || nrows > c.rows_most) return;
+  const float inv = pa_join_weights(c, blockIdx.x, pr_w);
+  __syncthreads();
+  pa_join_sums(c, blockIdx.x, sq.q0 + r / c.group, kvh * c.group + r % c.group, pr_w, inv, threadIdx.x, 128);
 }
 
-template <int BITS, int DP, bool R16>
+template <int BITS, int DP, bool R16, bool EXACT>
 static cudaError_t rows_go(const PaCall& c, int tiles, cudaStream_t st) {
   using S = PrShape<BITS, DP>;
-  constexpr size_t sums = (size_t)PR_WARPS * (R16 ? 16 : 8) * DP * 4, ring = (size_t)PR_WARPS * S::NST * S::STAGE;
+  constexpr size_t sums = (size_t)PR_WARPS * (R16 ? 16 : 8) * DP * 4, ring = (size_t)PR_WARPS * PrFit<BITS, DP, R16>::NST * S::STAGE;
   constexpr size_t smem = sums > ring ? sums : ring;
-  auto kern = attn_rows_kernel<BITS, DP, R16>;
+  auto kern = attn_rows_kernel<BITS, DP, R16, EXACT>;
   static unsigned long long attr_mask = 0;
   int dev = 0;
   cudaGetDevice(&dev);
@@ -536,11 +644,13 @@ static cudaError_t rows_go(const PaCall& c, int tiles, cudaStream_t st) {
   cfg.attrs = at; cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kern, c);
 }
-template <int BITS>
-static cudaError_t rows_pick(const PaCall& c, bool r16, int tiles, cudaStream_t st) {
-  if (c.g.hd <= 64) return r16 ? rows_go<BITS, 64, true>(c, tiles, st) : rows_go<BITS, 64, false>(c, tiles, st);
-  if (c.g.hd <= 128) return r16 ? rows_go<BITS, 128, true>(c, tiles, st) : rows_go<BITS, 128, false>(c, tiles, st);
-  return r16 ? rows_go<BITS, 256, true>(c, tiles, st) : rows_go<BITS, 256, false>(c, tiles, st);
+template <int BITS, bool R16>
+static cudaError_t rows_pick(const PaCall& c, int tiles, cudaStream_t st) {
+  if (c.g.hd == 64) return rows_go<BITS, 64, R16, true>(c, tiles, st);
+  if (c.g.hd == 128) return rows_go<BITS, 128, R16, true>(c, tiles, st);
+  if (c.g.hd < 64) return rows_go<BITS, 64, R16, false>(c, tiles, st);
+  if (c.g.hd < 128) return rows_go<BITS, 128, R16, false>(c, tiles, st);
+  return rows_go<BITS, 256, R16, false>(c, tiles, st);
 }
 
 int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* dq, int ldq, float* dout, int ldo, int heads, float scale,
@@ -583,11 +693,13 @@ int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* d
       r.ml = reinterpret_cast<float2*>(lease.p);
       r.acc = lease.p + 2 * n;
     }
-    cudaError_t e = kv.bits == 16 ? rows_pick<16>(r, r16, (int)tiles, st) : kv.bits == 8 ? rows_pick<8>(r, r16, (int)tiles, st) : rows_pick<4>(r, r16, (int)tiles, st);
+    cudaError_t e = kv.bits == 16 ? (r16 ? rows_pick<16, true>(r, (int)tiles, st) : rows_pick<16, false>(r, (int)tiles, st))
+                  : kv.bits == 8 ? (r16 ? rows_pick<8, true>(r, (int)tiles, st) : rows_pick<8, false>(r, (int)tiles, st))
+                                 : (r16 ? rows_pick<4, true>(r, (int)tiles, st) : rows_pick<4, false>(r, (int)tiles, st));
     if (e == cudaSuccess && ns > 1) {
       cudaLaunchConfig_t cfg = {};
       cudaLaunchAttribute at[1];
-      cfg.gridDim = dim3((unsigned)(b.num_seqs * c.g.kvh * per_head)); cfg.blockDim = dim3((c.g.hd + 31) & ~31); cfg.stream = st;
+      cfg.gridDim = dim3((unsigned)(b.num_seqs * c.g.kvh * per_head)); cfg.blockDim = dim3(128); cfg.dynamicSmemBytes = (size_t)ns * 4; cfg.stream = st;
       at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
       at[0].val.programmaticStreamSerializationAllowed = 1;
       cfg.attrs = at; cfg.numAttrs = 1;

@@ -1,10 +1,8 @@
 // What the kernels of the paged attention share: the weights' units, the split results and their merge.
 //
-// A key's logit is x = scale log2(e) q.k, its weight 2^x, its value row v = f 2^e c with c the codes, f in [1, 2) and 2^e the rest of the
-// row's scale. What goes through the tensor cores is 2^(x + e - M) f in two float16 pieces (22 bits), M the running maximum of
-// x + e over the keys seen so far, so that the largest contribution keeps its bits whatever the scales are; the divisor is
-// sum 2^(x - M). e is held to [-90, 100], the rest of a scale beyond that stays in f, so that the divisor's terms stay in range.
-// Both sums carry a factor of 2^13 that uses the float16 range and cancels.
+// A key's logit is x = scale log2(e) q.k, its weight 2^x, its value row v = f 2^E c with c the codes and 2^E the largest value scale's power
+// of two among the keys at hand. What goes through the tensor cores is 2^(x - m) f in two float16 pieces (22 bits), m the running
+// maximum of x; the divisor is sum 2^(x - m) in float32. Both sums carry a factor of 2^13 that uses the float16 range and cancels.
 #pragma once
 #include "wv_paged.cuh"
 #include <math.h>
@@ -27,13 +25,6 @@ struct PaCall {
 };
 
 __device__ __forceinline__ float pa_ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
-// A value row's scale as 2^e f; returns e, sets f and 2^-e.
-__device__ __forceinline__ float pa_split_scale(float s, float& f, float& inv) {
-  const int e = min(max((int)((__float_as_uint(s) >> 23) & 255u) - 127, -90), 100);
-  inv = __uint_as_float((unsigned)(127 - e) << 23);
-  f = s * inv;
-  return (float)e;
-}
 __device__ __forceinline__ unsigned pa_pack(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const unsigned*>(&h);
@@ -51,12 +42,19 @@ __device__ __forceinline__ unsigned pa_mul2(unsigned v, unsigned m) {
 // Integer bytes or nibbles become float16 without a conversion: a byte in the mantissa of 1024, then 1024 + offset is subtracted.
 // The low two (SEL 0x4140) or high two (0x4342) bytes of w, biased by 128, as signed values.
 template <unsigned SEL> __device__ __forceinline__ unsigned pa_bytes(unsigned w) { return pa_sub2(__byte_perm(w, 0x64646464u, SEL), 0x64806480u); }
-// Nibbles j and j + 4 of w, biased by 8, times the sub-scale in both halves of t.
-__device__ __forceinline__ unsigned pa_nibbles(unsigned w, int j, unsigned t) {
-  return pa_mul2(pa_sub2(((w >> (4 * j)) & 0x000f000fu) | 0x64006400u, 0x64086408u), t);
+// Nibbles j and j + 4 of w, biased by 8, times the sub-scales t (a pair of float16): the nibble n in the upper mantissa of 1 is
+// 1 + n / 16, and (1 + n / 16) 16 t - 24 t = (n - 8) t is exact in one instruction.
+struct PaSub { unsigned a, b; };
+__device__ __forceinline__ unsigned pa_nibbles(unsigned w, int j, const PaSub& t) {
+  const unsigned s = j == 0 ? w << 6 : j == 1 ? w << 2 : j == 2 ? w >> 2 : w >> 6, x = (s & 0x03c003c0u) | 0x3c003c00u;
+  const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&t.a), *reinterpret_cast<const __half2*>(&t.b));
+  return *reinterpret_cast<const unsigned*>(&r);
 }
-// Two bytes as a pair of float16.
-__device__ __forceinline__ unsigned pa_pair(unsigned a, unsigned b) { return pa_sub2(0x64006400u | a | (b << 16), 0x64006400u); }
+// Two sub-scales (bytes) as the factors of pa_nibbles.
+__device__ __forceinline__ PaSub pa_pair(unsigned a, unsigned b) {
+  const unsigned t = pa_sub2(0x64006400u | a | (b << 16), 0x64006400u);
+  return PaSub{pa_mul2(t, 0x4c004c00u), pa_mul2(t, 0xce00ce00u)};        // 16 t and -24 t
+}
 
 
 // The positions that a block of consecutive rows of a sequence sees: [lo, hi), lo cut down to a multiple of 16.
@@ -66,22 +64,45 @@ __device__ __forceinline__ void pa_range(const WvSeq& s, int tok0, int tok1, int
   lo = window > 0 ? max(0, p0 - window + 1) & ~15 : 0;
 }
 
-// One value of a row out of its splits' results, in their order.
-__device__ __forceinline__ void pa_join(const PaCall& c, size_t rec, int token, int head, int d) {
+// A row out of its splits' results, in two steps. By a whole warp (each of a block's may do it): the splits' weights into w[nsplit];
+// returns the divisor's reciprocal. All maxima and divisors are loaded at once: one after the other they were a chain of
+// round trips to L2 (33 splits took 12 us).
+__device__ __forceinline__ float pa_join_weights(const PaCall& c, size_t rec, float* w) {
+  const int lane = threadIdx.x & 31;
   const float2* ml = c.ml + rec * c.nsplit;
-  const float* acc = c.acc + rec * c.nsplit * c.g.hd + d;
-  float M = -INFINITY, L = 0.f, a = 0.f;
-  for (int s = 0; s < c.nsplit; s++) M = fmaxf(M, ml[s].x);
-  const float ref = M == -INFINITY ? 0.f : M;
-#pragma unroll 4
-  for (int s = 0; s < c.nsplit; s++) {
-    const float2 x = ml[s];
-    if (x.y == 0.f) continue;
-    const float w = x.x == -INFINITY ? 1.f : pa_ex2(x.x - ref);          // -inf with a divisor: NaN, which counts
-    L += x.y * w;
-    a += acc[(size_t)s * c.g.hd] * w;
+  float M = -INFINITY, L = 0.f;
+  for (int s0 = 0; s0 < c.nsplit; s0 += 128) {
+#pragma unroll
+    for (int u = 0; u < 4; u++) { const int s = s0 + 32 * u + lane; if (s < c.nsplit) M = fmaxf(M, ml[s].x); }
   }
-  c.out[(size_t)token * c.ldo + (size_t)head * c.g.hd + d] = L == 0.f ? 0.f : a / L;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+  const float ref = M == -INFINITY ? 0.f : M;
+  for (int s = lane; s < c.nsplit; s += 32) {
+    const float2 x = ml[s];
+    const float f = x.y == 0.f ? 0.f : x.x == -INFINITY ? 1.f : pa_ex2(x.x - ref);      // -inf with a divisor: NaN, which counts
+    if (f != 0.f) L += x.y * f;
+    w[s] = f;
+  }
+#pragma unroll
+  for (int o = 16; o; o >>= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+  return L == 0.f ? 0.f : 1.f / L;
+}
+// Values first, first + step, ... of the row: the sums of the splits with weight, in their order, eight loads at a time.
+__device__ __forceinline__ void pa_join_sums(const PaCall& c, size_t rec, int token, int head, const float* w, float inv, int first, int step) {
+  const float* acc = c.acc + rec * c.nsplit * c.g.hd;
+  float* out = c.out + (size_t)token * c.ldo + (size_t)head * c.g.hd;
+  for (int d = first; d < c.g.hd; d += step) {
+    float a = 0.f;
+    for (int s0 = 0; s0 < c.nsplit; s0 += 8) {
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; u++) v[u] = s0 + u < c.nsplit && w[s0 + u] != 0.f ? acc[(size_t)(s0 + u) * c.g.hd + d] : 0.f;
+#pragma unroll
+      for (int u = 0; u < 8; u++) if (s0 + u < c.nsplit) a += v[u] * w[s0 + u];
+    }
+    out[d] = a * inv;
+  }
 }
 
 int wv_launch_attn_chunk(PaCall c, int bits, long long keys, bool alike, cudaStream_t st);      // wv_attn_chunk.cu
