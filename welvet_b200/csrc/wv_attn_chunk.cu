@@ -11,9 +11,13 @@
 // where 16-bit activations would take one, which is what bounds the kernel (the tensor pipe runs 4096 cycles for 256 x 128 x
 // head_dim 128, the weights take some 1300 a tile on the other pipes, and the two tiles take turns).
 //
-// Roles: two warpgroups own a tile each (a thread a row: maximum, weights, sums), one warp issues the MMAs, three fill the ring of
-// three stages, K and V tiles in turn, turning 8- and 4-bit codes into float16 on the way (16-bit ones are copied asynchronously).
-// Codes of 4 bits lie in the order in which they unpack two at a time (0 4 1 5 2 6 3 7); Q follows, and the outputs are put back.
+// Roles: two warpgroups own a tile each (a thread a row: maximum, weights, sums), one warp issues the MMAs, four fill the ring, K and V
+// tiles in turn. Rows of 16 bits are copied asynchronously into one of three stages; codes of 8 and 4 bits are copied as they are, two
+// tiles ahead and each thread for itself, and turned into float16 on the way from there to one of two stages. Codes of 4 bits lie in
+// the order in which they unpack two at a time (0 4 1 5 2 6 3 7); Q follows, and the outputs are put back.
+//
+// The running maximum is raised only where a logit may lie 2^7 above it, which a bound tells (the row's largest product times the
+// tile's largest scale), so that most tiles are read once.
 //
 // A key's scale multiplies its column of S; a value row's, relative to the largest of its tile, its weight, and the tile's own power
 // of two goes into the sum over tiles. Where the scales in a tile lie further apart than the pieces' range holds (2^16), the tile's
@@ -26,11 +30,12 @@
 #include "wv_lease.h"
 #include <type_traits>
 
-#define PC_THREADS 384
+#define PC_THREADS 512
 #define PC_M 128                    // rows of a tile
 #define PC_N 128                    // keys of a tile
-#define PC_STAGES 3
-#define PC_PRODUCERS 96
+#define PC_PRODUCERS 128
+#define PC_LIFT 6.f                 // weights carry 2^6 and are at most 2^14 (2^7 over the reference, scales below 2)
+#define PC_SLACK 7.f
 #define PC_SPIN (1u << 20)          // polls of a wait
 
 int wv_sm_count();
@@ -68,11 +73,13 @@ __device__ __forceinline__ void pc_ld32(unsigned taddr, unsigned (&r)[32]) {
       : PC_R8(r, 0), PC_R8(r, 8), PC_R8(r, 16), PC_R8(r, 24) : "r"(taddr) : "memory");
 }
 __device__ __forceinline__ void pc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void pc_st32(unsigned taddr, const unsigned (&r)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, "
-      "%21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
-      ::"r"(taddr), PC_W8(r, 0), PC_W8(r, 8), PC_W8(r, 16), PC_W8(r, 24) : "memory");
+__device__ __forceinline__ void pc_ld16(unsigned taddr, unsigned (&r)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+               : PC_R8(r, 0), PC_R8(r, 8) : "r"(taddr) : "memory");
+}
+__device__ __forceinline__ void pc_st16(unsigned taddr, const unsigned (&r)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+               ::"r"(taddr), PC_W8(r, 0), PC_W8(r, 8) : "memory");
 }
 __device__ __forceinline__ unsigned pc_ld1(unsigned taddr) {
   unsigned v;
@@ -83,17 +90,25 @@ __device__ __forceinline__ unsigned pc_ld1(unsigned taddr) {
 template <int N> __device__ __forceinline__ void pc_regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> __device__ __forceinline__ void pc_regs_down() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-// Shared memory: Q [tile][piece][head_dim / 64][128 rows][128 bytes], the ring of K and V tiles [head_dim / 64][128 keys][128 bytes],
-// then this.
+// Shared memory: Q [tile][piece][head_dim / 64][128 rows][128 bytes], the ring of K and V tiles [head_dim / 64][128 keys][128 bytes], the
+// codes on their way (8 and 4 bits), then this.
 struct PcMeta {
   float kk[2][PC_N], fv[2][PC_N];           // of a key tile (two of them in turn): the keys' scales times q's, the value rows' scales over 2^e
-  float beta[2];                            // 2^e
+  float beta[2], kmax[2];                   // 2^e, the largest kk
   unsigned flags[2];                        // 1: some key of the tile is not there, 2: value scales too far apart
   unsigned valid[2][4];                     // which keys are there
-  unsigned long long bar[2 * PC_STAGES + 11];
+  unsigned long long bar[17];
   unsigned tmem, qmax;
   int abort;
   int seq, tile;
+};
+template <int BITS, int DP> struct PcShape {
+  static constexpr int STAGES = BITS == 16 ? 3 : 2, STAGE = DP / 64 * PC_N * 128, QPIECE = DP / 64 * PC_M * 128;
+  static constexpr int PIECES = BITS == 16 ? DP / 8 : DP / 16;                    // of a row: 16 bytes, or 16 codes
+  static constexpr int PER = PIECES * PC_N / PC_PRODUCERS;                        // of a tile, a thread
+  static constexpr int RAW = BITS == 16 ? 0 : PC_PRODUCERS * PER * (BITS == 8 ? 16 : 12);    // 4 bits: codes, then a word that holds the sub-scale
+  static constexpr size_t SMEM = (size_t)4 * QPIECE + STAGES * STAGE + 2 * RAW + sizeof(PcMeta);
+  static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
 // The flat-th tile of 256 rows of the sequences that have more than rows_most rows, found by a whole warp: its sequence (-1: none)
@@ -129,22 +144,24 @@ template <int BITS> __device__ __forceinline__ int pc_dim(int p) {      // the v
 
 template <int BITS, int DP>
 __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_constant__ PaCall c) {
-  constexpr int HALVES = DP / 64, STAGE = HALVES * PC_N * 128, QPIECE = HALVES * PC_M * 128;
+  using S = PcShape<BITS, DP>;
+  constexpr int STAGES = S::STAGES, STAGE = S::STAGE, QPIECE = S::QPIECE;
   constexpr unsigned IDESC_S = (1u << 4) | (PC_N / 8 << 17) | (PC_M / 16 << 24);                   // f32 sums, f16 operands, both K-major
   constexpr unsigned IDESC_O = (1u << 4) | (1u << 16) | (DP / 8 << 17) | (PC_M / 16 << 24);        // B with its columns innermost
   extern __shared__ __align__(1024) unsigned char pc_smem[];
   unsigned char* s_q = pc_smem;
   unsigned char* s_kv = pc_smem + 4 * QPIECE;
-  PcMeta& M = *reinterpret_cast<PcMeta*>(s_kv + PC_STAGES * STAGE);
+  unsigned char* s_raw = s_kv + STAGES * STAGE;
+  PcMeta& M = *reinterpret_cast<PcMeta*>(s_raw + 2 * S::RAW);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   auto full = [&](int s) { return smem_u32(&M.bar[s]); };
-  auto empty = [&](int s) { return smem_u32(&M.bar[PC_STAGES + s]); };
-  auto s_full = [&](int t) { return smem_u32(&M.bar[2 * PC_STAGES + t]); };
-  auto p_full = [&](int t) { return smem_u32(&M.bar[2 * PC_STAGES + 2 + t]); };
-  auto o_full = [&](int t) { return smem_u32(&M.bar[2 * PC_STAGES + 4 + t]); };
-  auto m_full = [&](int s) { return smem_u32(&M.bar[2 * PC_STAGES + 6 + s]); };
-  auto m_empty = [&](int s) { return smem_u32(&M.bar[2 * PC_STAGES + 8 + s]); };
-  const unsigned done = smem_u32(&M.bar[2 * PC_STAGES + 10]);
+  auto empty = [&](int s) { return smem_u32(&M.bar[3 + s]); };
+  auto s_full = [&](int t) { return smem_u32(&M.bar[6 + t]); };
+  auto p_full = [&](int t) { return smem_u32(&M.bar[8 + t]); };
+  auto o_full = [&](int t) { return smem_u32(&M.bar[10 + t]); };
+  auto m_full = [&](int s) { return smem_u32(&M.bar[12 + s]); };
+  auto m_empty = [&](int s) { return smem_u32(&M.bar[14 + s]); };
+  const unsigned done = smem_u32(&M.bar[16]);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (smem_u32(pc_smem) & 1023u) { if (tid == 0) atomicCAS_system(c.err - 1, 0, 799); return; }    // the swizzle counts from 1024-byte boundaries
@@ -178,7 +195,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
   const bool two = rn > PC_M;
 
   if (tid == 0) {
-    for (int s = 0; s < PC_STAGES; s++) { mbar_init(full(s), PC_PRODUCERS / 32); mbar_init(empty(s), 1); }
+    for (int s = 0; s < STAGES; s++) { mbar_init(full(s), PC_PRODUCERS / 32); mbar_init(empty(s), 1); }
     for (int t = 0; t < 2; t++) {
       mbar_init(s_full(t), 1); mbar_init(p_full(t), 4); mbar_init(o_full(t), 1);
       mbar_init(m_full(t), 1); mbar_init(m_empty(t), two ? 8 : 4);
@@ -186,7 +203,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
     mbar_init(done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 11) {
+  if (warp == 12) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&M.tmem)), "n"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -211,8 +228,8 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
   pc_fence_after();
   const unsigned tmem = __shfl_sync(0xffffffffu, *(volatile unsigned*)&M.tmem, 0);
   const int qe = min(max((int)(M.qmax >> 23) - 127 - 13, -100), 114);
-  const float qinv = __uint_as_float((unsigned)(127 - qe) << 23);
-  const float qf = c.scale * __uint_as_float((unsigned)(127 + qe) << 23);
+  const float qinv = copysignf(__uint_as_float((unsigned)(127 - qe) << 23), c.scale);              // a negative scale turns q, so that kk is positive
+  const float qf = fabsf(c.scale) * __uint_as_float((unsigned)(127 + qe) << 23);
   for (int i = tid; i < 256 * (DP / 8); i += PC_THREADS) {               // 8 places of a row at a time
     const int r = i / (DP / 8), j = i % (DP / 8);
     if (r >= PC_M && !two) break;
@@ -261,9 +278,8 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
         if (!mbar_wait(m_full(ms), (j >> 1) & 1, PC_SPIN) || !mbar_wait(s_full(t), j & 1, PC_SPIN)) { if (!dead()) fail(700 + t); ok = false; }
         if (__any_sync(0xffffffffu, !ok)) { ok = false; break; }
         pc_fence_after();
-        const float* kk = M.kk[ms];
-        const float* fv = M.fv[ms];
-        float beta = M.beta[ms], alpha;
+        const unsigned kk = smem_u32(M.kk[ms]), fv = smem_u32(M.fv[ms]);
+        float beta = M.beta[ms], alpha = 1.f;
         const unsigned flags = M.flags[ms];
         const bool masked = (flags & 1u) || key0 + PC_N - 1 > pmin || key0 + PC_N > k1 || (c.window != 0 && key0 <= pmax - c.window);
         // bit k of `see`: the row sees key 32 q + k of the tile
@@ -277,52 +293,60 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
             see[q] = w & M.valid[ms][q];
           }
         }
-        // ---- the maximum over the tile
-        float mx = m;
+        // ---- the reference: may a logit lie too far above it?
+        bool raise = masked;
         if (!masked) {
+          float top = 0.f;
+          unsigned a[2][16];
+          pc_ld16(ts, a[0]);
 #pragma unroll
-          for (int q = 0; q < 4; q++) {
-            unsigned s[32];
-            pc_ld32(ts + 32 * q, s);
+          for (int q = 0; q < 8; q++) {
+            pc_wait_ld();
+            if (q < 7) pc_ld16(ts + 16 * (q + 1), a[(q + 1) & 1]);
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) top = fmaxf(top, fmaxf(__uint_as_float(a[q & 1][i]), __uint_as_float(a[q & 1][i + 1])));
+          }
+          raise = !(top * M.kmax[ms] <= m + PC_SLACK);
+        }
+        if (__any_sync(0xffffffffu, raise)) {
+          float mx = m;
+#pragma unroll
+          for (int q = 0; q < 8; q++) {
+            unsigned a[16];
+            pc_ld16(ts + 16 * q, a);
             pc_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-              const float4 k4 = *reinterpret_cast<const float4*>(kk + 32 * q + i);
-              const float2 a = __fmul2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(k4.x, k4.y));
-              const float2 b = __fmul2_rn(make_float2(__uint_as_float(s[i + 2]), __uint_as_float(s[i + 3])), make_float2(k4.z, k4.w));
-              mx = fmaxf(mx, fmaxf(fmaxf(a.x, a.y), fmaxf(b.x, b.y)));
+            for (int i = 0; i < 16; i += 4) {
+              const uint4 k4 = lds128(kk + 4 * (16 * q + i));
+              const float x[4] = {__uint_as_float(a[i]) * __uint_as_float(k4.x), __uint_as_float(a[i + 1]) * __uint_as_float(k4.y),
+                                  __uint_as_float(a[i + 2]) * __uint_as_float(k4.z), __uint_as_float(a[i + 3]) * __uint_as_float(k4.w)};
+              if (!masked) mx = fmaxf(mx, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+              else {
+#pragma unroll
+                for (int u = 0; u < 4; u++) if ((see[q >> 1] >> (16 * (q & 1) + i + u)) & 1u) mx = fmaxf(mx, x[u]);
+              }
             }
           }
-        } else {
-#pragma unroll
-          for (int q = 0; q < 4; q++) {
-            unsigned s[32];
-            pc_ld32(ts + 32 * q, s);
-            pc_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 32; i++) if ((see[q] >> i) & 1u) mx = fmaxf(mx, __uint_as_float(s[i]) * kk[32 * q + i]);
-          }
+          alpha = mx > m ? pa_ex2(m - mx) : 1.f;                         // 0 while there was nothing
+          m = mx;
+          l2 = __fmul2_rn(l2, make_float2(alpha, alpha));
         }
-        const float ref = mx == -INFINITY ? 0.f : mx;
-        alpha = pa_ex2(m - ref);                                         // 0 while there was nothing
-        m = mx;
-        l2 = __fmul2_rn(l2, make_float2(alpha, alpha));
-        const float2 off = make_float2(PA_LIFT - ref, PA_LIFT - ref);
+        const float2 off = m == -INFINITY ? make_float2(0.f, 0.f) : make_float2(PC_LIFT - m, PC_LIFT - m);
         if (flags & 2u) {
           // ---- value by value in float32; P is zero
           const int e = 2 * j + 1;
-          if (!mbar_wait(full(e % PC_STAGES), (e / PC_STAGES) & 1, PC_SPIN)) { if (!dead()) fail(702); ok = false; }
+          if (!mbar_wait(full(e % STAGES), (e / STAGES) & 1, PC_SPIN)) { if (!dead()) fail(702); ok = false; }
           if (__any_sync(0xffffffffu, !ok)) { ok = false; break; }
-          const unsigned char* v = s_kv + (e % PC_STAGES) * STAGE;
+          const unsigned char* v = s_kv + (e % STAGES) * STAGE;
 #pragma unroll
           for (int d = 0; d < DP; d++) o[d] *= alpha;
           alpha = 1.f;
 #pragma unroll 1
           for (int k = 0; k < PC_N; k++) {
-            const float x = __uint_as_float(pc_ld1(ts + k)) * kk[k];
+            const float x = fmaf(__uint_as_float(pc_ld1(ts + k)), M.kk[ms][k], off.x);
             const unsigned word = k < 32 ? see[0] : k < 64 ? see[1] : k < 96 ? see[2] : see[3];
             const bool on = !masked || ((word >> (k & 31)) & 1u);
-            const float p = on ? pa_ex2(x + off.x) : 0.f, w = on ? p * fv[k] * beta : 0.f;
+            const float p = on ? pa_ex2(x) : 0.f, w = on ? p * M.fv[ms][k] * beta : 0.f;
             l2.x += p;
 #pragma unroll
             for (int g = 0; g < DP / 8; g++) {
@@ -333,40 +357,44 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
             }
           }
           beta = 0.f;
-          unsigned z[32];
+          unsigned z[16];
 #pragma unroll
-          for (int i = 0; i < 32; i++) z[i] = 0u;
+          for (int i = 0; i < 16; i++) z[i] = 0u;
 #pragma unroll
-          for (int q = 0; q < 4; q++) pc_st32(ts + 32 * q, z);
+          for (int q = 0; q < 8; q++) pc_st16(ts + 16 * q, z);
         } else {
-          // ---- weights: 32 keys of S become 16 columns of their hi pieces and 16 of their lo pieces
+          // ---- weights: 16 keys of S become 8 columns of their hi pieces and 8 of their lo pieces
           auto weights = [&](auto some) {
+            unsigned a[2][16];
+            pc_ld16(ts, a[0]);
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-              unsigned s[32], w[32];
-              pc_ld32(ts + 32 * q, s);
+            for (int q = 0; q < 8; q++) {
+              unsigned w[16];
               pc_wait_ld();
+              if (q < 7) pc_ld16(ts + 16 * (q + 1), a[(q + 1) & 1]);
+              const unsigned (&s)[16] = a[q & 1];
 #pragma unroll
-              for (int i = 0; i < 32; i += 4) {
-                const float4 k4 = *reinterpret_cast<const float4*>(kk + 32 * q + i), f4 = *reinterpret_cast<const float4*>(fv + 32 * q + i);
+              for (int i = 0; i < 16; i += 4) {
+                const uint4 k4 = lds128(kk + 4 * (16 * q + i)), f4 = lds128(fv + 4 * (16 * q + i));
 #pragma unroll
                 for (int u = 0; u < 4; u += 2) {
-                  const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[i + u]), __uint_as_float(s[i + u + 1])), u ? make_float2(k4.z, k4.w) : make_float2(k4.x, k4.y), off);
+                  const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[i + u]), __uint_as_float(s[i + u + 1])),
+                                              u ? make_float2(__uint_as_float(k4.z), __uint_as_float(k4.w)) : make_float2(__uint_as_float(k4.x), __uint_as_float(k4.y)), off);
                   float2 p = make_float2(pa_ex2(x.x), pa_ex2(x.y));
-                  float2 pf = __fmul2_rn(p, u ? make_float2(f4.z, f4.w) : make_float2(f4.x, f4.y));
+                  float2 pf = __fmul2_rn(p, u ? make_float2(__uint_as_float(f4.z), __uint_as_float(f4.w)) : make_float2(__uint_as_float(f4.x), __uint_as_float(f4.y)));
                   if constexpr (decltype(some)::value) {
-                    const bool a = (see[q] >> (i + u)) & 1u, b = (see[q] >> (i + u + 1)) & 1u;
-                    p = make_float2(a ? p.x : 0.f, b ? p.y : 0.f);
-                    pf = make_float2(a ? pf.x : 0.f, b ? pf.y : 0.f);
+                    const unsigned bits = see[q >> 1] >> (16 * (q & 1) + i + u);
+                    p = make_float2(bits & 1u ? p.x : 0.f, bits & 2u ? p.y : 0.f);
+                    pf = make_float2(bits & 1u ? pf.x : 0.f, bits & 2u ? pf.y : 0.f);
                   }
                   l2 = __fadd2_rn(l2, p);
                   const unsigned h = pa_pack(pf.x, pf.y);
-                  const float2 back = pa_unpack(h);
+                  const float2 lo_ = __ffma2_rn(pa_unpack(h), make_float2(-1.f, -1.f), pf);
                   w[(i + u) / 2] = h;
-                  w[16 + (i + u) / 2] = pa_pack(pf.x - back.x, pf.y - back.y);
+                  w[8 + (i + u) / 2] = pa_pack(lo_.x, lo_.y);
                 }
               }
-              pc_st32(ts + 32 * q, w);
+              pc_st16(ts + 16 * q, w);
             }
           };
           if (masked) weights(std::true_type()); else weights(std::false_type());
@@ -376,19 +404,26 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
         __syncwarp();
         if (lane == 0) { mbar_arrive(p_full(t)); mbar_arrive(m_empty(ms)); }
         // ---- this tile's part of the sum
+        const bool same = !__any_sync(0xffffffffu, alpha != 1.f);
         if (!mbar_wait(o_full(t), j & 1, PC_SPIN)) { if (!dead()) fail(704 + t); ok = false; }
         if (__any_sync(0xffffffffu, !ok)) { ok = false; break; }
         pc_fence_after();
+        if (!same) {
 #pragma unroll
-        for (int q = 0; q < DP / 32; q++) {
-          unsigned s[32];
-          pc_ld32(to + 32 * q, s);
-          pc_wait_ld();
+          for (int d = 0; d < DP; d += 2) { const float2 v = __fmul2_rn(make_float2(o[d], o[d + 1]), make_float2(alpha, alpha)); o[d] = v.x; o[d + 1] = v.y; }
+        }
+        {
+          unsigned a[2][16];
+          pc_ld16(to, a[0]);
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
-            const float2 a = __fmul2_rn(make_float2(o[32 * q + i], o[32 * q + i + 1]), make_float2(alpha, alpha));
-            const float2 v = __ffma2_rn(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(beta, beta), a);
-            o[32 * q + i] = v.x; o[32 * q + i + 1] = v.y;
+          for (int q = 0; q < DP / 16; q++) {
+            pc_wait_ld();
+            if (q < DP / 16 - 1) pc_ld16(to + 16 * (q + 1), a[(q + 1) & 1]);
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              const float2 v = __ffma2_rn(make_float2(__uint_as_float(a[q & 1][i]), __uint_as_float(a[q & 1][i + 1])), make_float2(beta, beta), make_float2(o[16 * q + i], o[16 * q + i + 1]));
+              o[16 * q + i] = v.x; o[16 * q + i + 1] = v.y;
+            }
           }
         }
       }
@@ -415,9 +450,9 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
         }
       }
     }
-  } else {
-    pc_regs_down<72>();
-    if (warp == 11) {
+  } else if (warp >= 12) {
+    pc_regs_down<32>();
+    if (warp == 12) {
       // ============================================================ MMAs
       const bool leader = pc_elect();
       const unsigned qa = smem_u32(s_q), kv = smem_u32(s_kv);
@@ -430,7 +465,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
       };
       auto scores = [&](int t, int e) {                                  // S of tile t with the K tile that is element e of the ring
         if (leader) {
-          const unsigned kb = kv + (e % PC_STAGES) * STAGE;
+          const unsigned kb = kv + (e % STAGES) * STAGE;
 #pragma unroll
           for (int p = 1; p >= 0; p--) {                                 // the small pieces first
             const unsigned qb = qa + (2 * t + p) * QPIECE;
@@ -444,17 +479,17 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
       };
       auto values = [&](int t, int e) {
         if (leader) {
-          const unsigned vb = kv + (e % PC_STAGES) * STAGE;
+          const unsigned vb = kv + (e % STAGES) * STAGE;
 #pragma unroll
           for (int p = 1; p >= 0; p--)
 #pragma unroll
             for (int k = 0; k < PC_N / 16; k++)
-              pc_mma_ts(tmem + 256 + t * 128, tmem + t * PC_N + (k >> 1) * 32 + p * 16 + (k & 1) * 8, pc_desc(vb + k * 2048, PC_N * 128), IDESC_O, !(p == 1 && k == 0));
+              pc_mma_ts(tmem + 256 + t * 128, tmem + t * PC_N + 16 * k + 8 * p, pc_desc(vb + k * 2048, PC_N * 128), IDESC_O, !(p == 1 && k == 0));
           pc_commit(o_full(t));
         }
         __syncwarp();
       };
-      auto release = [&](int e) { if (leader) pc_commit(empty(e % PC_STAGES)); __syncwarp(); };
+      auto release = [&](int e) { if (leader) pc_commit(empty(e % STAGES)); __syncwarp(); };
       if (wait(full(0), 0, 710)) {
         pc_fence_after();
         for (int t = 0; t < nt; t++) scores(t, 0);
@@ -462,14 +497,14 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
       }
       for (int j = 0; j < n && ok; j++) {
         const int ev = 2 * j + 1, ek = 2 * j + 2;
-        if (!wait(full(ev % PC_STAGES), ev / PC_STAGES, 711)) break;
+        if (!wait(full(ev % STAGES), ev / STAGES, 711)) break;
         for (int t = 0; t < nt && ok; t++) {
           if (!wait(p_full(t), j, 712 + t)) break;
           pc_fence_after();
           values(t, ev);
           if (t == nt - 1) release(ev);
           if (j + 1 < n) {
-            if (t == 0 && !wait(full(ek % PC_STAGES), ek / PC_STAGES, 714)) break;
+            if (t == 0 && !wait(full(ek % STAGES), ek / STAGES, 714)) break;
             pc_fence_after();
             scores(t, ek);
             if (t == nt - 1) release(ek);
@@ -481,129 +516,178 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
         __syncwarp();
         mbar_wait(done, 0, PC_SPIN);
       }
-    } else {
-      // ============================================================ K and V tiles
-      const int pw = warp - 8, pt = tid - 256;                           // 0 .. 2, 0 .. 95
-      const int code = c.g.code, page = c.g.page;
-      constexpr int PER = BITS == 16 ? DP / 8 : DP / 16;                 // pieces of a row: 16 bytes of codes (8 in 4 bits)
-      const int pieces = BITS == 16 ? hd / 8 : hd / 16;
-      bool ok = true;
-      for (int e = 0; e < 2 * n && ok; e++) {
-        const int j = e >> 1, key0 = k0 + j * PC_N, s = e % PC_STAGES;
-        const bool is_v = e & 1;
-        // page numbers of the tile's 8 groups of 16 keys, a lane each
-        int id = -1;
-        if (lane < 8 && key0 + 16 * lane < k1) {
-          id = c.b.pages[(size_t)seq * c.b.table_stride + (key0 + 16 * lane) / page];
-          if (id < 0 || id >= c.g.num_pages) { if (pw == 0) wv_paged_report(c.err, WV_PAGED_PAGE); id = -1; }
-        }
-        const int slot = (key0 + 16 * min(lane, 7)) % page;
-        if (e >= PC_STAGES && !mbar_wait(empty(s), (e / PC_STAGES - 1) & 1, PC_SPIN)) { if (!dead()) fail(720); ok = false; }
-        if (!is_v && pw == 0 && j >= 2 && ok && !mbar_wait(m_empty(j & 1), ((j >> 1) - 1) & 1, PC_SPIN)) { if (!dead()) fail(721); ok = false; }
-        if (__any_sync(0xffffffffu, !ok || dead())) { ok = false; break; }
-        if (!is_v && pw == 0) {
-          // what the weights need: four keys a lane
-          const int ms = j & 1, gi = lane >> 2, gid = __shfl_sync(0xffffffffu, id, gi), gs = __shfl_sync(0xffffffffu, slot, gi) + 4 * (lane & 3);
-          float4 ks = make_float4(0.f, 0.f, 0.f, 0.f), vs = ks;
-          if (gid >= 0) {
-            const unsigned char* block = c.g.pool + ((size_t)gid * c.g.kvh + kvh) * c.g.block;
-            ks = *reinterpret_cast<const float4*>(block + c.g.kscale + 4 * gs);
-            vs = *reinterpret_cast<const float4*>(block + c.g.vscale + 4 * gs);
-          }
-          const float kx[4] = {ks.x, ks.y, ks.z, ks.w}, vx[4] = {vs.x, vs.y, vs.z, vs.w};
-          int emax = -90, emin = 1000;
-          bool there = gid >= 0;
-#pragma unroll
-          for (int i = 0; i < 4; i++) {
-            const int ex = min((int)((__float_as_uint(vx[i]) >> 23) & 255u) - 127, 100);
-            if (there && key0 + 4 * lane + i < k1 && vx[i] == vx[i] && ex > -90) { emax = max(emax, ex); emin = min(emin, ex); }
-          }
-          emax = __reduce_max_sync(0xffffffffu, emax);
-          emin = __reduce_min_sync(0xffffffffu, emin);
-          const float down = __uint_as_float((unsigned)(127 - emax) << 23);
-          *reinterpret_cast<float4*>(&M.kk[ms][4 * lane]) = make_float4(kx[0] * qf, kx[1] * qf, kx[2] * qf, kx[3] * qf);
-          *reinterpret_cast<float4*>(&M.fv[ms][4 * lane]) = make_float4(vx[0] * down, vx[1] * down, vx[2] * down, vx[3] * down);
-          const unsigned have = __ballot_sync(0xffffffffu, there);       // a bit for 4 keys; 4 lanes of a group alike
-          if (lane < 4) {
-            unsigned w = 0;
-#pragma unroll
-            for (int i = 0; i < 8; i++) if ((have >> (8 * lane + i)) & 1u) w |= 15u << (4 * i);
-            M.valid[ms][lane] = w;
-          }
-          if (lane == 0) {
-            M.beta[ms] = __uint_as_float((unsigned)(127 + emax) << 23);
-            M.flags[ms] = (have != ~0u ? 1u : 0u) | (emin < emax - 16 ? 2u : 0u);
-          }
-          __syncwarp();
-          if (lane == 0) mbar_arrive(m_full(ms));
-        }
-        unsigned char* dst = s_kv + s * STAGE;
-        const int part = is_v ? page * code : 0;
+    }
+  } else {
+    // ============================================================== K and V tiles
+    pc_regs_down<48>();
+    const int pt = tid - 256, code = c.g.code, page = c.g.page;
+    // A thread's piece of each run of rows is the same one: 16 bytes (16 bits) or 16 codes of row r0_ + RUN k, k = 0 ..
+    constexpr int RUN = PC_PRODUCERS / S::PIECES;
+    const int x = pt % S::PIECES, r0_ = pt / S::PIECES;
+    const bool mine = BITS == 16 ? 8 * x < hd : 16 * x < hd;
+    const unsigned raw = smem_u32(s_raw) + 16 * pt;
+    // page numbers of 32 groups of 16 keys (four tiles) at a time, a lane each, as offsets in the pool (-1: not there)
+    long long blk = 0;
+    int slots = 0;
+    auto places = [&](int j) {
+      if ((j & 3) == 0) {
+        const int key = k0 + j * PC_N + 16 * lane, at = key / page;
+        int id = key < k1 ? c.b.pages[(size_t)seq * c.b.table_stride + at] : 0;
+        if (id < 0 || id >= c.g.num_pages) { if (warp == 8) wv_paged_report(c.err, WV_PAGED_PAGE); id = -1; }
+        blk = id < 0 || key >= k1 ? -1LL : ((long long)id * c.g.kvh + kvh) * c.g.block;
+        slots = key - at * page;
+      }
+    };
+    float4 ks = make_float4(0.f, 0.f, 0.f, 0.f), vs = ks;                // warp 8: four keys a lane of the next tile
+    bool there = true;
+    auto scales = [&](int j) {
+      const int g = 8 * (j & 3) + (lane >> 2);
+      const long long at = __shfl_sync(0xffffffffu, blk, g);
+      const int slot = __shfl_sync(0xffffffffu, slots, g) + 4 * (lane & 3);
+      there = at >= 0 || k0 + j * PC_N + 16 * (lane >> 2) >= k1;         // what lies beyond the keys is not missing
+      ks = vs = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (at >= 0) {
+        ks = *reinterpret_cast<const float4*>(c.g.pool + at + c.g.kscale + 4 * slot);
+        vs = *reinterpret_cast<const float4*>(c.g.pool + at + c.g.vscale + 4 * slot);
+      }
+    };
+    // the copies of element e: into its stage (16 bits), or as they are
+    auto copy = [&](int e) {
+      const int j = e >> 1, key0 = k0 + j * PC_N;
+      const bool is_v = e & 1;
+      const int part = is_v ? page * code : 0;
+      const unsigned stage = smem_u32(s_kv) + (e % STAGES) * STAGE, slot_raw = raw + (e & 1) * S::RAW;
+#pragma unroll 4
+      for (int k = 0; k < S::PER; k++) {
+        const int r = r0_ + RUN * k, g = 8 * (j & 3) + (r >> 4);
+        const long long at = __shfl_sync(0xffffffffu, blk, g);
+        const int slot = __shfl_sync(0xffffffffu, slots, g) + (r & 15);
+        const bool on = mine && at >= 0 && key0 + r < k1;
+        const unsigned char* block = c.g.pool + (at < 0 ? 0 : at);
         if constexpr (BITS == 16) {
-          for (int i = pt; i < PC_N * PER; i += PC_PRODUCERS) {
-            const int r = i / PER, x = i % PER;
-            const int gid = __shfl_sync(0xffffffffu, id, r >> 4), gs = __shfl_sync(0xffffffffu, slot, r >> 4);
-            const bool on = gid >= 0 && key0 + r < k1 && x < pieces;
-            const unsigned char* src = c.g.pool + ((size_t)max(gid, 0) * c.g.kvh + kvh) * c.g.block + part + (on ? (gs + (r & 15)) * code + 16 * x : 0);
-            const unsigned to = smem_u32(dst) + (x >> 3) * PC_N * 128 + r * 128 + (((x & 7) ^ (r & 7)) << 4);
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(src), "r"(on ? 16 : 0) : "memory");
-          }
-          asm volatile("cp.async.wait_all;" ::: "memory");
+          const unsigned to = stage + (x >> 3) * PC_N * 128 + r * 128 + (((x & 7) ^ (r & 7)) << 4);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(block + part + (on ? slot * code + 16 * x : 0)), "r"(on ? 16 : 0) : "memory");
+        } else if constexpr (BITS == 8) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot_raw + 16 * PC_PRODUCERS * k), "l"(block + part + (on ? slot * code + 16 * x : 0)), "r"(on ? 16 : 0) : "memory");
         } else {
-          constexpr int B = 4;                                           // pieces in flight a thread
-          const int sub = is_v ? c.g.vsub : c.g.ksub, n16 = hd / 16;
-          for (int i0 = pt; i0 < PC_N * PER; i0 += B * PC_PRODUCERS) {
-            uint4 w[B];
-            unsigned t[B];
-            bool on[B];
-#pragma unroll
-            for (int u = 0; u < B; u++) {
-              const int i = i0 + u * PC_PRODUCERS, r = min(i / PER, PC_N - 1), x = i % PER;
-              const int gid = __shfl_sync(0xffffffffu, id, r >> 4), gs = __shfl_sync(0xffffffffu, slot, r >> 4) + (r & 15);
-              on[u] = i < PC_N * PER && gid >= 0 && key0 + r < k1 && x < pieces;
-              const unsigned char* block = c.g.pool + ((size_t)max(gid, 0) * c.g.kvh + kvh) * c.g.block;
-              if constexpr (BITS == 8) {
-                if (on[u]) w[u] = *reinterpret_cast<const uint4*>(block + part + gs * code + 16 * x);
-              } else {
-                if (on[u]) {
-                  const uint2 v = *reinterpret_cast<const uint2*>(block + part + gs * code + 8 * x);
-                  w[u].x = v.x; w[u].y = v.y;
-                  t[u] = block[sub + gs * n16 + x];
-                }
-              }
-            }
-#pragma unroll
-            for (int u = 0; u < B; u++) {
-              const int i = i0 + u * PC_PRODUCERS, r = i / PER, x = i % PER;
-              if (i >= PC_N * PER) break;
-              unsigned v[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
-              if (on[u]) {
-                if constexpr (BITS == 8) {
-                  const unsigned q[4] = {w[u].x, w[u].y, w[u].z, w[u].w};
-#pragma unroll
-                  for (int k = 0; k < 4; k++) { const unsigned b = q[k] ^ 0x80808080u; v[2 * k] = pa_bytes<0x4140>(b); v[2 * k + 1] = pa_bytes<0x4342>(b); }
-                } else {
-                  const unsigned q[2] = {w[u].x, w[u].y};
-                  const PaSub t2 = pa_pair(t[u], t[u]);
-#pragma unroll
-                  for (int k = 0; k < 8; k++) v[k] = pa_nibbles(q[k >> 2], k & 3, t2);
-                }
-              }
-              unsigned char* at = dst + (x >> 2) * PC_N * 128 + r * 128;
-              *reinterpret_cast<uint4*>(at + ((((2 * x) & 7) ^ (r & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
-              *reinterpret_cast<uint4*>(at + ((((2 * x + 1) & 7) ^ (r & 7)) << 4)) = make_uint4(v[4], v[5], v[6], v[7]);
-            }
-          }
+          const int sub = (is_v ? c.g.vsub : c.g.ksub) + slot * (hd / 16) + x;
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(slot_raw - 8 * pt + 8 * PC_PRODUCERS * k), "l"(block + part + (on ? slot * code + 8 * x : 0)), "r"(on ? 8 : 0) : "memory");
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(slot_raw - 12 * pt + 8 * PC_PRODUCERS * S::PER + 4 * PC_PRODUCERS * k), "l"(block + (on ? sub & ~3 : 0)), "r"(on ? 4 : 0) : "memory");
         }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) mbar_arrive(full(s));
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    // element e out of its copies into its stage
+    auto convert = [&](int e) {
+      const int j = e >> 1;
+      const unsigned stage = smem_u32(s_kv) + (e % STAGES) * STAGE, slot_raw = raw + (e & 1) * S::RAW;
+#pragma unroll 4
+      for (int k = 0; k < S::PER; k++) {
+        const int r = r0_ + RUN * k;
+        unsigned v[8];
+        if constexpr (BITS == 8) {
+          const uint4 q = lds128(slot_raw + 16 * PC_PRODUCERS * k);
+          const unsigned w[4] = {q.x ^ 0x80808080u, q.y ^ 0x80808080u, q.z ^ 0x80808080u, q.w ^ 0x80808080u};
+#pragma unroll
+          for (int i = 0; i < 4; i++) { v[2 * i] = pa_bytes<0x4140>(w[i]); v[2 * i + 1] = pa_bytes<0x4342>(w[i]); }
+        } else {
+          const uint2 q = lds64(slot_raw - 8 * pt + 8 * PC_PRODUCERS * k);
+          const unsigned word = lds32(slot_raw - 12 * pt + 8 * PC_PRODUCERS * S::PER + 4 * PC_PRODUCERS * k);
+          const int n16 = hd / 16;
+          // which byte of the word: the block and its parts start on 16-byte boundaries
+          const int slot = (k0 + j * PC_N + r) % 16, byte = (slot * n16 + x) & 3;      // slots of 16 keys take 16 n16 bytes
+          const PaSub t2 = pa_pair((word >> (8 * byte)) & 255u, (word >> (8 * byte)) & 255u);
+          const unsigned w[2] = {q.x, q.y};
+#pragma unroll
+          for (int i = 0; i < 8; i++) v[i] = pa_nibbles(w[i >> 2], i & 3, t2);
+        }
+        const unsigned to = stage + (x >> 2) * PC_N * 128 + r * 128;
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + ((((2 * x) & 7) ^ (r & 7)) << 4)), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + ((((2 * x + 1) & 7) ^ (r & 7)) << 4)), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
+      }
+    };
+    // what the weights need of tile j
+    auto meta = [&](int j) {
+      const int ms = j & 1, key0 = k0 + j * PC_N;
+      const float kx[4] = {ks.x * qf, ks.y * qf, ks.z * qf, ks.w * qf}, vx[4] = {vs.x, vs.y, vs.z, vs.w};
+      int emax = -90, emin = 1000;
+      float kmax = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        const int ex = min((int)((__float_as_uint(vx[i]) >> 23) & 255u) - 127, 100);
+        if (key0 + 4 * lane + i < k1) {
+          if (vx[i] == vx[i] && ex > -90) { emax = max(emax, ex); emin = min(emin, ex); }
+          kmax = fmaxf(kmax, kx[i]);
+        }
+      }
+      emax = __reduce_max_sync(0xffffffffu, emax);
+      emin = __reduce_min_sync(0xffffffffu, emin);
+      kmax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(kmax)));
+      const float down = __uint_as_float((unsigned)(127 - emax) << 23);
+      *reinterpret_cast<float4*>(&M.kk[ms][4 * lane]) = make_float4(kx[0], kx[1], kx[2], kx[3]);
+      *reinterpret_cast<float4*>(&M.fv[ms][4 * lane]) = make_float4(vx[0] * down, vx[1] * down, vx[2] * down, vx[3] * down);
+      const unsigned have = __ballot_sync(0xffffffffu, there);           // a bit for 4 keys
+      if (lane < 4) {
+        unsigned w = 0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) if ((have >> (8 * lane + i)) & 1u) w |= 15u << (4 * i);
+        M.valid[ms][lane] = w;
+      }
+      if (lane == 0) {
+        M.beta[ms] = __uint_as_float((unsigned)(127 + emax) << 23);
+        M.kmax[ms] = kmax;
+        M.flags[ms] = (have != ~0u ? 1u : 0u) | (emin < emax - 10 ? 2u : 0u);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(m_full(ms));
+    };
+    auto arrive = [&](int e) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      __syncwarp();
+      if (lane == 0) mbar_arrive(full(e % STAGES));
+    };
+    bool ok = true;
+    auto wait = [&](unsigned bar, int use, int why) {
+      if (!mbar_wait(bar, use & 1, PC_SPIN)) { if (!dead()) fail(why); ok = false; }
+      ok = !__any_sync(0xffffffffu, !ok || dead());
+      return ok;
+    };
+    auto room = [&](int e) { return e < STAGES || wait(empty(e % STAGES), e / STAGES - 1, 720); };
+    // the tile's page numbers and scales, then its copies, are asked for two elements (one tile) ahead
+    auto ahead = [&](int e) {
+      if (e >= 2 * n) { asm volatile("cp.async.commit_group;" ::: "memory"); return; }
+      if (!(e & 1)) { places(e >> 1); if (warp == 8) scales(e >> 1); }
+      copy(e);
+    };
+    if constexpr (BITS == 16) {
+      ahead(0);
+      if (warp == 8) meta(0);
+      for (int e = 0; e < 2 * n && ok; e++) {
+        if (!(e & 1) && e > 0 && warp == 8) { const int j = e >> 1; if (j >= 2 && !wait(m_empty(j & 1), (j >> 1) - 1, 721)) break; meta(j); }
+        // one element further is on its way while this one is waited for
+        if (e + 1 < 2 * n) { if (!room(e + 1)) break; }
+        ahead(e + 1);
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        arrive(e);
+      }
+    } else {
+      ahead(0);
+      if (warp == 8) meta(0);
+      ahead(1);
+      for (int e = 0; e < 2 * n && ok; e++) {
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        if (!room(e)) break;
+        convert(e);
+        arrive(e);
+        if ((e & 1) && e + 1 < 2 * n && warp == 8) { const int j = (e + 1) >> 1; if (j >= 2 && !wait(m_empty(j & 1), (j >> 1) - 1, 721)) break; meta(j); }
+        ahead(e + 2);
       }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
   pc_fence_before();
   __syncthreads();
-  if (warp == 11) {
+  if (warp == 12) {
     pc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
   }
@@ -638,8 +722,7 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const __grid_constant__
 
 template <int BITS, int DP>
 static cudaError_t chunk_go(const PaCall& c, long long flat, cudaStream_t st) {
-  constexpr size_t smem = (size_t)(DP / 64) * 128 * (4 * PC_M + PC_STAGES * PC_N) + sizeof(PcMeta);
-  static_assert(smem <= 227 * 1024, "shared memory");
+  constexpr size_t smem = PcShape<BITS, DP>::SMEM;
   auto kern = attn_chunk_kernel<BITS, DP>;
   static unsigned long long attr_mask = 0;
   int dev = 0;
