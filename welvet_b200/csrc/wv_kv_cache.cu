@@ -1,15 +1,18 @@
 // The paged key/value cache: rows rounded to 16, 8 or 4 bits as they are written, with the rotary embedding of Q and K in the same
 // pass, and read back. include/welvet_cuda.h (WvKvPages) defines layout and arithmetic.
 //
-// Bound: HBM for prompts, latency for single tokens. A CTA takes one token (its angles are the same for all heads), a warp a row
-// of head_dim values at a time, a lane four consecutive values of it (and four more beyond 128): float4 in, 8 / 4 / 2 bytes of
-// codes out, and the row's maximum is five shuffles away.
+// Bound: HBM for prompts, latency for single tokens. A CTA takes one token or four (their angles are the same for all heads), a warp
+// two rows of head_dim values at a time, a lane four consecutive values of each (and four more beyond 128): float4 in, 8 / 4 / 2
+// bytes of codes out, and a row's maximum is one reduction away. Four tokens share the chain of loads that finds a token's place (its
+// sequence, length, page) and fill the CTA with their angles.
 #include "wv_paged.cuh"
 #include <float.h>
 #include <math.h>
 #include <string.h>
 
 #define KVC_WARPS 8
+#define KVC_BLOCKS 4            // an SM: 64 registers (3 and 5 blocks take 138 us for prompts that take 135 with 4)
+#define KVC_TOKENS 4            // of a CTA, where there are enough of them
 
 // theta^(2 d / head_dim) for every pair, computed on the host once per (theta, head_dim) and passed by value.
 struct WvRopeFreq { double p[128]; };
@@ -34,19 +37,32 @@ __device__ __forceinline__ KvPlace kv_place(const WvKvGeom& g, const WvKvBatch& 
 
 // a * c - b * s with c and s in two float32 pieces each: the products' errors by fma, the sum's by Knuth's two-sum, so that the
 // result is the float64 expression's, rounded, but for one in some 10^7. (float64 itself issues at half the float32 rate here and its
-// conversions at a sixteenth.) What is not finite goes through float64.
-__device__ __forceinline__ float rot(float a, float b, float ch, float cl, float sh, float sl) {
-  const float p = a * ch, q = b * sh;
-  const float t = fmaf(a, cl, fmaf(a, ch, -p)) - fmaf(b, sl, fmaf(b, sh, -q));
-  const float s = __fsub_rn(p, q), z = __fsub_rn(s, p);
-  const float e = __fadd_rn(__fsub_rn(p, __fsub_rn(s, z)), __fsub_rn(-q, z));
-  const float r = s + (e + t);
-  if (fabsf(r) <= FLT_MAX) return r;
-  return (float)((double)a * ((double)ch + (double)cl) - (double)b * ((double)sh + (double)sl));
+// conversions at a sixteenth.) Two values at a time; ns is -s. Where an operand is not finite, neither is the result, and rot64 has
+// to say which one it is.
+__device__ __forceinline__ float2 rot2(float2 a, float2 b, float2 ch, float2 cl, float2 nsh, float2 nsl) {
+  const float2 m1 = make_float2(-1.f, -1.f);
+  const float2 p = __fmul2_rn(a, ch), q = __fmul2_rn(b, nsh);
+  const float2 pe = __ffma2_rn(a, ch, __fmul2_rn(p, m1)), qe = __ffma2_rn(b, nsh, __fmul2_rn(q, m1));
+  const float2 t = __fadd2_rn(__ffma2_rn(a, cl, pe), __ffma2_rn(b, nsl, qe));
+  const float2 s = __fadd2_rn(p, q), z = __ffma2_rn(p, m1, s);
+  const float2 e = __fadd2_rn(__ffma2_rn(__ffma2_rn(z, m1, s), m1, p), __ffma2_rn(z, m1, q));
+  return __fadd2_rn(s, __fadd2_rn(e, t));
+}
+__device__ __noinline__ float rot64(float a, float b, float ch, float cl, float nsh, float nsl) {
+  return (float)((double)a * ((double)ch + (double)cl) + (double)b * ((double)nsh + (double)nsl));
+}
+// rint(x / s) of the float32 quotient for |x / s| < 2^22, as the low bits of the result: the product with the reciprocal is off by
+// two units in the last place at most, so the division is only needed near the middle between two whole numbers.
+__device__ __forceinline__ unsigned kv_round(float x, float s, float inv) {
+  const float magic = 12582912.f;                                  // 1.5 2^23: the sum's last bit is 1
+  const float q = x * inv;
+  float m = __fadd_rn(q, magic);
+  if (fabsf(fabsf(q - __fsub_rn(m, magic)) - 0.5f) < 1.f / 4096.f) m = __fadd_rn(__fdiv_rn(x, s), magic);
+  return __float_as_uint(m);
 }
 
 // One row of V4 x 4 x 32 values at most: lane l holds 4 l .. 4 l + 3 (and 128 + those), lanes past head_dim hold zeros.
-template <int BITS, int V4>
+template <int BITS, int V4, bool FULL>
 __device__ __forceinline__ void kv_store_row(const WvKvGeom& g, unsigned char* block, bool is_v, int slot, const float (&x)[V4][4], int lane) {
   unsigned m = 0;                  // the largest magnitude's bits; infinities and NaN are above all others
 #pragma unroll
@@ -70,27 +86,30 @@ __device__ __forceinline__ void kv_store_row(const WvKvGeom& g, unsigned char* b
   float s;
   if (BITS == 16) s = __uint_as_float((unsigned)max((int)(m >> 23) - 14, 1) << 23);   // a subnormal has exponent 0: the smallest scale
   else s = fmaxf(__fmul_rn(a, BITS == 8 ? 1.f / 127.f : 1.f / 1785.f), FLT_MIN);
+  const float inv = __fdiv_rn(1.f, s);                             // 16 bits: a power of two (s <= 2^113), exact
   unsigned char* codes = block + (is_v ? g.page * g.code : 0) + slot * g.code;
 #pragma unroll
   for (int i = 0; i < V4; i++) {
     const int d = 4 * (lane + 32 * i);
-    if (d >= g.hd) break;
+    if (!FULL && d >= g.hd) break;
     if (BITS == 16) {
-      const float inv = __fdiv_rn(1.f, s);                       // a power of two (s <= 2^113): exact
       __half2 h[2] = {__floats2half2_rn(fine ? x[i][0] * inv : 0.f, fine ? x[i][1] * inv : 0.f),
                       __floats2half2_rn(fine ? x[i][2] * inv : 0.f, fine ? x[i][3] * inv : 0.f)};
       *reinterpret_cast<uint2*>(codes + 2 * d) = make_uint2(*reinterpret_cast<unsigned*>(&h[0]), *reinterpret_cast<unsigned*>(&h[1]));
     } else if (BITS == 8) {
-      unsigned w = 0;
+      unsigned c[4];
 #pragma unroll
-      for (int e = 0; e < 4; e++) w |= ((unsigned)(fine ? (int)rintf(__fdiv_rn(x[i][e], s)) : 0) & 0xffu) << (8 * e);
-      *reinterpret_cast<unsigned*>(codes + d) = w;
+      for (int e = 0; e < 4; e++) c[e] = fine ? kv_round(x[i][e], s, inv) : 0u;
+      *reinterpret_cast<unsigned*>(codes + d) = __byte_perm(__byte_perm(c[0], c[1], 0x0040), __byte_perm(c[2], c[3], 0x0040), 0x5410);
     } else {
       const float t = fine ? fminf(fmaxf(ceilf(__fdiv_rn(__fmul_rn(__uint_as_float(mg[i]), 1.f / 7.f), s)), 1.f), 255.f) : 1.f;
-      const float st = __fmul_rn(s, t);
+      const float st = __fmul_rn(s, t), ist = __fdiv_rn(1.f, st);
       unsigned w = 0;
 #pragma unroll
-      for (int e = 0; e < 4; e++) w |= (unsigned)(fine ? (int)fminf(fmaxf(rintf(__fdiv_rn(x[i][e], st)), -7.f), 7.f) + 8 : 8) << (4 * e);
+      for (int e = 0; e < 4; e++) {
+        const int c = fine ? (int)(kv_round(x[i][e], st, ist) - 0x4b400000u) : 0;
+        w |= (unsigned)(min(max(c, -7), 7) + 8) << (4 * e);
+      }
       *reinterpret_cast<unsigned short*>(codes + d / 2) = (unsigned short)w;
       if ((lane & 3) == 0) block[(is_v ? g.vsub : g.ksub) + slot * (g.hd / 16) + d / 16] = (unsigned char)t;
     }
@@ -98,78 +117,148 @@ __device__ __forceinline__ void kv_store_row(const WvKvGeom& g, unsigned char* b
   if (lane == 0) *reinterpret_cast<float*>(block + (is_v ? g.vscale : g.kscale) + 4 * slot) = fine ? s : __uint_as_float(0x7fc00000u);
 }
 
-// grid (tokens, pieces of a token's rows): rows of K, then V, then Q
-template <int BITS, int V4>
-__global__ void __launch_bounds__(32 * KVC_WARPS) kv_write_kernel(const WvKvGeom g, const WvKvBatch b, const float* __restrict__ k, int ldk,
+// grid (tokens / TOK, pieces of a token's rows)
+template <int BITS, int V4, int TOK, bool FULL>
+__global__ void __launch_bounds__(32 * KVC_WARPS, V4 == 1 ? KVC_BLOCKS : 2) kv_write_kernel(const WvKvGeom g, const WvKvBatch b, const float* __restrict__ k, int ldk,
                                                                   const float* __restrict__ v, int ldv, const float* q, int ldq, float* q_out,
                                                                   int ldqo, int heads, int rotate, const __grid_constant__ WvRopeFreq freq,
                                                                   int* __restrict__ err) {
-  __shared__ float4 s_cs[128];      // cos and sin of a pair, in two pieces each
+  __shared__ __align__(16) float s_cs[TOK][4][128];      // cos and sin of a pair, in two pieces each
+  __shared__ KvPlace s_at[TOK];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = g.hd >> 1;
-  const KvPlace at = kv_place(g, b, row, err);
-  if (at.pos == INT_MIN) return;    // a row that no sequence owns
+  const int row0 = blockIdx.x * TOK, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hd = FULL ? 128 * V4 : g.hd, half = hd >> 1;
+  if (warp < TOK) {
+    KvPlace p{INT_MIN, -1, 0};      // a row that no sequence owns
+    if (row0 + warp < b.total_q) p = kv_place(g, b, row0 + warp, err);
+    if (lane == 0) s_at[warp] = p;
+  }
+  __syncthreads();
   if (rotate) {
-    for (int d = threadIdx.x; d < half; d += 32 * KVC_WARPS) {
+    for (int i = threadIdx.x; i < TOK * half; i += 32 * KVC_WARPS) {
+      const int t = TOK == 1 ? 0 : i / half, d = i - t * half;
+      if (s_at[t].pos == INT_MIN) continue;
       double c, s;
-      sincos((double)at.pos / freq.p[d], &s, &c);
-      s_cs[d] = make_float4((float)c, (float)(c - (double)(float)c), (float)s, (float)(s - (double)(float)s));
+      sincos((double)s_at[t].pos / freq.p[d], &s, &c);
+      s_cs[t][0][d] = (float)c; s_cs[t][1][d] = (float)(c - (double)(float)c);
+      s_cs[t][2][d] = (float)s; s_cs[t][3][d] = (float)(s - (double)(float)s);
     }
     __syncthreads();
   }
-  const int nr = 2 * g.kvh + heads;
-  for (int r = blockIdx.y * KVC_WARPS + warp; r < nr; r += gridDim.y * KVC_WARPS) {
-    const bool is_q = r >= 2 * g.kvh, is_v = !is_q && r >= g.kvh;
-    const int h = is_q ? r - 2 * g.kvh : (is_v ? r - g.kvh : r);
-    if (!is_q && at.page < 0) continue;
-    const float* src = (is_q ? q + (size_t)row * ldq : is_v ? v + (size_t)row * ldv : k + (size_t)row * ldk) + (size_t)h * g.hd;
-    float x[V4][4];
-#pragma unroll
-    for (int i = 0; i < V4; i++) {
-      const int d = 4 * (lane + 32 * i);
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f), w = o;
-      if (d < g.hd) {
-        o = *reinterpret_cast<const float4*>(src + d);
-        if (rotate && !is_v) w = *reinterpret_cast<const float4*>(src + (d < half ? d + half : d - half));
-      }
-      x[i][0] = o.x; x[i][1] = o.y; x[i][2] = o.z; x[i][3] = o.w;
-      if (rotate && !is_v && d < g.hd) {
-        const float p[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int e = 0; e < 4; e++) {          // first half: a c - b s; second half, with b the first one's value: b s + a c
-          const float4 cs = s_cs[(d < half ? d : d - half) + e];
-          const float sg = d < half ? 1.f : -1.f;
-          x[i][e] = rot(x[i][e], p[e], cs.x, cs.y, sg * cs.z, sg * cs.w);
-        }
-      }
-    }
-    if (is_q) {
-      if (q == q_out) __syncwarp();            // in place: every lane has its partner's value
-      float* dst = q_out + (size_t)row * ldqo + (size_t)h * g.hd;
+  const int gw = blockIdx.y * KVC_WARPS + warp, nw = gridDim.y * KVC_WARPS;
+  for (int tok = 0; tok < TOK; tok++) {
+    const KvPlace at = s_at[tok];
+    if (at.pos == INT_MIN) continue;
+    const size_t row = row0 + tok;
+    // the lane's angles, for all rows of the token: cos, and the sine's negative in the first half of a row (a c - b s), itself in
+    // the second (with b the first one's value, a c + b s)
+    float2 cs[V4][4][2];
+    if (rotate) {
 #pragma unroll
       for (int i = 0; i < V4; i++) {
         const int d = 4 * (lane + 32 * i);
-        if (d < g.hd) *reinterpret_cast<float4*>(dst + d) = make_float4(x[i][0], x[i][1], x[i][2], x[i][3]);
+#pragma unroll
+        for (int p = 0; p < 4; p++) {
+          const float4 c = (FULL || d < hd) ? *reinterpret_cast<const float4*>(&s_cs[tok][p][d < half ? d : d - half]) : make_float4(0.f, 0.f, 0.f, 0.f);
+          const float f = p < 2 || d >= half ? 1.f : -1.f;
+          cs[i][p][0] = make_float2(f * c.x, f * c.y); cs[i][p][1] = make_float2(f * c.z, f * c.w);
+        }
       }
-    } else {
-      kv_store_row<BITS, V4>(g, g.pool + ((size_t)at.page * g.kvh + h) * g.block, is_v, at.slot, x, lane);
+    }
+    auto load = [&](const float* src, float (&x)[V4][4], bool on) {
+#pragma unroll
+      for (int i = 0; i < V4; i++) {
+        const int d = 4 * (lane + 32 * i);
+        const float4 o = on && (FULL || d < hd) ? *reinterpret_cast<const float4*>(src + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[i][0] = o.x; x[i][1] = o.y; x[i][2] = o.z; x[i][3] = o.w;
+      }
+    };
+    auto partners = [&](const float* src, float (&x)[V4][4], bool on) {
+#pragma unroll
+      for (int i = 0; i < V4; i++) {
+        const int d = 4 * (lane + 32 * i);
+        const float4 o = on && (FULL || d < hd) ? *reinterpret_cast<const float4*>(src + (d < half ? d + half : d - half)) : make_float4(0.f, 0.f, 0.f, 0.f);
+        x[i][0] = o.x; x[i][1] = o.y; x[i][2] = o.z; x[i][3] = o.w;
+      }
+    };
+    auto turn = [&](float (&x)[V4][4], const float (&w)[V4][4]) {
+#pragma unroll
+      for (int i = 0; i < V4; i++) {
+        float y[4];
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          const float2 v = rot2(make_float2(x[i][e], x[i][e + 1]), make_float2(w[i][e], w[i][e + 1]), cs[i][0][e / 2], cs[i][1][e / 2], cs[i][2][e / 2], cs[i][3][e / 2]);
+          y[e] = v.x; y[e + 1] = v.y;
+        }
+        if (!(fmaxf(fmaxf(fabsf(y[0]), fabsf(y[1])), fmaxf(fabsf(y[2]), fabsf(y[3]))) <= FLT_MAX) || y[0] + y[1] + y[2] + y[3] != y[0] + y[1] + y[2] + y[3]) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float2 *c = &cs[i][0][e / 2];
+            if (!(fabsf(y[e]) <= FLT_MAX)) y[e] = e & 1 ? rot64(x[i][e], w[i][e], c[0].y, c[2].y, c[4].y, c[6].y) : rot64(x[i][e], w[i][e], c[0].x, c[2].x, c[4].x, c[6].x);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[i][e] = y[e];
+      }
+    };
+    // two query heads at a time
+    for (int h = 2 * gw; h < heads; h += 2 * nw) {
+      float x[2][V4][4], w[2][V4][4];
+      const float* src = q + row * ldq + (size_t)h * hd;
+      load(src, x[0], true); load(src + hd, x[1], h + 1 < heads);
+      if (rotate) { partners(src, w[0], true); partners(src + hd, w[1], h + 1 < heads); }
+      __syncwarp();                 // in place: every lane has its partner's value
+      float* dst = q_out + row * ldqo + (size_t)h * hd;
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        if (u && h + 1 >= heads) break;
+        if (rotate) turn(x[u], w[u]);
+#pragma unroll
+        for (int i = 0; i < V4; i++) {
+          const int d = 4 * (lane + 32 * i);
+          if ((FULL || d < hd)) *reinterpret_cast<float4*>(dst + u * hd + d) = make_float4(x[u][i][0], x[u][i][1], x[u][i][2], x[u][i][3]);
+        }
+      }
+    }
+    // a kv head's K and V, the last warps first: with few tokens they have no query heads
+    if (at.page < 0) continue;
+    for (int h = nw - 1 - gw; h < g.kvh; h += nw) {
+      float x[V4][4], w[V4][4], y[V4][4];
+      const float* src = k + row * ldk + (size_t)h * hd;
+      load(src, x, true);
+      if (rotate) partners(src, w, true);
+      load(v + row * ldv + (size_t)h * hd, y, true);
+      if (rotate) turn(x, w);
+      unsigned char* block = g.pool + ((size_t)at.page * g.kvh + h) * g.block;
+      kv_store_row<BITS, V4, FULL>(g, block, false, at.slot, x, lane);
+      kv_store_row<BITS, V4, FULL>(g, block, true, at.slot, y, lane);
     }
   }
 }
 
-template <int BITS, int V4>
+template <int BITS, int V4, int TOK>
 __global__ void __launch_bounds__(32 * KVC_WARPS) kv_read_kernel(const WvKvGeom g, const WvKvBatch b, float* __restrict__ k, int ldk,
                                                                  float* __restrict__ v, int ldv, int* __restrict__ err) {
+  __shared__ KvPlace s_at[TOK];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int row = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const KvPlace at = kv_place(g, b, row, err);
-  if (at.pos == INT_MIN) return;
-  for (int r = blockIdx.y * KVC_WARPS + warp; r < 2 * g.kvh; r += gridDim.y * KVC_WARPS) {
+  const int row0 = blockIdx.x * TOK, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (warp < TOK) {
+    KvPlace p{INT_MIN, -1, 0};
+    if (row0 + warp < b.total_q) p = kv_place(g, b, row0 + warp, err);
+    if (lane == 0) s_at[warp] = p;
+  }
+  __syncthreads();
+  const int nr = 2 * g.kvh;
+#pragma unroll 4
+  for (int i0 = blockIdx.y * KVC_WARPS + warp; i0 < TOK * nr; i0 += gridDim.y * KVC_WARPS) {
+    const int tok = TOK == 1 ? 0 : i0 / nr, r = i0 - tok * nr;
+    const KvPlace at = s_at[tok];
+    if (at.pos == INT_MIN) continue;
+    const size_t row = row0 + tok;
     const bool is_v = r >= g.kvh;
     const int h = is_v ? r - g.kvh : r;
-    float* dst = (is_v ? v + (size_t)row * ldv : k + (size_t)row * ldk) + (size_t)h * g.hd;
+    float* dst = (is_v ? v + row * ldv : k + row * ldk) + (size_t)h * g.hd;
     const unsigned char* block = g.pool + ((size_t)max(at.page, 0LL) * g.kvh + h) * g.block;
     const unsigned char* codes = block + (is_v ? g.page * g.code : 0) + at.slot * g.code;
     const float s = at.page < 0 ? 0.f : *reinterpret_cast<const float*>(block + (is_v ? g.vscale : g.kscale) + 4 * at.slot);
@@ -199,15 +288,16 @@ __global__ void __launch_bounds__(32 * KVC_WARPS) kv_read_kernel(const WvKvGeom 
   }
 }
 
-static cudaError_t kvc_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* at, int tokens, int rows, cudaStream_t st) {
-  // Enough CTAs for the chip where there are few tokens; with many, a CTA per token, which computes its angles once.
+// Enough CTAs for the chip where there are few tokens; with many, a CTA for KVC_TOKENS of them.
+static int kvc_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* at, int tokens, int rows, cudaStream_t st) {
+  const int tok = tokens >= 592 * KVC_TOKENS ? KVC_TOKENS : 1;
   const int most = (rows + KVC_WARPS - 1) / KVC_WARPS, want = 592 / tokens;
-  cfg.gridDim = dim3(tokens, want < 1 ? 1 : (want > most ? most : want));
+  cfg.gridDim = dim3((tokens + tok - 1) / tok, want < 1 ? 1 : (want > most ? most : want));
   cfg.blockDim = dim3(32 * KVC_WARPS); cfg.stream = st;
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at; cfg.numAttrs = 1;
-  return cudaSuccess;
+  return tok;
 }
 
 int wv_launch_kv_write(const WvKvPages& kv, const WvKvBatch& b, const float* dk, int ldk, const float* dv, int ldv, const float* dq, int ldq,
@@ -222,11 +312,14 @@ int wv_launch_kv_write(const WvKvPages& kv, const WvKvBatch& b, const float* dk,
   }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[1];
-  kvc_config(cfg, at, b.total_q, 2 * g.kvh + heads, st);
+  const bool many = kvc_config(cfg, at, b.total_q, (2 * g.kvh + heads + 1) / 2, st) > 1;      // two rows a warp
   auto go = [&](auto kern) { return cudaLaunchKernelEx(&cfg, kern, g, b, dk, ldk, dv, ldv, dq, ldq, dq_out, ldqo, heads, theta > 0.0 ? 1 : 0, freq, wv_paged_err_ptr()); };
   cudaError_t e;
-  if (g.hd > 128) e = kv.bits == 16 ? go(kv_write_kernel<16, 2>) : kv.bits == 8 ? go(kv_write_kernel<8, 2>) : go(kv_write_kernel<4, 2>);
-  else e = kv.bits == 16 ? go(kv_write_kernel<16, 1>) : kv.bits == 8 ? go(kv_write_kernel<8, 1>) : go(kv_write_kernel<4, 1>);
+#define KVC_GO(V4_, TOK_, FULL_) (kv.bits == 16 ? go(kv_write_kernel<16, V4_, TOK_, FULL_>) : kv.bits == 8 ? go(kv_write_kernel<8, V4_, TOK_, FULL_>) : go(kv_write_kernel<4, V4_, TOK_, FULL_>))
+  if (g.hd > 128) e = many ? KVC_GO(2, KVC_TOKENS, false) : KVC_GO(2, 1, false);
+  else if (g.hd == 128) e = many ? KVC_GO(1, KVC_TOKENS, true) : KVC_GO(1, 1, true);
+  else e = many ? KVC_GO(1, KVC_TOKENS, false) : KVC_GO(1, 1, false);
+#undef KVC_GO
   if (e != cudaSuccess) { wv_set_error("wv_kv_write_dev: launch: %s", cudaGetErrorString(cudaGetLastError())); return WV_ECUDA; }
   return WV_OK;
 }
@@ -235,11 +328,13 @@ int wv_launch_kv_read(const WvKvPages& kv, const WvKvBatch& b, float* dk, int ld
   const WvKvGeom g = wv_kv_geom(kv);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[1];
-  kvc_config(cfg, at, b.total_q, 2 * g.kvh, st);
+  const bool many = kvc_config(cfg, at, b.total_q, 2 * g.kvh, st) > 1;
   auto go = [&](auto kern) { return cudaLaunchKernelEx(&cfg, kern, g, b, dk, ldk, dv, ldv, wv_paged_err_ptr()); };
   cudaError_t e;
-  if (g.hd > 128) e = kv.bits == 16 ? go(kv_read_kernel<16, 2>) : kv.bits == 8 ? go(kv_read_kernel<8, 2>) : go(kv_read_kernel<4, 2>);
-  else e = kv.bits == 16 ? go(kv_read_kernel<16, 1>) : kv.bits == 8 ? go(kv_read_kernel<8, 1>) : go(kv_read_kernel<4, 1>);
+#define KVC_GO(V4_, TOK_) (kv.bits == 16 ? go(kv_read_kernel<16, V4_, TOK_>) : kv.bits == 8 ? go(kv_read_kernel<8, V4_, TOK_>) : go(kv_read_kernel<4, V4_, TOK_>))
+  if (g.hd > 128) e = many ? KVC_GO(2, KVC_TOKENS) : KVC_GO(2, 1);
+  else e = many ? KVC_GO(1, KVC_TOKENS) : KVC_GO(1, 1);
+#undef KVC_GO
   if (e != cudaSuccess) { wv_set_error("wv_kv_read_dev: launch: %s", cudaGetErrorString(cudaGetLastError())); return WV_ECUDA; }
   return WV_OK;
 }
