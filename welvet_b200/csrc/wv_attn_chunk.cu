@@ -11,13 +11,16 @@
 // where 16-bit activations would take one, which is what bounds the kernel (the tensor pipe runs 4096 cycles for 256 x 128 x
 // head_dim 128, the weights take some 1300 a tile on the other pipes, and the two tiles take turns).
 //
-// Roles: two warpgroups own a tile each (a thread a row: maximum, weights, sums), one warp issues the MMAs, four fill the ring, K and V
-// tiles in turn. Rows of 16 bits are copied asynchronously into one of three stages; codes of 8 and 4 bits are copied as they are, two
-// tiles ahead and each thread for itself, and turned into float16 on the way from there to one of two stages. Codes of 4 bits lie in
-// the order in which they unpack two at a time (0 4 1 5 2 6 3 7); Q follows, and the outputs are put back.
+// Roles: four warpgroups have a tile's half each (a thread a row: the weights of 64 of the 128 keys, the sums of half of the values),
+// one warp issues the MMAs, three fill the ring, K and V tiles in turn. With one warpgroup a tile the weights of 128 keys were a
+// chain of some 3500 cycles with nothing to issue beside it; with two the pairs hide one another's latencies. Rows of 16 bits are
+// copied asynchronously into one of three stages; codes of 8 and 4 bits are copied as they are, two tiles ahead and each thread for
+// itself, and turned into float16 on the way from there to one of two stages. Codes of 4 bits lie in the order in which they unpack two
+// at a time (0 4 1 5 2 6 3 7); Q follows, and the outputs are put back.
 //
 // The running maximum is raised only where a logit may lie 2^7 above it, which a bound tells (the row's largest product times the
-// tile's largest scale), so that most tiles are read once.
+// tile's largest scale), so that most tiles are read once; a row's two threads agree on that, and exchange their maxima through tensor
+// memory that the next tile's sums will overwrite.
 //
 // A key's scale multiplies its column of S; a value row's, relative to the largest of its tile, its weight, and the tile's own power
 // of two goes into the sum over tiles. Where the scales in a tile lie further apart than the pieces' range holds (2^16), the tile's
@@ -30,10 +33,11 @@
 #include "wv_lease.h"
 #include <type_traits>
 
-#define PC_THREADS 512
+#define PC_THREADS 640
+#define PC_MMA_WARP 19
 #define PC_M 128                    // rows of a tile
 #define PC_N 128                    // keys of a tile
-#define PC_PRODUCERS 128
+#define PC_PRODUCERS 3              // warps 16 - 18
 #define PC_LIFT 6.f                 // weights carry 2^6 and are at most 2^14 (2^7 over the reference, scales below 2)
 #define PC_SLACK 7.f
 #define PC_SPIN (1u << 20)          // polls of a wait
@@ -97,7 +101,8 @@ struct PcMeta {
   float beta[2], kmax[2];                   // 2^e, the largest kk
   unsigned flags[2];                        // 1: some key of the tile is not there, 2: value scales too far apart
   unsigned valid[2][4];                     // which keys are there
-  unsigned long long bar[17];
+  unsigned long long bar[21];
+  unsigned vote[2][2];
   unsigned tmem, qmax;
   int abort;
   int seq, tile;
@@ -105,8 +110,8 @@ struct PcMeta {
 template <int BITS, int DP> struct PcShape {
   static constexpr int STAGES = BITS == 16 ? 3 : 2, STAGE = DP / 64 * PC_N * 128, QPIECE = DP / 64 * PC_M * 128;
   static constexpr int PIECES = BITS == 16 ? DP / 8 : DP / 16;                    // of a row: 16 bytes, or 16 codes
-  static constexpr int PER = PIECES * PC_N / PC_PRODUCERS;                        // of a tile, a thread
-  static constexpr int RAW = BITS == 16 ? 0 : PC_PRODUCERS * PER * (BITS == 8 ? 16 : 12);    // 4 bits: codes, then a word that holds the sub-scale
+  static constexpr int PER = PIECES / 2;                                          // of 16 rows, a lane
+  static constexpr int RAW = BITS == 16 ? 0 : PIECES * PC_N * (BITS == 8 ? 16 : 12);         // 4 bits: codes, then a word that holds the sub-scale
   static constexpr size_t SMEM = (size_t)4 * QPIECE + STAGES * STAGE + 2 * RAW + sizeof(PcMeta);
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
@@ -162,6 +167,8 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
   auto m_full = [&](int s) { return smem_u32(&M.bar[12 + s]); };
   auto m_empty = [&](int s) { return smem_u32(&M.bar[14 + s]); };
   const unsigned done = smem_u32(&M.bar[16]);
+  auto v_bar = [&](int t) { return smem_u32(&M.bar[17 + t]); };
+  auto x_bar = [&](int t) { return smem_u32(&M.bar[19 + t]); };
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (smem_u32(pc_smem) & 1023u) { if (tid == 0) atomicCAS_system(c.err - 1, 0, 799); return; }    // the swizzle counts from 1024-byte boundaries
@@ -195,15 +202,17 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
   const bool two = rn > PC_M;
 
   if (tid == 0) {
-    for (int s = 0; s < STAGES; s++) { mbar_init(full(s), PC_PRODUCERS / 32); mbar_init(empty(s), 1); }
+    for (int s = 0; s < STAGES; s++) { mbar_init(full(s), PC_PRODUCERS); mbar_init(empty(s), 1); }
     for (int t = 0; t < 2; t++) {
-      mbar_init(s_full(t), 1); mbar_init(p_full(t), 4); mbar_init(o_full(t), 1);
-      mbar_init(m_full(t), 1); mbar_init(m_empty(t), two ? 8 : 4);
+      mbar_init(s_full(t), 1); mbar_init(p_full(t), 8); mbar_init(o_full(t), 1);
+      mbar_init(m_full(t), 1); mbar_init(m_empty(t), two ? 16 : 8);
+      mbar_init(v_bar(t), 8); mbar_init(x_bar(t), 8);
+      M.vote[t][0] = M.vote[t][1] = 0;
     }
     mbar_init(done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 12) {
+  if (warp == PC_MMA_WARP) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&M.tmem)), "n"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -259,59 +268,73 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
   auto fail = [&](int code) { atomicCAS_system(c.err - 1, 0, code); *(volatile int*)&M.abort = 1; };      // the word before is the waits'
   auto dead = [&]() { return *(volatile int*)&M.abort != 0; };
 
-  if (warp < 8) {
-    // ============================================================== a tile's rows: weights and sums, a thread a row
-    pc_regs_up<216>();
-    const int t = warp >> 2, row = tid & (PC_M - 1), r = t * PC_M + row;
+  if (warp < 16) {
+    // ============================================================== half a tile: weights of 64 keys, sums of half of the values
+    pc_regs_up<104>();
+    constexpr int HD = DP / 2, HK = PC_N / 2;
+    const int t = warp >> 3, hf = (warp >> 2) & 1, row = tid & (PC_M - 1), r = t * PC_M + row;
     if (t == 0 || two) {
       const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
-      const unsigned ts = tmem + lanes + t * PC_N, to = tmem + lanes + 256 + t * 128;
+      const unsigned ts = tmem + lanes + t * PC_N + hf * HK, to = tmem + lanes + 256 + t * 128 + hf * HD, tx = to + HD - 2 * hf * HD;
       const int prow = pos0 + (r0 + min(r, rn - 1)) / c.group;
       const int pmin = pos0 + (r0 + t * PC_M) / c.group, pmax = pos0 + (r0 + min(t * PC_M + PC_M, rn) - 1) / c.group;
-      float o[DP], m = -INFINITY;
+      float o[HD], m = -INFINITY;
       float2 l2 = make_float2(0.f, 0.f);
 #pragma unroll
-      for (int d = 0; d < DP; d++) o[d] = 0.f;
+      for (int d = 0; d < HD; d++) o[d] = 0.f;
       bool ok = true;
+      int nv = 0, nx = 0;                                                // votes and exchanges so far
+      // a wait of the whole warp; false when it ran out or the block has given up
+      auto wait = [&](unsigned bar, int use, int why) {
+        if (ok && !mbar_wait(bar, use & 1, PC_SPIN)) { if (!dead()) fail(why); ok = false; }
+        ok = !__any_sync(0xffffffffu, !ok);
+        return ok;
+      };
+      // the tile's eight warps meet
+      auto meet = [&](unsigned bar, int use, int why) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar);
+        return wait(bar, use, why);
+      };
       for (int j = 0; j < n; j++) {
         const int ms = j & 1, key0 = k0 + j * PC_N;
-        if (!mbar_wait(m_full(ms), (j >> 1) & 1, PC_SPIN) || !mbar_wait(s_full(t), j & 1, PC_SPIN)) { if (!dead()) fail(700 + t); ok = false; }
-        if (__any_sync(0xffffffffu, !ok)) { ok = false; break; }
+        if (!wait(m_full(ms), j >> 1, 700 + t) || !wait(s_full(t), j, 702 + t)) break;
         pc_fence_after();
-        const unsigned kk = smem_u32(M.kk[ms]), fv = smem_u32(M.fv[ms]);
+        const unsigned kk = smem_u32(M.kk[ms]) + 4 * HK * hf, fv = smem_u32(M.fv[ms]) + 4 * HK * hf;
         float beta = M.beta[ms], alpha = 1.f;
         const unsigned flags = M.flags[ms];
         const bool masked = (flags & 1u) || key0 + PC_N - 1 > pmin || key0 + PC_N > k1 || (c.window != 0 && key0 <= pmax - c.window);
-        // bit k of `see`: the row sees key 32 q + k of the tile
-        unsigned see[4];
-        if (masked) {
-#pragma unroll
-          for (int q = 0; q < 4; q++) {
-            const int a = key0 + 32 * q, last = min(prow, k1 - 1) - a, first = c.window ? prow - c.window + 1 - a : 0;
-            unsigned w = last < 0 ? 0u : last >= 31 ? ~0u : (2u << last) - 1u;
-            if (first > 0) w &= first > 31 ? 0u : ~0u << first;
-            see[q] = w & M.valid[ms][q];
-          }
-        }
+        // bit k of `see`: the row sees key 32 q + k of the half
+        auto sees = [&](int at, int word) {
+          const int a = key0 + 32 * at, last = min(prow, k1 - 1) - a, first = c.window ? prow - c.window + 1 - a : 0;
+          unsigned w = last < 0 ? 0u : last >= 31 ? ~0u : (2u << last) - 1u;
+          if (first > 0) w &= first > 31 ? 0u : ~0u << first;
+          return w & M.valid[ms][word];
+        };
+        unsigned see[2] = {~0u, ~0u};
+        if (masked) { see[0] = sees(2 * hf, 2 * hf); see[1] = sees(2 * hf + 1, 2 * hf + 1); }
         // ---- the reference: may a logit lie too far above it?
         bool raise = masked;
         if (!masked) {
           float top = 0.f;
-          unsigned a[2][16];
-          pc_ld16(ts, a[0]);
 #pragma unroll
-          for (int q = 0; q < 8; q++) {
+          for (int q = 0; q < 4; q++) {
+            unsigned a[16];
+            pc_ld16(ts + 16 * q, a);
             pc_wait_ld();
-            if (q < 7) pc_ld16(ts + 16 * (q + 1), a[(q + 1) & 1]);
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) top = fmaxf(top, fmaxf(__uint_as_float(a[q & 1][i]), __uint_as_float(a[q & 1][i + 1])));
+            for (int i = 0; i < 16; i += 2) top = fmaxf(top, fmaxf(__uint_as_float(a[i]), __uint_as_float(a[i + 1])));
           }
-          raise = !(top * M.kmax[ms] <= m + PC_SLACK);
+          if (__any_sync(0xffffffffu, !(top * M.kmax[ms] <= m + PC_SLACK)) && lane == 0) atomicOr(&M.vote[t][nv & 1], 1u);
+          if (!meet(v_bar(t), nv, 704 + t)) break;
+          raise = *(volatile unsigned*)&M.vote[t][nv & 1] != 0;
+          if ((warp & 7) == 0 && lane == 0) M.vote[t][(nv + 1) & 1] = 0; // nobody comes to the next vote before this warp's weights are there
+          nv++;
         }
-        if (__any_sync(0xffffffffu, raise)) {
+        if (raise) {
           float mx = m;
 #pragma unroll
-          for (int q = 0; q < 8; q++) {
+          for (int q = 0; q < 4; q++) {
             unsigned a[16];
             pc_ld16(ts + 16 * q, a);
             pc_wait_ld();
@@ -320,59 +343,62 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
               const uint4 k4 = lds128(kk + 4 * (16 * q + i));
               const float x[4] = {__uint_as_float(a[i]) * __uint_as_float(k4.x), __uint_as_float(a[i + 1]) * __uint_as_float(k4.y),
                                   __uint_as_float(a[i + 2]) * __uint_as_float(k4.z), __uint_as_float(a[i + 3]) * __uint_as_float(k4.w)};
-              if (!masked) mx = fmaxf(mx, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
-              else {
 #pragma unroll
-                for (int u = 0; u < 4; u++) if ((see[q >> 1] >> (16 * (q & 1) + i + u)) & 1u) mx = fmaxf(mx, x[u]);
-              }
+              for (int u = 0; u < 4; u++) if ((see[q >> 1] >> (16 * (q & 1) + i + u)) & 1u) mx = fmaxf(mx, x[u]);
             }
           }
+          asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(to), "r"(__float_as_uint(mx)) : "memory");
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+          pc_fence_before();
+          if (!meet(x_bar(t), nx++, 706 + t)) break;
+          pc_fence_after();
+          mx = fmaxf(mx, __uint_as_float(pc_ld1(tx)));
           alpha = mx > m ? pa_ex2(m - mx) : 1.f;                         // 0 while there was nothing
           m = mx;
           l2 = __fmul2_rn(l2, make_float2(alpha, alpha));
         }
         const float2 off = m == -INFINITY ? make_float2(0.f, 0.f) : make_float2(PC_LIFT - m, PC_LIFT - m);
         if (flags & 2u) {
-          // ---- value by value in float32; P is zero
+          // ---- value by value in float32: both threads of a row go through all 128 keys; then P is zero
           const int e = 2 * j + 1;
-          if (!mbar_wait(full(e % STAGES), (e / STAGES) & 1, PC_SPIN)) { if (!dead()) fail(702); ok = false; }
-          if (__any_sync(0xffffffffu, !ok)) { ok = false; break; }
+          if (!wait(full(e % STAGES), e / STAGES, 708)) break;
           const unsigned char* v = s_kv + (e % STAGES) * STAGE;
+          const unsigned tt = tmem + lanes + t * PC_N;
 #pragma unroll
-          for (int d = 0; d < DP; d++) o[d] *= alpha;
+          for (int d = 0; d < HD; d++) o[d] *= alpha;
           alpha = 1.f;
 #pragma unroll 1
           for (int k = 0; k < PC_N; k++) {
-            const float x = fmaf(__uint_as_float(pc_ld1(ts + k)), M.kk[ms][k], off.x);
-            const unsigned word = k < 32 ? see[0] : k < 64 ? see[1] : k < 96 ? see[2] : see[3];
-            const bool on = !masked || ((word >> (k & 31)) & 1u);
+            const float x = fmaf(__uint_as_float(pc_ld1(tt + k)), M.kk[ms][k], off.x);
+            const bool on = !masked || ((sees(k >> 5, k >> 5) >> (k & 31)) & 1u);
             const float p = on ? pa_ex2(x) : 0.f, w = on ? p * M.fv[ms][k] * beta : 0.f;
-            l2.x += p;
+            if (k / HK == hf) l2.x += p;
 #pragma unroll
-            for (int g = 0; g < DP / 8; g++) {
-              const uint4 q = *reinterpret_cast<const uint4*>(v + (g >> 3) * PC_N * 128 + k * 128 + (((g & 7) ^ (k & 7)) << 4));
+            for (int g = 0; g < HD / 8; g++) {
+              const int at = hf * (HD / 8) + g;                          // 16 bytes of the row
+              const uint4 q = *reinterpret_cast<const uint4*>(v + (at >> 3) * PC_N * 128 + k * 128 + (((at & 7) ^ (k & 7)) << 4));
               const float2 a = pa_unpack(q.x), b = pa_unpack(q.y), d = pa_unpack(q.z), f = pa_unpack(q.w);
               o[8 * g] += w * a.x; o[8 * g + 1] += w * a.y; o[8 * g + 2] += w * b.x; o[8 * g + 3] += w * b.y;
               o[8 * g + 4] += w * d.x; o[8 * g + 5] += w * d.y; o[8 * g + 6] += w * f.x; o[8 * g + 7] += w * f.y;
             }
           }
           beta = 0.f;
+          pc_fence_before();
+          if (!meet(x_bar(t), nx++, 706 + t)) break;                     // the row's other thread has read S
+          pc_fence_after();
           unsigned z[16];
 #pragma unroll
           for (int i = 0; i < 16; i++) z[i] = 0u;
 #pragma unroll
-          for (int q = 0; q < 8; q++) pc_st16(ts + 16 * q, z);
+          for (int q = 0; q < 4; q++) pc_st16(ts + 16 * q, z);
         } else {
           // ---- weights: 16 keys of S become 8 columns of their hi pieces and 8 of their lo pieces
           auto weights = [&](auto some) {
-            unsigned a[2][16];
-            pc_ld16(ts, a[0]);
 #pragma unroll
-            for (int q = 0; q < 8; q++) {
-              unsigned w[16];
+            for (int q = 0; q < 4; q++) {
+              unsigned s[16], w[16];
+              pc_ld16(ts + 16 * q, s);
               pc_wait_ld();
-              if (q < 7) pc_ld16(ts + 16 * (q + 1), a[(q + 1) & 1]);
-              const unsigned (&s)[16] = a[q & 1];
 #pragma unroll
               for (int i = 0; i < 16; i += 4) {
                 const uint4 k4 = lds128(kk + 4 * (16 * q + i)), f4 = lds128(fv + 4 * (16 * q + i));
@@ -404,55 +430,61 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
         __syncwarp();
         if (lane == 0) { mbar_arrive(p_full(t)); mbar_arrive(m_empty(ms)); }
         // ---- this tile's part of the sum
-        const bool same = !__any_sync(0xffffffffu, alpha != 1.f);
-        if (!mbar_wait(o_full(t), j & 1, PC_SPIN)) { if (!dead()) fail(704 + t); ok = false; }
-        if (__any_sync(0xffffffffu, !ok)) { ok = false; break; }
-        pc_fence_after();
-        if (!same) {
+        if (__any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll
-          for (int d = 0; d < DP; d += 2) { const float2 v = __fmul2_rn(make_float2(o[d], o[d + 1]), make_float2(alpha, alpha)); o[d] = v.x; o[d + 1] = v.y; }
+          for (int d = 0; d < HD; d += 2) { const float2 v = __fmul2_rn(make_float2(o[d], o[d + 1]), make_float2(alpha, alpha)); o[d] = v.x; o[d + 1] = v.y; }
         }
-        {
-          unsigned a[2][16];
-          pc_ld16(to, a[0]);
+        if (!wait(o_full(t), j, 710 + t)) break;
+        pc_fence_after();
 #pragma unroll
-          for (int q = 0; q < DP / 16; q++) {
-            pc_wait_ld();
-            if (q < DP / 16 - 1) pc_ld16(to + 16 * (q + 1), a[(q + 1) & 1]);
+        for (int q = 0; q < HD / 16; q++) {
+          unsigned a[16];
+          pc_ld16(to + 16 * q, a);
+          pc_wait_ld();
 #pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              const float2 v = __ffma2_rn(make_float2(__uint_as_float(a[q & 1][i]), __uint_as_float(a[q & 1][i + 1])), make_float2(beta, beta), make_float2(o[16 * q + i], o[16 * q + i + 1]));
-              o[16 * q + i] = v.x; o[16 * q + i + 1] = v.y;
-            }
+          for (int i = 0; i < 16; i += 2) {
+            const float2 v = __ffma2_rn(make_float2(__uint_as_float(a[i]), __uint_as_float(a[i + 1])), make_float2(beta, beta), make_float2(o[16 * q + i], o[16 * q + i + 1]));
+            o[16 * q + i] = v.x; o[16 * q + i + 1] = v.y;
           }
         }
       }
-      const float l = l2.x + l2.y;
+      // the row's divisor: the two halves' sums
+      float l = l2.x + l2.y;
+      if (ok) {
+        asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(to), "r"(__float_as_uint(l)) : "memory");
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        pc_fence_before();
+        if (meet(x_bar(t), nx++, 706 + t)) {
+          pc_fence_after();
+          l += __uint_as_float(pc_ld1(tx));
+        }
+      }
       if (r < rn) {
         float f = 1.f;
         float* dst;
         if (c.nsplit > 1) {
           dst = c.acc + ((rec0 + r) * c.nsplit + sp) * hd;
-          c.ml[(rec0 + r) * c.nsplit + sp] = make_float2(m, l);
+          if (hf == 0) c.ml[(rec0 + r) * c.nsplit + sp] = make_float2(m, l);
         } else {
           dst = c.out + (size_t)(sq.q0 + (r0 + r) / c.group) * c.ldo + (size_t)(kvh * c.group + (r0 + r) % c.group) * hd;
           f = l == 0.f ? 0.f : 1.f / l;
         }
 #pragma unroll
-        for (int g = 0; g < DP / 8; g++) {
-          if (8 * g < hd) {
+        for (int g = 0; g < HD / 8; g++) {
+          const int d = hf * HD + 8 * g;
+          if (d < hd) {
             float x[8];
 #pragma unroll
-            for (int p = 0; p < 8; p++) x[pc_dim<BITS>(p)] = ok ? (c.nsplit > 1 ? o[8 * g + p] : o[8 * g + p] * f) : NAN;
-            *reinterpret_cast<float4*>(dst + 8 * g) = make_float4(x[0], x[1], x[2], x[3]);
-            *reinterpret_cast<float4*>(dst + 8 * g + 4) = make_float4(x[4], x[5], x[6], x[7]);
+            for (int p = 0; p < 8; p++) x[pc_dim<BITS>(p)] = ok ? o[8 * g + p] * f : NAN;
+            *reinterpret_cast<float4*>(dst + d) = make_float4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<float4*>(dst + d + 4) = make_float4(x[4], x[5], x[6], x[7]);
           }
         }
       }
     }
-  } else if (warp >= 12) {
-    pc_regs_down<32>();
-    if (warp == 12) {
+  } else {
+    pc_regs_down<64>();
+    if (warp == PC_MMA_WARP) {
       // ============================================================ MMAs
       const bool leader = pc_elect();
       const unsigned qa = smem_u32(s_q), kv = smem_u32(s_kv);
@@ -516,16 +548,14 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
         __syncwarp();
         mbar_wait(done, 0, PC_SPIN);
       }
-    }
-  } else {
+    } else {
     // ============================================================== K and V tiles
-    pc_regs_down<48>();
-    const int pt = tid - 256, code = c.g.code, page = c.g.page;
-    // A thread's piece of each run of rows is the same one: 16 bytes (16 bits) or 16 codes of row r0_ + RUN k, k = 0 ..
-    constexpr int RUN = PC_PRODUCERS / S::PIECES;
-    const int x = pt % S::PIECES, r0_ = pt / S::PIECES;
+    const int pw = warp - 16, code = c.g.code, page = c.g.page;
+    // A warp takes the groups pw, pw + 3, .. of a tile's eight groups of 16 rows; a lane's piece (16 bytes of 16-bit rows, else 16 codes) is
+    // number x of rows lr, lr + STEP, ..
+    constexpr int STEP = 32 / S::PIECES, PER = S::PER;
+    const int x = lane % S::PIECES, lr = lane / S::PIECES, n16 = hd / 16;
     const bool mine = BITS == 16 ? 8 * x < hd : 16 * x < hd;
-    const unsigned raw = smem_u32(s_raw) + 16 * pt;
     // page numbers of 32 groups of 16 keys (four tiles) at a time, a lane each, as offsets in the pool (-1: not there)
     long long blk = 0;
     int slots = 0;
@@ -533,12 +563,12 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
       if ((j & 3) == 0) {
         const int key = k0 + j * PC_N + 16 * lane, at = key / page;
         int id = key < k1 ? c.b.pages[(size_t)seq * c.b.table_stride + at] : 0;
-        if (id < 0 || id >= c.g.num_pages) { if (warp == 8) wv_paged_report(c.err, WV_PAGED_PAGE); id = -1; }
+        if (id < 0 || id >= c.g.num_pages) { if (pw == 0) wv_paged_report(c.err, WV_PAGED_PAGE); id = -1; }
         blk = id < 0 || key >= k1 ? -1LL : ((long long)id * c.g.kvh + kvh) * c.g.block;
         slots = key - at * page;
       }
     };
-    float4 ks = make_float4(0.f, 0.f, 0.f, 0.f), vs = ks;                // warp 8: four keys a lane of the next tile
+    float4 ks = make_float4(0.f, 0.f, 0.f, 0.f), vs = ks;                // the first of the warps: four keys a lane of the next tile
     bool there = true;
     auto scales = [&](int j) {
       const int g = 8 * (j & 3) + (lane >> 2);
@@ -553,57 +583,64 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
     };
     // the copies of element e: into its stage (16 bits), or as they are
     auto copy = [&](int e) {
-      const int j = e >> 1, key0 = k0 + j * PC_N;
+      const int j = e >> 1;
       const bool is_v = e & 1;
-      const int part = is_v ? page * code : 0;
-      const unsigned stage = smem_u32(s_kv) + (e % STAGES) * STAGE, slot_raw = raw + (e & 1) * S::RAW;
-#pragma unroll 4
-      for (int k = 0; k < S::PER; k++) {
-        const int r = r0_ + RUN * k, g = 8 * (j & 3) + (r >> 4);
-        const long long at = __shfl_sync(0xffffffffu, blk, g);
-        const int slot = __shfl_sync(0xffffffffu, slots, g) + (r & 15);
-        const bool on = mine && at >= 0 && key0 + r < k1;
+      const unsigned stage = smem_u32(s_kv) + (e % STAGES) * STAGE, raw = smem_u32(s_raw) + (e & 1) * S::RAW;
+      for (int g = pw; g < 8; g += PC_PRODUCERS) {
+        const long long at = __shfl_sync(0xffffffffu, blk, 8 * (j & 3) + g);
+        const int slot = __shfl_sync(0xffffffffu, slots, 8 * (j & 3) + g) + lr;
+        const int left = at < 0 ? 0 : k1 - (k0 + j * PC_N + 16 * g) - lr;          // the lane's rows 0, STEP, .. below this exist
         const unsigned char* block = c.g.pool + (at < 0 ? 0 : at);
-        if constexpr (BITS == 16) {
-          const unsigned to = stage + (x >> 3) * PC_N * 128 + r * 128 + (((x & 7) ^ (r & 7)) << 4);
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(block + part + (on ? slot * code + 16 * x : 0)), "r"(on ? 16 : 0) : "memory");
-        } else if constexpr (BITS == 8) {
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(slot_raw + 16 * PC_PRODUCERS * k), "l"(block + part + (on ? slot * code + 16 * x : 0)), "r"(on ? 16 : 0) : "memory");
-        } else {
-          const int sub = (is_v ? c.g.vsub : c.g.ksub) + slot * (hd / 16) + x;
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(slot_raw - 8 * pt + 8 * PC_PRODUCERS * k), "l"(block + part + (on ? slot * code + 8 * x : 0)), "r"(on ? 8 : 0) : "memory");
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(slot_raw - 12 * pt + 8 * PC_PRODUCERS * S::PER + 4 * PC_PRODUCERS * k), "l"(block + (on ? sub & ~3 : 0)), "r"(on ? 4 : 0) : "memory");
+        const unsigned char* src = block + (is_v ? page * code : 0) + slot * code + (BITS == 4 ? 8 : 16) * x;
+        const int sub = (is_v ? c.g.vsub : c.g.ksub) + slot * n16 + x;
+#pragma unroll
+        for (int i = 0; i < PER; i++) {
+          const bool on = mine && STEP * i < left;
+          const unsigned char* s = on ? src + STEP * i * code : block;
+          if constexpr (BITS == 16) {
+            const int r = 16 * g + lr + STEP * i;
+            const unsigned to = stage + (x >> 3) * PC_N * 128 + r * 128 + (((x & 7) ^ (r & 7)) << 4);
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(s), "r"(on ? 16 : 0) : "memory");
+          } else if constexpr (BITS == 8) {
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(raw + ((g * PER + i) * 32 + lane) * 16), "l"(s), "r"(on ? 16 : 0) : "memory");
+          } else {
+            const int w = (sub + STEP * i * n16) & ~3;
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(raw + ((g * PER + i) * 32 + lane) * 8), "l"(s), "r"(on ? 8 : 0) : "memory");
+            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(raw + 8 * PER * 256 + ((g * PER + i) * 32 + lane) * 4), "l"(block + (on ? w : 0)), "r"(on ? 4 : 0) : "memory");
+          }
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    // element e out of its copies into its stage
+    // Element e out of its copies into its stage. A lane stores two neighbouring 16-byte pieces; those of the upper half of a row start
+    // with the second, so that eight lanes reach all banks.
     auto convert = [&](int e) {
-      const int j = e >> 1;
-      const unsigned stage = smem_u32(s_kv) + (e % STAGES) * STAGE, slot_raw = raw + (e & 1) * S::RAW;
-#pragma unroll 4
-      for (int k = 0; k < S::PER; k++) {
-        const int r = r0_ + RUN * k;
-        unsigned v[8];
-        if constexpr (BITS == 8) {
-          const uint4 q = lds128(slot_raw + 16 * PC_PRODUCERS * k);
-          const unsigned w[4] = {q.x ^ 0x80808080u, q.y ^ 0x80808080u, q.z ^ 0x80808080u, q.w ^ 0x80808080u};
+      const unsigned stage = smem_u32(s_kv) + (e % STAGES) * STAGE, raw = smem_u32(s_raw) + (e & 1) * S::RAW;
+      const bool turned = (x >> 2) & 1;
+      for (int g = pw; g < 8; g += PC_PRODUCERS) {
 #pragma unroll
-          for (int i = 0; i < 4; i++) { v[2 * i] = pa_bytes<0x4140>(w[i]); v[2 * i + 1] = pa_bytes<0x4342>(w[i]); }
-        } else {
-          const uint2 q = lds64(slot_raw - 8 * pt + 8 * PC_PRODUCERS * k);
-          const unsigned word = lds32(slot_raw - 12 * pt + 8 * PC_PRODUCERS * S::PER + 4 * PC_PRODUCERS * k);
-          const int n16 = hd / 16;
-          // which byte of the word: the block and its parts start on 16-byte boundaries
-          const int slot = (k0 + j * PC_N + r) % 16, byte = (slot * n16 + x) & 3;      // slots of 16 keys take 16 n16 bytes
-          const PaSub t2 = pa_pair((word >> (8 * byte)) & 255u, (word >> (8 * byte)) & 255u);
-          const unsigned w[2] = {q.x, q.y};
+        for (int i = 0; i < PER; i++) {
+          const int r15 = lr + STEP * i, r = 16 * g + r15;
+          unsigned v[8];
+          if constexpr (BITS == 8) {
+            const uint4 q = lds128(raw + ((g * PER + i) * 32 + lane) * 16);
+            const unsigned w[4] = {(turned ? q.z : q.x) ^ 0x80808080u, (turned ? q.w : q.y) ^ 0x80808080u, (turned ? q.x : q.z) ^ 0x80808080u, (turned ? q.y : q.w) ^ 0x80808080u};
 #pragma unroll
-          for (int i = 0; i < 8; i++) v[i] = pa_nibbles(w[i >> 2], i & 3, t2);
+            for (int k = 0; k < 4; k++) { v[2 * k] = pa_bytes<0x4140>(w[k]); v[2 * k + 1] = pa_bytes<0x4342>(w[k]); }
+          } else {
+            const uint2 q = lds64(raw + ((g * PER + i) * 32 + lane) * 8);
+            const unsigned word = lds32(raw + 8 * PER * 256 + ((g * PER + i) * 32 + lane) * 4);
+            // which byte of the word: a block, its parts and 16 slots' sub-scales start on 16-byte boundaries, and k0 is a multiple of 16
+            const unsigned sc = (word >> (8 * ((r15 * n16 + x) & 3))) & 255u;
+            const PaSub t2 = pa_pair(sc, sc);
+            const unsigned w[2] = {turned ? q.y : q.x, turned ? q.x : q.y};
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = pa_nibbles(w[k >> 2], k & 3, t2);
+          }
+          const unsigned to = stage + (x >> 2) * PC_N * 128 + r * 128 + ((((2 * x + turned) & 7) ^ (r & 7)) << 4);
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to ^ 16u), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
         }
-        const unsigned to = stage + (x >> 2) * PC_N * 128 + r * 128;
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + ((((2 * x) & 7) ^ (r & 7)) << 4)), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
-        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + ((((2 * x + 1) & 7) ^ (r & 7)) << 4)), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]) : "memory");
       }
     };
     // what the weights need of tile j
@@ -656,14 +693,14 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
     // the tile's page numbers and scales, then its copies, are asked for two elements (one tile) ahead
     auto ahead = [&](int e) {
       if (e >= 2 * n) { asm volatile("cp.async.commit_group;" ::: "memory"); return; }
-      if (!(e & 1)) { places(e >> 1); if (warp == 8) scales(e >> 1); }
+      if (!(e & 1)) { places(e >> 1); if (pw == 0) scales(e >> 1); }
       copy(e);
     };
     if constexpr (BITS == 16) {
       ahead(0);
-      if (warp == 8) meta(0);
+      if (pw == 0) meta(0);
       for (int e = 0; e < 2 * n && ok; e++) {
-        if (!(e & 1) && e > 0 && warp == 8) { const int j = e >> 1; if (j >= 2 && !wait(m_empty(j & 1), (j >> 1) - 1, 721)) break; meta(j); }
+        if (!(e & 1) && e > 0 && pw == 0) { const int j = e >> 1; if (j >= 2 && !wait(m_empty(j & 1), (j >> 1) - 1, 721)) break; meta(j); }
         // one element further is on its way while this one is waited for
         if (e + 1 < 2 * n) { if (!room(e + 1)) break; }
         ahead(e + 1);
@@ -672,22 +709,23 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
       }
     } else {
       ahead(0);
-      if (warp == 8) meta(0);
+      if (pw == 0) meta(0);
       ahead(1);
       for (int e = 0; e < 2 * n && ok; e++) {
         asm volatile("cp.async.wait_group 1;" ::: "memory");
         if (!room(e)) break;
         convert(e);
         arrive(e);
-        if ((e & 1) && e + 1 < 2 * n && warp == 8) { const int j = (e + 1) >> 1; if (j >= 2 && !wait(m_empty(j & 1), (j >> 1) - 1, 721)) break; meta(j); }
+        if ((e & 1) && e + 1 < 2 * n && pw == 0) { const int j = (e + 1) >> 1; if (j >= 2 && !wait(m_empty(j & 1), (j >> 1) - 1, 721)) break; meta(j); }
         ahead(e + 2);
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
+    }
   }
   pc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == PC_MMA_WARP) {
     pc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
   }
