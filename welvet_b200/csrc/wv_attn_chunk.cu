@@ -18,12 +18,12 @@
 // itself, and turned into float16 on the way from there to one of two stages. Codes of 4 bits lie in the order in which they unpack two
 // at a time (0 4 1 5 2 6 3 7); Q follows, and the outputs are put back.
 //
-// The running maximum is raised only where a logit may lie 2^7 above it, which a bound tells (the row's largest product times the
+// The running maximum is raised only where a logit may lie 2^10 above it, which a bound tells (the row's largest product times the
 // tile's largest scale), so that most tiles are read once; a row's two threads agree on that, and exchange their maxima through tensor
 // memory that the next tile's sums will overwrite.
 //
 // A key's scale multiplies its column of S; a value row's, relative to the largest of its tile, its weight, and the tile's own power
-// of two goes into the sum over tiles. Where the scales in a tile lie further apart than the pieces' range holds (2^16), the tile's
+// of two goes into the sum over tiles. Where the scales in a tile lie further apart than the pieces' range holds (2^8), the tile's
 // weighted sum is taken value by value in float32 instead.
 //
 // Every wait is bounded: when one runs out the block records a code, all roles leave their loops, and tensor memory is released
@@ -38,8 +38,8 @@
 #define PC_M 128                    // rows of a tile
 #define PC_N 128                    // keys of a tile
 #define PC_PRODUCERS 3              // warps 16 - 18
-#define PC_LIFT 6.f                 // weights carry 2^6 and are at most 2^14 (2^7 over the reference, scales below 2)
-#define PC_SLACK 7.f
+#define PC_LIFT 4.f                 // weights carry 2^4 and are at most 2^15 (2^10 over the reference, scales below 2)
+#define PC_SLACK 10.f
 #define PC_SPIN (1u << 20)          // polls of a wait
 
 int wv_sm_count();
@@ -111,7 +111,7 @@ template <int BITS, int DP> struct PcShape {
   static constexpr int STAGES = BITS == 16 ? 3 : 2, STAGE = DP / 64 * PC_N * 128, QPIECE = DP / 64 * PC_M * 128;
   static constexpr int PIECES = BITS == 16 ? DP / 8 : DP / 16;                    // of a row: 16 bytes, or 16 codes
   static constexpr int PER = PIECES / 2;                                          // of 16 rows, a lane
-  static constexpr int RAW = BITS == 16 ? 0 : PIECES * PC_N * (BITS == 8 ? 16 : 12);         // 4 bits: codes, then a word that holds the sub-scale
+  static constexpr int RAW = BITS == 16 ? 0 : PIECES * PC_N * (BITS == 8 ? 16 : 8) + (BITS == 4 ? 1024 : 0);      // 4 bits: codes, then sub-scales
   static constexpr size_t SMEM = (size_t)4 * QPIECE + STAGES * STAGE + 2 * RAW + sizeof(PcMeta);
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
@@ -333,18 +333,24 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
         }
         if (raise) {
           float mx = m;
-#pragma unroll
+#pragma unroll 1
           for (int q = 0; q < 4; q++) {
+            const unsigned bits = ((q < 2 ? see[0] : see[1]) >> (16 * (q & 1))) & 0xffffu;
+            if (!__any_sync(0xffffffffu, bits)) continue;                // keys that none of the warp's rows sees
             unsigned a[16];
             pc_ld16(ts + 16 * q, a);
             pc_wait_ld();
+            const bool all = __all_sync(0xffffffffu, bits == 0xffffu);
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
-              const uint4 k4 = lds128(kk + 4 * (16 * q + i));
-              const float x[4] = {__uint_as_float(a[i]) * __uint_as_float(k4.x), __uint_as_float(a[i + 1]) * __uint_as_float(k4.y),
-                                  __uint_as_float(a[i + 2]) * __uint_as_float(k4.z), __uint_as_float(a[i + 3]) * __uint_as_float(k4.w)};
+              const uint4 k4 = lds128(kk + 64 * q + 4 * i);
+              float x[4] = {__uint_as_float(a[i]) * __uint_as_float(k4.x), __uint_as_float(a[i + 1]) * __uint_as_float(k4.y),
+                            __uint_as_float(a[i + 2]) * __uint_as_float(k4.z), __uint_as_float(a[i + 3]) * __uint_as_float(k4.w)};
+              if (!all) {
 #pragma unroll
-              for (int u = 0; u < 4; u++) if ((see[q >> 1] >> (16 * (q & 1) + i + u)) & 1u) mx = fmaxf(mx, x[u]);
+                for (int u = 0; u < 4; u++) x[u] = (bits >> (i + u)) & 1u ? x[u] : -INFINITY;
+              }
+              mx = fmaxf(mx, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
             }
           }
           asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(to), "r"(__float_as_uint(mx)) : "memory");
@@ -393,37 +399,50 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
           for (int q = 0; q < 4; q++) pc_st16(ts + 16 * q, z);
         } else {
           // ---- weights: 16 keys of S become 8 columns of their hi pieces and 8 of their lo pieces
-          auto weights = [&](auto some) {
+          auto weights = [&](auto some, int q, unsigned bits) {
+            unsigned s[16], w[16];
+            pc_ld16(ts + 16 * q, s);
+            pc_wait_ld();
 #pragma unroll
-            for (int q = 0; q < 4; q++) {
-              unsigned s[16], w[16];
-              pc_ld16(ts + 16 * q, s);
-              pc_wait_ld();
+            for (int i = 0; i < 16; i += 4) {
+              const uint4 k4 = lds128(kk + 64 * q + 4 * i), f4 = lds128(fv + 64 * q + 4 * i);
 #pragma unroll
-              for (int i = 0; i < 16; i += 4) {
-                const uint4 k4 = lds128(kk + 4 * (16 * q + i)), f4 = lds128(fv + 4 * (16 * q + i));
-#pragma unroll
-                for (int u = 0; u < 4; u += 2) {
-                  const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[i + u]), __uint_as_float(s[i + u + 1])),
-                                              u ? make_float2(__uint_as_float(k4.z), __uint_as_float(k4.w)) : make_float2(__uint_as_float(k4.x), __uint_as_float(k4.y)), off);
-                  float2 p = make_float2(pa_ex2(x.x), pa_ex2(x.y));
-                  float2 pf = __fmul2_rn(p, u ? make_float2(__uint_as_float(f4.z), __uint_as_float(f4.w)) : make_float2(__uint_as_float(f4.x), __uint_as_float(f4.y)));
-                  if constexpr (decltype(some)::value) {
-                    const unsigned bits = see[q >> 1] >> (16 * (q & 1) + i + u);
-                    p = make_float2(bits & 1u ? p.x : 0.f, bits & 2u ? p.y : 0.f);
-                    pf = make_float2(bits & 1u ? pf.x : 0.f, bits & 2u ? pf.y : 0.f);
-                  }
-                  l2 = __fadd2_rn(l2, p);
-                  const unsigned h = pa_pack(pf.x, pf.y);
-                  const float2 lo_ = __ffma2_rn(pa_unpack(h), make_float2(-1.f, -1.f), pf);
-                  w[(i + u) / 2] = h;
-                  w[8 + (i + u) / 2] = pa_pack(lo_.x, lo_.y);
+              for (int u = 0; u < 4; u += 2) {
+                const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[i + u]), __uint_as_float(s[i + u + 1])),
+                                            u ? make_float2(__uint_as_float(k4.z), __uint_as_float(k4.w)) : make_float2(__uint_as_float(k4.x), __uint_as_float(k4.y)), off);
+                float2 p = make_float2(pa_ex2(x.x), pa_ex2(x.y));
+                float2 pf = __fmul2_rn(p, u ? make_float2(__uint_as_float(f4.z), __uint_as_float(f4.w)) : make_float2(__uint_as_float(f4.x), __uint_as_float(f4.y)));
+                if constexpr (decltype(some)::value) {
+                  const bool a = (bits >> (i + u)) & 1u, b = (bits >> (i + u + 1)) & 1u;
+                  p = make_float2(a ? p.x : 0.f, b ? p.y : 0.f);
+                  pf = make_float2(a ? pf.x : 0.f, b ? pf.y : 0.f);
                 }
+                l2 = __fadd2_rn(l2, p);
+                const unsigned h = pa_pack(pf.x, pf.y);
+                const float2 lo_ = __ffma2_rn(pa_unpack(h), make_float2(-1.f, -1.f), pf);
+                w[(i + u) / 2] = h;
+                w[8 + (i + u) / 2] = pa_pack(lo_.x, lo_.y);
               }
-              pc_st16(ts + 16 * q, w);
             }
+            pc_st16(ts + 16 * q, w);
           };
-          if (masked) weights(std::true_type()); else weights(std::false_type());
+          if (!masked) {
+#pragma unroll
+            for (int q = 0; q < 4; q++) weights(std::false_type(), q, 0u);
+          } else {
+#pragma unroll 1
+            for (int q = 0; q < 4; q++) {
+              const unsigned bits = ((q < 2 ? see[0] : see[1]) >> (16 * (q & 1))) & 0xffffu;
+              if (!__any_sync(0xffffffffu, bits)) {
+                unsigned z[16];
+#pragma unroll
+                for (int i = 0; i < 16; i++) z[i] = 0u;
+                pc_st16(ts + 16 * q, z);
+              } else {
+                weights(std::true_type(), q, bits);
+              }
+            }
+          }
         }
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         pc_fence_before();
@@ -527,21 +546,39 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
         for (int t = 0; t < nt; t++) scores(t, 0);
         release(0);
       }
-      for (int j = 0; j < n && ok; j++) {
-        const int ev = 2 * j + 1, ek = 2 * j + 2;
-        if (!wait(full(ev % STAGES), ev / STAGES, 711)) break;
-        for (int t = 0; t < nt && ok; t++) {
-          if (!wait(p_full(t), j, 712 + t)) break;
-          pc_fence_after();
-          values(t, ev);
-          if (t == nt - 1) release(ev);
-          if (j + 1 < n) {
-            if (t == 0 && !wait(full(ek % STAGES), ek / STAGES, 714)) break;
+      // From then on whatever is ready first: a tile's values of step pv[t] when its weights and V are there, its scores of the next
+      // step, which overwrite those weights, after that when K is. In a fixed order the pipe waited for K with another tile's
+      // weights at hand.
+      int pv[2] = {0, 0}, qk[2] = {1, 1};
+      auto ready = [&](unsigned bar, int use) {
+        unsigned yes;
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(yes) : "r"(bar), "r"(use & 1) : "memory");
+        return __any_sync(0xffffffffu, yes) != 0;
+      };
+      unsigned idle = 0;
+      while (ok && (pv[0] < n || (nt == 2 && pv[1] < n))) {
+        bool did = false;
+        for (int t = 0; t < nt; t++) {
+          if (pv[t] < n && pv[t] < qk[t] && ready(full((2 * pv[t] + 1) % STAGES), (2 * pv[t] + 1) / STAGES) && ready(p_full(t), pv[t])) {
             pc_fence_after();
-            scores(t, ek);
-            if (t == nt - 1) release(ek);
+            const int e = 2 * pv[t] + 1;
+            values(t, e);
+            pv[t]++;
+            if (nt == 1 || pv[t ^ 1] >= pv[t]) release(e);               // the other tile has used it, too
+            did = true;
+          }
+          if (qk[t] < n && pv[t] >= qk[t] && ready(full(2 * qk[t] % STAGES), 2 * qk[t] / STAGES)) {
+            pc_fence_after();
+            const int e = 2 * qk[t];
+            scores(t, e);
+            qk[t]++;
+            if (nt == 1 || qk[t ^ 1] >= qk[t]) release(e);
+            did = true;
           }
         }
+        idle = did ? 0 : idle + 1;
+        if (idle > PC_SPIN) { if (leader) fail(711); ok = false; }
+        if ((idle & 255) == 255 && __any_sync(0xffffffffu, dead())) ok = false;
       }
       if (!ok) {                                                         // what was issued has to end before tensor memory is given back
         if (leader) pc_commit(done);
@@ -592,7 +629,6 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
         const int left = at < 0 ? 0 : k1 - (k0 + j * PC_N + 16 * g) - lr;          // the lane's rows 0, STEP, .. below this exist
         const unsigned char* block = c.g.pool + (at < 0 ? 0 : at);
         const unsigned char* src = block + (is_v ? page * code : 0) + slot * code + (BITS == 4 ? 8 : 16) * x;
-        const int sub = (is_v ? c.g.vsub : c.g.ksub) + slot * n16 + x;
 #pragma unroll
         for (int i = 0; i < PER; i++) {
           const bool on = mine && STEP * i < left;
@@ -604,11 +640,13 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
           } else if constexpr (BITS == 8) {
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(raw + ((g * PER + i) * 32 + lane) * 16), "l"(s), "r"(on ? 16 : 0) : "memory");
           } else {
-            const int w = (sub + STEP * i * n16) & ~3;
             asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(raw + ((g * PER + i) * 32 + lane) * 8), "l"(s), "r"(on ? 8 : 0) : "memory");
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(raw + 8 * PER * 256 + ((g * PER + i) * 32 + lane) * 4), "l"(block + (on ? w : 0)), "r"(on ? 4 : 0) : "memory");
           }
         }
+        // the group's sub-scales, 16 n16 bytes; the warp shares them
+        if (BITS == 4 && lane < n16)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(raw + 8 * PER * 256 + g * 128 + 16 * lane),
+                       "l"(block + (at < 0 ? 0 : (is_v ? c.g.vsub : c.g.ksub) + (slot - lr) * n16 + 16 * lane)), "r"(at < 0 ? 0 : 16) : "memory");
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -618,24 +656,30 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
       const unsigned stage = smem_u32(s_kv) + (e % STAGES) * STAGE, raw = smem_u32(s_raw) + (e & 1) * S::RAW;
       const bool turned = (x >> 2) & 1;
       for (int g = pw; g < 8; g += PC_PRODUCERS) {
+        // all of a group's loads before the first store: the compiler may not move them past it
+        unsigned c4[PER][BITS == 8 ? 4 : 2], sc[PER];
 #pragma unroll
         for (int i = 0; i < PER; i++) {
-          const int r15 = lr + STEP * i, r = 16 * g + r15;
-          unsigned v[8];
           if constexpr (BITS == 8) {
             const uint4 q = lds128(raw + ((g * PER + i) * 32 + lane) * 16);
-            const unsigned w[4] = {(turned ? q.z : q.x) ^ 0x80808080u, (turned ? q.w : q.y) ^ 0x80808080u, (turned ? q.x : q.z) ^ 0x80808080u, (turned ? q.y : q.w) ^ 0x80808080u};
-#pragma unroll
-            for (int k = 0; k < 4; k++) { v[2 * k] = pa_bytes<0x4140>(w[k]); v[2 * k + 1] = pa_bytes<0x4342>(w[k]); }
+            c4[i][0] = turned ? q.z : q.x; c4[i][1] = turned ? q.w : q.y; c4[i][BITS == 8 ? 2 : 0] = turned ? q.x : q.z; c4[i][BITS == 8 ? 3 : 1] = turned ? q.y : q.w;
           } else {
             const uint2 q = lds64(raw + ((g * PER + i) * 32 + lane) * 8);
-            const unsigned word = lds32(raw + 8 * PER * 256 + ((g * PER + i) * 32 + lane) * 4);
-            // which byte of the word: a block, its parts and 16 slots' sub-scales start on 16-byte boundaries, and k0 is a multiple of 16
-            const unsigned sc = (word >> (8 * ((r15 * n16 + x) & 3))) & 255u;
-            const PaSub t2 = pa_pair(sc, sc);
-            const unsigned w[2] = {turned ? q.y : q.x, turned ? q.x : q.y};
+            c4[i][0] = turned ? q.y : q.x; c4[i][1] = turned ? q.x : q.y;
+            asm volatile("ld.shared.u8 %0, [%1];" : "=r"(sc[i]) : "r"(raw + 8 * PER * 256 + g * 128 + (lr + STEP * i) * n16 + x));
+          }
+        }
 #pragma unroll
-            for (int k = 0; k < 8; k++) v[k] = pa_nibbles(w[k >> 2], k & 3, t2);
+        for (int i = 0; i < PER; i++) {
+          const int r = 16 * g + lr + STEP * i;
+          unsigned v[8];
+          if constexpr (BITS == 8) {
+#pragma unroll
+            for (int k = 0; k < 4; k++) { const unsigned w = c4[i][k] ^ 0x80808080u; v[2 * k] = pa_bytes<0x4140>(w); v[2 * k + 1] = pa_bytes<0x4342>(w); }
+          } else {
+            const PaSub t2 = pa_pair(sc[i], sc[i]);
+#pragma unroll
+            for (int k = 0; k < 8; k++) v[k] = pa_nibbles(c4[i][k >> 2], k & 3, t2, c.one);
           }
           const unsigned to = stage + (x >> 2) * PC_N * 128 + r * 128 + ((((2 * x + turned) & 7) ^ (r & 7)) << 4);
           asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]) : "memory");
@@ -673,7 +717,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
       if (lane == 0) {
         M.beta[ms] = __uint_as_float((unsigned)(127 + emax) << 23);
         M.kmax[ms] = kmax;
-        M.flags[ms] = (have != ~0u ? 1u : 0u) | (emin < emax - 10 ? 2u : 0u);
+        M.flags[ms] = (have != ~0u ? 1u : 0u) | (emin < emax - 8 ? 2u : 0u);
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(m_full(ms));
@@ -699,13 +743,13 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
     if constexpr (BITS == 16) {
       ahead(0);
       if (pw == 0) meta(0);
+      ahead(1);
       for (int e = 0; e < 2 * n && ok; e++) {
-        if (!(e & 1) && e > 0 && pw == 0) { const int j = e >> 1; if (j >= 2 && !wait(m_empty(j & 1), (j >> 1) - 1, 721)) break; meta(j); }
-        // one element further is on its way while this one is waited for
-        if (e + 1 < 2 * n) { if (!room(e + 1)) break; }
-        ahead(e + 1);
         asm volatile("cp.async.wait_group 1;" ::: "memory");
         arrive(e);
+        if ((e & 1) && e + 1 < 2 * n && pw == 0) { const int j = (e + 1) >> 1; if (j >= 2 && !wait(m_empty(j & 1), (j >> 1) - 1, 721)) break; meta(j); }
+        if (e + 2 < 2 * n && !room(e + 2)) break;
+        ahead(e + 2);
       }
     } else {
       ahead(0);
@@ -713,6 +757,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
       ahead(1);
       for (int e = 0; e < 2 * n && ok; e++) {
         asm volatile("cp.async.wait_group 1;" ::: "memory");
+        __syncwarp();
         if (!room(e)) break;
         convert(e);
         arrive(e);

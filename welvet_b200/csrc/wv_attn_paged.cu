@@ -103,6 +103,7 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gl = lane >> 2, cl = lane & 3;
   unsigned char* ring = pr_smem + warp * NST * S::STAGE;
   if (tid == 0) s_qmax = 0;
+  const unsigned one = c.one;
   const int hd = EXACT ? DP : c.g.hd, n16 = hd / 16, code = EXACT ? RB : c.g.code;
   if (!EXACT) {                                                          // what lies beyond the head stays zero
     for (int i = tid * 16; i < PR_WARPS * NST * S::STAGE; i += 32 * PR_WARPS * 16) *reinterpret_cast<uint4*>(pr_smem + i) = make_uint4(0, 0, 0, 0);
@@ -310,8 +311,8 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
         const uint2 w = lds64(sa + kofs[0] + n * 8 * RB);
         const unsigned t1 = sc[128 + r * n16 + min(cl, n16 - 1)];
         const PaSub t = pa_pair(t1, t1);
-        step(0, pa_nibbles(w.x, 0, t), pa_nibbles(w.x, 1, t)); step(1, pa_nibbles(w.x, 2, t), pa_nibbles(w.x, 3, t));
-        step(2, pa_nibbles(w.y, 0, t), pa_nibbles(w.y, 1, t)); step(3, pa_nibbles(w.y, 2, t), pa_nibbles(w.y, 3, t));
+        step(0, pa_nibbles(w.x, 0, t, one), pa_nibbles(w.x, 1, t, one)); step(1, pa_nibbles(w.x, 2, t, one), pa_nibbles(w.x, 3, t, one));
+        step(2, pa_nibbles(w.y, 0, t, one), pa_nibbles(w.y, 1, t, one)); step(3, pa_nibbles(w.y, 2, t, one), pa_nibbles(w.y, 3, t, one));
       } else {
 #pragma unroll
         for (int i = 0; i < RB / 64; i++) {
@@ -334,8 +335,8 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
             const PaSub t2[2] = {pa_pair(ta, ta), pa_pair(tb, tb)};
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-              step(8 * i + 2 * j, pa_nibbles(w[j], 0, t2[j >> 1]), pa_nibbles(w[j], 1, t2[j >> 1]));
-              step(8 * i + 2 * j + 1, pa_nibbles(w[j], 2, t2[j >> 1]), pa_nibbles(w[j], 3, t2[j >> 1]));
+              step(8 * i + 2 * j, pa_nibbles(w[j], 0, t2[j >> 1], one), pa_nibbles(w[j], 1, t2[j >> 1], one));
+              step(8 * i + 2 * j + 1, pa_nibbles(w[j], 2, t2[j >> 1], one), pa_nibbles(w[j], 3, t2[j >> 1], one));
             }
           }
         }
@@ -504,7 +505,7 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
         for (int hf = 0; hf < 2; hf++) {
           const unsigned x = __byte_perm(v[0][w], v[1][w], hf ? 0x7632 : 0x5410), z = __byte_perm(v[2][w], v[3][w], hf ? 0x7632 : 0x5410);
 #pragma unroll
-          for (int j = 0; j < 4; j++) put(8 * w + 4 * hf + j, pa_nibbles(x, j, ta), pa_nibbles(z, j, tb));
+          for (int j = 0; j < 4; j++) put(8 * w + 4 * hf + j, pa_nibbles(x, j, ta, one), pa_nibbles(z, j, tb, one));
         }
       }
     }
@@ -662,6 +663,7 @@ int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* d
   c.heads = heads; c.group = heads / c.g.kvh;
   c.scale = scale * 1.4426950408889634f;
   c.window = window;
+  c.one = 0x3c003c00u;
   c.err = wv_paged_err_ptr();
   // Up to 32 rows (tokens x query heads of a kv head) a sequence is taken 8 or 16 rows at a time, beyond in tiles of 128.
   const long long most = (long long)b.max_q * c.group;

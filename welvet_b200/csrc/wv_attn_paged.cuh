@@ -17,6 +17,7 @@ struct PaCall {
   int heads, group;                // query heads, and those of one kv head
   float scale;                     // times log2(e)
   int window;                      // 0: none
+  unsigned one;                    // 0x3c003c00, for pa_nibbles
   int rows_most;                   // sequences with more rows (tokens x group) than this go to the chunk kernel
   int nsplit, per;                 // splits of a sequence's keys, keys of a split (a multiple of 16; of 128 for chunks)
   float2* ml;                      // split results [row][nsplit]: {M, divisor}; {-inf, 0} and no sums for a split without keys
@@ -43,10 +44,11 @@ __device__ __forceinline__ unsigned pa_mul2(unsigned v, unsigned m) {
 // The low two (SEL 0x4140) or high two (0x4342) bytes of w, biased by 128, as signed values.
 template <unsigned SEL> __device__ __forceinline__ unsigned pa_bytes(unsigned w) { return pa_sub2(__byte_perm(w, 0x64646464u, SEL), 0x64806480u); }
 // Nibbles j and j + 4 of w, biased by 8, times the sub-scales t (a pair of float16): the nibble n in the upper mantissa of 1 is
-// 1 + n / 16, and (1 + n / 16) 16 t - 24 t = (n - 8) t is exact in one instruction.
+// 1 + n / 16, and (1 + n / 16) 16 t - 24 t = (n - 8) t is exact in one instruction. `one` is that 1 twice, PaCall::one: a constant that
+// the compiler cannot see, so that it masks and merges in one instruction with it in a register.
 struct PaSub { unsigned a, b; };
-__device__ __forceinline__ unsigned pa_nibbles(unsigned w, int j, const PaSub& t) {
-  const unsigned s = j == 0 ? w << 6 : j == 1 ? w << 2 : j == 2 ? w >> 2 : w >> 6, x = (s & 0x03c003c0u) | 0x3c003c00u;
+__device__ __forceinline__ unsigned pa_nibbles(unsigned w, int j, const PaSub& t, unsigned one) {
+  const unsigned s = j == 0 ? w << 6 : j == 1 ? w << 2 : j == 2 ? w >> 2 : w >> 6, x = (s & 0x03c003c0u) | one;
   const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&t.a), *reinterpret_cast<const __half2*>(&t.b));
   return *reinterpret_cast<const unsigned*>(&r);
 }
