@@ -56,9 +56,8 @@ struct SmpArgs {
   const float* temperature; const int* top_k; const float* top_p; const float* min_p; const double* u;
   int* index; float* prob;
 };
-// Four neighbouring bins of a thread: counts and weights up to and including each.
-struct SmpScan { unsigned c[4], c0; u64 w[4], w0; };
-struct SmpSel { int bin; unsigned before, count; u64 weight_before; };
+// A bin, what comes before it (counts and weight), and its count.
+struct SmpSel { int bin; unsigned before, count, pad; u64 weight_before; };
 
 struct __align__(16) SmpShared {
   union {
@@ -66,11 +65,12 @@ struct __align__(16) SmpShared {
     u64 run[SMP_LIST];                     // afterwards: the list's running weights
   };
   u64 list[SMP_LIST];
-  u64 part[SMP_WARPS];
-  unsigned partc[SMP_WARPS];
+  u64 part[SMP_WARPS], tot_w[SMP_CLUSTER];
+  unsigned partc[SMP_WARPS], tot_c[SMP_CLUSTER];
   u64 best, least_sum, result_word, result_cum;
-  SmpSel sel;
-  unsigned filled;
+  SmpSel sel[2];
+  unsigned filled, turn;
+  int place;
 };
 
 __device__ __forceinline__ int smp_bin(float y, float top) {
@@ -78,19 +78,38 @@ __device__ __forceinline__ int smp_bin(float y, float top) {
   return min((int)(__fsub_rn(top, y) * 64.f), SMP_BINS - 1);             // rises as y falls: each step rounds monotonously
 }
 
-// Sums of the bins over the cluster and their running totals. Ends with every CTA past its reads of the others' bins.
-__device__ __forceinline__ void smp_scan(cg::cluster_group& cluster, SmpShared& S, SmpScan& r) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, ncta = (int)cluster.num_blocks();
-  unsigned c[4] = {0, 0, 0, 0};
-  u64 w[4] = {0, 0, 0, 0};
-  for (int q = 0; q < ncta; q++) {
-    const SmpShared* o = cluster.map_shared_rank(&S, q);
-    const uint4 a = reinterpret_cast<const uint4*>(o->hist[0])[tid], l = reinterpret_cast<const uint4*>(o->hist[1])[tid], h = reinterpret_cast<const uint4*>(o->hist[2])[tid];
-    c[0] += a.x; c[1] += a.y; c[2] += a.z; c[3] += a.w;
-    w[0] += l.x + ((u64)h.x << 16); w[1] += l.y + ((u64)h.y << 16); w[2] += l.z + ((u64)h.z << 16); w[3] += l.w + ((u64)h.w << 16);
+// A CTA adds up its share of the bins over the cluster, the shares' totals go to every CTA, and a place is announced by the CTA whose
+// share it is in: reading all bins of all CTAs everywhere (196 KB over distributed shared memory) took 10 us a row.
+template <int NCTA> struct SmpScan {
+  static constexpr int SHARE = SMP_BINS / NCTA, NB = SHARE > SMP_THREADS ? SHARE / SMP_THREADS : 1;
+  unsigned c0, c[NB];                      // counts before the thread's bins, and up to and including each
+  u64 w0, w[NB];
+  unsigned count;
+  u64 all;
+};
+template <int NCTA>
+__device__ __forceinline__ void smp_scan(cg::cluster_group& cluster, SmpShared& S, SmpScan<NCTA>& r) {
+  using R = SmpScan<NCTA>;
+  constexpr int NB = R::NB;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, rank = NCTA == 1 ? 0 : (int)cluster.block_rank();
+  const bool on = tid * NB < R::SHARE;
+  unsigned c[NB];
+  u64 w[NB];
+#pragma unroll
+  for (int i = 0; i < NB; i++) { c[i] = 0; w[i] = 0; }
+  if (on) {
+    const int b0 = rank * R::SHARE + tid * NB;
+#pragma unroll
+    for (int q = 0; q < NCTA; q++) {
+      const SmpShared* o = NCTA == 1 ? &S : cluster.map_shared_rank(&S, q);
+#pragma unroll
+      for (int i = 0; i < NB; i++) { c[i] += o->hist[0][b0 + i]; w[i] += o->hist[1][b0 + i] + ((u64)o->hist[2][b0 + i] << 16); }
+    }
   }
-  unsigned ct = c[0] + c[1] + c[2] + c[3];
-  u64 wt = w[0] + w[1] + w[2] + w[3];
+  unsigned ct = 0;
+  u64 wt = 0;
+#pragma unroll
+  for (int i = 0; i < NB; i++) { ct += c[i]; wt += w[i]; }
   const unsigned c_own = ct;
   const u64 w_own = wt;
 #pragma unroll
@@ -101,51 +120,83 @@ __device__ __forceinline__ void smp_scan(cg::cluster_group& cluster, SmpShared& 
   }
   if (lane == 31) { S.partc[warp] = ct; S.part[warp] = wt; }
   __syncthreads();
-  for (int q = 0; q < warp; q++) { ct += S.partc[q]; wt += S.part[q]; }
-  r.c0 = ct - c_own; r.w0 = wt - w_own;
+  unsigned tc = 0;
+  u64 tw = 0;
+#pragma unroll
+  for (int q = 0; q < SMP_WARPS; q++) {
+    if (q == warp) { ct += tc; wt += tw; }
+    tc += S.partc[q]; tw += S.part[q];
+  }
+  if (tid < NCTA) {
+    SmpShared* o = NCTA == 1 ? &S : cluster.map_shared_rank(&S, tid);
+    o->tot_c[rank] = tc; o->tot_w[rank] = tw;
+  }
+  if (NCTA == 1) __syncthreads(); else cluster.sync();                   // and every CTA is past its reads of the others' bins
+  unsigned cb = 0;
+  u64 wb = 0;
+  r.count = 0; r.all = 0;
+#pragma unroll
+  for (int q = 0; q < NCTA; q++) { if (q < rank) { cb += S.tot_c[q]; wb += S.tot_w[q]; } r.count += S.tot_c[q]; r.all += S.tot_w[q]; }
+  r.c0 = cb + ct - c_own; r.w0 = wb + wt - w_own;
   unsigned a = r.c0;
   u64 b = r.w0;
 #pragma unroll
-  for (int i = 0; i < 4; i++) { a += c[i]; b += w[i]; r.c[i] = a; r.w[i] = b; }
-  cluster.sync();
+  for (int i = 0; i < NB; i++) { a += c[i]; b += w[i]; r.c[i] = a; r.w[i] = b; }
 }
 // The bin in which the running count (or weight) reaches target.
-__device__ __forceinline__ SmpSel smp_select(SmpShared& S, const SmpScan& r, bool by_weight, u64 target) {
+template <int NCTA>
+__device__ __forceinline__ SmpSel smp_select(cg::cluster_group& cluster, SmpShared& S, const SmpScan<NCTA>& r, bool by_weight, u64 target, int& turn) {
+  using R = SmpScan<NCTA>;
+  const int rank = NCTA == 1 ? 0 : (int)cluster.block_rank();
   unsigned cb = r.c0;
   u64 wb = r.w0;
+  turn ^= 1;                               // the place of the select before this one may still be read
 #pragma unroll
-  for (int i = 0; i < 4; i++) {
-    if (by_weight ? (wb < target && r.w[i] >= target) : (cb < target && r.c[i] >= target)) S.sel = SmpSel{4 * (int)threadIdx.x + i, cb, r.c[i] - cb, wb};
+  for (int i = 0; i < R::NB; i++) {
+    if (by_weight ? (wb < target && r.w[i] >= target) : (cb < target && r.c[i] >= target)) {
+      const SmpSel s{rank * R::SHARE + (int)threadIdx.x * R::NB + i, cb, r.c[i] - cb, 0u, wb};
+#pragma unroll
+      for (int q = 0; q < NCTA; q++) (NCTA == 1 ? &S : cluster.map_shared_rank(&S, q))->sel[turn] = s;
+    }
     cb = r.c[i]; wb = r.w[i];
   }
-  __syncthreads();
-  const SmpSel s = S.sel;
-  __syncthreads();
-  return s;
+  if (NCTA == 1) __syncthreads(); else cluster.sync();
+  return S.sel[turn];
 }
-// The first cnt words of the list from the largest down, and their running weights.
+// The first cnt words of the list from the largest down, and their running weights. Up to 256 of them each find their own rank.
 __device__ __forceinline__ void smp_sort(SmpShared& S, int cnt, float top) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  int p2 = 1;
-  while (p2 < cnt) p2 <<= 1;
-  for (int i = cnt + tid; i < p2; i += SMP_THREADS) S.list[i] = 0ull;
-  __syncthreads();
-  for (int size = 2; size <= p2; size <<= 1)
-    for (int stride = size >> 1; stride > 0; stride >>= 1) {
-      for (int i = tid; i < p2 / 2; i += SMP_THREADS) {
-        const int a = 2 * i - (i & (stride - 1)), b = a + stride;
-        const u64 x = S.list[a], y = S.list[b];
-        if (((a & size) == 0) ? (x < y) : (x > y)) { S.list[a] = y; S.list[b] = x; }
-      }
-      // steps of up to 32 stay within the 64 words of a warp
-      const int next = stride > 1 ? stride >> 1 : size;
-      if (stride > 32 || next > 32 || p2 > 2 * SMP_THREADS) __syncthreads(); else __syncwarp();
+  if (cnt <= 256) {
+    const u64 mine = tid < cnt ? S.list[tid] : 0ull;
+    int at = 0;
+    if (warp * 32 < cnt) {
+#pragma unroll 4
+      for (int j = 0; j < cnt; j++) at += S.list[j] > mine ? 1 : 0;
     }
+    __syncthreads();
+    if (tid < cnt) S.list[at] = mine;
+  } else {
+    int p2 = 512;
+    while (p2 < cnt) p2 <<= 1;
+    for (int i = cnt + tid; i < p2; i += SMP_THREADS) S.list[i] = 0ull;
+    __syncthreads();
+    for (int size = 2; size <= p2; size <<= 1)
+      for (int stride = size >> 1; stride > 0; stride >>= 1) {
+        for (int i = tid; i < p2 / 2; i += SMP_THREADS) {
+          const int a = 2 * i - (i & (stride - 1)), b = a + stride;
+          const u64 x = S.list[a], y = S.list[b];
+          if (((a & size) == 0) ? (x < y) : (x > y)) { S.list[a] = y; S.list[b] = x; }
+        }
+        // steps of up to 32 stay within the 64 words of a warp
+        const int next = stride > 1 ? stride >> 1 : size;
+        if (stride > 32 || next > 32 || p2 > 2 * SMP_THREADS) __syncthreads(); else __syncwarp();
+      }
+  }
   __syncthreads();
   constexpr int PER = SMP_LIST / SMP_THREADS;
   u64 v[PER], t = 0;
 #pragma unroll
-  for (int i = 0; i < PER; i++) { const int q = PER * tid + i; t += q < cnt ? smp_units(smp_weight(smp_value(S.list[q]), top)) : 0u; v[i] = t; }
+  for (int i = 0; i < PER; i++) { const int q = PER * tid + i; if (q < cnt) t += smp_units(smp_weight(smp_value(S.list[q]), top)); v[i] = t; }
   u64 s = t;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) { const u64 b = __shfl_up_sync(0xffffffffu, s, o); if (lane >= o) s += b; }
@@ -157,46 +208,79 @@ __device__ __forceinline__ void smp_sort(SmpShared& S, int cnt, float top) {
   __syncthreads();
 }
 // The place in S.run[0 .. cnt) (rising) where the running weight reaches target; the last place if it does not.
-__device__ __forceinline__ int smp_place(const SmpShared& S, int cnt, u64 target) {
-  int lo = 0, hi = cnt - 1;
-  while (lo < hi) { const int m = (lo + hi) >> 1; if (S.run[m] >= target) hi = m; else lo = m + 1; }
-  return lo;
+__device__ __forceinline__ int smp_place(SmpShared& S, int cnt, u64 target) {
+  if (threadIdx.x == 0) S.place = cnt - 1;
+  __syncthreads();
+  constexpr int PER = SMP_LIST / SMP_THREADS;
+#pragma unroll
+  for (int i = 0; i < PER; i++) {
+    const int q = PER * (int)threadIdx.x + i;
+    if (q < cnt && S.run[q] >= target && (q == 0 || S.run[q - 1] < target)) S.place = q;
+  }
+  __syncthreads();
+  const int at = S.place;
+  __syncthreads();
+  return at;
 }
 
+template <int NCTA>
 __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const SmpArgs A, int per) {
   extern __shared__ __align__(16) unsigned char smp_smem[];
   SmpShared& S = *reinterpret_cast<SmpShared*>(smp_smem);
   float* s_y = reinterpret_cast<float*>(smp_smem + sizeof(SmpShared));
   cg::cluster_group cluster = cg::this_cluster();
-  const int ncta = (int)cluster.num_blocks(), rank = (int)cluster.block_rank(), row = blockIdx.x / ncta;
+  const int rank = NCTA == 1 ? 0 : (int)cluster.block_rank(), row = blockIdx.x / NCTA;
   const int tid = threadIdx.x, lane = tid & 31;
   const int i0 = min(A.n, rank * per), mine = min(A.n - i0, per);
+  auto all_sync = [&]() { if (NCTA == 1) __syncthreads(); else cluster.sync(); };
+  auto other = [&](int q) { return NCTA == 1 ? &S : cluster.map_shared_rank(&S, q); };
   for (int i = tid; i < 3 * SMP_BINS; i += SMP_THREADS) S.hist[0][i] = 0u;
   if (tid == 0) { S.best = 0ull; S.least_sum = 0ull; S.filled = 0u; }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const float* x = A.logits + (size_t)row * A.ld + i0;
   const float t = A.temperature[row];
   const int k = A.top_k[row];
   const bool greedy = t <= 0.f || k == 1;
   const float least = A.min_p[row];
   const double tp = (double)A.top_p[row], u = A.u[row];
-  const float* x = A.logits + (size_t)row * A.ld + i0;
   __syncthreads();
   // ---- the row's logits / T into shared memory, and the largest word
   {
     float best = -INFINITY;
     int at = -1;
-    for (int b = tid; b < mine; b += 8 * SMP_THREADS) {
-      float v[8];
+    auto take = [&](float v, int i) {
+      const float y = smp_y(v, t, greedy);
+      if (y > best || (y == best && at < 0)) { best = y; at = i; }       // a thread's places rise: the first of equals
+      return y;
+    };
+    if ((reinterpret_cast<uintptr_t>(x) & 15) == 0 && (per & 3) == 0) {  // i0 is a multiple of per
+      constexpr int U = 8;
+      const int n4 = mine >> 2;
+      for (int b = tid; b < n4; b += U * SMP_THREADS) {
+        float4 v[U];
 #pragma unroll
-      for (int q = 0; q < 8; q++) v[q] = b + q * SMP_THREADS < mine ? x[b + q * SMP_THREADS] : NAN;
+        for (int q = 0; q < U; q++) if (b + q * SMP_THREADS < n4) v[q] = __ldcs(reinterpret_cast<const float4*>(x) + b + q * SMP_THREADS);
 #pragma unroll
-      for (int q = 0; q < 8; q++) {
-        const int i = b + q * SMP_THREADS;
-        if (i >= mine) break;
-        const float y = smp_y(v[q], t, greedy);
-        s_y[i] = y;
-        if (y > best || (y == best && at < 0)) { best = y; at = i; }     // a thread's places rise: the first of equals
+        for (int q = 0; q < U; q++) {
+          const int i = 4 * (b + q * SMP_THREADS);
+          if (i >= 4 * n4) break;
+          const float y0 = take(v[q].x, i), y1 = take(v[q].y, i + 1), y2 = take(v[q].z, i + 2), y3 = take(v[q].w, i + 3);
+          *reinterpret_cast<float4*>(s_y + i) = make_float4(y0, y1, y2, y3);
+        }
+      }
+      if (tid < (mine & 3)) { const int i = 4 * n4 + tid; s_y[i] = take(x[i], i); }
+    } else {
+      for (int b = tid; b < mine; b += 16 * SMP_THREADS) {
+        float v[16];
+#pragma unroll
+        for (int q = 0; q < 16; q++) v[q] = b + q * SMP_THREADS < mine ? __ldcs(x + b + q * SMP_THREADS) : NAN;
+#pragma unroll
+        for (int q = 0; q < 16; q++) {
+          const int i = b + q * SMP_THREADS;
+          if (i >= mine) break;
+          s_y[i] = take(v[q], i);
+        }
       }
     }
     u64 w = at < 0 ? 0ull : smp_word(best, i0 + at);
@@ -204,61 +288,73 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const SmpAr
     for (int o = 16; o; o >>= 1) w = max(w, __shfl_xor_sync(0xffffffffu, w, o));
     if (lane == 0 && w) atomicMax(&S.best, w);
   }
-  cluster.sync();
+  all_sync();
   u64 best = 0ull;
-  for (int q = 0; q < ncta; q++) best = max(best, cluster.map_shared_rank(&S, q)->best);
+#pragma unroll
+  for (int q = 0; q < NCTA; q++) best = max(best, other(q)->best);
   const float top = smp_value(best);
   if (best == 0ull || greedy) {
     if (rank == 0 && tid == 0) { A.index[row] = best ? smp_index(best) : -1; if (A.prob) A.prob[row] = best ? 1.f : 0.f; }
-    cluster.sync();                        // nobody leaves while its shared memory may be read
+    all_sync();                            // nobody leaves while its shared memory may be read
     return;
   }
-  // ---- counts and weights of the bins, and the weight that min-p leaves
-  {
+  // ---- counts and weights of the bins, and the weight that min-p leaves. Up to 1024 of top-k need the counts alone: the weights of
+  // those candidates are taken when they have been sorted.
+  auto bins = [&](bool weights) {
     u64 ms = 0ull;
     for (int i = tid; i < mine; i += SMP_THREADS) {
       const float y = s_y[i];
       if (y != y) continue;
-      const float f = smp_weight(y, top);
-      const unsigned w = smp_units(f);
       const int b = smp_bin(y, top);
       atomicAdd(&S.hist[0][b], 1u);
-      if (w) { atomicAdd(&S.hist[1][b], w & 0xffffu); atomicAdd(&S.hist[2][b], w >> 16); }
-      if (f >= least) ms += w;
+      if (weights) {
+        const float f = smp_weight(y, top);
+        const unsigned w = smp_units(f);
+        if (w) { atomicAdd(&S.hist[1][b], w & 0xffffu); atomicAdd(&S.hist[2][b], w >> 16); }
+        if (f >= least) ms += w;
+      }
     }
+    if (weights) {
 #pragma unroll
-    for (int o = 16; o; o >>= 1) ms += __shfl_xor_sync(0xffffffffu, ms, o);
-    if (lane == 0 && ms) atomicAdd(&S.least_sum, ms);
-  }
-  cluster.sync();
+      for (int o = 16; o; o >>= 1) ms += __shfl_xor_sync(0xffffffffu, ms, o);
+      if (lane == 0 && ms) atomicAdd(&S.least_sum, ms);
+    }
+    all_sync();
+  };
+  int turn = 0;
+  SmpScan<NCTA> scan;
+  const bool few = k > 0 && k <= SMP_LIST / 2;
+  bins(!few);
+  smp_scan<NCTA>(cluster, S, scan);
+  const bool cut_k = k > 0 && (unsigned)k < scan.count, cut_p = !(tp >= 1.0);
   u64 wmin = 0ull;
-  for (int q = 0; q < ncta; q++) wmin += cluster.map_shared_rank(&S, q)->least_sum;
-  SmpScan scan;
-  smp_scan(cluster, S, scan);
-  if (tid == SMP_THREADS - 1) { S.partc[0] = scan.c[3]; S.part[0] = scan.w[3]; }
-  __syncthreads();
-  const unsigned count = S.partc[0];
-  const u64 all = S.part[0];
-  __syncthreads();
-  if (!(least <= 1.f)) wmin = 1ull;        // only the first candidate, and the draw finds no other
-  const bool cut_k = k > 0 && (unsigned)k < count, cut_p = !(tp >= 1.0);
-  const SmpSel end = cut_k ? smp_select(S, scan, false, (u64)k) : smp_select(S, scan, true, min(cut_p ? smp_target(tp, all) : all, wmin));
+  SmpSel end;
+  auto least_weight = [&]() {
+    wmin = 0ull;
+#pragma unroll
+    for (int q = 0; q < NCTA; q++) wmin += other(q)->least_sum;
+    if (!(least <= 1.f)) wmin = 1ull;      // only the first candidate, and the draw finds no other
+  };
+  if (!few) least_weight();
+  if (few && !cut_k) end = SmpSel{SMP_BINS - 1, 0u, scan.count, 0u, 0ull};
+  else end = cut_k ? smp_select<NCTA>(cluster, S, scan, false, (u64)k, turn) : smp_select<NCTA>(cluster, S, scan, true, min(cut_p ? smp_target(tp, scan.all) : scan.all, wmin), turn);
 
   // words of the logits in bins first .. last whose digits above `himask` are `prefix`, into CTA 0's list
   auto gather = [&](int first, int last, u64 himask, u64 prefix) {
-    unsigned* filled = &cluster.map_shared_rank(&S, 0)->filled;
-    u64* list = cluster.map_shared_rank(&S, 0)->list;
+    unsigned* filled = &other(0)->filled;
+    u64* list = other(0)->list;
+    const float from = (float)first, to = last >= SMP_BINS - 1 ? INFINITY : (float)(last + 1);
     for (int i = tid; i < mine; i += SMP_THREADS) {
       const float y = s_y[i];
       if (y != y) continue;
-      const int b = smp_bin(y, top);
-      if (b < first || b > last) continue;
+      const float d = y == top ? 0.f : __fsub_rn(top, y) * 64.f;        // what smp_bin cuts to a whole number
+      if (!(d >= from && (d < to || to == INFINITY))) continue;
       const u64 w = smp_word(y, i0 + i);
       if ((w & himask) != prefix) continue;
       const unsigned at = atomicAdd(filled, 1u);
       if (at < SMP_LIST) list[at] = w;
     }
-    cluster.sync();
+    all_sync();
   };
   auto finish = [&](u64 word, u64 kept) {
     A.index[row] = smp_index(word);
@@ -270,20 +366,39 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const SmpAr
     if (rank != 0) return;
     const int cnt = (int)(end.before + end.count);
     smp_sort(S, cnt, top);
-    if (tid == 0) {
-      const u64 wk = cut_k ? S.run[k - 1] : all;
-      u64 kept = wk;
-      if (cut_p) { const u64 line = smp_target(tp, wk); kept = wmin < line ? wmin : S.run[smp_place(S, cut_k ? k : cnt, line)]; }
-      if (wmin < kept) kept = wmin;
-      if (!(least <= 1.f)) kept = 1ull << 31;
-      finish(S.list[least <= 1.f ? smp_place(S, cnt, smp_target(u, kept)) : 0], kept);
+    const u64 wk = cut_k ? S.run[k - 1] : few ? S.run[cnt - 1] : scan.all;
+    if (few) {                             // the list's first ones that are heavy enough (or all of it, which is more than is kept)
+      int heavy = 0;
+      for (int q = tid; q < cnt; q += SMP_THREADS) heavy += smp_weight(smp_value(S.list[q]), top) >= least ? 1 : 0;
+#pragma unroll
+      for (int o = 16; o; o >>= 1) heavy += __shfl_xor_sync(0xffffffffu, heavy, o);
+      if (lane == 0) S.partc[tid >> 5] = (unsigned)heavy;
+      __syncthreads();
+      heavy = 0;
+#pragma unroll
+      for (int q = 0; q < SMP_WARPS; q++) heavy += (int)S.partc[q];
+      wmin = least <= 1.f ? S.run[max(heavy, 1) - 1] : 1ull;
     }
+    u64 kept = wk;
+    if (cut_p) { const u64 line = smp_target(tp, wk); kept = wmin < line ? wmin : S.run[smp_place(S, cut_k ? k : cnt, line)]; }
+    if (wmin < kept) kept = wmin;
+    if (!(least <= 1.f)) kept = 1ull << 31;
+    const int at = least <= 1.f ? smp_place(S, cnt, smp_target(u, kept)) : 0;
+    if (tid == 0) finish(S.list[at], kept);
     return;
   }
 
   // ---- too many to sort together: the three places one after the other
+  if (few) {                               // with weights, after all
+    all_sync();
+    for (int i = tid; i < 3 * SMP_BINS; i += SMP_THREADS) S.hist[0][i] = 0u;
+    __syncthreads();
+    bins(true);
+    smp_scan<NCTA>(cluster, S, scan);
+    least_weight();
+  }
   auto find = [&](bool by_weight, u64 target, u64& cum) -> u64 {
-    SmpSel s = smp_select(S, scan, by_weight, target);
+    SmpSel s = smp_select<NCTA>(cluster, S, scan, by_weight, target, turn);
     const int bin = s.bin;
     u64 himask = 0ull, prefix = 0ull, before_w = s.weight_before;
     u64 left = target - (by_weight ? s.weight_before : (u64)s.before);
@@ -300,39 +415,35 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const SmpAr
         atomicAdd(&S.hist[0][d], 1u);
         if (f) { atomicAdd(&S.hist[1][d], f & 0xffffu); atomicAdd(&S.hist[2][d], f >> 16); }
       }
-      cluster.sync();
-      SmpScan fine;
-      smp_scan(cluster, S, fine);
-      s = smp_select(S, fine, by_weight, left);
+      all_sync();
+      SmpScan<NCTA> fine;
+      smp_scan<NCTA>(cluster, S, fine);
+      s = smp_select<NCTA>(cluster, S, fine, by_weight, left, turn);
       left -= by_weight ? s.weight_before : (u64)s.before;
       before_w += s.weight_before;
       himask = shift ? ~0ull << shift : ~0ull;
       prefix = (prefix & ~((u64)(SMP_BINS - 1) << shift)) | (u64)(SMP_BINS - 1 - s.bin) << shift;
     }
-    if (rank == 0 && tid == 0) S.filled = 0u;
-    cluster.sync();
     gather(bin, bin, himask, prefix);
     if (rank == 0) {
       const int cnt = (int)s.count;
       smp_sort(S, cnt, top);
-      if (tid < ncta) {                    // a thread for each CTA tells it
-        const int at = by_weight ? smp_place(S, cnt, left) : (int)left - 1;
-        SmpShared* o = cluster.map_shared_rank(&S, tid);
-        o->result_word = S.list[at]; o->result_cum = before_w + S.run[at];
-      }
+      const int at = by_weight ? smp_place(S, cnt, left) : (int)left - 1;
+      if (tid < NCTA) { SmpShared* o = other(tid); o->result_word = S.list[at]; o->result_cum = before_w + S.run[at]; }      // a thread for each CTA tells it
+      if (tid == 0) S.filled = 0u;
     }
-    cluster.sync();
+    all_sync();
     cum = S.result_cum;
     return S.result_word;
   };
-  u64 kept = all, cum;
+  u64 kept = scan.all, cum;
   if (cut_k) { find(false, (u64)k, cum); kept = cum; }
   if (cut_p) { const u64 line = smp_target(tp, kept); if (wmin < line) kept = wmin; else { find(true, line, cum); kept = cum; } }
   if (wmin < kept) kept = wmin;
   const u64 word = least <= 1.f ? find(true, smp_target(u, kept), cum) : best;
   if (!(least <= 1.f)) kept = 1ull << 31;
   if (rank == 0 && tid == 0) finish(word, kept);
-  cluster.sync();
+  all_sync();
 }
 
 // ------------------------------------------------------------------ a row beyond the cluster's shared memory
@@ -445,10 +556,13 @@ extern "C" int wv_sample_rows_dev(const float* d_logits, int rows, int n, int64_
     cfg.gridDim = dim3(rows); cfg.blockDim = dim3(SMW_THREADS);
     e = cudaLaunchKernelEx(&cfg, sample_wide_kernel, A);
   } else {
-    const int ncta = n <= SMP_SMALL ? 1 : SMP_CLUSTER, per = (n - 1) / ncta + 1;
+    const int ncta = n <= SMP_SMALL ? 1 : SMP_CLUSTER, per = ((n - 1) / ncta + 4) & ~3;
+    auto kern = ncta == 1 ? sample_rows_kernel<1> : sample_rows_kernel<SMP_CLUSTER>;
     static unsigned long long attr_mask = 0;     // the attribute is set once per device
     if (dev >= 64 || !(attr_mask & (1ull << dev))) {
-      if (cudaFuncSetAttribute(sample_rows_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(sizeof(SmpShared) + SMP_CACHE * 4)) != cudaSuccess) {
+      const int most = (int)(sizeof(SmpShared) + SMP_CACHE * 4);
+      if (cudaFuncSetAttribute(sample_rows_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess ||
+          cudaFuncSetAttribute(sample_rows_kernel<SMP_CLUSTER>, cudaFuncAttributeMaxDynamicSharedMemorySize, most) != cudaSuccess) {
         wv_set_error("wv_sample_rows_dev: %s", cudaGetErrorString(cudaGetLastError())); return WV_ECUDA;
       }
       if (dev < 64) attr_mask |= 1ull << dev;
@@ -457,7 +571,7 @@ extern "C" int wv_sample_rows_dev(const float* d_logits, int rows, int n, int64_
     at[1].id = cudaLaunchAttributeClusterDimension;
     at[1].val.clusterDim.x = (unsigned)ncta; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
     cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, sample_rows_kernel, A, per);
+    e = cudaLaunchKernelEx(&cfg, kern, A, per);
   }
   if (e != cudaSuccess) { wv_set_error("wv_sample_rows_dev: launch: %s", cudaGetErrorString(cudaGetLastError())); return WV_ECUDA; }
   return WV_OK;
