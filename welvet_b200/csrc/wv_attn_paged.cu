@@ -678,12 +678,20 @@ int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* d
     const long long top = chunk ? c.rows_most : most;
     const bool r16 = top > 8;
     const long long tiles = (top + (r16 ? 15 : 7)) / (r16 ? 16 : 8), per_head = tiles * (r16 ? 16 : 8);
-    const long long blocks = (long long)b.num_seqs * tiles * c.g.kvh, want = 2LL * sms;
+    const long long blocks = (long long)b.num_seqs * tiles * c.g.kvh;
     if (blocks * (r16 ? 16 : 8) > INT_MAX) { wv_set_error("wv_attn_paged_dev: %d sequences are too many", b.num_seqs); return WV_ESHAPE; }
-    long long per = (keys * blocks + want - 1) / want;
-    per = (per + 63) & ~63LL;
-    if (per < 64) per = 64;
-    if (per > 1024) per = 1024;
+    // Splits of the keys: the number that fills 1, 2, .. 8 waves of the blocks that run at once and costs least, a wave being worth a
+    // warp's groups of 16 keys and some six more of start and end (2049 positions and eight blocks: 33 splits of 64; 131000: 55).
+    const long long slots = (long long)sms * (c.g.hd > 128 ? (r16 || kv.bits == 16 ? 1 : 2) : !r16 && (c.g.hd <= 64 || kv.bits < 16) ? 3 : 2);
+    long long per = 64, cost = -1;
+    for (long long w = 1; w <= 8; w++) {
+      long long n = w * slots / blocks;
+      if (n < 1) { if (w < 8) continue; n = 1; }
+      long long p = ((keys + n - 1) / n + 63) & ~63LL;
+      if (p < 64) p = 64;
+      const long long m = keys > p ? (keys + p - 1) / p : 1, k = (blocks * m + slots - 1) / slots * (p / 64 + 6);
+      if (cost < 0 || k < cost) { cost = k; per = p; }
+    }
     if (per < keys / 8192) per = (keys / 8192 + 63) & ~63LL;
     const long long ns = keys > per ? (keys + per - 1) / per : 1;
     PaCall r = c;
