@@ -44,3 +44,42 @@ def AttnPagedCUDA(pages: WvKvPages, batch: WvKvBatch, dq: int, dout: int, num_he
                   ldo: int = 0, stream: int = 0) -> None:
     """Causal attention of the new tokens over their sequence's cache, optionally the last `window` positions of it (wv_attn_paged_dev)."""
     check(lib().wv_attn_paged_dev(C.byref(pages), C.byref(batch), dq, ldq, dout, ldo, num_heads, scale, window, stream))
+
+
+class PagedBlockDecoder:
+    """One decoder block for a step of several sequences: decode.BlockDecoder's walk (model/transformer/forward.go:57-76) with all
+    new tokens of the batch as rows of one projection each, K and V rounded into the block's pages, and attention over them.
+
+    `cfg` is a decode.BlockConfig (MaxSeqLen is not used: the pages bound the lengths), `keys` maps q, k, v, o, gate, up, down to resident
+    blob keys, `bufs` maps the working matrices of up to `max_tokens` rows (norm and proj [DModel], q and attn [NumHeads * HeadDim], k and v
+    [NumKVHeads * HeadDim], gate and up [IntermediateDim]) and the weights attn_norm / ffn_norm to device pointers. A block has pages of its
+    own; the blocks of a stack share the working matrices and the batch."""
+
+    def __init__(self, cfg, keys: dict, bufs: dict, pages: WvKvPages, max_tokens: int, window: int = 0):
+        self.cfg, self.keys, self.bufs, self.pages, self.max_tokens, self.window = cfg, keys, bufs, pages, max_tokens, window
+        qd, kd = cfg.NumHeads * cfg.HeadDim, cfg.NumKVHeads * cfg.HeadDim
+
+        def group(names, outs):
+            n = len(names)
+            return (C.c_uint64 * n)(*[keys[m] for m in names]), (C.c_void_p * n)(*[bufs[m] for m in names]), (C.c_int * n)(*outs)
+        self._qkv, self._gu = group(("q", "k", "v"), (qd, kd, kd)), group(("gate", "up"), (cfg.IntermediateDim,) * 2)
+
+    def step(self, dh: int, batch: WvKvBatch, stream: int = 0) -> None:
+        """The rows of the hidden state [batch.total_q, DModel] at device address dh are updated in place."""
+        c, b, k, n, L = self.cfg, self.bufs, self.keys, batch.total_q, lib()
+        if n > self.max_tokens:
+            raise ValueError(f"{n} new tokens, but the working matrices have {self.max_tokens} rows")
+        if n == 0:
+            return
+        qd = c.NumHeads * c.HeadDim
+        check(L.wv_rmsnorm_dev(dh, b["attn_norm"], b["norm"], n, c.DModel, c.Eps, stream))
+        check(L.wv_matvec_dev_multi(self._qkv[0], 3, b["norm"], self._qkv[1], n, c.DModel, self._qkv[2], stream))
+        KVWriteCUDA(self.pages, batch, b["k"], b["v"], b["q"], b["q"], c.NumHeads, c.RoPETheta, stream=stream)
+        AttnPagedCUDA(self.pages, batch, b["q"], b["attn"], c.NumHeads, 1.0 / (c.HeadDim ** 0.5), window=self.window, stream=stream)
+        check(L.wv_matvec_dev(k["o"], b["attn"], b["proj"], n, qd, c.DModel, stream))
+        check(L.wv_residual_add_dev(dh, b["proj"], n * c.DModel, stream))
+        check(L.wv_rmsnorm_dev(dh, b["ffn_norm"], b["norm"], n, c.DModel, c.Eps, stream))
+        check(L.wv_matvec_dev_multi(self._gu[0], 2, b["norm"], self._gu[1], n, c.DModel, self._gu[2], stream))
+        check(L.wv_silu_mul_dev(b["gate"], b["up"], b["gate"], n * c.IntermediateDim, stream))
+        check(L.wv_matvec_dev(k["down"], b["gate"], b["proj"], n, c.IntermediateDim, c.DModel, stream))
+        check(L.wv_residual_add_dev(dh, b["proj"], n * c.DModel, stream))
