@@ -32,7 +32,9 @@ __device__ __forceinline__ float smp_value(u64 w) {
   return __uint_as_float((u & 0x80000000u) ? (u & 0x7FFFFFFFu) : ~u);
 }
 __device__ __forceinline__ int smp_index(u64 w) { return (int)(0xFFFFFFFFu - (unsigned)w); }
-__device__ __forceinline__ float smp_weight(float y, float top) { return y == top ? 1.f : expf(__fsub_rn(y, top)); }
+// top - y; 0 for the largest itself, be it an infinity.
+__device__ __forceinline__ float smp_distance(float y, float top) { return fmaxf(__fsub_rn(top, y), 0.f); }
+__device__ __forceinline__ float smp_weight(float y, float top) { return expf(-smp_distance(y, top)); }
 __device__ __forceinline__ unsigned smp_units(float w) { return __float2uint_rn(w * 2147483648.f); }
 // The smallest whole number that is at least f * total, between 1 and total.
 __device__ __forceinline__ u64 smp_target(double f, u64 total) {
@@ -42,6 +44,24 @@ __device__ __forceinline__ u64 smp_target(double f, u64 total) {
 }
 // logit / T; NaN for what is no candidate. A finite logit may become an infinity by the division: it stays a candidate.
 __device__ __forceinline__ float smp_y(float x, float t, bool greedy) { return !(x > -INFINITY) ? NAN : greedy ? x : __fdiv_rn(x, t); }
+// The same for four logits, by the reciprocal: with r the rounded 1/t, q within an ulp of x/t and the remainder x - q t exact, q + (x - q t) r
+// rounds to the rounded quotient (P. Markstein, Computation of elementary functions on the IBM RISC System/6000 processor, 1990). The
+// product x r is within one and a half ulps, so the step is done twice: 2.5 instructions a logit in pairs, where the division with its
+// test and branch takes about 14. The remainder is exact and nothing overflows for 2^-20 <= t <= 2^20 (`quick`) and
+// 2^-100 <= |x| <= 2^100; a group of four with another number is divided one by one. NaN stays NaN.
+__device__ __forceinline__ float4 smp_y4(float4 x, float t, float r, bool quick) {
+  const float hi = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
+  const float lo = fminf(fminf(fabsf(x.x), fabsf(x.y)), fminf(fabsf(x.z), fabsf(x.w)));
+  if (!(quick && hi <= 0x1p100f && lo >= 0x1p-100f)) return make_float4(smp_y(x.x, t, false), smp_y(x.y, t, false), smp_y(x.z, t, false), smp_y(x.w, t, false));
+  const float2 a = make_float2(x.x, x.y), b = make_float2(x.z, x.w), rr = make_float2(r, r), nt = make_float2(-t, -t);
+  float2 p = __fmul2_rn(a, rr), q = __fmul2_rn(b, rr);
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    p = __ffma2_rn(__ffma2_rn(p, nt, a), rr, p);
+    q = __ffma2_rn(__ffma2_rn(q, nt, b), rr, q);
+  }
+  return make_float4(p.x, p.y, q.x, q.y);
+}
 
 #define SMP_THREADS 512
 #define SMP_WARPS (SMP_THREADS / 32)
@@ -73,9 +93,10 @@ struct __align__(16) SmpShared {
   int place;
 };
 
+// The whole part of 64 times the distance, at most 2047, by a sum that rounds down: it rises as y falls, for each step rounds monotonously.
 __device__ __forceinline__ int smp_bin(float y, float top) {
-  if (y == top) return 0;
-  return min((int)(__fsub_rn(top, y) * 64.f), SMP_BINS - 1);             // rises as y falls: each step rounds monotonously
+  const float d = fminf(smp_distance(y, top), 31.999998f);
+  return __float_as_int(__fmaf_rd(d, 64.f, 8388608.f)) - 0x4b000000;
 }
 
 // A CTA adds up its share of the bins over the cluster, the shares' totals go to every CTA, and a place is announced by the CTA whose
@@ -163,10 +184,61 @@ __device__ __forceinline__ SmpSel smp_select(cg::cluster_group& cluster, SmpShar
   if (NCTA == 1) __syncthreads(); else cluster.sync();
   return S.sel[turn];
 }
-// The first cnt words of the list from the largest down, and their running weights. Up to 256 of them each find their own rank.
-__device__ __forceinline__ void smp_sort(SmpShared& S, int cnt, float top) {
+// The words of the list in 2048 buckets of equal width over bins first .. last, those of a bucket by their ranks among themselves. Nothing is
+// done, and false returned, where a bucket has more than 32 (equal logits).
+__device__ __forceinline__ bool smp_buckets(SmpShared& S, int cnt, float top, int first, int last) {
+  constexpr int PER = SMP_LIST / SMP_THREADS;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (cnt <= 256) {
+  const float width = (float)SMP_BINS / (float)(last - first + 1);
+  unsigned* start = S.hist[2];             // beyond what S.run takes
+  u64* spread = S.run;
+#pragma unroll
+  for (int q = 0; q < PER; q++) start[tid + q * SMP_THREADS] = 0u;
+  __syncthreads();
+  u64 w[PER];
+  int b[PER];
+  unsigned slot[PER];
+#pragma unroll
+  for (int q = 0; q < PER; q++) {
+    const int i = tid + q * SMP_THREADS;
+    if (i >= cnt) break;
+    w[q] = S.list[i];
+    const float d = __fmul_rn(__fsub_rn(smp_distance(smp_value(w[q]), top) * 64.f, (float)first), width);   // rises as the word falls
+    b[q] = (int)fminf(fmaxf(d, 0.f), (float)(SMP_BINS - 1));
+    slot[q] = atomicAdd(&start[b[q]], 1u);
+  }
+  __syncthreads();
+  unsigned c[PER], t = 0, most = 0;
+#pragma unroll
+  for (int q = 0; q < PER; q++) { const unsigned n = start[PER * tid + q]; c[q] = t; t += n; most = max(most, n); }
+  unsigned s = t;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) { const unsigned a = __shfl_up_sync(0xffffffffu, s, o); if (lane >= o) s += a; }
+  if (lane == 31) S.partc[warp] = s;
+  if (__syncthreads_or(most > 32)) return false;
+#pragma unroll
+  for (int q = 0; q < SMP_WARPS; q++) s += q < warp ? S.partc[q] : 0u;
+#pragma unroll
+  for (int q = 0; q < PER; q++) start[PER * tid + q] = s - t + c[q];
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < PER; q++) { if (tid + q * SMP_THREADS >= cnt) break; spread[start[b[q]] + slot[q]] = w[q]; }
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < PER; q++) {
+    if (tid + q * SMP_THREADS >= cnt) break;
+    const unsigned from = start[b[q]], to = b[q] + 1 < SMP_BINS ? start[b[q] + 1] : (unsigned)cnt;
+    unsigned at = from;
+    for (unsigned j = from; j < to; j++) at += spread[j] > w[q] ? 1u : 0u;
+    S.list[at] = w[q];
+  }
+  return true;
+}
+// The first cnt words of the list, all of bins first .. last, from the largest down, and their running weights. Up to 128 of them each find
+// their own rank; more are spread over buckets (2 us less than the 55 to 66 steps of a bitonic sort, which is left for many equal logits).
+__device__ __forceinline__ void smp_sort(SmpShared& S, int cnt, float top, int first, int last) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (cnt <= 128) {
     const u64 mine = tid < cnt ? S.list[tid] : 0ull;
     int at = 0;
     if (warp * 32 < cnt) {
@@ -175,8 +247,8 @@ __device__ __forceinline__ void smp_sort(SmpShared& S, int cnt, float top) {
     }
     __syncthreads();
     if (tid < cnt) S.list[at] = mine;
-  } else {
-    int p2 = 512;
+  } else if (!smp_buckets(S, cnt, top, first, last)) {
+    int p2 = 256;
     while (p2 < cnt) p2 <<= 1;
     for (int i = cnt + tid; i < p2; i += SMP_THREADS) S.list[i] = 0ull;
     __syncthreads();
@@ -245,45 +317,62 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const SmpAr
   const float least = A.min_p[row];
   const double tp = (double)A.top_p[row], u = A.u[row];
   __syncthreads();
-  // ---- the row's logits / T into shared memory, and the largest word
+  // ---- the row's logits / T into shared memory (a greedy row's stay where they are), and the largest
+  const int n4 = mine >> 2, n4up = (mine + 3) >> 2;                      // what pads the last four is no candidate
+  const bool quick = t >= 0x1p-20f && t <= 0x1p20f;
+  const float r = __frcp_rn(t);
+  float own = greedy ? -INFINITY : NAN;    // the thread's largest logit (or logit / T; NaN: no candidate)
+  int at = 0;                              // greedy: its place, the first of equals (a thread's places rise)
   {
-    float best = -INFINITY;
-    int at = -1;
-    auto take = [&](float v, int i) {
-      const float y = smp_y(v, t, greedy);
-      if (y > best || (y == best && at < 0)) { best = y; at = i; }       // a thread's places rise: the first of equals
+    auto four = [&](float4 v, int i, int step) {
+      const float m = fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w));
+      if (greedy) {
+        if (m > own) { own = m; at = v.x == m ? i : v.y == m ? i + step : v.z == m ? i + 2 * step : i + 3 * step; }
+        return v;
+      }
+      const float4 y = smp_y4(v, t, r, quick);
+      own = fmaxf(own, quick ? m : fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)));
       return y;
     };
     if ((reinterpret_cast<uintptr_t>(x) & 15) == 0 && (per & 3) == 0) {  // i0 is a multiple of per
       constexpr int U = 8;
-      const int n4 = mine >> 2;
       for (int b = tid; b < n4; b += U * SMP_THREADS) {
         float4 v[U];
 #pragma unroll
         for (int q = 0; q < U; q++) if (b + q * SMP_THREADS < n4) v[q] = __ldcs(reinterpret_cast<const float4*>(x) + b + q * SMP_THREADS);
 #pragma unroll
         for (int q = 0; q < U; q++) {
-          const int i = 4 * (b + q * SMP_THREADS);
-          if (i >= 4 * n4) break;
-          const float y0 = take(v[q].x, i), y1 = take(v[q].y, i + 1), y2 = take(v[q].z, i + 2), y3 = take(v[q].w, i + 3);
-          *reinterpret_cast<float4*>(s_y + i) = make_float4(y0, y1, y2, y3);
+          const int i = b + q * SMP_THREADS;
+          if (i >= n4) break;
+          const float4 y = four(v[q], 4 * i, 1);
+          if (!greedy) *reinterpret_cast<float4*>(s_y + 4 * i) = y;
         }
       }
-      if (tid < (mine & 3)) { const int i = 4 * n4 + tid; s_y[i] = take(x[i], i); }
+      if (tid == 0 && n4 < n4up) {
+        const int i = 4 * n4, left = mine & 3;
+        const float4 v = make_float4(x[i], left > 1 ? x[i + 1] : NAN, left > 2 ? x[i + 2] : NAN, NAN), y = four(v, i, 1);
+        if (!greedy) *reinterpret_cast<float4*>(s_y + i) = y;
+      }
     } else {
-      for (int b = tid; b < mine; b += 16 * SMP_THREADS) {
-        float v[16];
+      constexpr int U = 16;
+      for (int b = tid; b < 4 * n4up; b += U * SMP_THREADS) {
+        float v[U];
 #pragma unroll
-        for (int q = 0; q < 16; q++) v[q] = b + q * SMP_THREADS < mine ? __ldcs(x + b + q * SMP_THREADS) : NAN;
+        for (int q = 0; q < U; q++) v[q] = b + q * SMP_THREADS < mine ? __ldcs(x + b + q * SMP_THREADS) : NAN;
 #pragma unroll
-        for (int q = 0; q < 16; q++) {
+        for (int q = 0; q < U; q += 4) {
           const int i = b + q * SMP_THREADS;
-          if (i >= mine) break;
-          s_y[i] = take(v[q], i);
+          const float4 y = four(make_float4(v[q], v[q + 1], v[q + 2], v[q + 3]), i, SMP_THREADS);
+          if (greedy) continue;
+          if (i < 4 * n4up) s_y[i] = y.x;
+          if (i + SMP_THREADS < 4 * n4up) s_y[i + SMP_THREADS] = y.y;
+          if (i + 2 * SMP_THREADS < 4 * n4up) s_y[i + 2 * SMP_THREADS] = y.z;
+          if (i + 3 * SMP_THREADS < 4 * n4up) s_y[i + 3 * SMP_THREADS] = y.w;
         }
       }
     }
-    u64 w = at < 0 ? 0ull : smp_word(best, i0 + at);
+    if (quick && !greedy) own = smp_y(own, t, false);                     // the order of the quotients is that of the logits
+    u64 w = own != own || (greedy && !(own > -INFINITY)) ? 0ull : smp_word(own, i0 + at);
 #pragma unroll
     for (int o = 16; o; o >>= 1) w = max(w, __shfl_xor_sync(0xffffffffu, w, o));
     if (lane == 0 && w) atomicMax(&S.best, w);
@@ -298,13 +387,15 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const SmpAr
     all_sync();                            // nobody leaves while its shared memory may be read
     return;
   }
-  // ---- counts and weights of the bins, and the weight that min-p leaves. Up to 1024 of top-k need the counts alone: the weights of
-  // those candidates are taken when they have been sorted.
+  auto clear = [&]() {
+    for (int i = tid; i < 3 * SMP_BINS; i += SMP_THREADS) S.hist[0][i] = 0u;
+    __syncthreads();
+  };
+  // ---- counts (and weights) of the bins, and the weight that min-p leaves
   auto bins = [&](bool weights) {
     u64 ms = 0ull;
-    for (int i = tid; i < mine; i += SMP_THREADS) {
-      const float y = s_y[i];
-      if (y != y) continue;
+    auto one = [&](float y) {
+      if (y != y) return;
       const int b = smp_bin(y, top);
       atomicAdd(&S.hist[0][b], 1u);
       if (weights) {
@@ -313,6 +404,10 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const SmpAr
         if (w) { atomicAdd(&S.hist[1][b], w & 0xffffu); atomicAdd(&S.hist[2][b], w >> 16); }
         if (f >= least) ms += w;
       }
+    };
+    for (int i = tid; i < n4up; i += SMP_THREADS) {
+      const float4 y = *reinterpret_cast<const float4*>(s_y + 4 * i);
+      one(y.x); one(y.y); one(y.z); one(y.w);
     }
     if (weights) {
 #pragma unroll
@@ -321,12 +416,25 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const SmpAr
     }
     all_sync();
   };
+  // Up to 1024 of top-k: the k-th largest of the threads' largest is no larger than the k-th largest of all, so the bins down to its bin
+  // hold the k, and (4096 threads) hardly more than those: one entry a thread in place of one a logit. The weights of those
+  // candidates are taken when they have been sorted. Fewer threads than k with a candidate: the counts of all.
   int turn = 0;
   SmpScan<NCTA> scan;
   const bool few = k > 0 && k <= SMP_LIST / 2;
-  bins(!few);
-  smp_scan<NCTA>(cluster, S, scan);
-  const bool cut_k = k > 0 && (unsigned)k < scan.count, cut_p = !(tp >= 1.0);
+  bool part = few;                         // the bins hold the threads' largest alone
+  if (few) {
+    if (own == own) atomicAdd(&S.hist[0][smp_bin(own, top)], 1u);
+    all_sync();
+    smp_scan<NCTA>(cluster, S, scan);
+    part = scan.count >= (unsigned)k;
+    if (!part) clear();
+  }
+  if (!part) {
+    bins(!few);
+    smp_scan<NCTA>(cluster, S, scan);
+  }
+  const bool cut_k = part || (k > 0 && (unsigned)k < scan.count), cut_p = !(tp >= 1.0);
   u64 wmin = 0ull;
   SmpSel end;
   auto least_weight = [&]() {
@@ -343,16 +451,21 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const SmpAr
   auto gather = [&](int first, int last, u64 himask, u64 prefix) {
     unsigned* filled = &other(0)->filled;
     u64* list = other(0)->list;
-    const float from = (float)first, to = last >= SMP_BINS - 1 ? INFINITY : (float)(last + 1);
-    for (int i = tid; i < mine; i += SMP_THREADS) {
-      const float y = s_y[i];
-      if (y != y) continue;
-      const float d = y == top ? 0.f : __fsub_rn(top, y) * 64.f;        // what smp_bin cuts to a whole number
-      if (!(d >= from && (d < to || to == INFINITY))) continue;
+    // a distance that rounds to less than (last + 1) / 64 is less than that: all but the bins asked for go by one comparison
+    const float from = last >= SMP_BINS - 1 ? -INFINITY : __fsub_rd(top, (float)(last + 1) * 0.015625f);
+    auto one = [&](float y, int i) {
+      if (!(y >= from)) return;
+      const int b = smp_bin(y, top);
+      if (b < first || b > last) return;
       const u64 w = smp_word(y, i0 + i);
-      if ((w & himask) != prefix) continue;
+      if ((w & himask) != prefix) return;
       const unsigned at = atomicAdd(filled, 1u);
       if (at < SMP_LIST) list[at] = w;
+    };
+    for (int i = tid; i < n4up; i += SMP_THREADS) {
+      const float4 y = *reinterpret_cast<const float4*>(s_y + 4 * i);
+      if (!(fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)) >= from)) continue;
+      one(y.x, 4 * i); one(y.y, 4 * i + 1); one(y.z, 4 * i + 2); one(y.w, 4 * i + 3);
     }
     all_sync();
   };
@@ -363,36 +476,42 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const SmpAr
 
   if (end.before + end.count <= SMP_LIST) {
     gather(0, end.bin, 0ull, 0ull);
-    if (rank != 0) return;
-    const int cnt = (int)(end.before + end.count);
-    smp_sort(S, cnt, top);
-    const u64 wk = cut_k ? S.run[k - 1] : few ? S.run[cnt - 1] : scan.all;
-    if (few) {                             // the list's first ones that are heavy enough (or all of it, which is more than is kept)
-      int heavy = 0;
-      for (int q = tid; q < cnt; q += SMP_THREADS) heavy += smp_weight(smp_value(S.list[q]), top) >= least ? 1 : 0;
-#pragma unroll
-      for (int o = 16; o; o >>= 1) heavy += __shfl_xor_sync(0xffffffffu, heavy, o);
-      if (lane == 0) S.partc[tid >> 5] = (unsigned)heavy;
-      __syncthreads();
-      heavy = 0;
-#pragma unroll
-      for (int q = 0; q < SMP_WARPS; q++) heavy += (int)S.partc[q];
-      wmin = least <= 1.f ? S.run[max(heavy, 1) - 1] : 1ull;
+    const unsigned got = other(0)->filled;
+    if (NCTA > 1) cluster.barrier_arrive();                               // has read it
+    if (got <= SMP_LIST) {
+      if (rank != 0) { cluster.barrier_wait(); return; }
+      const int cnt = (int)got;
+      smp_sort(S, cnt, top, 0, end.bin);
+      const u64 wk = cut_k ? S.run[k - 1] : few ? S.run[cnt - 1] : scan.all;
+      if (few) {                             // the list's first ones that are heavy enough (or all of it, which is more than is kept)
+        int heavy = 0;
+        for (int q = tid; q < cnt; q += SMP_THREADS) heavy += smp_weight(smp_value(S.list[q]), top) >= least ? 1 : 0;
+  #pragma unroll
+        for (int o = 16; o; o >>= 1) heavy += __shfl_xor_sync(0xffffffffu, heavy, o);
+        if (lane == 0) S.partc[tid >> 5] = (unsigned)heavy;
+        __syncthreads();
+        heavy = 0;
+  #pragma unroll
+        for (int q = 0; q < SMP_WARPS; q++) heavy += (int)S.partc[q];
+        wmin = least <= 1.f ? S.run[max(heavy, 1) - 1] : 1ull;
+      }
+      u64 kept = wk;
+      if (cut_p) { const u64 line = smp_target(tp, wk); kept = wmin < line ? wmin : S.run[smp_place(S, cut_k ? k : cnt, line)]; }
+      if (wmin < kept) kept = wmin;
+      if (!(least <= 1.f)) kept = 1ull << 31;
+      const int at = least <= 1.f ? smp_place(S, cnt, smp_target(u, kept)) : 0;
+      if (tid == 0) finish(S.list[at], kept);
+      if (NCTA > 1) cluster.barrier_wait();  // CTA 0's memory outlives the others' reads of it
+      return;
     }
-    u64 kept = wk;
-    if (cut_p) { const u64 line = smp_target(tp, wk); kept = wmin < line ? wmin : S.run[smp_place(S, cut_k ? k : cnt, line)]; }
-    if (wmin < kept) kept = wmin;
-    if (!(least <= 1.f)) kept = 1ull << 31;
-    const int at = least <= 1.f ? smp_place(S, cnt, smp_target(u, kept)) : 0;
-    if (tid == 0) finish(S.list[at], kept);
-    return;
+    if (NCTA > 1) cluster.barrier_wait(); else __syncthreads();
+    if (rank == 0 && tid == 0) S.filled = 0u;
   }
 
   // ---- too many to sort together: the three places one after the other
   if (few) {                               // with weights, after all
     all_sync();
-    for (int i = tid; i < 3 * SMP_BINS; i += SMP_THREADS) S.hist[0][i] = 0u;
-    __syncthreads();
+    clear();
     bins(true);
     smp_scan<NCTA>(cluster, S, scan);
     least_weight();
@@ -403,8 +522,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const SmpAr
     u64 himask = 0ull, prefix = 0ull, before_w = s.weight_before;
     u64 left = target - (by_weight ? s.weight_before : (u64)s.before);
     for (int shift = 64 - 11; s.count > SMP_LIST; shift = max(shift - 11, 0)) {
-      for (int i = tid; i < 3 * SMP_BINS; i += SMP_THREADS) S.hist[0][i] = 0u;
-      __syncthreads();
+      clear();
       for (int i = tid; i < mine; i += SMP_THREADS) {
         const float y = s_y[i];
         if (y != y || smp_bin(y, top) != bin) continue;
@@ -427,7 +545,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const SmpAr
     gather(bin, bin, himask, prefix);
     if (rank == 0) {
       const int cnt = (int)s.count;
-      smp_sort(S, cnt, top);
+      smp_sort(S, cnt, top, bin, bin);
       const int at = by_weight ? smp_place(S, cnt, left) : (int)left - 1;
       if (tid < NCTA) { SmpShared* o = other(tid); o->result_word = S.list[at]; o->result_cum = before_w + S.run[at]; }      // a thread for each CTA tells it
       if (tid == 0) S.filled = 0u;
@@ -440,7 +558,7 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const SmpAr
   if (cut_k) { find(false, (u64)k, cum); kept = cum; }
   if (cut_p) { const u64 line = smp_target(tp, kept); if (wmin < line) kept = wmin; else { find(true, line, cum); kept = cum; } }
   if (wmin < kept) kept = wmin;
-  const u64 word = least <= 1.f ? find(true, smp_target(u, kept), cum) : best;
+  const u64 word = find(true, least <= 1.f ? smp_target(u, kept) : 1ull, cum);
   if (!(least <= 1.f)) kept = 1ull << 31;
   if (rank == 0 && tid == 0) finish(word, kept);
   all_sync();
