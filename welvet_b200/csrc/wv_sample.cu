@@ -89,8 +89,8 @@ struct __align__(16) SmpShared {
   unsigned partc[SMP_WARPS], tot_c[SMP_CLUSTER];
   u64 best, least_sum, result_word, result_cum;
   SmpSel sel[2];
-  unsigned filled, turn;
-  int place;
+  unsigned filled, own, from;              // words in CTA 0's list, the CTA's own of them, and where those begin
+  int place[2];
 };
 
 // The whole part of 64 times the distance, at most 2047, by a sum that rounds down: it rises as y falls, for each step rounds monotonously.
@@ -274,25 +274,24 @@ __device__ __forceinline__ void smp_sort(SmpShared& S, int cnt, float top, int f
   for (int o = 1; o < 32; o <<= 1) { const u64 b = __shfl_up_sync(0xffffffffu, s, o); if (lane >= o) s += b; }
   if (lane == 31) S.part[warp] = s;
   __syncthreads();
-  for (int q = 0; q < warp; q++) s += S.part[q];
+#pragma unroll
+  for (int q = 0; q < SMP_WARPS; q++) s += q < warp ? S.part[q] : 0ull;
 #pragma unroll
   for (int i = 0; i < PER; i++) S.run[PER * tid + i] = s - t + v[i];
   __syncthreads();
 }
-// The place in S.run[0 .. cnt) (rising) where the running weight reaches target; the last place if it does not.
-__device__ __forceinline__ int smp_place(SmpShared& S, int cnt, u64 target) {
-  if (threadIdx.x == 0) S.place = cnt - 1;
-  __syncthreads();
+// The place in S.run[0 .. cnt) (rising) where the running weight reaches target; the last place if it does not. The places of two calls in
+// a row stand apart, so that one barrier a call is enough.
+__device__ __forceinline__ int smp_place(SmpShared& S, int cnt, u64 target, int which) {
   constexpr int PER = SMP_LIST / SMP_THREADS;
+  const u64 to = min(target, S.run[cnt - 1]);
 #pragma unroll
   for (int i = 0; i < PER; i++) {
     const int q = PER * (int)threadIdx.x + i;
-    if (q < cnt && S.run[q] >= target && (q == 0 || S.run[q - 1] < target)) S.place = q;
+    if (q < cnt && S.run[q] >= to && (q == 0 || S.run[q - 1] < to)) S.place[which] = q;
   }
   __syncthreads();
-  const int at = S.place;
-  __syncthreads();
-  return at;
+  return S.place[which];
 }
 
 template <int NCTA>
@@ -447,10 +446,11 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const SmpAr
   if (few && !cut_k) end = SmpSel{SMP_BINS - 1, 0u, scan.count, 0u, 0ull};
   else end = cut_k ? smp_select<NCTA>(cluster, S, scan, false, (u64)k, turn) : smp_select<NCTA>(cluster, S, scan, true, min(cut_p ? smp_target(tp, scan.all) : scan.all, wmin), turn);
 
-  // words of the logits in bins first .. last whose digits above `himask` are `prefix`, into CTA 0's list
-  auto gather = [&](int first, int last, u64 himask, u64 prefix) {
-    unsigned* filled = &other(0)->filled;
-    u64* list = other(0)->list;
+  // Words of the logits in bins first .. last whose digits above `himask` are `prefix`: each CTA collects its own where the bins were, and
+  // writes them to CTA 0's list from a place that one atomic for all of them gives. More than fit the list: only their number.
+  auto gather = [&](int first, int last, u64 himask, u64 prefix) -> unsigned {
+    if (tid == 0) S.own = 0u;
+    __syncthreads();
     // a distance that rounds to less than (last + 1) / 64 is less than that: all but the bins asked for go by one comparison
     const float from = last >= SMP_BINS - 1 ? -INFINITY : __fsub_rd(top, (float)(last + 1) * 0.015625f);
     auto one = [&](float y, int i) {
@@ -459,52 +459,60 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const SmpAr
       if (b < first || b > last) return;
       const u64 w = smp_word(y, i0 + i);
       if ((w & himask) != prefix) return;
-      const unsigned at = atomicAdd(filled, 1u);
-      if (at < SMP_LIST) list[at] = w;
+      const unsigned at = atomicAdd(&S.own, 1u);
+      if (at < SMP_LIST) S.run[at] = w;
     };
     for (int i = tid; i < n4up; i += SMP_THREADS) {
       const float4 y = *reinterpret_cast<const float4*>(s_y + 4 * i);
       if (!(fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)) >= from)) continue;
       one(y.x, 4 * i); one(y.y, 4 * i + 1); one(y.z, 4 * i + 2); one(y.w, 4 * i + 3);
     }
+    __syncthreads();
+    const unsigned n = S.own;
+    if (tid == 0) S.from = atomicAdd(&other(0)->filled, n);
+    __syncthreads();
+    const unsigned at = S.from;
+    u64* list = other(0)->list;
+    if (at + n <= SMP_LIST) for (unsigned i = tid; i < n; i += SMP_THREADS) list[at + i] = S.run[i];
     all_sync();
+    const unsigned got = other(0)->filled;
+    if (NCTA > 1) cluster.barrier_arrive(); else __syncthreads();         // has read it: see `leave`
+    return got;
   };
+  auto leave = [&]() { if (NCTA > 1) cluster.barrier_wait(); };         // all CTAs have read the number
   auto finish = [&](u64 word, u64 kept) {
     A.index[row] = smp_index(word);
     if (A.prob) A.prob[row] = (float)((double)smp_weight(smp_value(word), top) * 2147483648.0 / (double)kept);
   };
 
   if (end.before + end.count <= SMP_LIST) {
-    gather(0, end.bin, 0ull, 0ull);
-    const unsigned got = other(0)->filled;
-    if (NCTA > 1) cluster.barrier_arrive();                               // has read it
+    const unsigned got = gather(0, end.bin, 0ull, 0ull);
     if (got <= SMP_LIST) {
-      if (rank != 0) { cluster.barrier_wait(); return; }
+      if (rank != 0) { leave(); return; }
       const int cnt = (int)got;
       smp_sort(S, cnt, top, 0, end.bin);
       const u64 wk = cut_k ? S.run[k - 1] : few ? S.run[cnt - 1] : scan.all;
-      if (few) {                             // the list's first ones that are heavy enough (or all of it, which is more than is kept)
+      if (few && least > 0.f) {              // the list's first ones that are heavy enough (or all of it, which is more than is kept)
         int heavy = 0;
         for (int q = tid; q < cnt; q += SMP_THREADS) heavy += smp_weight(smp_value(S.list[q]), top) >= least ? 1 : 0;
-  #pragma unroll
-        for (int o = 16; o; o >>= 1) heavy += __shfl_xor_sync(0xffffffffu, heavy, o);
+        heavy = __reduce_add_sync(0xffffffffu, heavy);
         if (lane == 0) S.partc[tid >> 5] = (unsigned)heavy;
         __syncthreads();
         heavy = 0;
-  #pragma unroll
+#pragma unroll
         for (int q = 0; q < SMP_WARPS; q++) heavy += (int)S.partc[q];
         wmin = least <= 1.f ? S.run[max(heavy, 1) - 1] : 1ull;
-      }
+      } else if (few) wmin = least <= 0.f ? S.run[cnt - 1] : 1ull;       // NaN: the first candidate alone
       u64 kept = wk;
-      if (cut_p) { const u64 line = smp_target(tp, wk); kept = wmin < line ? wmin : S.run[smp_place(S, cut_k ? k : cnt, line)]; }
+      if (cut_p) { const u64 line = smp_target(tp, wk); kept = wmin < line ? wmin : S.run[smp_place(S, cut_k ? k : cnt, line, 0)]; }
       if (wmin < kept) kept = wmin;
       if (!(least <= 1.f)) kept = 1ull << 31;
-      const int at = least <= 1.f ? smp_place(S, cnt, smp_target(u, kept)) : 0;
+      const int at = least <= 1.f ? smp_place(S, cnt, smp_target(u, kept), 1) : 0;
       if (tid == 0) finish(S.list[at], kept);
-      if (NCTA > 1) cluster.barrier_wait();  // CTA 0's memory outlives the others' reads of it
+      leave();
       return;
     }
-    if (NCTA > 1) cluster.barrier_wait(); else __syncthreads();
+    leave();
     if (rank == 0 && tid == 0) S.filled = 0u;
   }
 
@@ -542,11 +550,11 @@ __global__ void __launch_bounds__(SMP_THREADS, 2) sample_rows_kernel(const SmpAr
       himask = shift ? ~0ull << shift : ~0ull;
       prefix = (prefix & ~((u64)(SMP_BINS - 1) << shift)) | (u64)(SMP_BINS - 1 - s.bin) << shift;
     }
-    gather(bin, bin, himask, prefix);
+    const int cnt = (int)gather(bin, bin, himask, prefix);
+    leave();
     if (rank == 0) {
-      const int cnt = (int)s.count;
       smp_sort(S, cnt, top, bin, bin);
-      const int at = by_weight ? smp_place(S, cnt, left) : (int)left - 1;
+      const int at = by_weight ? smp_place(S, cnt, left, 0) : (int)left - 1;
       if (tid < NCTA) { SmpShared* o = other(tid); o->result_word = S.list[at]; o->result_cum = before_w + S.run[at]; }      // a thread for each CTA tells it
       if (tid == 0) S.filled = 0u;
     }
