@@ -372,14 +372,14 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
 #pragma unroll
     for (int i = 0; i < NR; i++) {
       mx[i] = fmaxf(fmaxf(y[i][0], y[i][1]), fmaxf(y[i][2], y[i][3]));
-      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
       up |= mx[i] > m[i] + PR_SLACK;
     }
     if (__any_sync(0xffffffffu, up)) {
       float fac[NR];
 #pragma unroll
       for (int i = 0; i < NR; i++) {
+        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
         fac[i] = mx[i] > m[i] ? pa_ex2(m[i] - mx[i]) : 1.f;              // 0 while there was nothing
         m[i] = fmaxf(m[i], mx[i]);
         l[i] *= fac[i];
@@ -510,6 +510,7 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
       }
     }
   };
+  const int seen_lo = c.window == 0 ? lo : max(lo, pmax - c.window + 1), seen_hi = min(pmin + 1, k1);         // what every row sees
   for (int it = 0; it < ng; it++) {
     pr_wait<NST - 2>();
     __syncwarp();                                                        // every lane has read the stage that is filled next
@@ -519,28 +520,35 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
     stage_out = stage_out + 1 == NST ? 0 : stage_out + 1;
     const int key = (g0 + it * PR_WARPS) * 16;
     const bool there = !((bad >> (it & 31)) & 1u);
-    const bool whole = key >= lo && key + 15 <= pmin && key + 16 <= k1 && (c.window == 0 || key > pmax - c.window) && there;
+    const bool whole = key >= seen_lo && key + 16 <= seen_hi && there;
     const uint2 v0 = *reinterpret_cast<const uint2*>(st + 32 * RB + 64 + 8 * cl), v1 = *reinterpret_cast<const uint2*>(st + 32 * RB + 96 + 8 * cl);
     unsigned vv[4] = {v0.x, v0.y, v1.x, v1.y};
-    // the largest and smallest exponent among the 16 value scales; a scale of NaN has none, one below 2^-90 is nothing
-    unsigned top = 0u, low = 255u << 23;
+    // Most groups: all 16 value scales within PR_FAR powers of two below the largest so far, by one difference a scale and one vote.
+    const unsigned least = (max(erun, PR_FAR + 37u) - PR_FAR) << 23, span = ((erun + 1u) << 23) - least;
+    const bool near = max(max(vv[0] - least, vv[1] - least), max(vv[2] - least, vv[3] - least)) < span;
+    bool easy = whole && __all_sync(0xffffffffu, near), far = false;
+    if (!easy) {
+      // the largest and smallest exponent among the 16 value scales; a scale of NaN has none, one below 2^-90 is nothing
+      unsigned top = 0u, low = 255u << 23;
 #pragma unroll
-    for (int j = 0; j < 4; j++) {
-      if (!whole && key + 8 * (j >> 1) + 2 * cl + (j & 1) >= k1) vv[j] = 0u;
-      const unsigned u = vv[j] < 0x7f800000u ? vv[j] : 0u;
-      top = max(top, u);
-      low = min(low, u < (37u << 23) ? 255u << 23 : u);
-    }
-    top = __reduce_max_sync(0xffffffffu, top) >> 23;
-    low = __reduce_min_sync(0xffffffffu, low) >> 23;
-    if (top > erun) {
-      const float down = __uint_as_float((unsigned)max(127 - (int)(top - erun), 0) << 23);
-      erun = top;
+      for (int j = 0; j < 4; j++) {
+        if (!whole && key + 8 * (j >> 1) + 2 * cl + (j & 1) >= k1) vv[j] = 0u;
+        const unsigned u = vv[j] < 0x7f800000u ? vv[j] : 0u;
+        top = max(top, u);
+        low = min(low, u < (37u << 23) ? 255u << 23 : u);
+      }
+      top = __reduce_max_sync(0xffffffffu, top) >> 23;
+      low = __reduce_min_sync(0xffffffffu, low) >> 23;
+      if (top > erun) {
+        const float down = __uint_as_float((unsigned)max(127 - (int)(top - erun), 0) << 23);
+        erun = top;
 #pragma unroll
-      for (int t = 0; t < NT; t++) { o[t][0] *= down; o[t][1] *= down; o[t][2] *= down; o[t][3] *= down; }
+        for (int t = 0; t < NT; t++) { o[t][0] *= down; o[t][1] *= down; o[t][2] *= down; o[t][3] *= down; }
+      }
+      far = low + PR_FAR < erun;
+      easy = whole && !far;
     }
-    const bool far = low + PR_FAR < erun;
-    if (whole && !far) group(std::true_type(), sa, st, key, vv, false, true);
+    if (easy) group(std::true_type(), sa, st, key, vv, false, true);
     else group(std::false_type(), sa, st, key, vv, far, there);
   }
 
