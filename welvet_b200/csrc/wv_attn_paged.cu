@@ -297,15 +297,15 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
   auto group = [&](auto plain, unsigned sa, const unsigned char* st, int key, const unsigned (&vv)[4], bool far, bool there) {
     constexpr bool PLAIN = decltype(plain)::value;
     const unsigned char* sc = st + 32 * RB;
-    // -------------------------------------------------------------- logits of two n-tiles of 8 keys, two chains of sums each
-    float s[2][2][4];
+    // -------------------------------------------------------------- logits of two n-tiles of 8 keys
+    float s[2][4];
 #pragma unroll
     for (int n = 0; n < 2; n++) {
       const int r = gl + 8 * n;
       auto step = [&](int k, unsigned b0, unsigned b1) {
-        if (k < 2) pr_mma0(s[n][k & 1], qfrag(R16 ? KS + k : k), b0, b1);
-        else pr_mma(s[n][k & 1], qfrag(R16 ? KS + k : k), b0, b1);
-        if (R16) pr_mma(s[n][k & 1], qfrag(k), b0, b1);                  // the small pieces first
+        if (k == 0) pr_mma0(s[n], qfrag(R16 ? KS + k : k), b0, b1);
+        else pr_mma(s[n], qfrag(R16 ? KS + k : k), b0, b1);
+        if (R16) pr_mma(s[n], qfrag(k), b0, b1);                  // the small pieces first
       };
       if constexpr (BITS == 4 && DP == 64) {
         const uint2 w = lds64(sa + kofs[0] + n * 8 * RB);
@@ -353,10 +353,10 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
       const int n = j >> 1, e = j & 1;
       f[j] = __uint_as_float(vv[j]) * inv;
       if (R16) {
-        y[0][j] = (s[n][0][e] + s[n][1][e]) * kk[j];
-        y[NR - 1][j] = (s[n][0][2 + e] + s[n][1][2 + e]) * kk[j];
+        y[0][j] = s[n][e] * kk[j];
+        y[NR - 1][j] = s[n][2 + e] * kk[j];
       } else {
-        y[0][j] = ((s[n][0][2 + e] + s[n][1][2 + e]) + (s[n][0][e] + s[n][1][e])) * kk[j];
+        y[0][j] = (s[n][2 + e] + s[n][e]) * kk[j];
       }
       if (!PLAIN) {
         const int p = key + 8 * n + 2 * cl + e;
