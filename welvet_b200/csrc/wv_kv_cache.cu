@@ -1,18 +1,27 @@
 // The paged key/value cache: rows rounded to 16, 8 or 4 bits as they are written, with the rotary embedding of Q and K in the same
 // pass, and read back. include/welvet_cuda.h (WvKvPages) defines layout and arithmetic.
 //
-// Bound: HBM for prompts, latency for single tokens. A CTA takes one token or four (their angles are the same for all heads), a warp
-// two rows of head_dim values at a time, a lane four consecutive values of each (and four more beyond 128): float4 in, 8 / 4 / 2
-// bytes of codes out, and a row's maximum is one reduction away. Four tokens share the chain of loads that finds a token's place (its
-// sequence, length, page) and fill the CTA with their angles.
+// Bound: HBM for prompts, latency for single tokens. A CTA takes one token or two (their angles are the same for all heads), a warp
+// a kv head's K and V and four query heads at a time, all of them under way at once (1.4 instructions wait for memory to one that
+// does not: it is the loads in flight that count); a lane holds four consecutive values of each row (and four more beyond 128): float4
+// in, 8 / 4 / 2 bytes of codes out, and a row's maximum is one reduction away. With heads of 128 the value that a value is turned with
+// comes from the lane 16 away; loading it a second time took 135 us for the prompts below. Two tokens share the chain of loads that finds
+// a token's place (its sequence, length, page) and fill the CTA with their angles.
+//
+// Prompts of 9900 tokens together, 32 query heads and 8 kv heads of 128, 8 bits, written and read back: 117 us, 4.4 TB/s
+// One token: 5.5 us; 200 tokens in 4 bits: 8.8 us (two launches each, captured in a graph).
 #include "wv_paged.cuh"
 #include <float.h>
 #include <math.h>
 #include <string.h>
 
 #define KVC_WARPS 8
-#define KVC_BLOCKS 4            // an SM: 64 registers (3 and 5 blocks take 138 us for prompts that take 135 with 4)
-#define KVC_TOKENS 4            // of a CTA, where there are enough of them
+// The prompts' times in us with other settings: 3 blocks 129, 5 blocks 134 (of 122 with 4); 2 heads 128 (122); 3, 4 and 6 tokens 119, 122, 124
+// (119); 2 rows 118 (117).
+#define KVC_BLOCKS 4            // an SM: 64 registers
+#define KVC_HEADS 4             // query heads of a warp at a time, heads of 128; else 2
+#define KVR_ROWS 4              // rows that a warp reads back at a time
+#define KVC_TOKENS 2            // of a CTA, where there are enough of them
 
 // theta^(2 d / head_dim) for every pair, computed on the host once per (theta, head_dim) and passed by value.
 struct WvRopeFreq { double p[128]; };
@@ -117,7 +126,7 @@ __device__ __forceinline__ void kv_store_row(const WvKvGeom& g, unsigned char* b
   if (lane == 0) *reinterpret_cast<float*>(block + (is_v ? g.vscale : g.kscale) + 4 * slot) = fine ? s : __uint_as_float(0x7fc00000u);
 }
 
-// grid (tokens / TOK, pieces of a token's rows)
+// grid (tokens / TOK, pieces of a token's rows). FULL: head_dim is 128.
 template <int BITS, int V4, int TOK, bool FULL>
 __global__ void __launch_bounds__(32 * KVC_WARPS, V4 == 1 ? KVC_BLOCKS : 2) kv_write_kernel(const WvKvGeom g, const WvKvBatch b, const float* __restrict__ k, int ldk,
                                                                   const float* __restrict__ v, int ldv, const float* q, int ldq, float* q_out,
@@ -127,7 +136,7 @@ __global__ void __launch_bounds__(32 * KVC_WARPS, V4 == 1 ? KVC_BLOCKS : 2) kv_w
   __shared__ KvPlace s_at[TOK];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int row0 = blockIdx.x * TOK, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hd = FULL ? 128 * V4 : g.hd, half = hd >> 1;
+  const int row0 = blockIdx.x * TOK, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hd = FULL ? 128 : g.hd, half = hd >> 1;
   if (warp < TOK) {
     KvPlace p{INT_MIN, -1, 0};      // a row that no sequence owns
     if (row0 + warp < b.total_q) p = kv_place(g, b, row0 + warp, err);
@@ -145,6 +154,7 @@ __global__ void __launch_bounds__(32 * KVC_WARPS, V4 == 1 ? KVC_BLOCKS : 2) kv_w
     }
     __syncthreads();
   }
+  constexpr int U = FULL ? KVC_HEADS : 2;
   const int gw = blockIdx.y * KVC_WARPS + warp, nw = gridDim.y * KVC_WARPS;
   for (int tok = 0; tok < TOK; tok++) {
     const KvPlace at = s_at[tok];
@@ -173,12 +183,18 @@ __global__ void __launch_bounds__(32 * KVC_WARPS, V4 == 1 ? KVC_BLOCKS : 2) kv_w
         x[i][0] = o.x; x[i][1] = o.y; x[i][2] = o.z; x[i][3] = o.w;
       }
     };
-    auto partners = [&](const float* src, float (&x)[V4][4], bool on) {
+    // what x is turned with: the value half a head away, which another lane holds
+    auto partners = [&](const float* src, const float (&x)[V4][4], float (&w)[V4][4], bool on) {
 #pragma unroll
       for (int i = 0; i < V4; i++) {
-        const int d = 4 * (lane + 32 * i);
-        const float4 o = on && (FULL || d < hd) ? *reinterpret_cast<const float4*>(src + (d < half ? d + half : d - half)) : make_float4(0.f, 0.f, 0.f, 0.f);
-        x[i][0] = o.x; x[i][1] = o.y; x[i][2] = o.z; x[i][3] = o.w;
+        if (FULL) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) w[i][e] = __shfl_xor_sync(0xffffffffu, x[i][e], 16);
+        } else {
+          const int d = 4 * (lane + 32 * i);
+          const float4 o = on && d < hd ? *reinterpret_cast<const float4*>(src + (d < half ? d + half : d - half)) : make_float4(0.f, 0.f, 0.f, 0.f);
+          w[i][0] = o.x; w[i][1] = o.y; w[i][2] = o.z; w[i][3] = o.w;
+        }
       }
     };
     auto turn = [&](float (&x)[V4][4], const float (&w)[V4][4]) {
@@ -201,34 +217,47 @@ __global__ void __launch_bounds__(32 * KVC_WARPS, V4 == 1 ? KVC_BLOCKS : 2) kv_w
         for (int e = 0; e < 4; e++) x[i][e] = y[e];
       }
     };
-    // two query heads at a time
-    for (int h = 2 * gw; h < heads; h += 2 * nw) {
-      float x[2][V4][4], w[2][V4][4];
+    // a kv head's K and V, the last warps first: with few tokens they have no query heads. They are under way while Q is turned.
+    const int hk = nw - 1 - gw;
+    const bool kv = at.page >= 0 && hk < g.kvh;
+    float x[V4][4], y[V4][4];
+    load(k + row * ldk + (size_t)hk * hd, x, kv);
+    load(v + row * ldv + (size_t)hk * hd, y, kv);
+    // U query heads at a time
+    for (int h = U * gw; h < heads; h += U * nw) {
+      float z[U][V4][4], w[FULL ? 1 : U][V4][4];
       const float* src = q + row * ldq + (size_t)h * hd;
-      load(src, x[0], true); load(src + hd, x[1], h + 1 < heads);
-      if (rotate) { partners(src, w[0], true); partners(src + hd, w[1], h + 1 < heads); }
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        load(src + u * hd, z[u], h + u < heads);
+        if (!FULL && rotate) partners(src + u * hd, z[u], w[FULL ? 0 : u], h + u < heads);
+      }
       __syncwarp();                 // in place: every lane has its partner's value
       float* dst = q_out + row * ldqo + (size_t)h * hd;
 #pragma unroll
-      for (int u = 0; u < 2; u++) {
-        if (u && h + 1 >= heads) break;
-        if (rotate) turn(x[u], w[u]);
+      for (int u = 0; u < U; u++) {
+        if (h + u >= heads) break;
+        if (FULL && rotate) partners(src, z[u], w[0], true);
+        if (rotate) turn(z[u], w[FULL ? 0 : u]);
 #pragma unroll
         for (int i = 0; i < V4; i++) {
           const int d = 4 * (lane + 32 * i);
-          if ((FULL || d < hd)) *reinterpret_cast<float4*>(dst + u * hd + d) = make_float4(x[u][i][0], x[u][i][1], x[u][i][2], x[u][i][3]);
+          if ((FULL || d < hd)) *reinterpret_cast<float4*>(dst + u * hd + d) = make_float4(z[u][i][0], z[u][i][1], z[u][i][2], z[u][i][3]);
         }
       }
     }
-    // a kv head's K and V, the last warps first: with few tokens they have no query heads
-    if (at.page < 0) continue;
-    for (int h = nw - 1 - gw; h < g.kvh; h += nw) {
-      float x[V4][4], w[V4][4], y[V4][4];
+    if (!kv) continue;
+    for (int h = hk; h < g.kvh; h += nw) {
       const float* src = k + row * ldk + (size_t)h * hd;
-      load(src, x, true);
-      if (rotate) partners(src, w, true);
-      load(v + row * ldv + (size_t)h * hd, y, true);
-      if (rotate) turn(x, w);
+      if (h != hk) {
+        load(src, x, true);
+        load(v + row * ldv + (size_t)h * hd, y, true);
+      }
+      if (rotate) {
+        float w[V4][4];
+        partners(src, x, w, true);
+        turn(x, w);
+      }
       unsigned char* block = g.pool + ((size_t)at.page * g.kvh + h) * g.block;
       kv_store_row<BITS, V4, FULL>(g, block, false, at.slot, x, lane);
       kv_store_row<BITS, V4, FULL>(g, block, true, at.slot, y, lane);
@@ -250,40 +279,59 @@ __global__ void __launch_bounds__(32 * KVC_WARPS) kv_read_kernel(const WvKvGeom 
   }
   __syncthreads();
   const int nr = 2 * g.kvh;
-#pragma unroll 4
-  for (int i0 = blockIdx.y * KVC_WARPS + warp; i0 < TOK * nr; i0 += gridDim.y * KVC_WARPS) {
-    const int tok = TOK == 1 ? 0 : i0 / nr, r = i0 - tok * nr;
-    const KvPlace at = s_at[tok];
-    if (at.pos == INT_MIN) continue;
-    const size_t row = row0 + tok;
-    const bool is_v = r >= g.kvh;
-    const int h = is_v ? r - g.kvh : r;
-    float* dst = (is_v ? v + row * ldv : k + row * ldk) + (size_t)h * g.hd;
-    const unsigned char* block = g.pool + ((size_t)max(at.page, 0LL) * g.kvh + h) * g.block;
-    const unsigned char* codes = block + (is_v ? g.page * g.code : 0) + at.slot * g.code;
-    const float s = at.page < 0 ? 0.f : *reinterpret_cast<const float*>(block + (is_v ? g.vscale : g.kscale) + 4 * at.slot);
+  // KVR_ROWS rows of a warp at a time: their loads are all under way before the first is stored
+  const int step = gridDim.y * KVC_WARPS;
+  for (int r0 = blockIdx.y * KVC_WARPS + warp; r0 < TOK * nr; r0 += KVR_ROWS * step) {
+    float* dst[KVR_ROWS];
+    float s[KVR_ROWS];
+    uint2 w[KVR_ROWS][V4];
+    int t[KVR_ROWS][V4];
 #pragma unroll
-    for (int i = 0; i < V4; i++) {
-      const int d = 4 * (lane + 32 * i);
-      if (d >= g.hd) break;
-      float c[4] = {0.f, 0.f, 0.f, 0.f};
-      if (at.page >= 0) {
-        if (BITS == 16) {
-          const uint2 w = *reinterpret_cast<const uint2*>(codes + 2 * d);
-          const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&w.x)), hi = __half22float2(*reinterpret_cast<const __half2*>(&w.y));
-          c[0] = lo.x; c[1] = lo.y; c[2] = hi.x; c[3] = hi.y;
-        } else if (BITS == 8) {
-          const unsigned w = *reinterpret_cast<const unsigned*>(codes + d);
+    for (int u = 0; u < KVR_ROWS; u++) {
+      const int i0 = r0 + u * step, tok = TOK == 1 ? 0 : i0 / nr, r = i0 - tok * nr;
+      dst[u] = nullptr;
+      if (i0 >= TOK * nr || s_at[tok].pos == INT_MIN) continue;
+      const KvPlace at = s_at[tok];
+      const size_t row = row0 + tok;
+      const bool is_v = r >= g.kvh;
+      const int h = is_v ? r - g.kvh : r;
+      dst[u] = (is_v ? v + row * ldv : k + row * ldk) + (size_t)h * g.hd;
+      const unsigned char* block = g.pool + ((size_t)max(at.page, 0LL) * g.kvh + h) * g.block;
+      const unsigned char* codes = block + (is_v ? g.page * g.code : 0) + at.slot * g.code;
+      s[u] = at.page < 0 ? 0.f : *reinterpret_cast<const float*>(block + (is_v ? g.vscale : g.kscale) + 4 * at.slot);
 #pragma unroll
-          for (int e = 0; e < 4; e++) c[e] = (float)(int)(signed char)(w >> (8 * e));
-        } else {
-          const unsigned w = *reinterpret_cast<const unsigned short*>(codes + d / 2);
-          const int t = block[(is_v ? g.vsub : g.ksub) + at.slot * (g.hd / 16) + d / 16];
-#pragma unroll
-          for (int e = 0; e < 4; e++) c[e] = (float)(((int)((w >> (4 * e)) & 15u) - 8) * t);
+      for (int i = 0; i < V4; i++) {
+        const int d = 4 * (lane + 32 * i);
+        w[u][i] = make_uint2(BITS == 4 ? 0x8888u : 0u, 0u);              // no page: zeros
+        t[u][i] = 0;
+        if (d >= g.hd || at.page < 0) continue;
+        if (BITS == 16) w[u][i] = *reinterpret_cast<const uint2*>(codes + 2 * d);
+        if (BITS == 8) w[u][i].x = *reinterpret_cast<const unsigned*>(codes + d);
+        if (BITS == 4) {
+          w[u][i].x = *reinterpret_cast<const unsigned short*>(codes + d / 2);
+          t[u][i] = block[(is_v ? g.vsub : g.ksub) + at.slot * (g.hd / 16) + d / 16];
         }
       }
-      *reinterpret_cast<float4*>(dst + d) = make_float4(s * c[0], s * c[1], s * c[2], s * c[3]);
+    }
+#pragma unroll
+    for (int u = 0; u < KVR_ROWS; u++) {
+      if (!dst[u]) continue;
+#pragma unroll
+      for (int i = 0; i < V4; i++) {
+        const int d = 4 * (lane + 32 * i);
+        if (d >= g.hd) break;
+        float c[4];
+        if (BITS == 16) {
+          const float2 lo = __half22float2(*reinterpret_cast<const __half2*>(&w[u][i].x)), hi = __half22float2(*reinterpret_cast<const __half2*>(&w[u][i].y));
+          c[0] = lo.x; c[1] = lo.y; c[2] = hi.x; c[3] = hi.y;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          if (BITS == 8) c[e] = (float)(int)(signed char)(w[u][i].x >> (8 * e));
+          if (BITS == 4) c[e] = (float)(((int)((w[u][i].x >> (4 * e)) & 15u) - 8) * t[u][i]);
+        }
+        *reinterpret_cast<float4*>(dst[u] + d) = make_float4(s[u] * c[0], s[u] * c[1], s[u] * c[2], s[u] * c[3]);
+      }
     }
   }
 }
