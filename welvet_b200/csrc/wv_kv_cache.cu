@@ -2,13 +2,12 @@
 // pass, and read back. include/welvet_cuda.h (WvKvPages) defines layout and arithmetic.
 //
 // Bound: HBM for prompts, latency for single tokens. A CTA takes one token or two (their angles are the same for all heads), a warp
-// a kv head's K and V and four query heads at a time, all of them under way at once (1.4 instructions wait for memory to one that
-// does not: it is the loads in flight that count); a lane holds four consecutive values of each row (and four more beyond 128): float4
-// in, 8 / 4 / 2 bytes of codes out, and a row's maximum is one reduction away. With heads of 128 the value that a value is turned with
-// comes from the lane 16 away; loading it a second time took 135 us for the prompts below. Two tokens share the chain of loads that finds
-// a token's place (its sequence, length, page) and fill the CTA with their angles.
+// a kv head's K and V and four query heads at a time, all of them under way at once; a lane holds four consecutive values of each row
+// (and four more beyond 128): float4 in, 8 / 4 / 2 bytes of codes out, and a row's maximum is one reduction away. With heads of 128 the
+// value that a value is turned with comes from the lane 16 away; loading it a second time took 135 us for the prompts below. Two tokens
+// share the chain of loads that finds a token's place (its sequence, length, page) and fill the CTA with their angles.
 //
-// Prompts of 9900 tokens together, 32 query heads and 8 kv heads of 128, 8 bits, written and read back: 117 us, 4.4 TB/s
+// Prompts of 9900 tokens together, 32 query heads and 8 kv heads of 128, 8 bits, written and read back: 117 us, 4.4 TB/s.
 // One token: 5.5 us; 200 tokens in 4 bits: 8.8 us (two launches each, captured in a graph).
 #include "wv_paged.cuh"
 #include <float.h>
