@@ -13,9 +13,14 @@
 // memory: the order of the products does not matter for K, and for V it only decides which output a lane holds. Rows lie in the
 // ring with their 16-byte pieces permuted so that both reading patterns are free of bank conflicts.
 //
-// Four warps a block, two blocks an SM, so that one block's start (three dependent loads: lengths, page numbers, rows) runs beside
-// another's keys. The keys of a sequence are split over blocks; the splits leave {M, divisor, sums} and a second kernel joins them
-// in order, so results do not depend on who ran first.
+// Four warps a block and three blocks an SM (two with 16-bit rows of 128 or 16 query rows, see pr_blocks), so that one block's start (three
+// dependent loads: lengths, page numbers, rows) runs beside another's keys. The keys of a sequence are split over blocks; the splits
+// leave {M, divisor, sums} and a second kernel joins them in order, so results do not depend on who ran first.
+//
+// Measured: one token over 2049 positions (32 heads, 8 kv heads of 128, 16 bits) 10 us; over 131000 positions in 4 bits (64 heads) 70 us,
+// 2.3 TB/s of codes and scales; 64 tokens over up to 8192 positions in 8 bits 127 us, 4.4 TB/s; 16 x 5 tokens over 3000, heads of 64 in
+// 16 bits, 26 us. What bounds the long ones is issue: 525 instructions per 16 keys in 4 bits, 450 in 8 bits, 0.55 a cycle and scheduler
+// with three blocks; a fourth (q's fragments out of shared memory, 128 registers) issues no more and took 79 and 191 us.
 #include "wv_attn_paged.cuh"
 #include "wv_tma_common.cuh"
 #include "wv_lease.h"
@@ -37,10 +42,14 @@ template <int BITS, int DP> struct PrShape {
   static constexpr int NCP = (RB + 31) / 32;                             // copies of 16 bytes that a lane makes for K's 16 rows (and for V's)
 };
 
-// Blocks an SM: three where the registers allow it (up to 8 rows of 128 values), and the stages of a warp's ring in what they leave.
+// Blocks an SM: three where the registers allow it (up to 8 rows of 128 values). wv_launch_attn_paged splits the keys over as many.
+__host__ __device__ constexpr int pr_blocks(int bits, int dp, bool r16) {
+  return dp == 256 && (bits == 16 || r16) ? 1 : !r16 && (dp == 64 || (dp == 128 && bits < 16)) ? 3 : 2;
+}
+// And the stages of a warp's ring in what they leave.
 template <int BITS, int DP, bool R16> struct PrFit {
   static constexpr int STAGE = PrShape<BITS, DP>::STAGE;
-  static constexpr int BLOCKS = DP == 256 && (BITS == 16 || R16) ? 1 : !R16 && (DP == 64 || (DP == 128 && BITS < 16)) ? 3 : 2;
+  static constexpr int BLOCKS = pr_blocks(BITS, DP, R16);
   static constexpr int FIT = (BLOCKS == 3 ? 35 * 512 : 25 * 1024) / STAGE;
   static constexpr int NST = FIT < 2 ? 2 : (FIT > 8 ? 8 : FIT);
 };
@@ -301,7 +310,7 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
     float s[2][4];
 #pragma unroll
     for (int n = 0; n < 2; n++) {
-      const int r = gl + 8 * n;
+      [[maybe_unused]] const int r = gl + 8 * n;
       auto step = [&](int k, unsigned b0, unsigned b1) {
         if (k == 0) pr_mma0(s[n], qfrag(R16 ? KS + k : k), b0, b1);
         else pr_mma(s[n], qfrag(R16 ? KS + k : k), b0, b1);
@@ -417,7 +426,7 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
       if (R16) pr_mma(o[t], pl, b0, b1);
       pr_mma(o[t], ph, b0, b1);
     };
-    const int rows4[4] = {2 * cl, 2 * cl + 1, 2 * cl + 8, 2 * cl + 9};
+    [[maybe_unused]] const int rows4[4] = {2 * cl, 2 * cl + 1, 2 * cl + 8, 2 * cl + 9};
     if (!PLAIN && far) {                                                 // value by value in float32
 #pragma unroll 1
       for (int j = 0; j < 16; j++) {
@@ -690,7 +699,7 @@ int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* d
     if (blocks * (r16 ? 16 : 8) > INT_MAX) { wv_set_error("wv_attn_paged_dev: %d sequences are too many", b.num_seqs); return WV_ESHAPE; }
     // Splits of the keys: the number that fills 1, 2, .. 8 waves of the blocks that run at once and costs least, a wave being worth a
     // warp's groups of 16 keys and some six more of start and end (2049 positions and eight blocks: 33 splits of 64; 131000: 55).
-    const long long slots = (long long)sms * (c.g.hd > 128 ? (r16 || kv.bits == 16 ? 1 : 2) : !r16 && (c.g.hd <= 64 || kv.bits < 16) ? 3 : 2);
+    const long long slots = (long long)sms * pr_blocks(kv.bits, c.g.hd <= 64 ? 64 : c.g.hd <= 128 ? 128 : 256, r16);
     long long per = 64, cost = -1;
     for (long long w = 1; w <= 8; w++) {
       long long n = w * slots / blocks;
