@@ -17,18 +17,20 @@
 // dependent loads: lengths, page numbers, rows) runs beside another's keys. The keys of a sequence are split over blocks; the splits
 // leave {M, divisor, sums} and a second kernel joins them in order, so results do not depend on who ran first.
 //
-// Measured: one token over 2049 positions (32 heads, 8 kv heads of 128, 16 bits) 10 us; over 131000 positions in 4 bits (64 heads) 70 us,
-// 2.3 TB/s of codes and scales; 64 tokens over up to 8192 positions in 8 bits 127 us, 4.4 TB/s; 16 x 5 tokens over 3000, heads of 64 in
-// 16 bits, 26 us. What bounds the long ones is issue: 525 instructions per 16 keys in 4 bits, 450 in 8 bits, 0.55 a cycle and scheduler
+// Measured: one token over 2049 positions (32 heads, 8 kv heads of 128, 16 bits) 10 us; over 131000 positions in 4 bits (64 heads) 71 us,
+// 2.3 TB/s of codes and scales; 64 tokens over up to 8192 positions in 8 bits 130 us, 4.3 TB/s; 16 x 5 tokens over 3000, heads of 64 in
+// 16 bits, 29 us. What bounds the long ones is issue: 535 instructions per 16 keys in 4 bits, 460 in 8 bits, 0.55 a cycle and scheduler
 // with three blocks; a fourth (q's fragments out of shared memory, 128 registers) issues no more and took 79 and 191 us.
 #include "wv_attn_paged.cuh"
 #include "wv_tma_common.cuh"
 #include "wv_lease.h"
+#include <algorithm>
 #include <type_traits>
 
 int wv_sm_count();
 
 #define PR_WARPS 4
+#define PR_CHAIN 40           // products that a warp adds to its sums at most, see wv_launch_attn_paged
 // The running maximum is raised only when a logit is 2^7 above it (the sums, 64 registers a lane, are multiplied each time), so weights
 // reach 2^7 and carry 2^6 instead of 2^13: at most 2^14, and 2^-30 of that is still there.
 #define PR_LIFT 6.f
@@ -306,15 +308,15 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
   auto group = [&](auto plain, unsigned sa, const unsigned char* st, int key, const unsigned (&vv)[4], bool far, bool there) {
     constexpr bool PLAIN = decltype(plain)::value;
     const unsigned char* sc = st + 32 * RB;
-    // -------------------------------------------------------------- logits of two n-tiles of 8 keys
-    float s[2][4];
+    // -------------------------------------------------------------- logits of two n-tiles of 8 keys, two chains of sums each
+    float s[2][2][4];
 #pragma unroll
     for (int n = 0; n < 2; n++) {
       [[maybe_unused]] const int r = gl + 8 * n;
       auto step = [&](int k, unsigned b0, unsigned b1) {
-        if (k == 0) pr_mma0(s[n], qfrag(R16 ? KS + k : k), b0, b1);
-        else pr_mma(s[n], qfrag(R16 ? KS + k : k), b0, b1);
-        if (R16) pr_mma(s[n], qfrag(k), b0, b1);                  // the small pieces first
+        if (k < 2) pr_mma0(s[n][k & 1], qfrag(R16 ? KS + k : k), b0, b1);
+        else pr_mma(s[n][k & 1], qfrag(R16 ? KS + k : k), b0, b1);
+        if (R16) pr_mma(s[n][k & 1], qfrag(k), b0, b1);                  // the small pieces first
       };
       if constexpr (BITS == 4 && DP == 64) {
         const uint2 w = lds64(sa + kofs[0] + n * 8 * RB);
@@ -362,10 +364,10 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
       const int n = j >> 1, e = j & 1;
       f[j] = __uint_as_float(vv[j]) * inv;
       if (R16) {
-        y[0][j] = s[n][e] * kk[j];
-        y[NR - 1][j] = s[n][2 + e] * kk[j];
+        y[0][j] = (s[n][0][e] + s[n][1][e]) * kk[j];
+        y[NR - 1][j] = (s[n][0][2 + e] + s[n][1][2 + e]) * kk[j];
       } else {
-        y[0][j] = (s[n][2 + e] + s[n][e]) * kk[j];
+        y[0][j] = ((s[n][0][2 + e] + s[n][1][2 + e]) + (s[n][0][e] + s[n][1][e])) * kk[j];
       }
       if (!PLAIN) {
         const int p = key + 8 * n + 2 * cl + e;
@@ -700,11 +702,14 @@ int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* d
     // Splits of the keys: the number that fills 1, 2, .. 8 waves of the blocks that run at once and costs least, a wave being worth a
     // warp's groups of 16 keys and some six more of start and end (2049 positions and eight blocks: 33 splits of 64; 131000: 55).
     const long long slots = (long long)sms * pr_blocks(kv.bits, c.g.hd <= 64 ? 64 : c.g.hd <= 128 ? 128 : 256, r16);
+    // The tensor core cuts instead of rounding as it adds, so the error grows with the products that a warp adds to its sums one
+    // after the other (two a group with 16 rows): 3e-7 after 8, 9e-7 after 38, 7e-6 after 380. No more than 40 of them.
+    const long long longest = 64 * (r16 ? PR_CHAIN / 2 : PR_CHAIN);
     long long per = 64, cost = -1;
     for (long long w = 1; w <= 8; w++) {
       long long n = w * slots / blocks;
       if (n < 1) { if (w < 8) continue; n = 1; }
-      long long p = ((keys + n - 1) / n + 63) & ~63LL;
+      long long p = std::min(((keys + n - 1) / n + 63) & ~63LL, longest);
       if (p < 64) p = 64;
       const long long m = keys > p ? (keys + p - 1) / p : 1, k = (blocks * m + slots - 1) / slots * (p / 64 + 6);
       if (cost < 0 || k < cost) { cost = k; per = p; }
