@@ -299,6 +299,32 @@ def test_attention_sharp_and_flat(wv):
         check_attn(wv, 16, 16, 4, 2, 128, [(1, 1000), (70, 500)], seed=3, spread=spread)
 
 
+@pytest.mark.parametrize("nq", [1, 3])
+def test_long_sequences_of_a_full_batch(wv, nq):
+    """So many sequences that none has to be split to fill the chip: the sums over 12000 positions are as exact as those over a few.
+    Bound: at most 40 additions that cut off up to 2^-23 of a sum one after the other, half of that on average, and as much again for
+    weights, divisor and the sums of the parts."""
+    seqs, kv, heads, hd, dev = 160, 12000, 4, 64, "cuda"
+    gen = torch.Generator(device=dev).manual_seed(5)
+    rand = lambda *n: torch.randn(*n, device=dev, generator=gen)  # noqa: E731
+    c = Cache(wv, 8, 64, 1, hd, [(nq, kv)])
+    c.fill(rand(kv, hd), rand(kv, hd))
+    k, v = torch.zeros(kv, hd, device=dev), torch.zeros(kv, hd, device=dev)
+    whole, keep = c.batch_of([(kv, kv)])
+    wv.paged.KVReadCUDA(c.pages, whole, k.data_ptr(), v.data_ptr())
+    table = c.d_table.repeat(seqs, 1)                                     # one sequence's pages for all of them
+    start, lens = torch.arange(seqs + 1, dtype=torch.int32, device=dev) * nq, torch.full((seqs,), kv, dtype=torch.int32, device=dev)
+    b = wv.paged.Batch(start.data_ptr(), lens.data_ptr(), table.data_ptr(), seqs, table.shape[1], seqs * nq, nq, kv)
+    q, out = rand(seqs * nq, heads * hd), torch.zeros(seqs * nq, heads * hd, device=dev)
+    wv.paged.AttnPagedCUDA(c.pages, b, q.data_ptr(), out.data_ptr(), heads, 0.125)
+    torch.cuda.synchronize()
+    s = q.double().view(seqs, nq, heads, hd) @ k.double().T * 0.125
+    last = kv - nq + torch.arange(nq, device=dev)
+    s = s.masked_fill(torch.arange(kv, device=dev) > last[:, None, None], -math.inf)
+    want = (torch.softmax(s, -1) @ v.double()).view(seqs * nq, heads * hd)
+    assert ((out.double() - want).norm() / want.norm()).item() <= 2 * 40 * 2.0 ** -24
+
+
 def test_rows_that_see_nothing(wv):
     """More new tokens than the cache holds: positions before 0 give zeros."""
     lens = [(5, 3), (70, 64), (2, 0)]
