@@ -293,6 +293,20 @@ def test_attention_window(wv, window, lens):
         check_attn(wv, bits, 16, 4, 2, 64, lens, window=window, seed=window)
 
 
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 2, 2 ** 30, 301, 300, 299, -5])
+@pytest.mark.parametrize("lens", [[(2, 300), (5, 3), (2, 0)], [(310, 300), (70, 64), (1, 90)]])
+def test_windows_wider_than_the_cache(wv, window, lens):
+    """A window that no sequence fills, up to the largest number, is none, with rows before position 0 as well."""
+    for bits in (16, 4):
+        check_attn(wv, bits, 16, 4, 1, 64, lens, window=max(window, 0))
+        c = Cache(wv, bits, 16, 1, 64, lens)
+        n, total = sum(k for _, k in lens), sum(q for q, _ in lens)
+        c.fill(torch.randn(n, 64, device="cuda"), torch.randn(n, 64, device="cuda"))
+        q = torch.randn(total, 256, device="cuda")
+        if window < 0 or window >= 300:
+            assert np.array_equal(run_attn(c, q, 4, 0.125, window=window), run_attn(c, q, 4, 0.125))
+
+
 def test_attention_sharp_and_flat(wv):
     """Weights on a single key, and equal keys: the running maximum has to move and to stay."""
     for spread in (30.0, 0.0, 1e-3):

@@ -473,5 +473,6 @@ extern "C" int wv_attn_paged_dev(const WvKvPages* kv, const WvKvBatch* batch, co
   const long long qw = (long long)num_heads * kv->head_dim;
   if ((rc = kv_rows(who, "q", dq, &ldq, qw)) || (rc = kv_rows(who, "out", dout, &ldo, qw))) return rc;
   if (none) return WV_OK;
-  return wv_launch_attn_paged(*kv, *batch, dq, ldq, dout, ldo, num_heads, scale, window > 0 ? window : 0, static_cast<cudaStream_t>(stream));
+  if (window < 0 || window >= batch->max_kv) window = 0;              // wider than any sequence: none
+  return wv_launch_attn_paged(*kv, *batch, dq, ldq, dout, ldo, num_heads, scale, window, static_cast<cudaStream_t>(stream));
 }
