@@ -831,7 +831,7 @@ static cudaError_t chunk_go(const PaCall& c, long long flat, cudaStream_t st) {
   return cudaLaunchKernelEx(&cfg, chunk_join_kernel, c);
 }
 
-// keys: what a sequence's new tokens see at most; alike: every sequence has max_q new tokens.
+// keys: what a sequence's new tokens see at most; alike: every sequence can have max_q new tokens.
 int wv_launch_attn_chunk(PaCall c, int bits, long long keys, bool alike, cudaStream_t st) {
   const long long each = ((long long)c.b.max_q * c.group + 255) / 256, upto = (long long)c.b.total_q * c.group / 256 + c.b.num_seqs;
   const long long flat = alike || c.b.num_seqs * each < upto ? c.b.num_seqs * each : upto, blocks = flat * c.g.kvh;

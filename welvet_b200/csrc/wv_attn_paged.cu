@@ -687,8 +687,11 @@ int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* d
   // Up to 32 rows (tokens x query heads of a kv head) a sequence is taken 8 or 16 rows at a time, beyond in tiles of 128.
   const long long most = (long long)b.max_q * c.group;
   c.rows_most = c.g.hd <= 128 ? 32 : INT_MAX;
-  const bool alike = (long long)b.num_seqs * b.max_q == b.total_q;       // every sequence has max_q new tokens
+  // Where every sequence can have max_q new tokens they are expected to, and one kernel takes them all. They need not (the lengths are
+  // the device's, and may be others in each replay of a graph): that kernel then takes the short ones too.
+  const bool alike = (long long)b.num_seqs * b.max_q == b.total_q;
   const bool chunk = most > c.rows_most, rows = !chunk || !alike;
+  if (!rows) c.rows_most = 0;
   if ((long long)b.total_q * heads > INT_MAX) { wv_set_error("wv_attn_paged_dev: %d rows of %d heads are too many", b.total_q, heads); return WV_ESHAPE; }
   // what a sequence's new tokens can see together
   const long long keys = window > 0 && (long long)window + b.max_q + 16 < b.max_kv ? (long long)window + b.max_q + 16 : b.max_kv;

@@ -18,7 +18,7 @@ struct PaCall {
   float scale;                     // times log2(e)
   int window;                      // 0: none
   unsigned one;                    // 0x3c003c00, for pa_nibbles
-  int rows_most;                   // sequences with more rows (tokens x group) than this go to the chunk kernel
+  int rows_most;                   // sequences with more rows (tokens x group) than this go to the chunk kernel (0: all that have any)
   int nsplit, per;                 // splits of a sequence's keys, keys of a split (a multiple of 16; of 128 for chunks)
   float2* ml;                      // split results [row][nsplit]: {M, divisor}; {-inf, 0} and no sums for a split without keys
   float* acc;                      // [row][nsplit][head_dim]
