@@ -171,7 +171,8 @@ int wv_topk_sample(const float* d_logits, int n, int top_k, float temperature, i
  * it are not touched), kv_len[num_seqs] tokens of each sequence in the cache, its new ones included, pages[num_seqs][table_stride] the
  * page that holds tokens i * page_size and on. A sequence may have no new tokens, or none at all. max_q and max_kv bound the
  * lengths. A length, row or page number beyond these bounds is cut to them on the device, its page is not read or
- * written, and wv_device_status() then reports WV_ESHAPE. A sequence must not hold a page twice, nor two sequences a page that
+ * written, and wv_device_status() then reports WV_ESHAPE. Of a sequence with more than max_q new tokens the first max_q are taken, at
+ * the positions that they have; the other rows belong to nobody. A sequence must not hold a page twice, nor two sequences a page that
  * either of them writes.
  *
  * Row strides (ld*) count floats, 0 stands for rows without a gap; they are multiples of 4 and the vectors 16-byte

@@ -91,3 +91,59 @@ def test_few_and_many_tokens_under_loose_bounds(wv):
         want, tol = want_attn(c, lens, q, heads, 0.125)
         assert (np.abs(out.cpu().numpy().reshape(total, heads, hd) - want) <= tol).all(), lens
         assert wv._lib.lib().wv_device_status() == 0
+
+
+@pytest.mark.parametrize("max_q,long", [(4, 7), (4, 60), (64, 67), (64, 150)])
+def test_more_tokens_than_max_q(wv, max_q, long):
+    """A sequence in the midst of others with more new tokens than max_q: reported, its first max_q ones are taken at the places that
+    they have, the others' rows and places are left as they were, and the other sequences do not notice; in all three calls."""
+    heads, kvh, hd, scale = 8, 2, 64, 0.125
+    lens = [(3, 90), (long, 200), (max_q, 100)]
+    c = Cache(wv, 8, 16, kvh, hd, lens, seed=long)
+    rng = np.random.default_rng(long)
+    n, total = sum(k for _, k in lens), sum(q for q, _ in lens)
+    rand = lambda *s: torch.from_numpy(rng.normal(0, 1, s).astype(np.float32)).cuda()  # noqa: E731
+    c.fill(rand(n, kvh * hd), rand(n, kvh * hd))
+    status = wv._lib.lib().wv_device_status
+    batch, keep = c.batch_of(lens, max_q=max_q)
+    whole = c.keep, c.batch
+    mine = np.ones(total, bool)
+    mine[3 + max_q:3 + long] = False                                      # the rows that nobody takes
+    q = rng.normal(0, 1, (total, heads * hd)).astype(np.float32)
+    out = torch.full((total, heads * hd), 7.0, device="cuda")
+    wv.paged.AttnPagedCUDA(c.pages, batch, torch.from_numpy(q).cuda().data_ptr(), out.data_ptr(), heads, scale)
+    torch.cuda.synchronize()
+    assert status() == wv._lib.WV_ESHAPE
+    got = out.cpu().numpy().reshape(total, heads, hd)
+    want, tol = want_attn(c, lens, q, heads, scale)
+    assert (np.abs(got - want) <= tol)[mine].all() and (got[~mine] == 7.0).all()
+    # what the cache holds, read back
+    full = [torch.full((total, kvh * hd), 5.0, device="cuda") for _ in range(2)]
+    part = [torch.full((total, kvh * hd), 5.0, device="cuda") for _ in range(2)]
+    wv.paged.KVReadCUDA(c.pages, whole[1], *[t.data_ptr() for t in full])
+    torch.cuda.synchronize()
+    assert status() == 0
+    wv.paged.KVReadCUDA(c.pages, batch, *[t.data_ptr() for t in part])
+    torch.cuda.synchronize()
+    assert status() == wv._lib.WV_ESHAPE
+    m = torch.from_numpy(mine).cuda()
+    for f, p in zip(full, part):
+        assert torch.equal(p[m], f[m]) and (p[~m] == 5.0).all()
+    # written anew, with the queries turned
+    k, v, before = rand(total, kvh * hd), rand(total, kvh * hd), c.pool.clone()
+    dq, qo = rand(total, heads * hd), torch.full((total, heads * hd), 5.0, device="cuda")
+    qf = torch.zeros_like(qo)
+    wv.paged.KVWriteCUDA(c.pages, batch, k.data_ptr(), v.data_ptr(), dq.data_ptr(), qo.data_ptr(), heads, 10000.0)
+    torch.cuda.synchronize()
+    assert status() == wv._lib.WV_ESHAPE
+    some = [torch.zeros_like(t) for t in full]
+    wv.paged.KVReadCUDA(c.pages, whole[1], *[t.data_ptr() for t in some])
+    c.pool.copy_(before)
+    wv.paged.KVWriteCUDA(c.pages, whole[1], k.data_ptr(), v.data_ptr(), dq.data_ptr(), qf.data_ptr(), heads, 10000.0)
+    every = [torch.zeros_like(t) for t in full]
+    wv.paged.KVReadCUDA(c.pages, whole[1], *[t.data_ptr() for t in every])
+    torch.cuda.synchronize()
+    assert status() == 0
+    assert torch.equal(qo[m], qf[m]) and (qo[~m] == 5.0).all()
+    for f, s, e in zip(full, some, every):
+        assert torch.equal(s[m], e[m]) and torch.equal(s[~m], f[~m])

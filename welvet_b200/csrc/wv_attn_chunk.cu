@@ -131,7 +131,7 @@ __device__ __forceinline__ void pc_find(const PaCall& c, int flat, int* err, int
     if (s0 + lane < c.b.num_seqs) {
       const WvSeq q = wv_seq(c.b, c.g.page, s0 + lane, err);
       const long long rows = (long long)(q.q1 - q.q0) * c.group;
-      n = rows > c.rows_most && q.q1 - q.q0 <= c.b.max_q ? (int)((rows + 255) / 256) : 0;
+      n = rows > c.rows_most ? (int)((rows + 255) / 256) : 0;
     }
     int upto = n;
 #pragma unroll
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
   int lo, hi;
   pa_range(sq, r0 / c.group, (r0 + rn - 1) / c.group, c.window, lo, hi);
   const int k0 = lo + sp * c.per, k1 = min(hi, k0 + c.per);
-  const int hd = c.g.hd, pos0 = sq.kv - (sq.q1 - sq.q0);
+  const int hd = c.g.hd, pos0 = sq.p0;
   const size_t rec0 = ((size_t)flat * c.g.kvh + kvh) * 256;               // this block's rows in the split results
   if (k0 >= k1) {
     if (c.nsplit > 1) { if (tid < rn) c.ml[(rec0 + tid) * c.nsplit + sp] = make_float2(-INFINITY, 0.f); }

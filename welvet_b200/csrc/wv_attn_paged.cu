@@ -223,7 +223,7 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
   for (int i = 0; i < NR; i++) {
     const int r = r0 + min(gl + 8 * i, rn - 1), tok = r / c.group, h = kvh * c.group + r - tok * c.group;
     qrow[i] = c.q + (size_t)(sq.q0 + tok) * c.ldq + (size_t)h * hd;
-    plast[i] = sq.kv - (sq.q1 - sq.q0) + tok;
+    plast[i] = sq.p0 + tok;
     where[i] = h * hd;
   }
   float qv[NR][KS / PR_WARPS][4];                                        // the lane's fragment values of steps warp, warp + 4, ...
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
   }
   auto qfrag = [&](int i) -> uint4 { if constexpr (QREG) return qr[i]; else return s_qf[i * 32 + lane]; };
 
-  const int pmin = sq.kv - (sq.q1 - sq.q0) + r0 / c.group, pmax = sq.kv - (sq.q1 - sq.q0) + (r0 + rn - 1) / c.group;
+  const int pmin = sq.p0 + r0 / c.group, pmax = sq.p0 + (r0 + rn - 1) / c.group;
 
   float o[NT][4], m[NR], l[NR];
 #pragma unroll
@@ -604,7 +604,7 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
       to = c.acc + rec(r) * hd;
       if (warp == 0 && cl == 0) c.ml[rec(r)] = make_float2(M, L);
     } else {
-      to = c.out + (size_t)(sq.q0 + plast[i] - (sq.kv - (sq.q1 - sq.q0))) * c.ldo + where[i];
+      to = c.out + (size_t)(sq.q0 + plast[i] - sq.p0) * c.ldo + where[i];
       scale = L == 0.f ? 0.f : 1.f / L;
     }
     for (int t4 = warp; t4 < NT / 4; t4 += PR_WARPS) {                   // four neighbouring values at a time, twice

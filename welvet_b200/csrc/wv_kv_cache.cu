@@ -34,7 +34,7 @@ __device__ __forceinline__ KvPlace kv_place(const WvKvGeom& g, const WvKvBatch& 
   if (s >= b.num_seqs) { p.pos = INT_MIN; return p; }
   const WvSeq q = wv_seq(b, g.page, s, err);
   if (row < q.q0 || row >= q.q1) { p.pos = INT_MIN; return p; }
-  p.pos = q.kv - (q.q1 - q.q0) + (row - q.q0);
+  p.pos = q.p0 + (row - q.q0);
   if (p.pos < 0) return p;
   const int i = p.pos / g.page, id = b.pages[(size_t)s * b.table_stride + i];
   p.slot = p.pos - i * g.page;

@@ -32,15 +32,18 @@ __host__ __device__ inline WvKvGeom wv_kv_geom(const WvKvPages& p) {
 #define WV_PAGED_PAGE 2          // a page number outside the pool
 __device__ __forceinline__ void wv_paged_report(int* err, int code) { if (err) atomicCAS_system(err, 0, code); }
 
-// A sequence of the batch, cut to the call's bounds.
-struct WvSeq { int q0, q1, kv; };      // rows q0 .. q1 - 1 of q, kv tokens in the cache
+// A sequence of the batch, cut to the call's bounds: rows q0 .. q1 - 1 of q, the first of them at position p0; kv tokens in the cache.
+// Of more than max_q new tokens the first ones stay, at their places.
+struct WvSeq { int q0, q1, kv, p0; };
 __device__ __forceinline__ WvSeq wv_seq(const WvKvBatch& b, int page, int s, int* err) {
   WvSeq q;
   const int a = b.q_start[s], e = b.q_start[s + 1], k = b.kv_len[s];
   q.q0 = min(max(a, 0), b.total_q);
   q.q1 = min(max(e, q.q0), b.total_q);
   q.kv = min(max(k, 0), b.max_kv);      // max_kv <= table_stride * page_size: the host checked
+  q.p0 = q.kv - (q.q1 - q.q0);
   if (q.q0 != a || q.q1 != e || q.kv != k || q.q1 - q.q0 > b.max_q) wv_paged_report(err, WV_PAGED_LENGTH);
+  if (q.q1 - q.q0 > b.max_q) q.q1 = q.q0 + b.max_q;
   return q;
 }
 // The sequence that row `row` of q belongs to (num_seqs: none), found by a whole warp: the first s with q_start[s + 1] > row.
