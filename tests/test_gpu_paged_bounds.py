@@ -147,3 +147,78 @@ def test_more_tokens_than_max_q(wv, max_q, long):
     assert torch.equal(qo[m], qf[m]) and (qo[~m] == 5.0).all()
     for f, s, e in zip(full, some, every):
         assert torch.equal(s[m], e[m]) and torch.equal(s[~m], f[~m])
+
+
+SCRATCH = 256 << 20                               # what a call of the attention may keep for the results of its splits
+
+
+def taken(call):
+    """Device memory that a captured call and its replay leave taken (the graph is still there)."""
+    call(torch.cuda.current_stream().cuda_stream)                        # kernels loaded, the stream's own scratch allocated
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    g, st = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    with torch.cuda.graph(g, stream=st):
+        call(torch.cuda.current_stream().cuda_stream)
+    g.replay()
+    torch.cuda.synchronize()
+    return free - torch.cuda.mem_get_info()[0], g
+
+
+def close(got, want):
+    """As in a full batch's long sequences: 40 additions that cut off up to 2^-23 of a sum, half of that on average, and as much again."""
+    assert ((got.double() - want).norm() / want.norm()).item() <= 2 * 40 * 2.0 ** -24
+
+
+def test_scratch_of_a_long_prompt_with_wide_heads(wv):
+    """Heads beyond 128 go 16 rows at a time, and their keys in splits: a prompt of 8192 tokens (131072 rows, 7 splits of 258 numbers)
+    takes its scratch in parts. Tokens from its start, middle and end against 64 bits."""
+    n, heads, kvh, hd = 8192, 16, 8, 256
+    c = Cache(wv, 8, 64, kvh, hd, [(n, n)])
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=gen)  # noqa: E731
+    k, v, q = rand(n, kvh * hd), rand(n, kvh * hd), rand(n, heads * hd)
+    c.fill(k, v)
+    wv.paged.KVReadCUDA(c.pages, c.batch, k.data_ptr(), v.data_ptr())
+    out = torch.zeros(n, heads * hd, device="cuda")
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    took, g = taken(lambda st: wv.paged.AttnPagedCUDA(c.pages, c.batch, q.data_ptr(), out.data_ptr(), heads, 0.0625, stream=st))
+    assert took <= SCRATCH + (4 << 20), took
+    kd, vd = (t.view(n, kvh, hd).double() for t in (k, v))
+    for t0 in (0, 1279, 4090, 8176):
+        qs = q[t0:t0 + 16].view(16, kvh, heads // kvh, hd).double()
+        s = torch.einsum("tgrd,kgd->tgrk", qs, kd[:t0 + 16]) * 0.0625
+        s = s.masked_fill(torch.arange(t0 + 16, device="cuda") > t0 + torch.arange(16, device="cuda")[:, None, None, None], float("-inf"))
+        close(out[t0:t0 + 16], torch.einsum("tgrk,kgd->tgrd", torch.softmax(s, -1), vd[:t0 + 16]).reshape(16, -1))
+
+
+@pytest.mark.parametrize("piece", [1, 64])
+def test_scratch_of_many_sequences_under_a_long_bound(wv, piece):
+    """256 short sequences, a piece of a prompt among them or not, under the bound of a model with a context of 131072."""
+    seqs, heads, kvh, hd, most, page = 256, 32, 8, 128, 131072, 64
+    c = Cache(wv, 8, page, kvh, hd, [(1, 400)])
+    gen = torch.Generator(device="cuda").manual_seed(3)
+    rand = lambda *s: torch.randn(*s, device="cuda", generator=gen)  # noqa: E731
+    k, v = rand(400, kvh * hd), rand(400, kvh * hd)
+    c.fill(k, v)
+    whole, keep = c.batch_of([(400, 400)])
+    wv.paged.KVReadCUDA(c.pages, whole, k.data_ptr(), v.data_ptr())
+    table = torch.full((seqs, most // page), -1, dtype=torch.int32, device="cuda")
+    table[:, :c.table.shape[1]] = c.d_table                               # one sequence's pages for all of them
+    new = [1] * seqs
+    new[100] = piece
+    new[7] = 0
+    start = torch.tensor(np.concatenate([[0], np.cumsum(new)]), dtype=torch.int32, device="cuda")
+    kv = torch.randint(64, 401, (seqs,), device="cuda", dtype=torch.int32, generator=gen)
+    total = sum(new)
+    q, out = rand(total, heads * hd), torch.zeros(total, heads * hd, device="cuda")
+    b = wv.paged.Batch(start.data_ptr(), kv.data_ptr(), table.data_ptr(), seqs, table.shape[1], total, piece, most)
+    took, g = taken(lambda st: wv.paged.AttnPagedCUDA(c.pages, b, q.data_ptr(), out.data_ptr(), heads, 0.09, stream=st))
+    assert took <= SCRATCH + (4 << 20), took
+    seq = torch.repeat_interleave(torch.arange(seqs, device="cuda"), torch.tensor(new, device="cuda"))
+    pos = kv[seq] - (start[seq + 1] - torch.arange(total, device="cuda"))
+    s = torch.einsum("tgrd,kgd->tgrk", q.view(total, kvh, heads // kvh, hd).double(), k.view(400, kvh, hd).double()) * 0.09
+    s = s.masked_fill(torch.arange(400, device="cuda") > pos[:, None, None, None], float("-inf"))
+    close(out, torch.einsum("tgrk,kgd->tgrd", torch.softmax(s, -1), v.view(400, kvh, hd).double()).reshape(total, -1))
+    assert wv._lib.lib().wv_device_status() == 0

@@ -841,7 +841,7 @@ int wv_launch_attn_chunk(PaCall c, int bits, long long keys, bool alike, cudaStr
   const long long tiles = (keys + PC_N - 1) / PC_N, sms = wv_sm_count();
   long long best = 1, cost = -1;
   for (long long ns = 1; ns <= 16 && ns <= tiles; ns++) {      // 16: chunk_join_kernel's room for weights
-    if (ns > 1 && blocks * 256 * ns * (c.g.hd + 2) * 4 > (256LL << 20)) break;
+    if (ns > 1 && blocks * 256 * ns * (c.g.hd + 2) * 4 > PA_SCRATCH) break;
     const long long t = (tiles + ns - 1) / ns, w = (blocks * ns + sms - 1) / sms * (t + 4 + (ns > 1 ? 2 : 0));
     if (cost < 0 || w < cost) { cost = w; best = ns; }
   }

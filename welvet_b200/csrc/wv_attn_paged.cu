@@ -123,8 +123,8 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  const int tiles = gridDim.x / (c.b.num_seqs * c.g.kvh);
-  const int kvh = blockIdx.x % c.g.kvh, tile = blockIdx.x / c.g.kvh % tiles, seq = blockIdx.x / c.g.kvh / tiles, sp = blockIdx.y;
+  const unsigned flat = c.first + blockIdx.x, of_head = flat / (unsigned)c.g.kvh;
+  const int kvh = flat - of_head * c.g.kvh, seq = of_head / c.tiles, tile = of_head - seq * c.tiles, sp = blockIdx.y;
   const WvSeq sq = wv_seq(c.b, c.g.page, seq, sp == 0 && kvh == 0 && tile == 0 ? c.err : nullptr);
   const int nrows = (sq.q1 - sq.q0) * c.group, r0 = tile * NROW;
   if (r0 >= nrows || nrows > c.rows_most) return;
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
   int lo, hi;
   pa_range(sq, r0 / c.group, (r0 + rn - 1) / c.group, c.window, lo, hi);
   const int k0 = lo + sp * c.per, k1 = min(hi, k0 + c.per);              // this block's keys; k0 is a multiple of 16
-  auto rec = [&](int r) { return (((size_t)seq * c.g.kvh + kvh) * (tiles * NROW) + r0 + r) * c.nsplit + sp; };      // a row's split result
+  auto rec = [&](int r) { return ((size_t)blockIdx.x * c.kept + r) * c.nsplit + sp; };      // a row's split result
   if (k0 >= k1) {
     if (c.nsplit > 1) { if (tid < rn) c.ml[rec(tid)] = make_float2(-INFINITY, 0.f); }
     else for (int i = tid; i < rn * hd; i += 32 * PR_WARPS) {            // rows that see nothing
@@ -628,12 +628,13 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
   }
 }
 
-// The splits' results joined in their order: a block per (sequence, kv head, row).
-__global__ void __launch_bounds__(128) rows_join_kernel(const __grid_constant__ PaCall c, int per_head) {
+// The splits' results joined in their order: a block per row (tokens x query heads) of the blocks of attn_rows_kernel, which took `nrow` each.
+__global__ void __launch_bounds__(128) rows_join_kernel(const __grid_constant__ PaCall c, int nrow) {
   extern __shared__ float pr_w[];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  const int r = blockIdx.x % per_head, kvh = blockIdx.x / per_head % c.g.kvh, seq = blockIdx.x / per_head / c.g.kvh;
+  const unsigned block = blockIdx.x / c.kept, flat = c.first + block, of_head = flat / (unsigned)c.g.kvh;
+  const int kvh = flat - of_head * c.g.kvh, seq = of_head / c.tiles, r = (of_head - seq * c.tiles) * nrow + blockIdx.x - block * c.kept;
   const WvSeq sq = wv_seq(c.b, c.g.page, seq, nullptr);
   const int nrows = (sq.q1 - sq.q0) * c.group;
   if (r >= nrows || nrows > c.rows_most) return;
@@ -643,7 +644,7 @@ __global__ void __launch_bounds__(128) rows_join_kernel(const __grid_constant__ 
 }
 
 template <int BITS, int DP, bool R16, bool EXACT>
-static cudaError_t rows_go(const PaCall& c, int tiles, cudaStream_t st) {
+static cudaError_t rows_go(const PaCall& c, int blocks, cudaStream_t st) {
   using S = PrShape<BITS, DP>;
   constexpr size_t sums = (size_t)PR_WARPS * (R16 ? 16 : 8) * DP * 4, ring = (size_t)PR_WARPS * PrFit<BITS, DP, R16>::NST * S::STAGE;
   constexpr size_t smem = sums > ring ? sums : ring;
@@ -658,19 +659,19 @@ static cudaError_t rows_go(const PaCall& c, int tiles, cudaStream_t st) {
   }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[1];
-  cfg.gridDim = dim3((unsigned)(c.b.num_seqs * tiles * c.g.kvh), (unsigned)c.nsplit); cfg.blockDim = dim3(32 * PR_WARPS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+  cfg.gridDim = dim3((unsigned)blocks, (unsigned)c.nsplit); cfg.blockDim = dim3(32 * PR_WARPS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at; cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kern, c);
 }
 template <int BITS, bool R16>
-static cudaError_t rows_pick(const PaCall& c, int tiles, cudaStream_t st) {
-  if (c.g.hd == 64) return rows_go<BITS, 64, R16, true>(c, tiles, st);
-  if (c.g.hd == 128) return rows_go<BITS, 128, R16, true>(c, tiles, st);
-  if (c.g.hd < 64) return rows_go<BITS, 64, R16, false>(c, tiles, st);
-  if (c.g.hd < 128) return rows_go<BITS, 128, R16, false>(c, tiles, st);
-  return rows_go<BITS, 256, R16, false>(c, tiles, st);
+static cudaError_t rows_pick(const PaCall& c, int blocks, cudaStream_t st) {
+  if (c.g.hd == 64) return rows_go<BITS, 64, R16, true>(c, blocks, st);
+  if (c.g.hd == 128) return rows_go<BITS, 128, R16, true>(c, blocks, st);
+  if (c.g.hd < 64) return rows_go<BITS, 64, R16, false>(c, blocks, st);
+  if (c.g.hd < 128) return rows_go<BITS, 128, R16, false>(c, blocks, st);
+  return rows_go<BITS, 256, R16, false>(c, blocks, st);
 }
 
 int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* dq, int ldq, float* dout, int ldo, int heads, float scale,
@@ -699,9 +700,10 @@ int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* d
   if (rows) {
     const long long top = chunk ? c.rows_most : most;
     const bool r16 = top > 8;
-    const long long tiles = (top + (r16 ? 15 : 7)) / (r16 ? 16 : 8), per_head = tiles * (r16 ? 16 : 8);
+    const int nrow = r16 ? 16 : 8;
+    const long long tiles = (top + nrow - 1) / nrow;
     const long long blocks = (long long)b.num_seqs * tiles * c.g.kvh;
-    if (blocks * (r16 ? 16 : 8) > INT_MAX) { wv_set_error("wv_attn_paged_dev: %d sequences are too many", b.num_seqs); return WV_ESHAPE; }
+    if (blocks * nrow > INT_MAX) { wv_set_error("wv_attn_paged_dev: %d sequences are too many", b.num_seqs); return WV_ESHAPE; }
     // Splits of the keys: the number that fills 1, 2, .. 8 waves of the blocks that run at once and costs least, a wave being worth a
     // warp's groups of 16 keys and some six more of start and end (2049 positions and eight blocks: 33 splits of 64; 131000: 55).
     const long long slots = (long long)sms * pr_blocks(kv.bits, c.g.hd <= 64 ? 64 : c.g.hd <= 128 ? 128 : 256, r16);
@@ -721,25 +723,34 @@ int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* d
     if (per < keys / 8192) per = (keys / 8192 + 63) & ~63LL;
     const long long ns = keys > per ? (keys + per - 1) / per : 1;
     PaCall r = c;
-    r.per = (int)per; r.nsplit = (int)ns;
+    r.per = (int)per; r.nsplit = (int)ns; r.tiles = (unsigned)tiles; r.kept = (unsigned)(top < nrow ? top : nrow);
+    // The splits' results of all rows may be more than a call should keep (a prompt of 8192 tokens and 16 heads of 256: 0.9 GB): the blocks
+    // then go in parts of equal size, one after the other through the same scratch. A part holds 600 blocks of 16 rows or more up to 26
+    // splits of the widest heads, so it still fills the chip.
+    const long long bytes = (long long)r.kept * ns * (2 + c.g.hd) * 4, most_blocks = ns == 1 || bytes * blocks <= PA_SCRATCH ? blocks : std::max(PA_SCRATCH / bytes, 1LL);
+    const long long parts = (blocks + most_blocks - 1) / most_blocks, part = (blocks + parts - 1) / parts;
     WvLease lease;
     if (ns > 1) {
-      const size_t n = (size_t)(b.num_seqs * c.g.kvh) * per_head * ns;
-      if (const int rc = wv_lease(lease, n * (2 + c.g.hd), st, "wv_attn_paged_dev: the splits' results")) return rc;
+      const size_t n = (size_t)part * r.kept * ns, sums = (2 * n + 3) & ~(size_t)3;      // the sums are stored 16 bytes at a time
+      if (const int rc = wv_lease(lease, sums + n * c.g.hd, st, "wv_attn_paged_dev: the splits' results")) return rc;
       r.ml = reinterpret_cast<float2*>(lease.p);
-      r.acc = lease.p + 2 * n;
+      r.acc = lease.p + sums;
     }
-    cudaError_t e = kv.bits == 16 ? (r16 ? rows_pick<16, true>(r, (int)tiles, st) : rows_pick<16, false>(r, (int)tiles, st))
-                  : kv.bits == 8 ? (r16 ? rows_pick<8, true>(r, (int)tiles, st) : rows_pick<8, false>(r, (int)tiles, st))
-                                 : (r16 ? rows_pick<4, true>(r, (int)tiles, st) : rows_pick<4, false>(r, (int)tiles, st));
-    if (e == cudaSuccess && ns > 1) {
+    cudaError_t e = cudaSuccess;
+    for (long long at0 = 0; at0 < blocks && e == cudaSuccess; at0 += part) {
+      const int now = (int)std::min(part, blocks - at0);
+      r.first = (unsigned)at0;
+      e = kv.bits == 16 ? (r16 ? rows_pick<16, true>(r, now, st) : rows_pick<16, false>(r, now, st))
+        : kv.bits == 8 ? (r16 ? rows_pick<8, true>(r, now, st) : rows_pick<8, false>(r, now, st))
+                       : (r16 ? rows_pick<4, true>(r, now, st) : rows_pick<4, false>(r, now, st));
+      if (e != cudaSuccess || ns == 1) continue;
       cudaLaunchConfig_t cfg = {};
       cudaLaunchAttribute at[1];
-      cfg.gridDim = dim3((unsigned)(b.num_seqs * c.g.kvh * per_head)); cfg.blockDim = dim3(128); cfg.dynamicSmemBytes = (size_t)ns * 4; cfg.stream = st;
+      cfg.gridDim = dim3((unsigned)(now * r.kept)); cfg.blockDim = dim3(128); cfg.dynamicSmemBytes = (size_t)ns * 4; cfg.stream = st;
       at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
       at[0].val.programmaticStreamSerializationAllowed = 1;
       cfg.attrs = at; cfg.numAttrs = 1;
-      e = cudaLaunchKernelEx(&cfg, rows_join_kernel, r, (int)per_head);
+      e = cudaLaunchKernelEx(&cfg, rows_join_kernel, r, nrow);
     }
     if (e != cudaSuccess) { wv_set_error("wv_attn_paged_dev: launch: %s", cudaGetErrorString(cudaGetLastError())); return WV_ECUDA; }
   }

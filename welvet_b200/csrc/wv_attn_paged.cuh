@@ -8,6 +8,7 @@
 #include <math.h>
 
 #define PA_LIFT 13.f
+#define PA_SCRATCH (256LL << 20)        // bytes that a call may keep for its splits' results
 
 struct PaCall {
   WvKvGeom g;
@@ -20,6 +21,7 @@ struct PaCall {
   unsigned one;                    // 0x3c003c00, for pa_nibbles
   int rows_most;                   // sequences with more rows (tokens x group) than this go to the chunk kernel (0: all that have any)
   int nsplit, per;                 // splits of a sequence's keys, keys of a split (a multiple of 16; of 128 for chunks)
+  unsigned tiles, first, kept;     // few rows: tiles of a sequence, the launch's first block of rows, rows of a block with split results
   float2* ml;                      // split results [row][nsplit]: {M, divisor}; {-inf, 0} and no sums for a split without keys
   float* acc;                      // [row][nsplit][head_dim]
   int* err;
