@@ -222,3 +222,20 @@ def test_scratch_of_many_sequences_under_a_long_bound(wv, piece):
     s = s.masked_fill(torch.arange(400, device="cuda") > pos[:, None, None, None], float("-inf"))
     close(out, torch.einsum("tgrk,kgd->tgrd", torch.softmax(s, -1), v.view(400, kvh, hd).double()).reshape(total, -1))
     assert wv._lib.lib().wv_device_status() == 0
+
+
+def test_no_more_positions_than_the_attention_counts(wv):
+    """A billion cached tokens and more under one table row are refused: keys are counted in 32 bits."""
+    c = Cache(wv, 8, 16, 2, 64, [(1, 20)])
+    x, o = torch.zeros(1, 256, device="cuda"), torch.zeros(1, 256, device="cuda")
+    start, kv = arrays(c, [(1, 20)])
+    for most, ok in ((2 ** 30, True), (2 ** 30 + 1, False), (2 ** 31 - 16, False)):
+        b = wv.paged.Batch(start.data_ptr(), kv.data_ptr(), c.d_table.data_ptr(), 1, 2 ** 27, 1, 1, most)
+        if ok:
+            wv.paged.AttnPagedCUDA(c.pages, b, x.data_ptr(), o.data_ptr(), 4, 0.125)
+        else:
+            with pytest.raises(wv.WelvetError) as e:
+                wv.paged.AttnPagedCUDA(c.pages, b, x.data_ptr(), o.data_ptr(), 4, 0.125)
+            assert e.value.code == wv._lib.WV_ESHAPE
+    torch.cuda.synchronize()
+    assert wv._lib.lib().wv_device_status() == 0

@@ -191,7 +191,8 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
   const int nrows = (sq.q1 - sq.q0) * c.group, r0 = M.tile * 256, rn = min(256, nrows - r0);
   int lo, hi;
   pa_range(sq, r0 / c.group, (r0 + rn - 1) / c.group, c.window, lo, hi);
-  const int k0 = lo + sp * c.per, k1 = min(hi, k0 + c.per);
+  const unsigned first = (unsigned)lo + (unsigned)(sp * c.per);
+  const int k0 = (int)min(first, (unsigned)hi), k1 = min(hi, k0 + c.per);
   const int hd = c.g.hd, pos0 = sq.p0;
   const size_t rec0 = ((size_t)flat * c.g.kvh + kvh) * 256;               // this block's rows in the split results
   if (k0 >= k1) {

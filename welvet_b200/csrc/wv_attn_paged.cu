@@ -131,7 +131,8 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
   const int rn = min(NROW, nrows - r0);
   int lo, hi;
   pa_range(sq, r0 / c.group, (r0 + rn - 1) / c.group, c.window, lo, hi);
-  const int k0 = lo + sp * c.per, k1 = min(hi, k0 + c.per);              // this block's keys; k0 is a multiple of 16
+  const unsigned first = (unsigned)lo + (unsigned)(sp * c.per);
+  const int k0 = (int)min(first, (unsigned)hi), k1 = min(hi, k0 + c.per);      // this block's keys; k0 is a multiple of 16 if there are any
   auto rec = [&](int r) { return ((size_t)blockIdx.x * c.kept + r) * c.nsplit + sp; };      // a row's split result
   if (k0 >= k1) {
     if (c.nsplit > 1) { if (tid < rn) c.ml[rec(tid)] = make_float2(-INFINITY, 0.f); }

@@ -62,7 +62,8 @@ __device__ __forceinline__ PaSub pa_pair(unsigned a, unsigned b) {
 
 
 // The positions that a block of consecutive rows of a sequence sees: [lo, hi), lo cut down to a multiple of 16. The first row may stand
-// before position 0, where p0 - window has no room in 32 bits for the widest windows.
+// before position 0, where p0 - window has no room in 32 bits for the widest windows. A split's first key lo + split * per may lie past
+// hi; with at most 2^30 cached tokens it stays below 2^32, and k0 + per of a split with keys below 2^31.
 __device__ __forceinline__ void pa_range(const WvSeq& s, int tok0, int tok1, int window, int& lo, int& hi) {
   const int p0 = s.p0 + tok0;
   hi = max(0, s.p0 + tok1 + 1);

@@ -470,6 +470,7 @@ extern "C" int wv_attn_paged_dev(const WvKvPages* kv, const WvKvBatch* batch, co
   const bool none = rc == 1;
   if (num_heads < 1 || num_heads % kv->num_kv_heads) { wv_set_error("%s: %d heads over %d kv heads", who, num_heads, kv->num_kv_heads); return WV_ESHAPE; }
   if (!(scale == scale) || scale - scale != 0.f) { wv_set_error("%s: the scale is not finite", who); return WV_EARG; }
+  if (batch->max_kv > 1 << 30) { wv_set_error("%s: max_kv %d (at most 2^30)", who, batch->max_kv); return WV_ESHAPE; }
   const long long qw = (long long)num_heads * kv->head_dim;
   if ((rc = kv_rows(who, "q", dq, &ldq, qw)) || (rc = kv_rows(who, "out", dout, &ldo, qw))) return rc;
   if (none) return WV_OK;
