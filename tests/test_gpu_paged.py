@@ -403,6 +403,39 @@ def test_large_and_small_values(wv):
             a += kv
 
 
+@pytest.mark.parametrize("bits", [16, 8, 4])
+@pytest.mark.parametrize("large", [3e7, 1e9, 1e12, 1e30])
+def test_logits_of_any_size(wv, bits, large):
+    """Logits far beyond 2^24, whose float32 steps are wider than a weight's range: few rows and chunks, within a tile and over many. The
+    weight is all on the largest logit where the next one lies further below it than both may be off (`bound`'s first term) and 64 more,
+    which leaves e^-64 to the others; the output is then that key's value, but for the weight's 2^-19."""
+    heads, kvh, hd = 4, 2, 64
+    lens = [(3, 90), (100, 700), (70, 70)]
+    c = Cache(wv, bits, 16, kvh, hd, lens)
+    rng = np.random.default_rng(bits)
+    n, total = sum(k for _, k in lens), sum(a for a, _ in lens)
+    c.fill(*(torch.from_numpy(rng.normal(0, 1, (n, kvh * hd)).astype(np.float32)).cuda() for _ in range(2)))
+    q = rng.normal(0, large, (total, heads, hd)).astype(np.float32)
+    got = run_attn(c, torch.from_numpy(q.reshape(total, -1)).cuda(), heads, 0.125).reshape(total, heads, hd)
+    assert np.isfinite(got).all()
+    kk, vv = c.rows("k"), c.rows("v")
+    r = a = clear = 0
+    for nq, kv in lens:
+        for i in range(nq):
+            for h in range(heads):
+                seen = slice(a, a + kv - nq + i + 1)
+                x = kk[seen, h // 2] @ q[r + i, h].astype(np.float64) * 0.125
+                off = 2 * hd * 2.0 ** -23 * (np.abs(kk[seen, h // 2]) @ np.abs(q[r + i, h].astype(np.float64))).max() * 0.125
+                o = np.argsort(-x)
+                if len(x) > 1 and x[o[0]] - x[o[1]] <= 2 * off + 64:
+                    continue
+                clear += 1
+                v = vv[seen, h // 2]
+                assert (np.abs(got[r + i, h] - v[o[0]]) <= 2.0 ** -19 * np.abs(v).max()).all(), (nq, i, h)
+        r, a = r + nq, a + kv
+    assert clear > total * heads * 0.9
+
+
 def test_strides_and_rows_of_nobody(wv):
     """Gaps between rows stay as they are, and so do rows past the last sequence's."""
     heads, kvh, hd = 4, 2, 64

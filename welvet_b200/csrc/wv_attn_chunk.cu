@@ -26,6 +26,10 @@
 // tile's largest scale), so that most tiles are read once; a row's two threads agree on that, and exchange their maxima through tensor
 // memory that the next tile's sums will overwrite.
 //
+// A logit is S times its key's scale, in one fused step with the subtraction of the reference. The reference is a rounded product, so from
+// 2^24 on the two may lie further apart than a weight's range: where a warp's reference is 2^20 or more, and in tiles with a mask, the
+// product is rounded first.
+//
 // A key's scale multiplies its column of S; a value row's, relative to the largest of its tile, its weight, and the tile's own power
 // of two goes into the sum over tiles. Where the scales in a tile lie further apart than the pieces' range holds (2^8), the tile's
 // weighted sum is taken value by value in float32 instead.
@@ -380,7 +384,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
           alpha = 1.f;
 #pragma unroll 1
           for (int k = 0; k < PC_N; k++) {
-            const float x = fmaf(__uint_as_float(pc_ld1(tt + k)), M.kk[ms][k], off.x);
+            const float x = __fadd_rn(__fmul_rn(__uint_as_float(pc_ld1(tt + k)), M.kk[ms][k]), off.x);
             const bool on = !masked || ((sees(k >> 5, k >> 5) >> (k & 31)) & 1u);
             const float p = on ? pa_ex2(x) : 0.f, w = on ? p * M.fv[ms][k] * beta : 0.f;
             if (k / HK == hf) l2.x += p;
@@ -413,8 +417,11 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
               const uint4 k4 = lds128(kk + 64 * q + 4 * i), f4 = lds128(fv + 64 * q + 4 * i);
 #pragma unroll
               for (int u = 0; u < 4; u += 2) {
-                const float2 x = __ffma2_rn(make_float2(__uint_as_float(s[i + u]), __uint_as_float(s[i + u + 1])),
-                                            u ? make_float2(__uint_as_float(k4.z), __uint_as_float(k4.w)) : make_float2(__uint_as_float(k4.x), __uint_as_float(k4.y)), off);
+                const float2 sv = make_float2(__uint_as_float(s[i + u]), __uint_as_float(s[i + u + 1]));
+                const float2 kv = u ? make_float2(__uint_as_float(k4.z), __uint_as_float(k4.w)) : make_float2(__uint_as_float(k4.x), __uint_as_float(k4.y));
+                float2 x;                                                // (a packed product and sum may still be fused)
+                if constexpr (decltype(some)::value) x = make_float2(__fadd_rn(__fmul_rn(sv.x, kv.x), off.x), __fadd_rn(__fmul_rn(sv.y, kv.y), off.x));
+                else x = __ffma2_rn(sv, kv, off);
                 float2 p = make_float2(pa_ex2(x.x), pa_ex2(x.y));
                 float2 pf = __fmul2_rn(p, u ? make_float2(__uint_as_float(f4.z), __uint_as_float(f4.w)) : make_float2(__uint_as_float(f4.x), __uint_as_float(f4.y)));
                 if constexpr (decltype(some)::value) {
@@ -431,7 +438,8 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
             }
             pc_st16(ts + 16 * q, w);
           };
-          if (!masked) {
+          const unsigned far = (__float_as_uint(m) & 0x7fffffffu) - __float_as_uint(1048576.f);      // 2^20 up to infinity: large
+          if (!masked && !__any_sync(0xffffffffu, far < 0x7f800000u - __float_as_uint(1048576.f))) {
 #pragma unroll
             for (int q = 0; q < 4; q++) weights(std::false_type(), q, 0u);
           } else {
