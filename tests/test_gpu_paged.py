@@ -436,6 +436,42 @@ def test_logits_of_any_size(wv, bits, large):
     assert clear > total * heads * 0.9
 
 
+@pytest.mark.parametrize("bits", [16, 8, 4])
+@pytest.mark.parametrize("far", [1e9, 1e20, 1e36])
+def test_queries_far_larger_than_their_neighbours(wv, bits, far):
+    """A query row's own magnitude is what its products are exact to: other rows, those of tokens that see nothing among them, do not
+    matter, for 1 to 8 rows, up to 16, and chunks."""
+    heads, kvh, hd = 4, 2, 64
+    lens = [(2, 90), (7, 200), (5, 3), (100, 130), (90, 64)]
+    c = Cache(wv, bits, 16, kvh, hd, lens)
+    rng = np.random.default_rng(bits)
+    n, total = sum(k for _, k in lens), sum(a for a, _ in lens)
+    c.fill(*(torch.from_numpy(rng.normal(0, 1, (n, kvh * hd)).astype(np.float32)).cuda() for _ in range(2)))
+    q = rng.normal(0, 1, (total, heads, hd)).astype(np.float32)
+    r = 0
+    for nq, kv in lens:
+        q[r, 0], q[r, 3] = q[r, 0] * np.float32(far), q[r, 3] / np.float32(far)   # the first token: before position 0 in the third and fifth
+        if nq > 60:
+            q[r + 60, 1] *= np.float32(far)
+        r += nq
+    kk, vv = c.rows("k"), c.rows("v")
+    for some in ([0], [1], [2], [3], [4], [0, 1, 2, 3, 4]):
+        take = np.concatenate([np.arange(lens[i][0]) + sum(a for a, _ in lens[:i]) for i in some])
+        part = [lens[i] for i in some]
+        b, keep = c.batch_of(part)
+        table = c.d_table[some].contiguous()
+        b.pages = table.data_ptr()
+        got = run_attn(c, torch.from_numpy(q[take].reshape(len(take), -1)).cuda(), heads, 0.125, batch=b).reshape(len(take), heads, hd)
+        r = 0
+        for i in some:
+            nq, kv = lens[i]
+            k0 = sum(k for _, k in lens[:i])
+            want, mag, reach = attn64(q[take][r:r + nq], kk[k0:k0 + kv], vv[k0:k0 + kv], 0.125, 0, kv - nq)
+            err = np.abs(got[r:r + nq] - want)
+            assert (err <= bound(mag, reach, hd, kv)).all(), (some, i, float((err / bound(mag, reach, hd, kv)).max()))
+            r += nq
+
+
 def test_strides_and_rows_of_nobody(wv):
     """Gaps between rows stay as they are, and so do rows past the last sequence's."""
     heads, kvh, hd = 4, 2, 64

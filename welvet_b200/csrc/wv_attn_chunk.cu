@@ -112,6 +112,7 @@ struct PcMeta {
   unsigned long long bar[21];
   unsigned vote[2][2];
   unsigned tmem, qmax;
+  unsigned char qexp[2 * PC_M], lift[2 * PC_M];      // of a row: exponent field of its largest |q|, and what it is lifted by
   int abort;
   int seq, tile;
 };
@@ -225,21 +226,27 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&M.tmem)), "n"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  // ---------------------------------------------------------------- Q: a common power of two, two pieces, the operand's layout
+  // ---------------------------------------------------------------- Q: a power of two, two pieces, the operand's layout
+  // The power of two is that of the block's largest row, so that the keys' scales carry it for all rows. A row that lies further below
+  // than its pieces reach (by more than 2^15: the second piece then ends above 2^-24 of the row's largest) is lifted by its own, and its
+  // sums are put down again, by warps that have such a row. Rows before position 0 see nothing and are zeros, whatever they hold.
   auto qrow = [&](int r) { return c.q + (size_t)(sq.q0 + (r0 + r) / c.group) * c.ldq + (size_t)(kvh * c.group + (r0 + r) % c.group) * hd; };
   {
-    unsigned m = 0;
+    unsigned top = 0;
     for (int r = warp; r < rn; r += PC_THREADS / 32) {
       const float* src = qrow(r);
+      unsigned m = 0;
       for (int d = 4 * lane; d < hd; d += 128) {
         const float4 v = *reinterpret_cast<const float4*>(src + d);
         const float x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
         for (int e = 0; e < 4; e++) { const unsigned u = __float_as_uint(x[e]) & 0x7fffffffu; if (u < 0x7f800000u) m = max(m, u); }
       }
+      m = __reduce_max_sync(0xffffffffu, m);
+      if (pos0 + (r0 + r) / c.group >= 0) top = max(top, m);
+      if (lane == 0) M.qexp[r] = (unsigned char)(m >> 23);
     }
-    m = __reduce_max_sync(0xffffffffu, m);
-    if (lane == 0) atomicMax(&M.qmax, m);
+    if (lane == 0) atomicMax(&M.qmax, top);
   }
   pc_fence_before();
   __syncthreads();
@@ -248,16 +255,22 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
   const int qe = min(max((int)(M.qmax >> 23) - 127 - 13, -100), 114);
   const float qinv = copysignf(__uint_as_float((unsigned)(127 - qe) << 23), c.scale);              // a negative scale turns q, so that kk is positive
   const float qf = fabsf(c.scale) * __uint_as_float((unsigned)(127 + qe) << 23);
+  auto lift = [&](int r) {
+    const int own = M.qexp[r], up = qe - max(own - 127 - 13, -100);
+    return own && up > 15 ? min(up, 100) : 0;
+  };
+  if (tid < 2 * PC_M) M.lift[tid] = (unsigned char)(tid < rn ? lift(tid) : 0);
   for (int i = tid; i < 256 * (DP / 8); i += PC_THREADS) {               // 8 places of a row at a time
     const int r = i / (DP / 8), j = i % (DP / 8);
     if (r >= PC_M && !two) break;
     unsigned h[4] = {0u, 0u, 0u, 0u}, l[4] = {0u, 0u, 0u, 0u};
-    if (r < rn && 8 * j < hd) {
+    if (r < rn && 8 * j < hd && pos0 + (r0 + r) / c.group >= 0) {
       const float* src = qrow(r) + 8 * j;
+      const float f = qinv * __uint_as_float((unsigned)(127 + lift(r)) << 23);
       const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
       float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
-      for (int e = 0; e < 8; e++) x[e] = x[e] - x[e] == 0.f ? x[e] * qinv : NAN;
+      for (int e = 0; e < 8; e++) x[e] = x[e] - x[e] == 0.f ? x[e] * f : NAN;
 #pragma unroll
       for (int p = 0; p < 4; p++) {
         const float u = x[pc_dim<BITS>(2 * p)], v = x[pc_dim<BITS>(2 * p + 1)];
@@ -311,6 +324,8 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
         pc_fence_after();
         const unsigned kk = smem_u32(M.kk[ms]) + 4 * HK * hf, fv = smem_u32(M.fv[ms]) + 4 * HK * hf;
         float beta = M.beta[ms], alpha = 1.f;
+        const unsigned lifted = M.lift[r];
+        const float down = __uint_as_float((127u - lifted) << 23);
         const unsigned flags = M.flags[ms];
         const bool masked = (flags & 1u) || key0 + PC_N - 1 > pmin || key0 + PC_N > k1 || (c.window != 0 && key0 <= pmax - c.window);
         // bit k of `see`: the row sees key 32 q + k of the half
@@ -334,7 +349,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
 #pragma unroll
             for (int i = 0; i < 16; i += 2) top = fmaxf(top, fmaxf(__uint_as_float(a[i]), __uint_as_float(a[i + 1])));
           }
-          if (__any_sync(0xffffffffu, !(top * M.kmax[ms] <= m + PC_SLACK)) && lane == 0) atomicOr(&M.vote[t][nv & 1], 1u);
+          if (__any_sync(0xffffffffu, !(top * down * M.kmax[ms] <= m + PC_SLACK)) && lane == 0) atomicOr(&M.vote[t][nv & 1], 1u);
           if (!meet(v_bar(t), nv, 704 + t)) break;
           raise = *(volatile unsigned*)&M.vote[t][nv & 1] != 0;
           if ((warp & 7) == 0 && lane == 0) M.vote[t][(nv + 1) & 1] = 0; // nobody comes to the next vote before this warp's weights are there
@@ -353,8 +368,10 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
               const uint4 k4 = lds128(kk + 64 * q + 4 * i);
-              float x[4] = {__uint_as_float(a[i]) * __uint_as_float(k4.x), __uint_as_float(a[i + 1]) * __uint_as_float(k4.y),
-                            __uint_as_float(a[i + 2]) * __uint_as_float(k4.z), __uint_as_float(a[i + 3]) * __uint_as_float(k4.w)};
+              const float2 dd = make_float2(down, down);
+              const float2 xa = __fmul2_rn(__fmul2_rn(make_float2(__uint_as_float(a[i]), __uint_as_float(a[i + 1])), dd), make_float2(__uint_as_float(k4.x), __uint_as_float(k4.y)));
+              const float2 xb = __fmul2_rn(__fmul2_rn(make_float2(__uint_as_float(a[i + 2]), __uint_as_float(a[i + 3])), dd), make_float2(__uint_as_float(k4.z), __uint_as_float(k4.w)));
+              float x[4] = {xa.x, xa.y, xb.x, xb.y};
               if (!all) {
 #pragma unroll
                 for (int u = 0; u < 4; u++) x[u] = (bits >> (i + u)) & 1u ? x[u] : -INFINITY;
@@ -384,7 +401,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
           alpha = 1.f;
 #pragma unroll 1
           for (int k = 0; k < PC_N; k++) {
-            const float x = __fadd_rn(__fmul_rn(__uint_as_float(pc_ld1(tt + k)), M.kk[ms][k]), off.x);
+            const float x = __fadd_rn(__fmul_rn(__uint_as_float(pc_ld1(tt + k)) * down, M.kk[ms][k]), off.x);
             const bool on = !masked || ((sees(k >> 5, k >> 5) >> (k & 31)) & 1u);
             const float p = on ? pa_ex2(x) : 0.f, w = on ? p * M.fv[ms][k] * beta : 0.f;
             if (k / HK == hf) l2.x += p;
@@ -417,7 +434,8 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
               const uint4 k4 = lds128(kk + 64 * q + 4 * i), f4 = lds128(fv + 64 * q + 4 * i);
 #pragma unroll
               for (int u = 0; u < 4; u += 2) {
-                const float2 sv = make_float2(__uint_as_float(s[i + u]), __uint_as_float(s[i + u + 1]));
+                float2 sv = make_float2(__uint_as_float(s[i + u]), __uint_as_float(s[i + u + 1]));
+                if constexpr (decltype(some)::value) sv = __fmul2_rn(sv, make_float2(down, down));
                 const float2 kv = u ? make_float2(__uint_as_float(k4.z), __uint_as_float(k4.w)) : make_float2(__uint_as_float(k4.x), __uint_as_float(k4.y));
                 float2 x;                                                // (a packed product and sum may still be fused)
                 if constexpr (decltype(some)::value) x = make_float2(__fadd_rn(__fmul_rn(sv.x, kv.x), off.x), __fadd_rn(__fmul_rn(sv.y, kv.y), off.x));
@@ -439,7 +457,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
             pc_st16(ts + 16 * q, w);
           };
           const unsigned far = (__float_as_uint(m) & 0x7fffffffu) - __float_as_uint(1048576.f);      // 2^20 up to infinity: large
-          if (!masked && !__any_sync(0xffffffffu, far < 0x7f800000u - __float_as_uint(1048576.f))) {
+          if (!masked && !__any_sync(0xffffffffu, lifted || far < 0x7f800000u - __float_as_uint(1048576.f))) {
 #pragma unroll
             for (int q = 0; q < 4; q++) weights(std::false_type(), q, 0u);
           } else {

@@ -110,10 +110,10 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
   extern __shared__ __align__(128) unsigned char pr_smem[];
   __shared__ uint4 s_qf[(R16 ? 2 : 1) * KS * 32];
   __shared__ float2 s_ml[PR_WARPS][NROW];
-  __shared__ unsigned s_qmax;
+  __shared__ unsigned s_qmax[NROW];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, gl = lane >> 2, cl = lane & 3;
   unsigned char* ring = pr_smem + warp * NST * S::STAGE;
-  if (tid == 0) s_qmax = 0;
+  if (tid < NROW) s_qmax[tid] = 0;
   const unsigned one = c.one;
   const int hd = EXACT ? DP : c.g.hd, n16 = hd / 16, code = EXACT ? RB : c.g.code;
   if (!EXACT) {                                                          // what lies beyond the head stays zero
@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
 #pragma unroll
   for (int i = 0; i < NST - 1; i++) start(i);
 
-  // ---------------------------------------------------------------- q: a common power of two, then two float16 pieces, as fragments
+  // ---------------------------------------------------------------- q: a power of two for each row, then two float16 pieces, as fragments
   constexpr int NR = R16 ? 2 : 1;
   const float* qrow[NR];                                                 // of the lane's rows
   int plast[NR], where[NR];                                              // the last position that they see; token and head as an offset in out
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
   }
   float qv[NR][KS / PR_WARPS][4];                                        // the lane's fragment values of steps warp, warp + 4, ...
   {
-    unsigned m = 0;
+    unsigned m[NR] = {};
 #pragma unroll
     for (int k = 0; k < KS / PR_WARPS; k++)
 #pragma unroll
@@ -247,16 +247,24 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
           qv[i][k][0] = v.x; qv[i][k][1] = v.y; qv[i][k][2] = v.z; qv[i][k][3] = v.w;
         }
 #pragma unroll
-        for (int e = 0; e < 4; e++) { const unsigned u = __float_as_uint(qv[i][k][e]) & 0x7fffffffu; if (u < 0x7f800000u) m = max(m, u); }
+        for (int e = 0; e < 4; e++) { const unsigned u = __float_as_uint(qv[i][k][e]) & 0x7fffffffu; if (u < 0x7f800000u) m[i] = max(m[i], u); }
       }
-    m = __reduce_max_sync(0xffffffffu, m);
     __syncthreads();
-    if (lane == 0) atomicMax(&s_qmax, m);
+#pragma unroll
+    for (int i = 0; i < NR; i++) {
+      m[i] = max(m[i], __shfl_xor_sync(0xffffffffu, m[i], 1));
+      m[i] = max(m[i], __shfl_xor_sync(0xffffffffu, m[i], 2));
+      if (cl == 0) atomicMax(&s_qmax[gl + 8 * i], m[i]);
+    }
     __syncthreads();
   }
-  const int qe = min(max((int)(s_qmax >> 23) - 127 - 13, -100), 114);    // max |q| 2^-qe in [2^13, 2^14)
-  const float qinv = __uint_as_float((unsigned)(127 - qe) << 23);
-  const float qf = c.scale * __uint_as_float((unsigned)(127 + qe) << 23);
+  float qinv[NR], qf[NR];
+#pragma unroll
+  for (int i = 0; i < NR; i++) {
+    const int qe = min(max((int)(s_qmax[gl + 8 * i] >> 23) - 127 - 13, -100), 114);      // max |q| 2^-qe in [2^13, 2^14)
+    qinv[i] = __uint_as_float((unsigned)(127 - qe) << 23);
+    qf[i] = c.scale * __uint_as_float((unsigned)(127 + qe) << 23);
+  }
 #pragma unroll
   for (int k = 0; k < KS / PR_WARPS; k++) {
     unsigned h_[NR][2], l_[NR][2];                                       // [row g, row g + 8][k half]
@@ -265,8 +273,8 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
 #pragma unroll
       for (int p = 0; p < 2; p++) {
         float x = qv[i][k][2 * p], z = qv[i][k][2 * p + 1];
-        x = x - x == 0.f ? x * qinv : NAN;                               // not finite: the row's sums are NaN
-        z = z - z == 0.f ? z * qinv : NAN;
+        x = x - x == 0.f ? x * qinv[i] : NAN;                            // not finite: the row's sums are NaN
+        z = z - z == 0.f ? z * qinv[i] : NAN;
         h_[i][p] = pa_pack(x, z);
         const float2 b = pa_unpack(h_[i][p]);
         l_[i][p] = pa_pack(x - b.x, z - b.y);
@@ -356,7 +364,9 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
     }
     // -------------------------------------------------------------- weights of the lane's four keys 2c, 2c + 1, 2c + 8, 2c + 9
     const float2 k0_ = *reinterpret_cast<const float2*>(sc + 8 * cl), k1_ = *reinterpret_cast<const float2*>(sc + 32 + 8 * cl);
-    const float kk[4] = {k0_.x * qf, k0_.y * qf, k1_.x * qf, k1_.y * qf};
+    float kk[NR][4];
+#pragma unroll
+    for (int i = 0; i < NR; i++) { kk[i][0] = k0_.x * qf[i]; kk[i][1] = k0_.y * qf[i]; kk[i][2] = k1_.x * qf[i]; kk[i][3] = k1_.y * qf[i]; }
     const float inv = __uint_as_float((254u - erun) << 23);
     float y[NR][4], f[4];
     bool seen[NR][4];
@@ -365,10 +375,10 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
       const int n = j >> 1, e = j & 1;
       f[j] = __uint_as_float(vv[j]) * inv;
       if (R16) {
-        y[0][j] = (s[n][0][e] + s[n][1][e]) * kk[j];
-        y[NR - 1][j] = (s[n][0][2 + e] + s[n][1][2 + e]) * kk[j];
+        y[0][j] = (s[n][0][e] + s[n][1][e]) * kk[0][j];
+        y[NR - 1][j] = (s[n][0][2 + e] + s[n][1][2 + e]) * kk[NR - 1][j];
       } else {
-        y[0][j] = ((s[n][0][2 + e] + s[n][1][2 + e]) + (s[n][0][e] + s[n][1][e])) * kk[j];
+        y[0][j] = ((s[n][0][2 + e] + s[n][1][2 + e]) + (s[n][0][e] + s[n][1][e])) * kk[0][j];
       }
       if (!PLAIN) {
         const int p = key + 8 * n + 2 * cl + e;
