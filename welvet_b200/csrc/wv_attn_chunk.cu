@@ -572,7 +572,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
         __syncwarp();
       };
       auto release = [&](int e) { if (leader) pc_commit(empty(e % STAGES)); __syncwarp(); };
-      if (wait(full(0), 0, 710)) {
+      if (wait(full(0), 0, 712)) {
         pc_fence_after();
         for (int t = 0; t < nt; t++) scores(t, 0);
         release(0);
@@ -608,7 +608,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
           }
         }
         idle = did ? 0 : idle + 1;
-        if (idle > PC_SPIN) { if (leader) fail(711); ok = false; }
+        if (idle > PC_SPIN) { if (leader) fail(713); ok = false; }
         if ((idle & 255) == 255 && __any_sync(0xffffffffu, dead())) ok = false;
       }
       if (!ok) {                                                         // what was issued has to end before tensor memory is given back
