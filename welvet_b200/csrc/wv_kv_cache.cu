@@ -335,10 +335,12 @@ __global__ void __launch_bounds__(32 * KVC_WARPS) kv_read_kernel(const WvKvGeom 
   }
 }
 
+int wv_sm_count();
 // Enough CTAs for the chip where there are few tokens; with many, a CTA for KVC_TOKENS of them.
 static int kvc_config(cudaLaunchConfig_t& cfg, cudaLaunchAttribute* at, int tokens, int rows, cudaStream_t st) {
-  const int tok = tokens >= 592 * KVC_TOKENS ? KVC_TOKENS : 1;
-  const int most = (rows + KVC_WARPS - 1) / KVC_WARPS, want = 592 / tokens;
+  const int ctas = KVC_BLOCKS * wv_sm_count();
+  const int tok = tokens / KVC_TOKENS >= ctas ? KVC_TOKENS : 1;
+  const int most = (rows + KVC_WARPS - 1) / KVC_WARPS, want = ctas / tokens;
   cfg.gridDim = dim3((tokens + tok - 1) / tok, want < 1 ? 1 : (want > most ? most : want));
   cfg.blockDim = dim3(32 * KVC_WARPS); cfg.stream = st;
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
