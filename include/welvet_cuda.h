@@ -198,8 +198,14 @@ int wv_kv_read_dev(const WvKvPages* kv, const WvKvBatch* batch, float* dk, int l
 /* Attention of the new tokens over the cached ones (mha/attn.go:15-120 for a chunk): the token at position p sees positions
  * max(0, p - window + 1) .. p (window <= 0: from 0), out = sum of softmax(scale q.k) v over them, zeros where it sees
  * none, NaN for a query that is not finite; query head h reads kv head h / (num_heads / num_kv_heads). max_q == 1 is a decode step;
- * max_kv is at most 2^30. Scratch for the results of splits, at most 256 MB, belongs to the stream (or to the graph, in a capture): the
- * first call for a larger shape allocates it. */
+ * max_kv is at most 2^30.
+ *
+ * Sums are float32; q and the weights enter the products as two float16 pieces each (22 bits). In the sum (not in the divisor) a
+ * weight counts to 2^-28 of its row's largest, so a key with less may be missing; a value row whose scale is below 2^-90 counts as
+ * zeros (all of it below some 1e-23 in 16 bits, 1e-25 in 8), and values beyond 2^90 (1e27) may overflow.
+ *
+ * Scratch for the results of splits, at most 256 MB, belongs to the stream (or to the graph, in a capture): the first call for a
+ * larger shape allocates it. */
 int wv_attn_paged_dev(const WvKvPages* kv, const WvKvBatch* batch, const float* dq, int ldq, float* dout, int ldo, int num_heads,
                       float scale, int window, void* stream);
 

@@ -194,6 +194,26 @@ def test_rows_are_rounded_as_stated(wv, bits, hd):
 
 
 @pytest.mark.parametrize("bits", [16, 8, 4])
+@pytest.mark.parametrize("largest", [1e37, 2.0 ** 127, 3.3e38])
+def test_rows_of_the_largest_magnitudes(wv, bits, largest):
+    """Rows whose largest value is near the end of float32's range, which one that rounds up to the next power of two would pass."""
+    c = Cache(wv, bits, 16, 2, 128, [(20, 20)])
+    rng = np.random.default_rng(bits)
+    k, v = (rng.uniform(-1, 1, (20, 2, 128)) * largest for _ in range(2))
+    k[:, :, 5], v[:, :, 100] = largest, -largest
+    k, v = k.astype(np.float32), v.astype(np.float32)
+    assert np.isfinite(k).all() and np.isfinite(v).all()
+    c.fill(torch.from_numpy(k.reshape(20, 256)).cuda(), torch.from_numpy(v.reshape(20, 256)).cuda())
+    back = [torch.zeros(20, 256, device="cuda") for _ in range(2)]
+    wv.paged.KVReadCUDA(c.pages, c.batch, back[0].data_ptr(), back[1].data_ptr())
+    torch.cuda.synchronize()
+    for x, which, b in ((k, "k", back[0]), (v, "v", back[1])):
+        want = quantise(x, bits)
+        assert np.isfinite(want).all() and np.array_equal(c.rows(which), want)
+        assert np.array_equal(b.cpu().numpy().reshape(20, 2, 128), want.astype(np.float32))
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
 @pytest.mark.parametrize("hd,theta", [(64, 10000.0), (128, 500000.0), (80, 10000.0), (256, 10000.0)])
 def test_rotation_and_places(wv, bits, hd, theta):
     """Q and K are rotated by their position as wv_rope_cache_dev does, in place or not, with gaps between rows; only the new
@@ -401,6 +421,52 @@ def test_large_and_small_values(wv):
             want, mag, reach = attn64(q[r:r + nq].reshape(nq, 2, 64), kk[a:a + kv], vv[a:a + kv], 0.125, 0, kv - nq)
             assert (np.abs(got[r:r + nq] - want) <= bound(mag, reach, 64, kv)).all(), bits
             a += kv
+
+
+def attn_of(c, q, heads, scale, lens):
+    """A call's outputs against 64 bits: error and bound of every value. A weight is a multiple of 2^-24 in the products, where the row's
+    largest is 2^4 or more (chunks; 2^6 for few rows): rounding leaves 2^-25 / 2^4 of the largest a key, times value codes that reach
+    twice the largest value in units of the largest scale. Where the keys with weight have the code 0, that is all there is."""
+    got = run_attn(c, torch.from_numpy(q.reshape(q.shape[0], -1)).cuda(), heads, scale).reshape(q.shape)
+    kk, vv = c.rows("k"), c.rows("v")
+    err, tol = np.zeros(q.shape), np.zeros(q.shape)
+    r = a = 0
+    for nq, kv in lens:
+        want, mag, reach = attn64(q[r:r + nq], kk[a:a + kv], vv[a:a + kv], scale, 0, kv - nq)
+        err[r:r + nq] = np.abs(got[r:r + nq] - want)
+        tol[r:r + nq] = bound(mag, reach, c.hd, kv) + kv * 2.0 ** -28 * (np.abs(vv[a:a + kv]).max() if kv else 0)
+        r, a = r + nq, a + kv
+    return err, tol
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
+@pytest.mark.parametrize("scale", [-0.125, -2.0, 0.0, -0.0, 1e-20, 3.0])
+def test_scales_of_any_sign(wv, bits, scale):
+    """A scale below 0 turns the order of the keys, one of 0 gives their mean; few rows and chunks."""
+    lens = [(1, 90), (12, 40), (100, 400), (6, 3)]
+    c = Cache(wv, bits, 16, 2, 64, lens)
+    rng = np.random.default_rng(bits)
+    n, total = sum(k for _, k in lens), sum(a for a, _ in lens)
+    c.fill(*(torch.from_numpy(rng.normal(0, 1, (n, 128)).astype(np.float32)).cuda() for _ in range(2)))
+    q = rng.normal(0, 1, (total, 4, 64)).astype(np.float32)
+    err, tol = attn_of(c, q, 4, scale, lens)
+    assert (err <= tol).all(), float((err / np.maximum(tol, 1e-30)).max())
+
+
+@pytest.mark.parametrize("bits", [16, 8, 4])
+@pytest.mark.parametrize("size", [2.0 ** 90, 1e20, 1e-20, 1e-22])
+def test_values_over_the_stated_range(wv, bits, size):
+    """V from the smallest scales that count (2^-90) to the largest values (2^90), over enough keys for several tiles and splits."""
+    lens = [(1, 2000), (12, 40), (100, 900)]
+    c = Cache(wv, bits, 16, 2, 64, lens)
+    rng = np.random.default_rng(bits)
+    n, total = sum(k for _, k in lens), sum(a for a, _ in lens)
+    v = rng.uniform(-1, 1, (n, 2, 64))
+    v[:, :, 9] = np.sign(v[:, :, 9])                                      # every row reaches 1
+    c.fill(torch.from_numpy(rng.normal(0, 1, (n, 128)).astype(np.float32)).cuda(), torch.from_numpy((v * size).astype(np.float32).reshape(n, 128)).cuda())
+    q = rng.normal(0, 1, (total, 4, 64)).astype(np.float32)
+    err, tol = attn_of(c, q, 4, 0.125, lens)
+    assert (err <= tol - 1e-30).all(), float((err / tol).max())          # without the absolute part
 
 
 @pytest.mark.parametrize("bits", [16, 8, 4])
