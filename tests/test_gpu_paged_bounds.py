@@ -224,6 +224,31 @@ def test_scratch_of_many_sequences_under_a_long_bound(wv, piece):
     assert wv._lib.lib().wv_device_status() == 0
 
 
+@pytest.mark.parametrize("heads,kvh,hd,max_q,most", [(8, 2, 256, 2048, 400), (4, 4, 144, 300, 5000), (16, 1, 192, 131072, 131072)])
+def test_wide_heads_under_loose_bounds(wv, heads, kvh, hd, max_q, most):
+    """Heads beyond 128: single tokens, a piece of a prompt and empty sequences in a batch whose bounds allow each far more (256 sequences
+    of 131072 tokens have more tiles of rows than a grid)."""
+    lens = ([(1, 60), (40, 90), (0, 0), (3, 3), (1, 300), (70, 70), (1, 1), (9, 200)] + [(1, 17), (0, 5)] * 16) if max_q < 131072 else [(1, 60), (33, 90)] + [(0, 0)] * 254
+    c = Cache(wv, 8, 16, kvh, hd, lens, seed=hd)
+    rng = np.random.default_rng(hd)
+    n, total = sum(k for _, k in lens), sum(q for q, _ in lens)
+    c.fill(*(torch.from_numpy(rng.normal(0, 1, (n, kvh * hd)).astype(np.float32)).cuda() for _ in range(2)))
+    q = rng.normal(0, 1, (total, heads * hd)).astype(np.float32)
+    dq, out = torch.from_numpy(q).cuda(), torch.full((total + 5, heads * hd), 7.0, device="cuda")
+    table = torch.full((len(lens), -(-most // 16)), -1, dtype=torch.int32, device="cuda")
+    table[:, :c.table.shape[1]] = c.d_table
+    start, kv = arrays(c, lens)
+    b = wv.paged.Batch(start.data_ptr(), kv.data_ptr(), table.data_ptr(), len(lens), table.shape[1], total + 5, max_q, most)
+    scale = hd ** -0.5
+    wv.paged.AttnPagedCUDA(c.pages, b, dq.data_ptr(), out.data_ptr(), heads, scale)
+    torch.cuda.synchronize()
+    assert wv._lib.lib().wv_device_status() == 0
+    got = out.cpu().numpy()
+    assert (got[total:] == 7.0).all()
+    want, tol = want_attn(c, lens, q, heads, scale)
+    assert (np.abs(got[:total].reshape(total, heads, hd) - want) <= tol).all()
+
+
 def test_no_more_positions_than_the_attention_counts(wv):
     """A billion cached tokens and more under one table row are refused: keys are counted in 32 bits."""
     c = Cache(wv, 8, 16, 2, 64, [(1, 20)])

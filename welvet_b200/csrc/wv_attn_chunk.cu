@@ -125,32 +125,6 @@ template <int BITS, int DP> struct PcShape {
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
-// The flat-th tile of 256 rows of the sequences that have more than rows_most rows, found by a whole warp: its sequence (-1: none)
-// and its place in it, the later tokens, which see most, first.
-__device__ __forceinline__ void pc_find(const PaCall& c, int flat, int* err, int& seq, int& tile) {
-  const int lane = threadIdx.x & 31;
-  int before = 0;
-  seq = -1; tile = 0;
-  for (int s0 = 0; s0 < c.b.num_seqs && seq < 0; s0 += 32) {
-    int n = 0;
-    if (s0 + lane < c.b.num_seqs) {
-      const WvSeq q = wv_seq(c.b, c.g.page, s0 + lane, err);
-      const long long rows = (long long)(q.q1 - q.q0) * c.group;
-      n = rows > c.rows_most ? (int)((rows + 255) / 256) : 0;
-    }
-    int upto = n;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += v; }
-    const unsigned hit = __ballot_sync(0xffffffffu, before + upto > flat);
-    if (hit) {
-      const int at = __ffs(hit) - 1;
-      seq = s0 + at;
-      tile = before + __shfl_sync(0xffffffffu, upto, at) - 1 - flat;
-    }
-    before += __shfl_sync(0xffffffffu, upto, 31);
-  }
-}
-
 template <int BITS> __device__ __forceinline__ int pc_dim(int p) {      // the value that stands at place p of a row
   if constexpr (BITS == 4) return (p & ~7) | ((p & 7) >> 1) | (p & 1) << 2;
   return p;
@@ -186,7 +160,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
   const int kvh = blockIdx.x % c.g.kvh, flat = blockIdx.x / c.g.kvh, sp = blockIdx.y;
   if (warp == 0) {
     int seq, tile;
-    pc_find(c, flat, blockIdx.x == 0 && sp == 0 ? c.err : nullptr, seq, tile);
+    pa_find(c, flat, 256, c.rows_most, blockIdx.x == 0 && sp == 0 ? c.err : nullptr, seq, tile);
     if (lane == 0) { M.seq = seq; M.tile = tile; M.qmax = 0; M.abort = 0; }
   }
   __syncthreads();
@@ -816,7 +790,7 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const __grid_constant__
   const int kvh = blockIdx.x % c.g.kvh, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   if (warp == 0) {
     int seq, tile;
-    pc_find(c, blockIdx.x / c.g.kvh, nullptr, seq, tile);
+    pa_find(c, blockIdx.x / c.g.kvh, 256, c.rows_most, nullptr, seq, tile);
     if (lane == 0) { s_at[0] = seq; s_at[1] = tile; }
   }
   __syncthreads();

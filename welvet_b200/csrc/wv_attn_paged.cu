@@ -124,7 +124,20 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   const unsigned flat = c.first + blockIdx.x, of_head = flat / (unsigned)c.g.kvh;
-  const int kvh = flat - of_head * c.g.kvh, seq = of_head / c.tiles, tile = of_head - seq * c.tiles, sp = blockIdx.y;
+  const int kvh = flat - of_head * c.g.kvh, sp = blockIdx.y;
+  int seq, tile;
+  if (DP == 256 && c.tiles == 0) {                                       // see wv_launch_attn_paged
+    __shared__ int s_at[2];
+    if (warp == 0) {
+      pa_find(c, of_head, NROW, 0, nullptr, seq, tile);
+      if (lane == 0) { s_at[0] = seq; s_at[1] = tile; }
+    }
+    __syncthreads();
+    seq = s_at[0]; tile = s_at[1];
+    if (seq < 0) return;
+  } else {
+    seq = of_head / c.tiles; tile = of_head - seq * c.tiles;
+  }
   const WvSeq sq = wv_seq(c.b, c.g.page, seq, sp == 0 && kvh == 0 && tile == 0 ? c.err : nullptr);
   const int nrows = (sq.q1 - sq.q0) * c.group, r0 = tile * NROW;
   if (r0 >= nrows || nrows > c.rows_most) return;
@@ -645,7 +658,15 @@ __global__ void __launch_bounds__(128) rows_join_kernel(const __grid_constant__ 
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const unsigned block = blockIdx.x / c.kept, flat = c.first + block, of_head = flat / (unsigned)c.g.kvh;
-  const int kvh = flat - of_head * c.g.kvh, seq = of_head / c.tiles, r = (of_head - seq * c.tiles) * nrow + blockIdx.x - block * c.kept;
+  const int kvh = flat - of_head * c.g.kvh;
+  int seq, tile;
+  if (c.tiles == 0) {                                                    // each of the warps for itself
+    pa_find(c, of_head, nrow, 0, nullptr, seq, tile);
+    if (seq < 0) return;
+  } else {
+    seq = of_head / c.tiles; tile = of_head - seq * c.tiles;
+  }
+  const int r = tile * nrow + blockIdx.x - block * c.kept;
   const WvSeq sq = wv_seq(c.b, c.g.page, seq, nullptr);
   const int nrows = (sq.q1 - sq.q0) * c.group;
   if (r >= nrows || nrows > c.rows_most) return;
@@ -713,7 +734,11 @@ int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* d
     const bool r16 = top > 8;
     const int nrow = r16 ? 16 : 8;
     const long long tiles = (top + nrow - 1) / nrow;
-    const long long blocks = (long long)b.num_seqs * tiles * c.g.kvh;
+    // Heads beyond 128 come here with prompts as well. Beside short sequences most of the tiles that max_q allows for each are then empty
+    // (and may be more than a grid holds): where total_q allows a quarter of them or less, a block looks its sequence up.
+    const long long rows_tiles = (long long)b.num_seqs * tiles, full_tiles = (long long)b.total_q * c.group / nrow + b.num_seqs;
+    const bool look = c.g.hd > 128 && full_tiles <= rows_tiles / 4;
+    const long long blocks = (look ? full_tiles : rows_tiles) * c.g.kvh;
     if (blocks * nrow > INT_MAX) { wv_set_error("wv_attn_paged_dev: %d sequences are too many", b.num_seqs); return WV_ESHAPE; }
     // Splits of the keys: the number that fills 1, 2, .. 8 waves of the blocks that run at once and costs least, a wave being worth a
     // warp's groups of 16 keys and some six more of start and end (2049 positions and eight blocks: 33 splits of 64; 131000: 55).
@@ -734,7 +759,7 @@ int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* d
     if (per < keys / 8192) per = (keys / 8192 + 63) & ~63LL;
     const long long ns = keys > per ? (keys + per - 1) / per : 1;
     PaCall r = c;
-    r.per = (int)per; r.nsplit = (int)ns; r.tiles = (unsigned)tiles; r.kept = (unsigned)(top < nrow ? top : nrow);
+    r.per = (int)per; r.nsplit = (int)ns; r.tiles = look ? 0u : (unsigned)tiles; r.kept = (unsigned)(top < nrow ? top : nrow);
     // The splits' results of all rows may be more than a call should keep (a prompt of 8192 tokens and 16 heads of 256: 0.9 GB): the blocks
     // then go in parts of equal size, one after the other through the same scratch. A part holds 600 blocks of 16 rows or more up to 26
     // splits of the widest heads, so it still fills the chip.

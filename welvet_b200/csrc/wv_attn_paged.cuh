@@ -21,7 +21,7 @@ struct PaCall {
   unsigned one;                    // 0x3c003c00, for pa_nibbles
   int rows_most;                   // sequences with more rows (tokens x group) than this go to the chunk kernel (0: all that have any)
   int nsplit, per;                 // splits of a sequence's keys, keys of a split (a multiple of 16; of 128 for chunks)
-  unsigned tiles, first, kept;     // few rows: tiles of a sequence, the launch's first block of rows, rows of a block with split results
+  unsigned tiles, first, kept;     // few rows: tiles of a sequence (0: see pa_find), the launch's first block of rows, rows of a block with split results
   float2* ml;                      // split results [row][nsplit]: {M, divisor}; {-inf, 0} and no sums for a split without keys
   float* acc;                      // [row][nsplit][head_dim]
   int* err;
@@ -68,6 +68,32 @@ __device__ __forceinline__ void pa_range(const WvSeq& s, int tok0, int tok1, int
   const int p0 = s.p0 + tok0;
   hi = max(0, s.p0 + tok1 + 1);
   lo = window > 0 ? max(0, max(p0, 0) - window + 1) & ~15 : 0;
+}
+
+// The flat-th tile of `size` rows (tokens x group) of the sequences that have more than `above` rows, found by a whole warp: its sequence
+// (-1: none) and its place in it, the later tokens, which see most, first.
+__device__ __forceinline__ void pa_find(const PaCall& c, int flat, int size, int above, int* err, int& seq, int& tile) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  seq = -1; tile = 0;
+  for (int s0 = 0; s0 < c.b.num_seqs && seq < 0; s0 += 32) {
+    int n = 0;
+    if (s0 + lane < c.b.num_seqs) {
+      const WvSeq q = wv_seq(c.b, c.g.page, s0 + lane, err);
+      const long long rows = (long long)(q.q1 - q.q0) * c.group;
+      n = rows > above ? (int)((rows + size - 1) / size) : 0;
+    }
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += v; }
+    const unsigned hit = __ballot_sync(0xffffffffu, before + upto > flat);
+    if (hit) {
+      const int at = __ffs(hit) - 1;
+      seq = s0 + at;
+      tile = before + __shfl_sync(0xffffffffu, upto, at) - 1 - flat;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
 }
 
 // A row out of its splits' results, in two steps. By a whole warp (each of a block's may do it): the splits' weights into w[nsplit];
