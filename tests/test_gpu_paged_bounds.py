@@ -249,6 +249,33 @@ def test_wide_heads_under_loose_bounds(wv, heads, kvh, hd, max_q, most):
     assert (np.abs(got[:total].reshape(total, heads, hd) - want) <= tol).all()
 
 
+@pytest.mark.parametrize("hd", [64, 256])
+@pytest.mark.parametrize("what", ["kv_len", "q_start"])
+@pytest.mark.parametrize("total", [96 * 42, 96 * 42 + 200, 130])
+def test_lengths_out_of_bounds_behind_the_first_sequence(wv, hd, what, total):
+    """A length out of its bounds is reported wherever it stands, with tokens of its own or none, whichever kernels run."""
+    lens = [(96, 100)] + [(0, 50)] * 40 + [(30, 50)]
+    c = Cache(wv, 8, 16, 2, hd, lens)
+    c.fill(torch.randn(2150, 2 * hd, device="cuda"), torch.randn(2150, 2 * hd, device="cuda"))
+    q, out = torch.randn(total, 8 * hd, device="cuda"), torch.zeros(total, 8 * hd, device="cuda")
+    start, kv = arrays(c, lens)
+    status = wv._lib.lib().wv_device_status
+    b = wv.paged.Batch(start.data_ptr(), kv.data_ptr(), c.d_table.data_ptr(), 42, c.table.shape[1], total, 96, 100)
+
+    def call():
+        wv.paged.AttnPagedCUDA(c.pages, b, q.data_ptr(), out.data_ptr(), 8, 0.1)
+        torch.cuda.synchronize()
+        return status()
+    assert call() == 0
+    for i, bad in ((35, 101), (35, -1), (41, 10 ** 9)) if what == "kv_len" else ((36, 90), (42, 96 + 97), (42, total + 1)):
+        a = kv if what == "kv_len" else start
+        saved = int(a[i])
+        a[i] = bad
+        assert call() == wv._lib.WV_ESHAPE, (i, bad)
+        a[i] = saved
+    assert call() == 0
+
+
 def test_no_more_positions_than_the_attention_counts(wv):
     """A billion cached tokens and more under one table row are refused: keys are counted in 32 bits."""
     c = Cache(wv, 8, 16, 2, 64, [(1, 20)])

@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
   if (DP == 256 && c.tiles == 0) {                                       // see wv_launch_attn_paged
     __shared__ int s_at[2];
     if (warp == 0) {
-      pa_find(c, of_head, NROW, 0, nullptr, seq, tile);
+      pa_find(c, of_head, NROW, 0, flat == 0 && sp == 0 ? c.err : nullptr, seq, tile);
       if (lane == 0) { s_at[0] = seq; s_at[1] = tile; }
     }
     __syncthreads();

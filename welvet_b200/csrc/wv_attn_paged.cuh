@@ -71,12 +71,12 @@ __device__ __forceinline__ void pa_range(const WvSeq& s, int tok0, int tok1, int
 }
 
 // The flat-th tile of `size` rows (tokens x group) of the sequences that have more than `above` rows, found by a whole warp: its sequence
-// (-1: none) and its place in it, the later tokens, which see most, first.
+// (-1: none) and its place in it, the later tokens, which see most, first. With err it reads on through all sequences and reports.
 __device__ __forceinline__ void pa_find(const PaCall& c, int flat, int size, int above, int* err, int& seq, int& tile) {
   const int lane = threadIdx.x & 31;
   int before = 0;
   seq = -1; tile = 0;
-  for (int s0 = 0; s0 < c.b.num_seqs && seq < 0; s0 += 32) {
+  for (int s0 = 0; s0 < c.b.num_seqs && (seq < 0 || err); s0 += 32) {
     int n = 0;
     if (s0 + lane < c.b.num_seqs) {
       const WvSeq q = wv_seq(c.b, c.g.page, s0 + lane, err);
@@ -87,7 +87,7 @@ __device__ __forceinline__ void pa_find(const PaCall& c, int flat, int size, int
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += v; }
     const unsigned hit = __ballot_sync(0xffffffffu, before + upto > flat);
-    if (hit) {
+    if (hit && seq < 0) {
       const int at = __ffs(hit) - 1;
       seq = s0 + at;
       tile = before + __shfl_sync(0xffffffffu, upto, at) - 1 - flat;
