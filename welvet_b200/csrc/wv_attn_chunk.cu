@@ -294,11 +294,14 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
       };
       for (int j = 0; j < n; j++) {
         const int ms = j & 1, key0 = k0 + j * PC_N;
+        // rows that are lifted or have a reference of 2^20 or more: the warp rounds its logits first
+        const unsigned lifted = M.lift[r];
+        auto apart = [&]() { return __any_sync(0xffffffffu, lifted || (__float_as_uint(m) & 0x7fffffffu) - __float_as_uint(1048576.f) < 0x7f800000u - __float_as_uint(1048576.f)); };
+        bool slow = apart();
         if (!wait(m_full(ms), j >> 1, 700 + t) || !wait(s_full(t), j, 702 + t)) break;
         pc_fence_after();
         const unsigned kk = smem_u32(M.kk[ms]) + 4 * HK * hf, fv = smem_u32(M.fv[ms]) + 4 * HK * hf;
         float beta = M.beta[ms], alpha = 1.f;
-        const unsigned lifted = M.lift[r];
         const float down = __uint_as_float((127u - lifted) << 23);
         const unsigned flags = M.flags[ms];
         const bool masked = (flags & 1u) || key0 + PC_N - 1 > pmin || key0 + PC_N > k1 || (c.window != 0 && key0 <= pmax - c.window);
@@ -361,6 +364,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
           mx = fmaxf(mx, __uint_as_float(pc_ld1(tx)));
           alpha = mx > m ? pa_ex2(m - mx) : 1.f;                         // 0 while there was nothing
           m = mx;
+          slow = apart();
           l2 = __fmul2_rn(l2, make_float2(alpha, alpha));
         }
         const float2 off = m == -INFINITY ? make_float2(0.f, 0.f) : make_float2(PC_LIFT - m, PC_LIFT - m);
@@ -430,8 +434,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
             }
             pc_st16(ts + 16 * q, w);
           };
-          const unsigned far = (__float_as_uint(m) & 0x7fffffffu) - __float_as_uint(1048576.f);      // 2^20 up to infinity: large
-          if (!masked && !__any_sync(0xffffffffu, lifted || far < 0x7f800000u - __float_as_uint(1048576.f))) {
+          if (!masked && !slow) {
 #pragma unroll
             for (int q = 0; q < 4; q++) weights(std::false_type(), q, 0u);
           } else {

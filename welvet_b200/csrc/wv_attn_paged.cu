@@ -712,7 +712,7 @@ int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* d
   c.g = wv_kv_geom(kv);
   c.b = b;
   c.q = dq; c.ldq = ldq; c.out = dout; c.ldo = ldo;
-  c.heads = heads; c.group = heads / c.g.kvh;
+  c.group = heads / c.g.kvh;
   c.scale = scale * 1.4426950408889634f;
   c.window = window;
   c.one = 0x3c003c00u;

@@ -7,7 +7,6 @@
 #include "wv_paged.cuh"
 #include <math.h>
 
-#define PA_LIFT 13.f
 #define PA_SCRATCH (256LL << 20)        // bytes that a call may keep for its splits' results
 
 struct PaCall {
@@ -15,7 +14,7 @@ struct PaCall {
   WvKvBatch b;
   const float* q; int ldq;
   float* out; int ldo;
-  int heads, group;                // query heads, and those of one kv head
+  int group;                       // query heads of one kv head
   float scale;                     // times log2(e)
   int window;                      // 0: none
   unsigned one;                    // 0x3c003c00, for pa_nibbles
