@@ -3,7 +3,7 @@
 // A block takes 256 rows (tokens x query heads of one kv head, so that a cached row is read once for the group) as two tiles of 128
 // and walks the keys, 128 at a time, with a running maximum:
 //   S = Q K^T    Q (two float16 pieces, hi and lo) and K in shared memory, S in tensor memory       2 x 128 x 128 x head_dim products
-//   P            weights in two float16 pieces, written over S, 32 keys a piece pair                 one row a thread
+//   P            weights in two float16 pieces, written over S, 16 keys a piece pair                 two threads a row
 //   O_j = P V    P out of tensor memory, V in shared memory, keys being V's rows                     2 x 128 x head_dim x 128
 // O is summed up over the key tiles in registers (128 float32 a row): the tensor core cuts instead of rounding as it adds, which over
 // thousands of keys would show, a tile's 128 do not; and the maximum's correction is a factor in that sum instead of a pass over
@@ -12,8 +12,8 @@
 // 8000 now: the weights alone 2600 of issue on every scheduler (ten cycles an element: ex2 eight, beside it the conversions and the
 // packed products), the maxima, the sums in registers and the waits between the roles the rest.
 //
-// Measured, heads of 128: prompts of up to 4096 tokens, four together, 32 heads in 16 bits, 531 us (floor of the doubled products 238); 2048
-// tokens of 10000 with a window of 4000, 64 heads in 4 bits, 665 us (323); 512 tokens over 4608 positions, 32 heads in 8 bits, 118 us (44).
+// Measured, heads of 128: prompts of up to 4096 tokens, four together, 32 heads in 16 bits, 546 us (floor of the doubled products 238); 2048
+// tokens of 10000 with a window of 4000, 64 heads in 4 bits, 669 us (323); 512 tokens over 4608 positions, 32 heads in 8 bits, 120 us (44).
 //
 // Roles: four warpgroups have a tile's half each (a thread a row: the weights of 64 of the 128 keys, the sums of half of the values),
 // one warp issues the MMAs, three fill the ring, K and V tiles in turn. With one warpgroup a tile the weights of 128 keys were a

@@ -8,7 +8,7 @@
 // registers; with 9 to 16 rows there is an instruction for each.
 //
 // A warp works alone: it takes 16 keys at a time, copies their K and V rows, scales and sub-scales into its own ring of shared memory
-// (cp.async, 20 to 25 KB in flight a warp, no barrier but its own), turns codes into float16 as it reads them, and keeps maximum,
+// (cp.async, 9 to 17 KB in flight a warp, no barrier but its own), turns codes into float16 as it reads them, and keeps maximum,
 // divisor and the weighted sum in registers. Which 8 or 16 values of a row a lane reads is chosen so that they are neighbours in
 // memory: the order of the products does not matter for K, and for V it only decides which output a lane holds. Rows lie in the
 // ring with their 16-byte pieces permuted so that both reading patterns are free of bank conflicts.
@@ -17,10 +17,11 @@
 // dependent loads: lengths, page numbers, rows) runs beside another's keys. The keys of a sequence are split over blocks; the splits
 // leave {M, divisor, sums} and a second kernel joins them in order, so results do not depend on who ran first.
 //
-// Measured: one token over 2049 positions (32 heads, 8 kv heads of 128, 16 bits) 10 us; over 131000 positions in 4 bits (64 heads) 71 us,
+// Measured: one token over 2049 positions (32 heads, 8 kv heads of 128, 16 bits) 10 us; over 131000 positions in 4 bits (64 heads) 72 us,
 // 2.3 TB/s of codes and scales; 64 tokens over up to 8192 positions in 8 bits 130 us, 4.3 TB/s; 16 x 5 tokens over 3000, heads of 64 in
-// 16 bits, 29 us. What bounds the long ones is issue: 535 instructions per 16 keys in 4 bits, 460 in 8 bits, 0.55 a cycle and scheduler
-// with three blocks; a fourth (q's fragments out of shared memory, 128 registers) issues no more and took 79 and 191 us.
+// 16 bits, 29 us. Neither DRAM (30 and 53 %) nor issue (0.55 a cycle and scheduler) is full in the long ones: what bounds them is latency
+// within a warp, one dependent chain a group of 16 keys (535 instructions in 4 bits, 460 in 8 bits) with 2.8 warps a scheduler to
+// hide it. A fourth block (q's fragments out of shared memory, 128 registers) issued no more and took 79 and 191 us.
 #include "wv_attn_paged.cuh"
 #include "wv_tma_common.cuh"
 #include "wv_lease.h"

@@ -1,8 +1,10 @@
 // What the kernels of the paged attention share: the weights' units, the split results and their merge.
 //
 // A key's logit is x = scale log2(e) q.k, its weight 2^x, its value row v = f 2^E c with c the codes and 2^E the largest value scale's power
-// of two among the keys at hand. What goes through the tensor cores is 2^(x - m) f in two float16 pieces (22 bits), m the running
-// maximum of x; the divisor is sum 2^(x - m) in float32. Both sums carry a factor of 2^13 that uses the float16 range and cancels.
+// of two among the keys at hand. What goes through the tensor cores is 2^(x - m) f in two float16 pieces (22 bits), the divisor is
+// sum 2^(x - m) in float32. m follows the running maximum of x and may lie 2^7 (few rows) or 2^10 (chunks) below it; both sums carry a
+// factor, 2^6 and 2^4, that uses the float16 range and cancels. With f below 2 a weight is at most 2^14 and 2^15, and what rounds away of
+// one is below 2^-30 and 2^-28 of the largest.
 #pragma once
 #include "wv_paged.cuh"
 #include <math.h>

@@ -7,8 +7,10 @@
 // value that a value is turned with comes from the lane 16 away; loading it a second time took 135 us for the prompts below. Two tokens
 // share the chain of loads that finds a token's place (its sequence, length, page) and fill the CTA with their angles.
 //
-// Prompts of 9900 tokens together, 32 query heads and 8 kv heads of 128, 8 bits, written and read back: 117 us, 4.4 TB/s.
-// One token: 5.5 us; 200 tokens in 4 bits: 8.8 us (two launches each, captured in a graph).
+// Prompts of 9900 tokens together, 32 query heads and 8 kv heads of 128, 8 bits, written and read back: 118 us, 4.4 TB/s; neither DRAM
+// (46 %) nor issue (50 %) is full, a CTA asks for a token's rows and then waits for them.
+// One token: 5.7 us; 200 tokens in 4 bits: 9.0 us (two launches each, captured in a graph; called one by one, the host's part of the
+// two calls makes it 13 us for either).
 #include "wv_paged.cuh"
 #include <float.h>
 #include <math.h>
