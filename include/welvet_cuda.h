@@ -196,9 +196,9 @@ int wv_kv_write_dev(const WvKvPages* kv, const WvKvBatch* batch, const float* dk
 /* The same tokens' K and V out of the pages, as float32 (rows of tokens before position 0 or in pages out of bounds: zeros). */
 int wv_kv_read_dev(const WvKvPages* kv, const WvKvBatch* batch, float* dk, int ldk, float* dv, int ldv, void* stream);
 /* Attention of the new tokens over the cached ones (mha/attn.go:15-120 for a chunk): the token at position p sees positions
- * max(0, p - window + 1) .. p (window <= 0: from 0), out = sum of softmax(scale q.k) v over them, zeros where it sees
- * none, NaN for a query that is not finite; query head h reads kv head h / (num_heads / num_kv_heads). max_q == 1 is a decode step;
- * max_kv is at most 2^30.
+ * max(0, p - window + 1) .. p (window <= 0: from 0), out = sum of softmax(scale q.k) v over them; zeros where it sees
+ * none, whatever its query holds, else NaN for a query that is not finite. Query head h reads kv head h / (num_heads /
+ * num_kv_heads). max_q == 1 is a decode step; max_kv is at most 2^30.
  *
  * Sums are float32; q and the weights enter the products as two float16 pieces each (22 bits). In the sum (not in the divisor) a
  * weight counts to 2^-28 of its row's largest, so a key with less may be missing; a value row whose scale is below 2^-90 counts as

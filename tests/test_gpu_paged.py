@@ -553,6 +553,37 @@ def test_strides_and_rows_of_nobody(wv):
         assert (got[:, heads * hd:] == 7.0).all() and (got[2 * nq:] == 7.0).all()
 
 
+@pytest.mark.parametrize("bits", [16, 4])
+def test_a_pool_beyond_4_gb(wv, bits):
+    """Pages whose bytes start past 2^32: written, read back, and attended over by few rows and chunks as from a small pool."""
+    lens, kvh, hd, page = [(1, 200), (60, 130)], 8, 128, 16
+    n = sum(k for _, k in lens)
+    gen = torch.Generator(device="cuda").manual_seed(bits)
+    k, v, q = (torch.randn(r, w, device="cuda", generator=gen) for r, w in ((n, kvh * hd), (n, kvh * hd), (61, 16 * hd)))
+    small = Cache(wv, bits, page, kvh, hd, lens)
+    big = Cache(wv, bits, page, kvh, hd, lens)
+    pages = 2 ** 32 // (kvh * big.bytes) + big.num_pages
+    first = pages - big.num_pages
+    big.pool = torch.zeros(pages, kvh, big.bytes, dtype=torch.uint8, device="cuda")
+    big.table = np.where(big.table < 0, -1, big.table + first).astype(np.int32)
+    big.d_table = torch.from_numpy(big.table).cuda()
+    big.pages = wv.paged.KVPages(big.pool.data_ptr(), bits, pages, page, kvh, hd)
+    big.batch, big.keep = big.batch_of(lens)
+    back = []
+    for c in (small, big):
+        c.fill(k, v)
+        b, keep = c.batch_of([(m, m) for _, m in lens])
+        kv = [torch.zeros(n, kvh * hd, device="cuda") for _ in range(2)]
+        wv.paged.KVReadCUDA(c.pages, b, kv[0].data_ptr(), kv[1].data_ptr())
+        first_only, keep2 = c.batch_of([lens[0]])
+        one, all_ = run_attn(c, q[:1], 16, 0.09, batch=first_only), run_attn(c, q, 16, 0.09)
+        back.append([t.cpu().numpy() for t in kv] + [one, all_])
+    assert not big.pool[:first].any() and torch.equal(big.pool[first:], small.pool)
+    for a, b in zip(*back):
+        assert np.array_equal(a, b) and np.isfinite(a).all() and a.any()
+    assert wv._lib.lib().wv_device_status() == 0
+
+
 def test_results_do_not_change_from_run_to_run(wv):
     for lens in ([(1, 3000), (1, 40)], [(300, 900)]):
         c = Cache(wv, 8, 16, 2, 128, lens)

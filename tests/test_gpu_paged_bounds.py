@@ -249,6 +249,27 @@ def test_wide_heads_under_loose_bounds(wv, heads, kvh, hd, max_q, most):
     assert (np.abs(got[:total].reshape(total, heads, hd) - want) <= tol).all()
 
 
+@pytest.mark.parametrize("hd", [64, 128, 256])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), -3e38])
+def test_queries_before_position_0(wv, hd, what):
+    """What the rows of tokens that see nothing hold does not matter: they are zeros, and the others do not notice."""
+    lens = [(9, 5), (1, 0), (3, 1), (90, 60), (40, 0)]
+    c = Cache(wv, 8, 16, 2, hd, lens)
+    rng = np.random.default_rng(hd)
+    n, total = sum(k for _, k in lens), sum(q for q, _ in lens)
+    c.fill(*(torch.from_numpy(rng.normal(0, 1, (n, 2 * hd)).astype(np.float32)).cuda() for _ in range(2)))
+    q = rng.normal(0, 1, (total, 4 * hd)).astype(np.float32)
+    want, tol = want_attn(c, lens, q, 4, hd ** -0.5)
+    r = 0
+    for nq, kv in lens:
+        q[r:r + max(0, nq - kv)] = what
+        r += nq
+    out = torch.full((total, 4 * hd), 7.0, device="cuda")
+    wv.paged.AttnPagedCUDA(c.pages, c.batch, torch.from_numpy(q).cuda().data_ptr(), out.data_ptr(), 4, hd ** -0.5)
+    torch.cuda.synchronize()
+    assert (np.abs(out.cpu().numpy().reshape(total, 4, hd) - want) <= tol).all()
+
+
 @pytest.mark.parametrize("hd", [64, 256])
 @pytest.mark.parametrize("what", ["kv_len", "q_start"])
 @pytest.mark.parametrize("total", [96 * 42, 96 * 42 + 200, 130])
