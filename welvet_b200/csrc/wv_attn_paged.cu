@@ -19,7 +19,7 @@
 //
 // Measured: one token over 2049 positions (32 heads, 8 kv heads of 128, 16 bits) 10 us; over 131000 positions in 4 bits (64 heads) 72 us,
 // 2.3 TB/s of codes and scales; 64 tokens over up to 8192 positions in 8 bits 130 us, 4.3 TB/s; 16 x 5 tokens over 3000, heads of 64 in
-// 16 bits, 29 us. Neither DRAM (30 and 53 %) nor issue (0.55 a cycle and scheduler) is full in the long ones: what bounds them is latency
+// 16 bits, 29 us. Neither DRAM (32 and 54 %) nor issue (0.55 a cycle and scheduler) is full in the long ones: what bounds them is latency
 // within a warp, one dependent chain a group of 16 keys (535 instructions in 4 bits, 460 in 8 bits) with 2.8 warps a scheduler to
 // hide it. A fourth block (q's fragments out of shared memory, 128 registers) issued no more and took 79 and 191 us.
 #include "wv_attn_paged.cuh"

@@ -8,7 +8,7 @@
 // share the chain of loads that finds a token's place (its sequence, length, page) and fill the CTA with their angles.
 //
 // Prompts of 9900 tokens together, 32 query heads and 8 kv heads of 128, 8 bits, written and read back: 118 us, 4.4 TB/s; neither DRAM
-// (46 %) nor issue (50 %) is full, a CTA asks for a token's rows and then waits for them.
+// (52 %) nor issue (56 %) is full, a CTA asks for a token's rows and then waits for them.
 // One token: 5.7 us; 200 tokens in 4 bits: 9.0 us (two launches each, captured in a graph; called one by one, the host's part of the
 // two calls makes it 13 us for either).
 #include "wv_paged.cuh"
