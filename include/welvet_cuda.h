@@ -209,6 +209,40 @@ int wv_kv_read_dev(const WvKvPages* kv, const WvKvBatch* batch, float* dk, int l
 int wv_attn_paged_dev(const WvKvPages* kv, const WvKvBatch* batch, const float* dq, int ldq, float* dout, int ldo, int num_heads,
                       float scale, int window, void* stream);
 
+/* Page tables on the device. refs[num_pages] counts for every page the places of the tables that hold it (0: the page is free),
+ * pages[num_seqs][table_stride] and kv_len[num_seqs] are a batch's: sequence s holds pages[s][0 .. ceil(kv_len[s] / page_size) - 1].
+ * All-zero refs and kv_len are an empty cache. The calls below change all three and nothing else, but for the copies of pages that
+ * extend and compact make in `pools` (the caches of all blocks that use the table: pages of one size in tokens and number, of any width;
+ * num_pools may be 0). They are asynchronous on `stream`, hold no state of their own and can be captured; calls that share a table are
+ * ordered by the caller. An entry that breaks a rule is left out and wv_device_status() then reports WV_ESHAPE. Results are the same in
+ * every run.
+ *
+ * wv_kv_fork_dev: for i < n, the empty sequence d_dst[i] becomes the first d_keep[i] tokens (d_keep NULL: all of them) of sequence
+ *   d_src[i], in the same pages. No target is a source of the call; of entries with the same target the first one counts.
+ * wv_kv_extend_dev: sequence s gets room for d_add[s] more tokens (kv_len counts them from then on, so that the table is the batch's for the
+ *   step that writes them): new pages where it needs them, and a copy of its last page where that is partly filled and held more than
+ *   once. The free pages go, in rising order, to the sequences in theirs (to one's copy first); a sequence whose pages, added to those of all before
+ *   it, are more than were free before the call is refused, and so is one that would not fit its row of the table: it stays as it is.
+ *   d_granted[s] (may be NULL) is 1 or 0.
+ * wv_kv_trim_dev: for i < n, sequence d_seqs[i] (d_seqs NULL: i) is cut to d_keep[i] tokens (d_keep NULL: 0, the sequence is freed); its pages
+ *   behind them are given back and their places in the table are -1. One that is no longer than that stays as it is; of entries with
+ *   the same sequence the first one counts.
+ * wv_kv_compact_dev: with L pages held, the k-th held page from L on moves to the k-th free page in front of L, in all pools and tables. *d_live
+ *   becomes L; the pages from L on are free then (what stood in them stays).
+ * wv_kv_copy_dev: for i < n, page d_src[i] of every pool is copied to page d_dst[i]. The pages of d_dst differ from one another and from those of d_src
+ *   (but a page may be copied to itself, which does nothing). */
+typedef struct WvKvTable {
+  int* refs;
+  int* pages;
+  int* kv_len;
+  int num_pages, page_size, num_seqs, table_stride;
+} WvKvTable;
+int wv_kv_fork_dev(const WvKvTable* table, const int* d_src, const int* d_dst, const int* d_keep, int n, void* stream);
+int wv_kv_extend_dev(const WvKvTable* table, const int* d_add, int* d_granted, const WvKvPages* pools, int num_pools, void* stream);
+int wv_kv_trim_dev(const WvKvTable* table, const int* d_seqs, const int* d_keep, int n, void* stream);
+int wv_kv_compact_dev(const WvKvTable* table, const WvKvPages* pools, int num_pools, int* d_live, void* stream);
+int wv_kv_copy_dev(const WvKvPages* pools, int num_pools, const int* d_src, const int* d_dst, int n, void* stream);
+
 /* The next token of each of `rows` rows of n logits (row r at d_logits + r * ld, ld 0: n). Parameters are device arrays, one
  * value a row: temperature T, top_k, top_p, min_p and the draw u in [0, 1]. Candidates are the logits that are neither NaN nor
  * -inf, ordered by logit / T from the largest down, equal ones by rising index. Kept are the first top_k (all for

@@ -39,6 +39,7 @@ SOURCES = {
     "wv_gemv_rows.cu": [],
     "wv_decode.cu": [],
     "wv_kv_cache.cu": [],
+    "wv_kv_pages.cu": [],
     "wv_attn_paged.cu": [],
     "wv_attn_chunk.cu": [],
     "wv_sample.cu": [],

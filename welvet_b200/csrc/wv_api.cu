@@ -1027,7 +1027,8 @@ extern "C" int wv_matvec_bias_act(uint64_t key, const float* x, const double* bi
 extern "C" int wv_device_status(void) {
   if (int te = wv_tma_take_error()) { wv_set_error("a bounded device wait ran out (code %d)", te); return WV_ETIMEOUT; }
   if (int pe = wv_paged_take_error()) {
-    wv_set_error("paged call: %s", pe == 1 ? "a q_start or kv_len is outside its bounds" : "a page number is outside the pool");
+    wv_set_error("paged call: %s", pe == 1 ? "a q_start, kv_len or length is outside its bounds" : pe == 2 ? "a page number is outside the pool"
+                                   : pe == 3 ? "a sequence's number is out of range, or a sequence is used twice or is not empty" : "a page was given back more often than it was held");
     return WV_ESHAPE;
   }
   return WV_OK;

@@ -395,13 +395,10 @@ int wv_api_bind_device();
 int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* dq, int ldq, float* dout, int ldo, int heads, float scale,
                          int window, cudaStream_t st);
 
-static bool kv_shape_ok(int bits, int page_size, int head_dim) {
-  return (bits == 16 || bits == 8 || bits == 4) && page_size >= 16 && page_size % 16 == 0 && page_size <= 65536 && head_dim >= 16 && head_dim % 16 == 0 && head_dim <= 256;
-}
 extern "C" int wv_kv_block_bytes(int bits, int page_size, int head_dim, uint64_t* bytes) {
   if (!bytes) { wv_set_error("wv_kv_block_bytes: null pointer"); return WV_EARG; }
   if (bits != 16 && bits != 8 && bits != 4) { wv_set_error("wv_kv_block_bytes: %d bits (16, 8 or 4)", bits); return WV_EFORMAT; }
-  if (!kv_shape_ok(bits, page_size, head_dim)) { wv_set_error("wv_kv_block_bytes: page_size %d, head_dim %d (multiples of 16, head_dim at most 256)", page_size, head_dim); return WV_ESHAPE; }
+  if (!wv_kv_shape_ok(bits, page_size, head_dim)) { wv_set_error("wv_kv_block_bytes: page_size %d, head_dim %d (multiples of 16, head_dim at most 256)", page_size, head_dim); return WV_ESHAPE; }
   WvKvPages p = {nullptr, bits, 1, page_size, 1, head_dim};
   *bytes = (uint64_t)wv_kv_geom(p).block;
   return WV_OK;
@@ -411,7 +408,7 @@ extern "C" int wv_kv_block_bytes(int bits, int page_size, int head_dim, uint64_t
 static int kv_check(const char* who, const WvKvPages* kv, const WvKvBatch* b) {
   if (!kv || !b || !kv->pool || !b->q_start || !b->kv_len || !b->pages) { wv_set_error("%s: null pointer", who); return WV_EARG; }
   if (kv->bits != 16 && kv->bits != 8 && kv->bits != 4) { wv_set_error("%s: %d bits (16, 8 or 4)", who, kv->bits); return WV_EFORMAT; }
-  if (!kv_shape_ok(kv->bits, kv->page_size, kv->head_dim) || kv->num_pages < 1 || kv->num_kv_heads < 1) {
+  if (!wv_kv_shape_ok(kv->bits, kv->page_size, kv->head_dim) || kv->num_pages < 1 || kv->num_kv_heads < 1) {
     wv_set_error("%s: %d pages of %d, %d kv heads of %d (page_size and head_dim are multiples of 16, head_dim at most 256)", who, kv->num_pages, kv->page_size,
                  kv->num_kv_heads, kv->head_dim);
     return WV_ESHAPE;

@@ -27,9 +27,15 @@ __host__ __device__ inline WvKvGeom wv_kv_geom(const WvKvPages& p) {
   return g;
 }
 
+inline bool wv_kv_shape_ok(int bits, int page_size, int head_dim) {
+  return (bits == 16 || bits == 8 || bits == 4) && page_size >= 16 && page_size % 16 == 0 && page_size <= 65536 && head_dim >= 16 && head_dim % 16 == 0 && head_dim <= 256;
+}
+
 // Codes in the sticky status word of paged calls.
 #define WV_PAGED_LENGTH 1        // q_start or kv_len outside its bounds
 #define WV_PAGED_PAGE 2          // a page number outside the pool
+#define WV_PAGED_SEQ 3           // a table's call: a sequence's number, or a sequence used twice or not empty
+#define WV_PAGED_REFS 4          // a table's call: a page given back more often than it was held
 __device__ __forceinline__ void wv_paged_report(int* err, int code) { if (err) atomicCAS_system(err, 0, code); }
 
 // A sequence of the batch, cut to the call's bounds: rows q0 .. q1 - 1 of q, the first of them at position p0; kv tokens in the cache.

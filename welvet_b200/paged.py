@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 
-from ._lib import WvKvBatch, WvKvPages, check, lib
+from ._lib import WvKvBatch, WvKvPages, WvKvTable, check, lib
 
 
 def KVBlockBytes(bits: int, page_size: int, head_dim: int) -> int:
@@ -44,6 +44,43 @@ def AttnPagedCUDA(pages: WvKvPages, batch: WvKvBatch, dq: int, dout: int, num_he
                   ldo: int = 0, stream: int = 0) -> None:
     """Causal attention of the new tokens over their sequence's cache, optionally the last `window` positions of it (wv_attn_paged_dev)."""
     check(lib().wv_attn_paged_dev(C.byref(pages), C.byref(batch), dq, ldq, dout, ldo, num_heads, scale, window, stream))
+
+
+def KVTable(refs: int, pages: int, kv_len: int, num_pages: int, page_size: int, num_seqs: int, table_stride: int) -> WvKvTable:
+    """The page tables of a cache on the device (WvKvTable): int32 refs[num_pages], pages[num_seqs, table_stride] and kv_len[num_seqs], zeroed for
+    an empty cache. pages and kv_len are the ones that a Batch names; all blocks of a stack share one table."""
+    return WvKvTable(refs, pages, kv_len, num_pages, page_size, num_seqs, table_stride)
+
+
+def KVBlocks(pools):
+    """The caches of all blocks that use a table, as KVExtendCUDA, KVCompactCUDA and KVCopyCUDA take them: a list of KVPages."""
+    return (WvKvPages * len(pools))(*pools)
+
+
+def KVForkCUDA(table: WvKvTable, dsrc: int, ddst: int, n: int, dkeep: int = 0, stream: int = 0) -> None:
+    """The empty sequences ddst[:n] become the first dkeep (0: all) tokens of the sequences dsrc[:n], in the same pages (wv_kv_fork_dev)."""
+    check(lib().wv_kv_fork_dev(C.byref(table), dsrc, ddst, dkeep or None, n, stream))
+
+
+def KVExtendCUDA(table: WvKvTable, dadd: int, dgranted: int = 0, pools=None, stream: int = 0) -> None:
+    """Room for dadd[s] more tokens of every sequence, counted in kv_len; shared last pages are copied in all `pools` (KVBlocks). dgranted[s]: 1, or 0
+    for a sequence that was refused (wv_kv_extend_dev)."""
+    check(lib().wv_kv_extend_dev(C.byref(table), dadd, dgranted or None, pools, len(pools) if pools is not None else 0, stream))
+
+
+def KVTrimCUDA(table: WvKvTable, n: int, dkeep: int = 0, dseqs: int = 0, stream: int = 0) -> None:
+    """The sequences dseqs[:n] (0: the first n) are cut to dkeep[:n] tokens (0: freed) and their pages behind them given back (wv_kv_trim_dev)."""
+    check(lib().wv_kv_trim_dev(C.byref(table), dseqs or None, dkeep or None, n, stream))
+
+
+def KVCompactCUDA(table: WvKvTable, pools, dlive: int, stream: int = 0) -> None:
+    """The pages in use move to the front of the pools (KVBlocks, or None); their number goes to dlive (wv_kv_compact_dev)."""
+    check(lib().wv_kv_compact_dev(C.byref(table), pools, len(pools) if pools is not None else 0, dlive, stream))
+
+
+def KVCopyCUDA(pools, dsrc: int, ddst: int, n: int, stream: int = 0) -> None:
+    """Pages dsrc[:n] of all `pools` (KVBlocks) copied to pages ddst[:n] (wv_kv_copy_dev)."""
+    check(lib().wv_kv_copy_dev(pools, len(pools), dsrc, ddst, n, stream))
 
 
 class PagedBlockDecoder:
