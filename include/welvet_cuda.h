@@ -209,6 +209,21 @@ int wv_kv_read_dev(const WvKvPages* kv, const WvKvBatch* batch, float* dk, int l
 int wv_attn_paged_dev(const WvKvPages* kv, const WvKvBatch* batch, const float* dq, int ldq, float* dout, int ldo, int num_heads,
                       float scale, int window, void* stream);
 
+/* wv_attn_paged_dev (without a window) for sequences that share a long prefix, such as forks of one: the keys of the first tokens of a group of
+ * sequences are read and multiplied once, for all rows of the group. Group g is the sequences start[g] .. start[g + 1] - 1 (start[num_groups + 1]
+ * rising, on the device; sequences before start[0] and behind the last are on their own), whose tables name the same pages for their first
+ * shared[g] tokens. Only whole pages count, and only as far as every new token of the group sees them: whatever the lengths are, the
+ * result is that of wv_attn_paged_dev, to its accuracy. max_shared bounds shared[]; a start or shared[g] outside its bounds is cut and reported as a batch's lengths
+ * are (the rows of its sequences are then undefined, as they are where the tables differ). max_shared and max_kv - max_shared plan the call's splits. Scratch as
+ * wv_attn_paged_dev; with num_groups or max_shared 0, or more rows than it holds two results for, the call is that one. */
+typedef struct WvKvGroups {
+  const int* start;
+  const int* shared;
+  int num_groups, max_shared;
+} WvKvGroups;
+int wv_attn_shared_dev(const WvKvPages* kv, const WvKvBatch* batch, const WvKvGroups* groups, const float* dq, int ldq, float* dout, int ldo, int num_heads,
+                       float scale, void* stream);
+
 /* Page tables on the device. refs[num_pages] counts for every page the places of the tables that hold it (0: the page is free),
  * pages[num_seqs][table_stride] and kv_len[num_seqs] are a batch's: sequence s holds pages[s][0 .. ceil(kv_len[s] / page_size) - 1].
  * All-zero refs and kv_len are an empty cache. The calls below change all three and nothing else, but for the copies of pages that

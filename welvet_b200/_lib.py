@@ -24,7 +24,7 @@ SYMBOLS = [
     "wv_attn_decode_dev", "wv_silu_mul_dev", "wv_residual_add_dev",
     "wv_topk_sample_dev", "wv_topk_sample", "wv_decode_row", "wv_decode_row_dev",
     "wv_kv_block_bytes", "wv_kv_write_dev", "wv_kv_read_dev", "wv_attn_paged_dev", "wv_sample_rows_dev",
-    "wv_kv_fork_dev", "wv_kv_extend_dev", "wv_kv_trim_dev", "wv_kv_compact_dev", "wv_kv_copy_dev",
+    "wv_kv_fork_dev", "wv_kv_extend_dev", "wv_kv_trim_dev", "wv_kv_compact_dev", "wv_kv_copy_dev", "wv_attn_shared_dev",
 ]
 
 # Development hooks (csrc/wv_dev_hooks.h): only in a library built with -DWV_DEV_HOOKS (libwelvet_cuda_dev.so),
@@ -55,6 +55,11 @@ class WvKvBatch(C.Structure):
     """WvKvBatch of include/welvet_cuda.h."""
     _fields_ = [("q_start", C.c_void_p), ("kv_len", C.c_void_p), ("pages", C.c_void_p), ("num_seqs", C.c_int), ("table_stride", C.c_int),
                 ("total_q", C.c_int), ("max_q", C.c_int), ("max_kv", C.c_int)]
+
+
+class WvKvGroups(C.Structure):
+    """WvKvGroups of include/welvet_cuda.h."""
+    _fields_ = [("start", C.c_void_p), ("shared", C.c_void_p), ("num_groups", C.c_int), ("max_shared", C.c_int)]
 
 
 class WvKvTable(C.Structure):
@@ -134,6 +139,7 @@ def lib() -> C.CDLL:
         L.wv_kv_write_dev.argtypes = [C.POINTER(WvKvPages), C.POINTER(WvKvBatch), vp, i, vp, i, vp, i, vp, i, i, C.c_double, vp]
         L.wv_kv_read_dev.argtypes = [C.POINTER(WvKvPages), C.POINTER(WvKvBatch), vp, i, vp, i, vp]
         L.wv_attn_paged_dev.argtypes = [C.POINTER(WvKvPages), C.POINTER(WvKvBatch), vp, i, vp, i, i, C.c_float, i, vp]
+        L.wv_attn_shared_dev.argtypes = [C.POINTER(WvKvPages), C.POINTER(WvKvBatch), C.POINTER(WvKvGroups), vp, i, vp, i, i, C.c_float, vp]
         L.wv_kv_fork_dev.argtypes = [C.POINTER(WvKvTable), vp, vp, vp, i, vp]
         L.wv_kv_extend_dev.argtypes = [C.POINTER(WvKvTable), vp, vp, C.POINTER(WvKvPages), i, vp]
         L.wv_kv_trim_dev.argtypes = [C.POINTER(WvKvTable), vp, vp, i, vp]

@@ -48,6 +48,7 @@
 #define PC_PRODUCERS 3              // warps 16 - 18
 #define PC_LIFT 4.f                 // weights carry 2^4 and are at most 2^15 (2^10 over the reference, scales below 2)
 #define PC_SLACK 10.f
+#define PC_JOIN 4.f                 // 2^6 / 2^4: results that are joined with those of few rows carry the same factor
 #define PC_SPIN (1u << 20)          // polls of a wait
 
 int wv_sm_count();
@@ -114,7 +115,7 @@ struct PcMeta {
   unsigned tmem, qmax;
   unsigned char qexp[2 * PC_M], lift[2 * PC_M];      // of a row: exponent field of its largest |q|, and what it is lifted by
   int abort;
-  int seq, tile;
+  int seq, tile, shared, table;
 };
 template <int BITS, int DP> struct PcShape {
   static constexpr int STAGES = BITS == 16 ? 3 : 2, STAGE = DP / 64 * PC_N * 128, QPIECE = DP / 64 * PC_M * 128;
@@ -130,7 +131,8 @@ template <int BITS> __device__ __forceinline__ int pc_dim(int p) {      // the v
   return p;
 }
 
-template <int BITS, int DP>
+// SHARED: a part of wv_attn_shared_dev.
+template <int BITS, int DP, bool SHARED>
 __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_constant__ PaCall c) {
   using S = PcShape<BITS, DP>;
   constexpr int STAGES = S::STAGES, STAGE = S::STAGE, QPIECE = S::QPIECE;
@@ -159,23 +161,53 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
   // ---------------------------------------------------------------- which rows: tiles of 256 of the sequences that have more than rows_most
   const int kvh = blockIdx.x % c.g.kvh, flat = blockIdx.x / c.g.kvh, sp = blockIdx.y;
   if (warp == 0) {
-    int seq, tile;
-    pa_find(c, flat, 256, c.rows_most, blockIdx.x == 0 && sp == 0 ? c.err : nullptr, seq, tile);
-    if (lane == 0) { M.seq = seq; M.tile = tile; M.qmax = 0; M.abort = 0; }
+    int seq, tile, shared = 0, table = 0;
+    int* err = blockIdx.x == 0 && sp == 0 ? c.err : nullptr;
+    if (SHARED && c.part == 1) {
+      pa_find_group(c, flat, 256, err, seq, tile);
+      if (seq >= 0) shared = pa_shared_keys(c, seq, pa_group(c, seq, nullptr), table);
+      if (shared == 0) seq = -1;
+    } else {
+      pa_find(c, flat, 256, c.rows_most, err, seq, tile);
+      table = seq;
+      if (SHARED && seq >= 0) shared = pa_shared_of(c, seq);
+    }
+    if (lane == 0) { M.seq = seq; M.tile = tile; M.qmax = 0; M.abort = 0; if (SHARED) { M.shared = shared; M.table = table; } }
   }
   __syncthreads();
   const int seq = M.seq;
   if (seq < 0) return;
-  const WvSeq sq = wv_seq(c.b, c.g.page, seq, sp == 0 && kvh == 0 ? c.err : nullptr);
+  const int table = SHARED ? M.table : seq;                              // the sequence whose pages are read
+  WvSeq sq;
+  if (SHARED && c.part == 1) {                                           // the rows of a group's sequences, all behind its shared keys
+    const PaGroup g = pa_group(c, seq, nullptr);
+    sq = WvSeq{g.q0, g.q1, M.shared, M.shared};
+  } else {
+    sq = wv_seq(c.b, c.g.page, seq, sp == 0 && kvh == 0 ? c.err : nullptr);
+  }
   const int nrows = (sq.q1 - sq.q0) * c.group, r0 = M.tile * 256, rn = min(256, nrows - r0);
-  int lo, hi;
+  int lo, hi, per = c.per;
   pa_range(sq, r0 / c.group, (r0 + rn - 1) / c.group, c.window, lo, hi);
-  const unsigned first = (unsigned)lo + (unsigned)(sp * c.per);
-  const int k0 = (int)min(first, (unsigned)hi), k1 = min(hi, k0 + c.per);
-  const int hd = c.g.hd, pos0 = sq.p0;
   const size_t rec0 = ((size_t)flat * c.g.kvh + kvh) * 256;               // this block's rows in the split results
+  auto rec = [&](int r) {
+    if (SHARED) return ((size_t)(sq.q0 + (r0 + r) / c.group) * (c.group * c.g.kvh) + kvh * c.group + (r0 + r) % c.group) * c.nslots + c.slot0 + sp;
+    return (rec0 + r) * c.nsplit + sp;
+  };
+  if (SHARED) {
+    if (c.part == 1) {
+      hi = min(hi, M.shared);
+    } else {
+      lo = max(lo, M.shared);
+      if (hi > lo) per = max(per, ((hi - lo + c.nsplit - 1) / c.nsplit + PC_N - 1) & ~(PC_N - 1));      // planned for less where little is shared
+      if (M.shared == 0 && sp == 0)                                      // nobody else writes these rows' results of part 1
+        for (int i = tid; i < rn * c.slot0; i += PC_THREADS) c.ml[rec(i / c.slot0) - c.slot0 + i % c.slot0] = make_float2(-INFINITY, 0.f);
+    }
+  }
+  const unsigned first = (unsigned)lo + (unsigned)sp * (unsigned)per;
+  const int k0 = (int)min(first, (unsigned)hi), k1 = min(hi, k0 + per);
+  const int hd = c.g.hd, pos0 = sq.p0;
   if (k0 >= k1) {
-    if (c.nsplit > 1) { if (tid < rn) c.ml[(rec0 + tid) * c.nsplit + sp] = make_float2(-INFINITY, 0.f); }
+    if (SHARED || c.nsplit > 1) { if (tid < rn) c.ml[rec(tid)] = make_float2(-INFINITY, 0.f); }
     else for (int i = tid; i < rn * hd; i += PC_THREADS) {
       const int r = r0 + i / hd;
       c.out[(size_t)(sq.q0 + r / c.group) * c.ldo + (size_t)(kvh * c.group + r % c.group) * hd + i % hd] = 0.f;
@@ -489,9 +521,10 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
       if (r < rn) {
         float f = 1.f;
         float* dst;
-        if (c.nsplit > 1) {
-          dst = c.acc + ((rec0 + r) * c.nsplit + sp) * hd;
-          if (hf == 0) c.ml[(rec0 + r) * c.nsplit + sp] = make_float2(m, l);
+        if (SHARED || c.nsplit > 1) {
+          dst = c.acc + rec(r) * hd;
+          if (SHARED) f = PC_JOIN;
+          if (hf == 0) c.ml[rec(r)] = make_float2(m, l * f);
         } else {
           dst = c.out + (size_t)(sq.q0 + (r0 + r) / c.group) * c.ldo + (size_t)(kvh * c.group + (r0 + r) % c.group) * hd;
           f = l == 0.f ? 0.f : 1.f / l;
@@ -607,7 +640,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
     auto places = [&](int j) {
       if ((j & 3) == 0) {
         const int key = k0 + j * PC_N + 16 * lane, at = key / page;
-        int id = key < k1 ? c.b.pages[(size_t)seq * c.b.table_stride + at] : 0;
+        int id = key < k1 ? c.b.pages[(size_t)table * c.b.table_stride + at] : 0;
         if (id < 0 || id >= c.g.num_pages) { if (pw == 0) wv_paged_report(c.err, WV_PAGED_PAGE); id = -1; }
         blk = id < 0 || key >= k1 ? -1LL : ((long long)id * c.g.kvh + kvh) * c.g.block;
         slots = key - at * page;
@@ -804,17 +837,17 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const __grid_constant__
     const int r = s_at[1] * 256 + i;
     if (r >= nrows) break;
     const size_t rec = (size_t)blockIdx.x * 256 + i;
-    const float inv = pa_join_weights(c, rec, s_w[warp]);
+    const float inv = pa_join_weights(c, rec, c.nsplit, s_w[warp]);
     __syncwarp();
-    pa_join_sums(c, rec, sq.q0 + r / c.group, kvh * c.group + r % c.group, s_w[warp], inv, lane, 32);
+    pa_join_sums(c, rec, c.nsplit, sq.q0 + r / c.group, kvh * c.group + r % c.group, s_w[warp], inv, lane, 32);
     __syncwarp();
   }
 }
 
-template <int BITS, int DP>
+template <int BITS, int DP, bool SHARED>
 static cudaError_t chunk_go(const PaCall& c, long long flat, cudaStream_t st) {
   constexpr size_t smem = PcShape<BITS, DP>::SMEM;
-  auto kern = attn_chunk_kernel<BITS, DP>;
+  auto kern = attn_chunk_kernel<BITS, DP, SHARED>;
   static unsigned long long attr_mask = 0;
   int dev = 0;
   cudaGetDevice(&dev);
@@ -830,10 +863,18 @@ static cudaError_t chunk_go(const PaCall& c, long long flat, cudaStream_t st) {
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at; cfg.numAttrs = 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kern, c);
-  if (e != cudaSuccess || c.nsplit == 1) return e;
+  if (SHARED || e != cudaSuccess || c.nsplit == 1) return e;
   cfg.gridDim = dim3((unsigned)(flat * c.g.kvh), 16); cfg.blockDim = dim3(256); cfg.dynamicSmemBytes = 0;
   return cudaLaunchKernelEx(&cfg, chunk_join_kernel, c);
 }
+
+template <bool SHARED> static cudaError_t chunk_any(const PaCall& c, int bits, long long flat, cudaStream_t st) {
+  const bool small = c.g.hd <= 64;
+  return bits == 16 ? (small ? chunk_go<16, 64, SHARED>(c, flat, st) : chunk_go<16, 128, SHARED>(c, flat, st))
+       : bits == 8 ? (small ? chunk_go<8, 64, SHARED>(c, flat, st) : chunk_go<8, 128, SHARED>(c, flat, st))
+                   : (small ? chunk_go<4, 64, SHARED>(c, flat, st) : chunk_go<4, 128, SHARED>(c, flat, st));
+}
+cudaError_t wv_launch_chunk_part(const PaCall& c, int bits, long long flat, cudaStream_t st) { return chunk_any<true>(c, bits, flat, st); }
 
 // keys: what a sequence's new tokens see at most; alike: every sequence can have max_q new tokens.
 int wv_launch_attn_chunk(PaCall c, int bits, long long keys, bool alike, cudaStream_t st) {
@@ -859,10 +900,7 @@ int wv_launch_attn_chunk(PaCall c, int bits, long long keys, bool alike, cudaStr
     c.ml = reinterpret_cast<float2*>(lease.p);
     c.acc = lease.p + 2 * n;
   }
-  const bool small = c.g.hd <= 64;
-  const cudaError_t e = bits == 16 ? (small ? chunk_go<16, 64>(c, flat, st) : chunk_go<16, 128>(c, flat, st))
-                      : bits == 8 ? (small ? chunk_go<8, 64>(c, flat, st) : chunk_go<8, 128>(c, flat, st))
-                                  : (small ? chunk_go<4, 64>(c, flat, st) : chunk_go<4, 128>(c, flat, st));
+  const cudaError_t e = chunk_any<false>(c, bits, flat, st);
   if (e != cudaSuccess) { wv_set_error("wv_attn_paged_dev: launch: %s", cudaGetErrorString(cudaGetLastError())); return WV_ECUDA; }
   return WV_OK;
 }

@@ -102,8 +102,8 @@ template <int BITS, int DP> __device__ __forceinline__ int pr_vdim(int t, int n)
   return n * (DP / 8) + t;
 }
 
-// EXACT: head_dim is DP, known at compile time; otherwise it is smaller and what lies beyond it is zero.
-template <int BITS, int DP, bool R16, bool EXACT>
+// EXACT: head_dim is DP, known at compile time; otherwise it is smaller and what lies beyond it is zero. SHARED: a part of wv_attn_shared_dev.
+template <int BITS, int DP, bool R16, bool EXACT, bool SHARED>
 __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) attn_rows_kernel(const __grid_constant__ PaCall c) {
   using S = PrShape<BITS, DP>;
   constexpr int RB = S::RB, KS = DP / 16, NT = DP / 8, NROW = R16 ? 16 : 8, NST = PrFit<BITS, DP, R16>::NST;
@@ -126,30 +126,56 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
 
   const unsigned flat = c.first + blockIdx.x, of_head = flat / (unsigned)c.g.kvh;
   const int kvh = flat - of_head * c.g.kvh, sp = blockIdx.y;
-  int seq, tile;
-  if (DP == 256 && c.tiles == 0) {                                       // see wv_launch_attn_paged
-    __shared__ int s_at[2];
-    if (warp == 0) {
-      pa_find(c, of_head, NROW, 0, flat == 0 && sp == 0 ? c.err : nullptr, seq, tile);
-      if (lane == 0) { s_at[0] = seq; s_at[1] = tile; }
-    }
-    __syncthreads();
-    seq = s_at[0]; tile = s_at[1];
+  int seq, tile, table, shared = 0;                                      // table: the sequence whose pages are read
+  WvSeq sq;
+  if (SHARED && c.part == 1) {                                           // the rows of a group's sequences, all behind its shared keys
+    pa_find_group(c, of_head, NROW, flat == 0 && sp == 0 && warp == 0 ? c.err : nullptr, seq, tile);
     if (seq < 0) return;
+    const PaGroup g = pa_group(c, seq, nullptr);
+    shared = pa_shared_keys(c, seq, g, table);
+    if (shared == 0) return;
+    sq = WvSeq{g.q0, g.q1, shared, shared};
   } else {
-    seq = of_head / c.tiles; tile = of_head - seq * c.tiles;
+    if (DP == 256 && !SHARED && c.tiles == 0) {                          // see wv_launch_attn_paged
+      __shared__ int s_at[2];
+      if (warp == 0) {
+        pa_find(c, of_head, NROW, 0, flat == 0 && sp == 0 ? c.err : nullptr, seq, tile);
+        if (lane == 0) { s_at[0] = seq; s_at[1] = tile; }
+      }
+      __syncthreads();
+      seq = s_at[0]; tile = s_at[1];
+      if (seq < 0) return;
+    } else {
+      seq = of_head / c.tiles; tile = of_head - seq * c.tiles;
+    }
+    sq = wv_seq(c.b, c.g.page, seq, sp == 0 && kvh == 0 && tile == 0 ? c.err : nullptr);
+    table = seq;
   }
-  const WvSeq sq = wv_seq(c.b, c.g.page, seq, sp == 0 && kvh == 0 && tile == 0 ? c.err : nullptr);
   const int nrows = (sq.q1 - sq.q0) * c.group, r0 = tile * NROW;
   if (r0 >= nrows || nrows > c.rows_most) return;
   const int rn = min(NROW, nrows - r0);
-  int lo, hi;
+  if (SHARED && c.part == 2) shared = pa_shared_of(c, seq);
+  int lo, hi, per = c.per;
   pa_range(sq, r0 / c.group, (r0 + rn - 1) / c.group, c.window, lo, hi);
-  const unsigned first = (unsigned)lo + (unsigned)(sp * c.per);
-  const int k0 = (int)min(first, (unsigned)hi), k1 = min(hi, k0 + c.per);      // this block's keys; k0 is a multiple of 16 if there are any
-  auto rec = [&](int r) { return ((size_t)blockIdx.x * c.kept + r) * c.nsplit + sp; };      // a row's split result
+  auto rec = [&](int r) {                                                // a row's split result
+    if (SHARED) return ((size_t)(sq.q0 + (r0 + r) / c.group) * (c.group * c.g.kvh) + kvh * c.group + (r0 + r) % c.group) * c.nslots + c.slot0 + sp;
+    return ((size_t)blockIdx.x * c.kept + r) * c.nsplit + sp;
+  };
+  if (SHARED) {
+    if (c.part == 1) {
+      hi = min(hi, shared);
+    } else {
+      lo = max(lo, shared);
+      // planned for what lies behind the longest prefix; where less is shared the splits are longer
+      if (hi > lo) per = max(per, ((hi - lo + c.nsplit - 1) / c.nsplit + 63) & ~63);
+      if (shared == 0 && sp == 0)                                        // nobody else writes these rows' results of part 1
+        for (int i = tid; i < rn * c.slot0; i += 32 * PR_WARPS) c.ml[rec(i / c.slot0) - c.slot0 + i % c.slot0] = make_float2(-INFINITY, 0.f);
+    }
+  }
+  const unsigned first = (unsigned)lo + (unsigned)sp * (unsigned)per;
+  const int k0 = (int)min(first, (unsigned)hi), k1 = min(hi, k0 + per);        // this block's keys; k0 is a multiple of 16 if there are any
   if (k0 >= k1) {
-    if (c.nsplit > 1) { if (tid < rn) c.ml[rec(tid)] = make_float2(-INFINITY, 0.f); }
+    if (SHARED || c.nsplit > 1) { if (tid < rn) c.ml[rec(tid)] = make_float2(-INFINITY, 0.f); }
     else for (int i = tid; i < rn * hd; i += 32 * PR_WARPS) {            // rows that see nothing
       const int r = i / hd, t = sq.q0 + (r0 + r) / c.group, h = kvh * c.group + (r0 + r) % c.group;
       c.out[(size_t)t * c.ldo + (size_t)h * hd + i % hd] = 0.f;
@@ -179,7 +205,7 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
   auto start = [&](int it) {
     if ((it & 31) == 0) {
       const int key = (g0 + (it + lane) * PR_WARPS) * 16, at = key / c.g.page;
-      int id = it + lane < ng ? c.b.pages[(size_t)seq * c.b.table_stride + at] : 0;
+      int id = it + lane < ng ? c.b.pages[(size_t)table * c.b.table_stride + at] : 0;
       if (id < 0 || id >= c.g.num_pages) { wv_paged_report(c.err, WV_PAGED_PAGE); id = -1; }
       blk = id < 0 ? -1LL : ((long long)id * c.g.kvh + kvh) * c.g.block;
       slots = key - at * c.g.page;
@@ -625,7 +651,7 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
     }
     float* to;
     float scale = 1.f;
-    if (c.nsplit > 1) {
+    if (SHARED || c.nsplit > 1) {
       to = c.acc + rec(r) * hd;
       if (warp == 0 && cl == 0) c.ml[rec(r)] = make_float2(M, L);
     } else {
@@ -671,17 +697,35 @@ __global__ void __launch_bounds__(128) rows_join_kernel(const __grid_constant__ 
   const WvSeq sq = wv_seq(c.b, c.g.page, seq, nullptr);
   const int nrows = (sq.q1 - sq.q0) * c.group;
   if (r >= nrows || nrows > c.rows_most) return;
-  const float inv = pa_join_weights(c, blockIdx.x, pr_w);
+  const float inv = pa_join_weights(c, blockIdx.x, c.nsplit, pr_w);
   __syncthreads();
-  pa_join_sums(c, blockIdx.x, sq.q0 + r / c.group, kvh * c.group + r % c.group, pr_w, inv, threadIdx.x, 128);
+  pa_join_sums(c, blockIdx.x, c.nsplit, sq.q0 + r / c.group, kvh * c.group + r % c.group, pr_w, inv, threadIdx.x, 128);
 }
 
-template <int BITS, int DP, bool R16, bool EXACT>
+// The same for the rows of wv_attn_shared_dev: a block for eight heads of a token, a warp each.
+__global__ void __launch_bounds__(256) shared_join_kernel(const __grid_constant__ PaCall c) {
+  extern __shared__ float pr_w[];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int token = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, head = blockIdx.y * 8 + warp, heads = c.group * c.g.kvh;
+  if (head >= heads) return;
+  const int s = wv_seq_of_row(c.b, token);
+  if (s >= c.b.num_seqs) return;
+  const WvSeq q = wv_seq(c.b, c.g.page, s, nullptr);
+  if (token < q.q0 || token >= q.q1) return;                             // a row that belongs to nobody
+  const size_t rec = (size_t)token * heads + head;
+  float* w = pr_w + warp * c.nslots;
+  const float inv = pa_join_weights(c, rec, c.nslots, w);
+  __syncwarp();
+  pa_join_sums(c, rec, c.nslots, token, head, w, inv, lane, 32);
+}
+
+template <int BITS, int DP, bool R16, bool EXACT, bool SHARED>
 static cudaError_t rows_go(const PaCall& c, int blocks, cudaStream_t st) {
   using S = PrShape<BITS, DP>;
   constexpr size_t sums = (size_t)PR_WARPS * (R16 ? 16 : 8) * DP * 4, ring = (size_t)PR_WARPS * PrFit<BITS, DP, R16>::NST * S::STAGE;
   constexpr size_t smem = sums > ring ? sums : ring;
-  auto kern = attn_rows_kernel<BITS, DP, R16, EXACT>;
+  auto kern = attn_rows_kernel<BITS, DP, R16, EXACT, SHARED>;
   static unsigned long long attr_mask = 0;
   int dev = 0;
   cudaGetDevice(&dev);
@@ -698,13 +742,38 @@ static cudaError_t rows_go(const PaCall& c, int blocks, cudaStream_t st) {
   cfg.attrs = at; cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kern, c);
 }
-template <int BITS, bool R16>
+template <int BITS, bool R16, bool SHARED>
 static cudaError_t rows_pick(const PaCall& c, int blocks, cudaStream_t st) {
-  if (c.g.hd == 64) return rows_go<BITS, 64, R16, true>(c, blocks, st);
-  if (c.g.hd == 128) return rows_go<BITS, 128, R16, true>(c, blocks, st);
-  if (c.g.hd < 64) return rows_go<BITS, 64, R16, false>(c, blocks, st);
-  if (c.g.hd < 128) return rows_go<BITS, 128, R16, false>(c, blocks, st);
-  return rows_go<BITS, 256, R16, false>(c, blocks, st);
+  if (c.g.hd == 64) return rows_go<BITS, 64, R16, true, SHARED>(c, blocks, st);
+  if (c.g.hd == 128) return rows_go<BITS, 128, R16, true, SHARED>(c, blocks, st);
+  if (c.g.hd < 64) return rows_go<BITS, 64, R16, false, SHARED>(c, blocks, st);
+  if (c.g.hd < 128) return rows_go<BITS, 128, R16, false, SHARED>(c, blocks, st);
+  return rows_go<BITS, 256, R16, false, SHARED>(c, blocks, st);
+}
+template <bool SHARED> static cudaError_t rows_any(const PaCall& c, int bits, bool r16, int blocks, cudaStream_t st) {
+  return bits == 16 ? (r16 ? rows_pick<16, true, SHARED>(c, blocks, st) : rows_pick<16, false, SHARED>(c, blocks, st))
+       : bits == 8 ? (r16 ? rows_pick<8, true, SHARED>(c, blocks, st) : rows_pick<8, false, SHARED>(c, blocks, st))
+                   : (r16 ? rows_pick<4, true, SHARED>(c, blocks, st) : rows_pick<4, false, SHARED>(c, blocks, st));
+}
+
+// Splits of the keys: the number that fills 1, 2, .. 8 waves of the blocks that run at once and costs least, a wave being worth a
+// warp's groups of 16 keys and some six more of start and end (2049 positions and eight blocks: 33 splits of 64; 131000: 55).
+// The tensor core cuts instead of rounding as it adds, so the error grows with the products that a warp adds to its sums one
+// after the other (two a group with 16 rows): 12 rows over 12000 keys in one chain of 376 were off by 6.7e-6, in chains of 40 by
+// 7e-7; 131000 keys in chains of 38 by 9e-7. So no more than 40, at 2 us of 26 for the drafted tokens and 4 of 126 for the batch above.
+static long long rows_per_split(long long keys, long long blocks, const WvKvGeom& g, int bits, bool r16) {
+  const long long slots = (long long)wv_sm_count() * pr_blocks(bits, g.hd <= 64 ? 64 : g.hd <= 128 ? 128 : 256, r16);
+  const long long longest = 64 * (r16 ? PR_CHAIN / 2 : PR_CHAIN);
+  long long per = 64, cost = -1;
+  for (long long w = 1; w <= 8; w++) {
+    long long n = w * slots / blocks;
+    if (n < 1) { if (w < 8) continue; n = 1; }
+    long long p = std::min(((keys + n - 1) / n + 63) & ~63LL, longest);
+    if (p < 64) p = 64;
+    const long long m = keys > p ? (keys + p - 1) / p : 1, k = (blocks * m + slots - 1) / slots * (p / 64 + 6);
+    if (cost < 0 || k < cost) { cost = k; per = p; }
+  }
+  return per;
 }
 
 int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* dq, int ldq, float* dout, int ldo, int heads, float scale,
@@ -729,7 +798,6 @@ int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* d
   if ((long long)b.total_q * heads > INT_MAX) { wv_set_error("wv_attn_paged_dev: %d rows of %d heads are too many", b.total_q, heads); return WV_ESHAPE; }
   // what a sequence's new tokens can see together
   const long long keys = window > 0 && (long long)window + b.max_q + 16 < b.max_kv ? (long long)window + b.max_q + 16 : b.max_kv;
-  const int sms = wv_sm_count();
   if (rows) {
     const long long top = chunk ? c.rows_most : most;
     const bool r16 = top > 8;
@@ -741,22 +809,7 @@ int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* d
     const bool look = c.g.hd > 128 && full_tiles <= rows_tiles / 4;
     const long long blocks = (look ? full_tiles : rows_tiles) * c.g.kvh;
     if (blocks * nrow > INT_MAX) { wv_set_error("wv_attn_paged_dev: %d sequences are too many", b.num_seqs); return WV_ESHAPE; }
-    // Splits of the keys: the number that fills 1, 2, .. 8 waves of the blocks that run at once and costs least, a wave being worth a
-    // warp's groups of 16 keys and some six more of start and end (2049 positions and eight blocks: 33 splits of 64; 131000: 55).
-    const long long slots = (long long)sms * pr_blocks(kv.bits, c.g.hd <= 64 ? 64 : c.g.hd <= 128 ? 128 : 256, r16);
-    // The tensor core cuts instead of rounding as it adds, so the error grows with the products that a warp adds to its sums one
-    // after the other (two a group with 16 rows): 12 rows over 12000 keys in one chain of 376 were off by 6.7e-6, in chains of 40 by
-    // 7e-7; 131000 keys in chains of 38 by 9e-7. So no more than 40, at 2 us of 26 for the drafted tokens and 4 of 126 for the batch above.
-    const long long longest = 64 * (r16 ? PR_CHAIN / 2 : PR_CHAIN);
-    long long per = 64, cost = -1;
-    for (long long w = 1; w <= 8; w++) {
-      long long n = w * slots / blocks;
-      if (n < 1) { if (w < 8) continue; n = 1; }
-      long long p = std::min(((keys + n - 1) / n + 63) & ~63LL, longest);
-      if (p < 64) p = 64;
-      const long long m = keys > p ? (keys + p - 1) / p : 1, k = (blocks * m + slots - 1) / slots * (p / 64 + 6);
-      if (cost < 0 || k < cost) { cost = k; per = p; }
-    }
+    long long per = rows_per_split(keys, blocks, c.g, kv.bits, r16);
     if (per < keys / 8192) per = (keys / 8192 + 63) & ~63LL;
     const long long ns = keys > per ? (keys + per - 1) / per : 1;
     PaCall r = c;
@@ -777,9 +830,7 @@ int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* d
     for (long long at0 = 0; at0 < blocks && e == cudaSuccess; at0 += part) {
       const int now = (int)std::min(part, blocks - at0);
       r.first = (unsigned)at0;
-      e = kv.bits == 16 ? (r16 ? rows_pick<16, true>(r, now, st) : rows_pick<16, false>(r, now, st))
-        : kv.bits == 8 ? (r16 ? rows_pick<8, true>(r, now, st) : rows_pick<8, false>(r, now, st))
-                       : (r16 ? rows_pick<4, true>(r, now, st) : rows_pick<4, false>(r, now, st));
+      e = rows_any<false>(r, kv.bits, r16, now, st);
       if (e != cudaSuccess || ns == 1) continue;
       cudaLaunchConfig_t cfg = {};
       cudaLaunchAttribute at[1];
@@ -792,4 +843,93 @@ int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* d
     if (e != cudaSuccess) { wv_set_error("wv_attn_paged_dev: launch: %s", cudaGetErrorString(cudaGetLastError())); return WV_ECUDA; }
   }
   return chunk ? wv_launch_attn_chunk(c, kv.bits, keys, alike, st) : WV_OK;
+}
+
+// The shared keys of every group for all rows of its sequences (part 1), every sequence's own keys (part 2), and the two joined. Part 1
+// runs on tcgen05 where a group has more than 32 rows of a kv head on average, part 2 where a sequence can have; otherwise 8 or 16 rows a pass.
+int wv_launch_attn_shared(const WvKvPages& kv, const WvKvBatch& b, const WvKvGroups& share, const float* dq, int ldq, float* dout, int ldo, int heads, float scale,
+                          cudaStream_t st) {
+  PaCall c = {};
+  c.g = wv_kv_geom(kv);
+  c.b = b;
+  c.share = share;
+  c.q = dq; c.ldq = ldq; c.out = dout; c.ldo = ldo;
+  c.group = heads / c.g.kvh;
+  c.scale = scale * 1.4426950408889634f;
+  c.one = 0x3c003c00u;
+  c.err = wv_paged_err_ptr();
+  c.rows_most = INT_MAX;
+  if (c.share.max_shared > b.max_kv) c.share.max_shared = b.max_kv;
+  const long long rows = (long long)b.total_q * heads, each = ((long long)b.total_q + share.num_groups - 1) / std::max(share.num_groups, 1);      // tokens of a group
+  const long long front = (long long)c.share.max_shared / c.g.page * c.g.page;
+  // two results a row at least
+  const long long most_slots = std::min(PA_SCRATCH / std::max(rows * (c.g.hd + 2) * 4, 1LL), 1024LL);
+  if (share.num_groups == 0 || front == 0 || most_slots < 2)            // nothing is shared, or there are so many rows that it gains nothing
+    return wv_launch_attn_paged(kv, b, dq, ldq, dout, ldo, heads, scale, 0, st);
+  if (rows > INT_MAX || (long long)b.num_seqs * ((long long)b.max_q * c.group / 8 + 1) * c.g.kvh > INT_MAX) {
+    wv_set_error("wv_attn_shared_dev: %d rows of %d heads, %d sequences of %d tokens are too many", b.total_q, heads, b.num_seqs, b.max_q); return WV_ESHAPE;
+  }
+  struct Part { bool chunk, r16; long long grid, per, n; } part[2];
+  for (int i = 0; i < 2; i++) {
+    Part& p = part[i];
+    const long long top = i ? (long long)b.max_q * c.group : each * c.group;      // rows of a kv head: of a sequence at most, of a group on average
+    const long long keys = i ? std::max((long long)b.max_kv - front, 1LL) : front;
+    p.chunk = c.g.hd <= 128 && top > 32;
+    p.r16 = top > 8;
+    const int size = p.chunk ? 256 : p.r16 ? 16 : 8;
+    const long long upto = (long long)b.total_q * c.group / size + (i ? b.num_seqs : share.num_groups), sure = (top + size - 1) / size;
+    const long long likely = i && p.chunk ? std::min(b.num_seqs * sure, upto) : (i ? b.num_seqs : share.num_groups) * sure;
+    p.grid = i ? likely : upto;
+    if (p.chunk) {
+      const long long tiles = (keys + 127) / 128, sms = wv_sm_count(), blocks = likely * c.g.kvh;
+      long long best = 1, cost = -1;
+      for (long long n = 1; n <= 64 && n <= tiles; n++) {
+        const long long t = (tiles + n - 1) / n, w = (blocks * n + sms - 1) / sms * (t + 4);
+        if (cost < 0 || w < cost) { cost = w; best = n; }
+      }
+      p.per = (tiles + best - 1) / best * 128;
+    } else {
+      p.per = rows_per_split(keys, likely * c.g.kvh, c.g, kv.bits, p.r16);
+    }
+    p.n = (keys + p.per - 1) / p.per;
+  }
+  if (part[0].n + part[1].n > most_slots) {                              // fewer and longer splits
+    for (int i = 1; i >= 0; i--) {
+      const long long n = std::min(part[i].n, i ? std::max(most_slots / 2, 1LL) : most_slots - part[1].n), keys = i ? std::max((long long)b.max_kv - front, 1LL) : front;
+      part[i].per = ((keys + n - 1) / n + 127) & ~127LL;
+      part[i].n = (keys + part[i].per - 1) / part[i].per;
+    }
+  }
+  c.nslots = (int)(part[0].n + part[1].n);
+  WvLease lease;
+  const size_t n = (size_t)rows * c.nslots, sums = (2 * n + 3) & ~(size_t)3;
+  if (const int rc = wv_lease(lease, sums + n * c.g.hd, st, "wv_attn_shared_dev: the splits' results")) return rc;
+  c.ml = reinterpret_cast<float2*>(lease.p);
+  c.acc = lease.p + sums;
+  cudaError_t e = cudaSuccess;
+  for (int i = 0; i < 2 && e == cudaSuccess; i++) {
+    PaCall r = c;
+    r.part = i + 1;
+    r.slot0 = i ? (int)part[0].n : 0;
+    r.per = (int)part[i].per; r.nsplit = (int)part[i].n;
+    if (part[i].chunk) {
+      r.rows_most = 0;
+      e = wv_launch_chunk_part(r, kv.bits, part[i].grid, st);
+    } else {
+      const int size = part[i].r16 ? 16 : 8;
+      r.tiles = i ? (unsigned)(((long long)b.max_q * c.group + size - 1) / size) : 1u;
+      e = rows_any<true>(r, kv.bits, part[i].r16, (int)(part[i].grid * c.g.kvh), st);
+    }
+  }
+  if (e == cudaSuccess) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at[1];
+    cfg.gridDim = dim3((unsigned)b.total_q, (unsigned)((heads + 7) / 8)); cfg.blockDim = dim3(256); cfg.dynamicSmemBytes = (size_t)8 * c.nslots * 4; cfg.stream = st;
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at; cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, shared_join_kernel, c);
+  }
+  if (e != cudaSuccess) { wv_set_error("wv_attn_shared_dev: launch: %s", cudaGetErrorString(cudaGetLastError())); return WV_ECUDA; }
+  return WV_OK;
 }

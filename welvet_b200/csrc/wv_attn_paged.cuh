@@ -26,6 +26,10 @@ struct PaCall {
   float2* ml;                      // split results [row][nsplit]: {M, divisor}; {-inf, 0} and no sums for a split without keys
   float* acc;                      // [row][nsplit][head_dim]
   int* err;
+  // wv_attn_shared_dev alone: groups of sequences whose first keys are the same pages. A launch takes those of all groups (part 1) or every
+  // sequence's own behind them (part 2); a row, token * heads + head, has nslots results, the launch's from slot0 on.
+  WvKvGroups share;
+  int part, slot0, nslots;
 };
 
 __device__ __forceinline__ float pa_ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
@@ -97,21 +101,92 @@ __device__ __forceinline__ void pa_find(const PaCall& c, int flat, int size, int
   }
 }
 
+// ------------------------------------------------------------------ shared prefixes
+// The sequences [s0, s1) of group g, cut to the batch, and the rows [q0, q1) of their new tokens.
+struct PaGroup { int s0, s1, q0, q1; };
+__device__ __forceinline__ PaGroup pa_group(const PaCall& c, int g, int* err) {
+  PaGroup r;
+  const int a = c.share.start[g], e = c.share.start[g + 1];
+  r.s0 = min(max(a, 0), c.b.num_seqs);
+  r.s1 = min(max(e, r.s0), c.b.num_seqs);
+  const int q0 = c.b.q_start[r.s0], q1 = c.b.q_start[r.s1], n = c.share.shared[g];
+  r.q0 = min(max(q0, 0), c.b.total_q);
+  r.q1 = min(max(q1, r.q0), c.b.total_q);
+  if (r.s0 != a || r.s1 != e || n < 0 || n > c.share.max_shared) wv_paged_report(err, WV_PAGED_LENGTH);
+  return r;
+}
+// By a whole warp: the keys that the group's rows all see and that lie in whole pages, which is what they share, and the first of its sequences
+// with new tokens, whose row of the table says where they are.
+__device__ __forceinline__ int pa_shared_keys(const PaCall& c, int g, const PaGroup& r, int& table) {
+  const int lane = threadIdx.x & 31;
+  int n = min(max(c.share.shared[g], 0), c.share.max_shared), first = INT_MAX;
+  for (int s0 = r.s0; s0 < r.s1; s0 += 32) {
+    const int s = s0 + lane;
+    if (s < r.s1) {
+      const WvSeq q = wv_seq(c.b, c.g.page, s, nullptr);
+      if (q.q1 > q.q0) { n = min(n, max(q.p0 + 1, 0)); first = min(first, s); }
+    }
+  }
+  n = __reduce_min_sync(0xffffffffu, n);
+  first = __reduce_min_sync(0xffffffffu, first);
+  table = first == INT_MAX ? 0 : first;
+  return first == INT_MAX ? 0 : n / c.g.page * c.g.page;
+}
+// The group that holds sequence seq (-1: none), found by a whole warp.
+__device__ __forceinline__ int pa_group_of(const PaCall& c, int seq) {
+  const int lane = threadIdx.x & 31;
+  for (int g0 = 0; g0 < c.share.num_groups; g0 += 32) {
+    const int g = g0 + lane;
+    const unsigned m = __ballot_sync(0xffffffffu, g < c.share.num_groups && c.share.start[g] <= seq && seq < c.share.start[g + 1]);
+    if (m) return g0 + __ffs(m) - 1;
+  }
+  return -1;
+}
+// What sequence seq shares with its group, by a whole warp.
+__device__ __forceinline__ int pa_shared_of(const PaCall& c, int seq) {
+  const int g = pa_group_of(c, seq);
+  int table;
+  return g < 0 ? 0 : pa_shared_keys(c, g, pa_group(c, g, nullptr), table);
+}
+// The flat-th tile of `size` rows (tokens x group) of the groups: its group (-1: none) and its place in it. As pa_find.
+__device__ __forceinline__ void pa_find_group(const PaCall& c, int flat, int size, int* err, int& group, int& tile) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  group = -1; tile = 0;
+  for (int g0 = 0; g0 < c.share.num_groups && (group < 0 || err); g0 += 32) {
+    int n = 0;
+    if (g0 + lane < c.share.num_groups) {
+      const PaGroup r = pa_group(c, g0 + lane, err);
+      n = (int)(((long long)(r.q1 - r.q0) * c.group + size - 1) / size);
+    }
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += v; }
+    const unsigned hit = __ballot_sync(0xffffffffu, before + upto > flat);
+    if (hit && group < 0) {
+      const int at = __ffs(hit) - 1;
+      group = g0 + at;
+      tile = flat - before - __shfl_sync(0xffffffffu, upto - n, at);
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+}
+
 // A row out of its splits' results, in two steps. By a whole warp (each of a block's may do it): the splits' weights into w[nsplit];
 // returns the divisor's reciprocal. All maxima and divisors are loaded at once: one after the other they were a chain of
 // round trips to L2 (33 splits took 12 us).
-__device__ __forceinline__ float pa_join_weights(const PaCall& c, size_t rec, float* w) {
+__device__ __forceinline__ float pa_join_weights(const PaCall& c, size_t rec, int nsplit, float* w) {
   const int lane = threadIdx.x & 31;
-  const float2* ml = c.ml + rec * c.nsplit;
+  const float2* ml = c.ml + rec * nsplit;
   float M = -INFINITY, L = 0.f;
-  for (int s0 = 0; s0 < c.nsplit; s0 += 128) {
+  for (int s0 = 0; s0 < nsplit; s0 += 128) {
 #pragma unroll
-    for (int u = 0; u < 4; u++) { const int s = s0 + 32 * u + lane; if (s < c.nsplit) M = fmaxf(M, ml[s].x); }
+    for (int u = 0; u < 4; u++) { const int s = s0 + 32 * u + lane; if (s < nsplit) M = fmaxf(M, ml[s].x); }
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
   const float ref = M == -INFINITY ? 0.f : M;
-  for (int s = lane; s < c.nsplit; s += 32) {
+  for (int s = lane; s < nsplit; s += 32) {
     const float2 x = ml[s];
     const float f = x.y == 0.f ? 0.f : x.x == -INFINITY ? 1.f : pa_ex2(x.x - ref);      // -inf with a divisor: NaN, which counts
     if (f != 0.f) L += x.y * f;
@@ -122,20 +197,21 @@ __device__ __forceinline__ float pa_join_weights(const PaCall& c, size_t rec, fl
   return L == 0.f ? 0.f : 1.f / L;
 }
 // Values first, first + step, ... of the row: the sums of the splits with weight, in their order, eight loads at a time.
-__device__ __forceinline__ void pa_join_sums(const PaCall& c, size_t rec, int token, int head, const float* w, float inv, int first, int step) {
-  const float* acc = c.acc + rec * c.nsplit * c.g.hd;
+__device__ __forceinline__ void pa_join_sums(const PaCall& c, size_t rec, int nsplit, int token, int head, const float* w, float inv, int first, int step) {
+  const float* acc = c.acc + rec * nsplit * c.g.hd;
   float* out = c.out + (size_t)token * c.ldo + (size_t)head * c.g.hd;
   for (int d = first; d < c.g.hd; d += step) {
     float a = 0.f;
-    for (int s0 = 0; s0 < c.nsplit; s0 += 8) {
+    for (int s0 = 0; s0 < nsplit; s0 += 8) {
       float v[8];
 #pragma unroll
-      for (int u = 0; u < 8; u++) v[u] = s0 + u < c.nsplit && w[s0 + u] != 0.f ? acc[(size_t)(s0 + u) * c.g.hd + d] : 0.f;
+      for (int u = 0; u < 8; u++) v[u] = s0 + u < nsplit && w[s0 + u] != 0.f ? acc[(size_t)(s0 + u) * c.g.hd + d] : 0.f;
 #pragma unroll
-      for (int u = 0; u < 8; u++) if (s0 + u < c.nsplit) a += v[u] * w[s0 + u];
+      for (int u = 0; u < 8; u++) if (s0 + u < nsplit) a += v[u] * w[s0 + u];
     }
     out[d] = a * inv;
   }
 }
 
 int wv_launch_attn_chunk(PaCall c, int bits, long long keys, bool alike, cudaStream_t st);      // wv_attn_chunk.cu
+cudaError_t wv_launch_chunk_part(const PaCall& c, int bits, long long flat, cudaStream_t st);                                // a part of wv_attn_shared_dev

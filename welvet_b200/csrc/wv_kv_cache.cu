@@ -394,6 +394,8 @@ int wv_launch_kv_read(const WvKvPages& kv, const WvKvBatch& b, float* dk, int ld
 int wv_api_bind_device();
 int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* dq, int ldq, float* dout, int ldo, int heads, float scale,
                          int window, cudaStream_t st);
+int wv_launch_attn_shared(const WvKvPages& kv, const WvKvBatch& b, const WvKvGroups& share, const float* dq, int ldq, float* dout, int ldo, int heads, float scale,
+                          cudaStream_t st);
 
 extern "C" int wv_kv_block_bytes(int bits, int page_size, int head_dim, uint64_t* bytes) {
   if (!bytes) { wv_set_error("wv_kv_block_bytes: null pointer"); return WV_EARG; }
@@ -477,4 +479,25 @@ extern "C" int wv_attn_paged_dev(const WvKvPages* kv, const WvKvBatch* batch, co
   if (none) return WV_OK;
   if (window < 0 || window >= batch->max_kv) window = 0;              // wider than any sequence: none
   return wv_launch_attn_paged(*kv, *batch, dq, ldq, dout, ldo, num_heads, scale, window, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int wv_attn_shared_dev(const WvKvPages* kv, const WvKvBatch* batch, const WvKvGroups* groups, const float* dq, int ldq, float* dout, int ldo,
+                                  int num_heads, float scale, void* stream) {
+  const char* who = "wv_attn_shared_dev";
+  int rc = wv_api_bind_device();
+  if (rc < 0) return rc;
+  if ((rc = kv_check(who, kv, batch)) < 0) return rc;
+  const bool none = rc == 1;
+  if (!groups) { wv_set_error("%s: null pointer", who); return WV_EARG; }
+  if (groups->num_groups < 0 || groups->num_groups > batch->num_seqs || groups->max_shared < 0) {
+    wv_set_error("%s: %d groups of %d sequences, %d tokens shared", who, groups->num_groups, batch->num_seqs, groups->max_shared); return WV_EARG;
+  }
+  if (groups->num_groups > 0 && (!groups->start || !groups->shared)) { wv_set_error("%s: null pointer", who); return WV_EARG; }
+  if (num_heads < 1 || num_heads % kv->num_kv_heads) { wv_set_error("%s: %d heads over %d kv heads", who, num_heads, kv->num_kv_heads); return WV_ESHAPE; }
+  if (!(scale == scale) || scale - scale != 0.f) { wv_set_error("%s: the scale is not finite", who); return WV_EARG; }
+  if (batch->max_kv > 1 << 30) { wv_set_error("%s: max_kv %d (at most 2^30)", who, batch->max_kv); return WV_ESHAPE; }
+  const long long qw = (long long)num_heads * kv->head_dim;
+  if ((rc = kv_rows(who, "q", dq, &ldq, qw)) || (rc = kv_rows(who, "out", dout, &ldo, qw))) return rc;
+  if (none) return WV_OK;
+  return wv_launch_attn_shared(*kv, *batch, *groups, dq, ldq, dout, ldo, num_heads, scale, static_cast<cudaStream_t>(stream));
 }

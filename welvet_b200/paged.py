@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 
-from ._lib import WvKvBatch, WvKvPages, WvKvTable, check, lib
+from ._lib import WvKvBatch, WvKvGroups, WvKvPages, WvKvTable, check, lib
 
 
 def KVBlockBytes(bits: int, page_size: int, head_dim: int) -> int:
@@ -44,6 +44,18 @@ def AttnPagedCUDA(pages: WvKvPages, batch: WvKvBatch, dq: int, dout: int, num_he
                   ldo: int = 0, stream: int = 0) -> None:
     """Causal attention of the new tokens over their sequence's cache, optionally the last `window` positions of it (wv_attn_paged_dev)."""
     check(lib().wv_attn_paged_dev(C.byref(pages), C.byref(batch), dq, ldq, dout, ldo, num_heads, scale, window, stream))
+
+
+def Groups(start: int, shared: int, num_groups: int, max_shared: int) -> WvKvGroups:
+    """Groups of a batch's sequences that share a prefix: device arrays of int32 (start[num_groups + 1] first sequences, shared[num_groups] tokens in the same
+    pages) and the bound of what the second holds."""
+    return WvKvGroups(start, shared, num_groups, max_shared)
+
+
+def AttnSharedCUDA(pages: WvKvPages, batch: WvKvBatch, groups: WvKvGroups, dq: int, dout: int, num_heads: int, scale: float, ldq: int = 0, ldo: int = 0,
+                   stream: int = 0) -> None:
+    """AttnPagedCUDA without a window, the keys that a group's sequences share read once for all of them (wv_attn_shared_dev)."""
+    check(lib().wv_attn_shared_dev(C.byref(pages), C.byref(batch), C.byref(groups), dq, ldq, dout, ldo, num_heads, scale, stream))
 
 
 def KVTable(refs: int, pages: int, kv_len: int, num_pages: int, page_size: int, num_seqs: int, table_stride: int) -> WvKvTable:
