@@ -258,6 +258,31 @@ int wv_kv_trim_dev(const WvKvTable* table, const int* d_seqs, const int* d_keep,
 int wv_kv_compact_dev(const WvKvTable* table, const WvKvPages* pools, int num_pools, int* d_live, void* stream);
 int wv_kv_copy_dev(const WvKvPages* pools, int num_pools, const int* d_src, const int* d_dst, int n, void* stream);
 
+/* Low-rank adapters of many requests beside a shared projection: y[r] = base[r] + scale[s] B_s (A_s x[r]) with s = slot[r], the adapter of row r.
+ *
+ * WvAdapters are the adapters of one projection: `slots` of them (at most 8192), a[slots][max_rank][in] and b[slots][out][max_rank] of `dtype` (a core.DType value: 1 = f32,
+ * 2 = f16, 3 = bf16), of which the first rank[s] ranks count (rank NULL: max_rank; what stands behind them is not used, whatever it is),
+ * scale[s] (NULL: 1). rank and scale are device arrays, so that an adapter can be exchanged between the replays of a graph. max_rank is a multiple of 8 up to
+ * 256, in a multiple of 8; the matrices are 16-byte aligned.
+ *
+ * wv_adapter_plan_dev sorts the rows of a step by adapter (d_slot[rows], -1: none) into a plan of wv_adapter_plan_bytes(), which the caller keeps while
+ * the step's calls use it; it is 16-byte aligned. wv_adapter_apply_dev adds the adapters of up to four projections on the same x (of the same slots, in and dtype): dy[i]
+ * [rows, out_i] = dbase[i] + ..., in place where dbase is NULL or names dy[i]; rows without an adapter are copied. x and the sums are
+ * float32 (products carry 24 bits, but for values of x or A x below 2^-100); a row of x that is not finite gives NaN where it has an adapter, and so does an
+ * adapter's value. A slot or rank out of bounds is taken as none or cut, and a plan of other rows or slots does nothing; wv_device_status()
+ * then reports WV_ESHAPE. Row strides as above (ldb, ldy NULL: rows without a gap); asynchronous on `stream`. */
+typedef struct WvAdapters {
+  const void* a;
+  const void* b;
+  const int* rank;
+  const float* scale;
+  int slots, max_rank, in, out, dtype;
+} WvAdapters;
+int wv_adapter_plan_bytes(int rows, int slots, uint64_t* bytes);
+int wv_adapter_plan_dev(const int* d_slot, int rows, int slots, void* d_plan, void* stream);
+int wv_adapter_apply_dev(const WvAdapters* targets, int n, const void* d_plan, int rows, const float* dx, int ldx, const float* const* dbase, const int* ldb,
+                         float* const* dy, const int* ldy, void* stream);
+
 /* The next token of each of `rows` rows of n logits (row r at d_logits + r * ld, ld 0: n). Parameters are device arrays, one
  * value a row: temperature T, top_k, top_p, min_p and the draw u in [0, 1]. Candidates are the logits that are neither NaN nor
  * -inf, ordered by logit / T from the largest down, equal ones by rising index. Kept are the first top_k (all for

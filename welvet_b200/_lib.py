@@ -25,6 +25,7 @@ SYMBOLS = [
     "wv_topk_sample_dev", "wv_topk_sample", "wv_decode_row", "wv_decode_row_dev",
     "wv_kv_block_bytes", "wv_kv_write_dev", "wv_kv_read_dev", "wv_attn_paged_dev", "wv_sample_rows_dev",
     "wv_kv_fork_dev", "wv_kv_extend_dev", "wv_kv_trim_dev", "wv_kv_compact_dev", "wv_kv_copy_dev", "wv_attn_shared_dev",
+    "wv_adapter_plan_bytes", "wv_adapter_plan_dev", "wv_adapter_apply_dev",
 ]
 
 # Development hooks (csrc/wv_dev_hooks.h): only in a library built with -DWV_DEV_HOOKS (libwelvet_cuda_dev.so),
@@ -66,6 +67,12 @@ class WvKvTable(C.Structure):
     """WvKvTable of include/welvet_cuda.h."""
     _fields_ = [("refs", C.c_void_p), ("pages", C.c_void_p), ("kv_len", C.c_void_p), ("num_pages", C.c_int), ("page_size", C.c_int),
                 ("num_seqs", C.c_int), ("table_stride", C.c_int)]
+
+
+class WvAdapters(C.Structure):
+    """WvAdapters of include/welvet_cuda.h."""
+    _fields_ = [("a", C.c_void_p), ("b", C.c_void_p), ("rank", C.c_void_p), ("scale", C.c_void_p), ("slots", C.c_int), ("max_rank", C.c_int),
+                ("in_", C.c_int), ("out", C.c_int), ("dtype", C.c_int)]
 
 
 class WelvetError(RuntimeError):
@@ -140,6 +147,9 @@ def lib() -> C.CDLL:
         L.wv_kv_read_dev.argtypes = [C.POINTER(WvKvPages), C.POINTER(WvKvBatch), vp, i, vp, i, vp]
         L.wv_attn_paged_dev.argtypes = [C.POINTER(WvKvPages), C.POINTER(WvKvBatch), vp, i, vp, i, i, C.c_float, i, vp]
         L.wv_attn_shared_dev.argtypes = [C.POINTER(WvKvPages), C.POINTER(WvKvBatch), C.POINTER(WvKvGroups), vp, i, vp, i, i, C.c_float, vp]
+        L.wv_adapter_plan_bytes.argtypes = [i, i, C.POINTER(u64)]
+        L.wv_adapter_plan_dev.argtypes = [vp, i, i, vp, vp]
+        L.wv_adapter_apply_dev.argtypes = [C.POINTER(WvAdapters), i, vp, i, vp, i, C.POINTER(vp), C.POINTER(i), C.POINTER(vp), C.POINTER(i), vp]
         L.wv_kv_fork_dev.argtypes = [C.POINTER(WvKvTable), vp, vp, vp, i, vp]
         L.wv_kv_extend_dev.argtypes = [C.POINTER(WvKvTable), vp, vp, C.POINTER(WvKvPages), i, vp]
         L.wv_kv_trim_dev.argtypes = [C.POINTER(WvKvTable), vp, vp, i, vp]

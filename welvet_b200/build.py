@@ -43,6 +43,7 @@ SOURCES = {
     "wv_attn_paged.cu": [],
     "wv_attn_chunk.cu": [],
     "wv_sample.cu": [],
+    "wv_adapter.cu": [],
     "wv_gemv_tc.cu": [],
     "wv_gemm_tcgen05.cu": [],
     "wv_api.cu": [],

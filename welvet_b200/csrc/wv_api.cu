@@ -1028,7 +1028,8 @@ extern "C" int wv_device_status(void) {
   if (int te = wv_tma_take_error()) { wv_set_error("a bounded device wait ran out (code %d)", te); return WV_ETIMEOUT; }
   if (int pe = wv_paged_take_error()) {
     wv_set_error("paged call: %s", pe == 1 ? "a q_start, kv_len or length is outside its bounds" : pe == 2 ? "a page number is outside the pool"
-                                   : pe == 3 ? "a sequence's number is out of range, or a sequence is used twice or is not empty" : "a page was given back more often than it was held");
+                                   : pe == 3 ? "a sequence's number is out of range, or a sequence is used twice or is not empty"
+                                   : pe == 4 ? "a page was given back more often than it was held" : "an adapter's number or rank is outside its bounds, or the plan is another call's");
     return WV_ESHAPE;
   }
   return WV_OK;

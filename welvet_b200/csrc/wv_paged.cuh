@@ -36,6 +36,7 @@ inline bool wv_kv_shape_ok(int bits, int page_size, int head_dim) {
 #define WV_PAGED_PAGE 2          // a page number outside the pool
 #define WV_PAGED_SEQ 3           // a table's call: a sequence's number, or a sequence used twice or not empty
 #define WV_PAGED_REFS 4          // a table's call: a page given back more often than it was held
+#define WV_PAGED_ADAPTER 5       // an adapter's number or rank outside its bounds, or a plan of another call
 __device__ __forceinline__ void wv_paged_report(int* err, int code) { if (err) atomicCAS_system(err, 0, code); }
 
 // A sequence of the batch, cut to the call's bounds: rows q0 .. q1 - 1 of q, the first of them at position p0; kv tokens in the cache.
