@@ -39,6 +39,7 @@
 #include "wv_attn_paged.cuh"
 #include "wv_tma_common.cuh"
 #include "wv_lease.h"
+#include <stddef.h>
 #include <type_traits>
 
 #define PC_THREADS 640
@@ -115,7 +116,7 @@ struct PcMeta {
   unsigned tmem, qmax;
   unsigned char qexp[2 * PC_M], lift[2 * PC_M];      // of a row: exponent field of its largest |q|, and what it is lifted by
   int abort;
-  int seq, tile, shared, table;
+  int seq, tile, shared, table, q0, q1;
 };
 template <int BITS, int DP> struct PcShape {
   static constexpr int STAGES = BITS == 16 ? 3 : 2, STAGE = DP / 64 * PC_N * 128, QPIECE = DP / 64 * PC_M * 128;
@@ -161,12 +162,14 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
   // ---------------------------------------------------------------- which rows: tiles of 256 of the sequences that have more than rows_most
   const int kvh = blockIdx.x % c.g.kvh, flat = blockIdx.x / c.g.kvh, sp = blockIdx.y;
   if (warp == 0) {
-    int seq, tile, shared = 0, table = 0;
+    int seq, tile = 0, shared = 0, table = 0;
     int* err = blockIdx.x == 0 && sp == 0 ? c.err : nullptr;
     if (SHARED && c.part == 1) {
-      pa_find_group(c, flat, 256, err, seq, tile);
-      if (seq >= 0) shared = pa_shared_keys(c, seq, pa_group(c, seq, nullptr), table);
-      if (shared == 0) seq = -1;
+      PaGroup g;
+      int q0 = 0, q1 = 0;
+      if (pa_find_group(c, flat, 256, err, g, q0, q1, tile)) shared = pa_shared_keys(c, g, table);
+      seq = shared == 0 ? -1 : 0;
+      if (lane == 0) { M.q0 = q0; M.q1 = q1; }
     } else {
       pa_find(c, flat, 256, c.rows_most, err, seq, tile);
       table = seq;
@@ -180,8 +183,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
   const int table = SHARED ? M.table : seq;                              // the sequence whose pages are read
   WvSeq sq;
   if (SHARED && c.part == 1) {                                           // the rows of a group's sequences, all behind its shared keys
-    const PaGroup g = pa_group(c, seq, nullptr);
-    sq = WvSeq{g.q0, g.q1, M.shared, M.shared};
+    sq = WvSeq{M.q0, M.q1, M.shared, M.shared};
   } else {
     sq = wv_seq(c.b, c.g.page, seq, sp == 0 && kvh == 0 ? c.err : nullptr);
   }
@@ -232,25 +234,123 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&M.tmem)), "n"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  // ---------------------------------------------------------------- K and V tiles: what their warps know of the pages, and the copies
+  const int pw = warp - 16, code = c.g.code, page = c.g.page;
+  // A warp takes the groups pw, pw + 3, .. of a tile's eight groups of 16 rows; a lane's piece (16 bytes of 16-bit rows, else 16 codes) is
+  // number x of rows lr, lr + STEP, ..
+  constexpr int STEP = 32 / S::PIECES, PER = S::PER;
+  const int x = lane % S::PIECES, lr = lane / S::PIECES, n16 = hd / 16;
+  const bool mine = BITS == 16 ? 8 * x < hd : 16 * x < hd;
+  // page numbers of 32 groups of 16 keys (four tiles) at a time, a lane each, as offsets in the pool (-1: not there)
+  long long blk = 0;
+  int slots = 0;
+  auto places = [&](int j) {
+    if ((j & 3) == 0) {
+      const int key = k0 + j * PC_N + 16 * lane, at = key / page;
+      int id = key < k1 ? c.b.pages[(size_t)table * c.b.table_stride + at] : 0;
+      if (id < 0 || id >= c.g.num_pages) { if (pw == 0) wv_paged_report(c.err, WV_PAGED_PAGE); id = -1; }
+      blk = id < 0 || key >= k1 ? -1LL : ((long long)id * c.g.kvh + kvh) * c.g.block;
+      slots = key - at * page;
+    }
+  };
+  float4 ks = make_float4(0.f, 0.f, 0.f, 0.f), vs = ks;                // the first of the warps: four keys a lane of the next tile
+  bool there = true;
+  auto scales = [&](int j) {
+    const int g = 8 * (j & 3) + (lane >> 2);
+    const long long at = __shfl_sync(0xffffffffu, blk, g);
+    const int slot = __shfl_sync(0xffffffffu, slots, g) + 4 * (lane & 3);
+    there = at >= 0 || k0 + j * PC_N + 16 * (lane >> 2) >= k1;         // what lies beyond the keys is not missing
+    ks = vs = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (at >= 0) {
+      ks = *reinterpret_cast<const float4*>(c.g.pool + at + c.g.kscale + 4 * slot);
+      vs = *reinterpret_cast<const float4*>(c.g.pool + at + c.g.vscale + 4 * slot);
+    }
+  };
+  // the copies of element e: into its stage (16 bits), or as they are
+  auto copy = [&](int e) {
+    const int j = e >> 1;
+    const bool is_v = e & 1;
+    const unsigned stage = smem_u32(s_kv) + (e % STAGES) * STAGE, raw = smem_u32(s_raw) + (e & 1) * S::RAW;
+    for (int g = pw; g < 8; g += PC_PRODUCERS) {
+      const long long at = __shfl_sync(0xffffffffu, blk, 8 * (j & 3) + g);
+      const int slot = __shfl_sync(0xffffffffu, slots, 8 * (j & 3) + g) + lr;
+      const int left = at < 0 ? 0 : k1 - (k0 + j * PC_N + 16 * g) - lr;          // the lane's rows 0, STEP, .. below this exist
+      const unsigned char* block = c.g.pool + (at < 0 ? 0 : at);
+      const unsigned char* src = block + (is_v ? page * code : 0) + slot * code + (BITS == 4 ? 8 : 16) * x;
+#pragma unroll
+      for (int i = 0; i < PER; i++) {
+        const bool on = mine && STEP * i < left;
+        const unsigned char* s = on ? src + STEP * i * code : block;
+        if constexpr (BITS == 16) {
+          const int r = 16 * g + lr + STEP * i;
+          const unsigned to = stage + (x >> 3) * PC_N * 128 + r * 128 + (((x & 7) ^ (r & 7)) << 4);
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(s), "r"(on ? 16 : 0) : "memory");
+        } else if constexpr (BITS == 8) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(raw + ((g * PER + i) * 32 + lane) * 16), "l"(s), "r"(on ? 16 : 0) : "memory");
+        } else {
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(raw + ((g * PER + i) * 32 + lane) * 8), "l"(s), "r"(on ? 8 : 0) : "memory");
+        }
+      }
+      // the group's sub-scales, 16 n16 bytes; the warp shares them
+      if (BITS == 4 && lane < n16)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(raw + 8 * PER * 256 + g * 128 + 16 * lane),
+                     "l"(block + (at < 0 ? 0 : (is_v ? c.g.vsub : c.g.ksub) + (slot - lr) * n16 + 16 * lane)), "r"(at < 0 ? 0 : 16) : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  // the tile's page numbers and scales, then its copies, are asked for two elements (one tile) ahead
+  auto ahead = [&](int e) {
+    if (e >= 2 * n) { asm volatile("cp.async.commit_group;" ::: "memory"); return; }
+    if (!(e & 1)) { places(e >> 1); if (pw == 0) scales(e >> 1); }
+    copy(e);
+  };
   // ---------------------------------------------------------------- Q: a power of two, two pieces, the operand's layout
   // The power of two is that of the block's largest row, so that the keys' scales carry it for all rows. A row that lies further below
   // than its pieces reach (by more than 2^15: the second piece then ends above 2^-24 of the row's largest) is lifted by its own, and its
   // sums are put down again, by warps that have such a row. Rows before position 0 see nothing and are zeros, whatever they hold.
-  auto qrow = [&](int r) { return c.q + (size_t)(sq.q0 + (r0 + r) / c.group) * c.ldq + (size_t)(kvh * c.group + (r0 + r) % c.group) * hd; };
-  {
+  // The warps of K and V ask for the first tile meanwhile; the others have eight rows under way at a time (one by one they were a chain of 13
+  // round trips). Where the rows are is worked out once and kept in the room of the keys' scales: what runs once costs what its instructions
+  // take to arrive, and a division for every row of an unrolled loop was 11 us of them.
+  constexpr int QW = PC_THREADS / 32 - PC_PRODUCERS;
+  const bool feeds = warp >= 16 && warp < 16 + PC_PRODUCERS;
+  const int qw = warp < 16 ? warp : 16, qt = 32 * qw + lane;
+  long long* q_at = reinterpret_cast<long long*>(M.kk);                  // of a row, as an offset; inverted if the row stands before position 0
+  static_assert(sizeof(M.kk) + sizeof(M.fv) >= 256 * sizeof(long long) && offsetof(PcMeta, fv) == sizeof(M.kk), "room for the rows' offsets");
+  if (tid < rn) {
+    const int tok = (r0 + tid) / c.group;
+    const long long at = (long long)(sq.q0 + tok) * c.ldq + (long long)(kvh * c.group + (r0 + tid) - tok * c.group) * hd;
+    q_at[tid] = pos0 + tok >= 0 ? at : ~at;
+  }
+  __syncthreads();
+  if (feeds) {
+    ahead(0);
+    ahead(1);
+  } else {
     unsigned top = 0;
-    for (int r = warp; r < rn; r += PC_THREADS / 32) {
-      const float* src = qrow(r);
-      unsigned m = 0;
-      for (int d = 4 * lane; d < hd; d += 128) {
-        const float4 v = *reinterpret_cast<const float4*>(src + d);
-        const float x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll 1
+    for (int r0_ = qw; r0_ < rn; r0_ += 8 * QW) {
+      float4 v[8];
+      unsigned seen = 0;
 #pragma unroll
-        for (int e = 0; e < 4; e++) { const unsigned u = __float_as_uint(x[e]) & 0x7fffffffu; if (u < 0x7f800000u) m = max(m, u); }
+      for (int u = 0; u < 8; u++) {
+        const int r = r0_ + QW * u;
+        v[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (r < rn) {
+          const long long at = q_at[r];
+          seen |= (unsigned)(at >= 0) << u;
+          if (4 * lane < hd) v[u] = *reinterpret_cast<const float4*>(c.q + (at < 0 ? ~at : at) + 4 * lane);
+        }
       }
-      m = __reduce_max_sync(0xffffffffu, m);
-      if (pos0 + (r0 + r) / c.group >= 0) top = max(top, m);
-      if (lane == 0) M.qexp[r] = (unsigned char)(m >> 23);
+#pragma unroll
+      for (int u = 0; u < 8; u++) {
+        const float x[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+        unsigned m = 0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) { const unsigned w = __float_as_uint(x[e]) & 0x7fffffffu; m = max(m, w < 0x7f800000u ? w : 0u); }
+        m = __reduce_max_sync(0xffffffffu, m);
+        if ((seen >> u) & 1u) top = max(top, m);
+        if (lane == 0 && r0_ + QW * u < rn) M.qexp[r0_ + QW * u] = (unsigned char)(m >> 23);
+      }
     }
     if (lane == 0) atomicMax(&M.qmax, top);
   }
@@ -266,12 +366,12 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
     return own && up > 15 ? min(up, 100) : 0;
   };
   if (tid < 2 * PC_M) M.lift[tid] = (unsigned char)(tid < rn ? lift(tid) : 0);
-  for (int i = tid; i < 256 * (DP / 8); i += PC_THREADS) {               // 8 places of a row at a time
+  for (int i = feeds ? 256 * (DP / 8) : qt; i < (two ? 256 : PC_M) * (DP / 8); i += 32 * QW) {      // 8 places of a row at a time
     const int r = i / (DP / 8), j = i % (DP / 8);
-    if (r >= PC_M && !two) break;
     unsigned h[4] = {0u, 0u, 0u, 0u}, l[4] = {0u, 0u, 0u, 0u};
-    if (r < rn && 8 * j < hd && pos0 + (r0 + r) / c.group >= 0) {
-      const float* src = qrow(r) + 8 * j;
+    const long long at = r < rn ? q_at[r] : -1;
+    if (at >= 0 && 8 * j < hd) {
+      const float* src = c.q + at + 8 * j;
       const float f = qinv * __uint_as_float((unsigned)(127 + lift(r)) << 23);
       const float4 a = *reinterpret_cast<const float4*>(src), b = *reinterpret_cast<const float4*>(src + 4);
       float x[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
@@ -628,69 +728,6 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
       }
     } else {
     // ============================================================== K and V tiles
-    const int pw = warp - 16, code = c.g.code, page = c.g.page;
-    // A warp takes the groups pw, pw + 3, .. of a tile's eight groups of 16 rows; a lane's piece (16 bytes of 16-bit rows, else 16 codes) is
-    // number x of rows lr, lr + STEP, ..
-    constexpr int STEP = 32 / S::PIECES, PER = S::PER;
-    const int x = lane % S::PIECES, lr = lane / S::PIECES, n16 = hd / 16;
-    const bool mine = BITS == 16 ? 8 * x < hd : 16 * x < hd;
-    // page numbers of 32 groups of 16 keys (four tiles) at a time, a lane each, as offsets in the pool (-1: not there)
-    long long blk = 0;
-    int slots = 0;
-    auto places = [&](int j) {
-      if ((j & 3) == 0) {
-        const int key = k0 + j * PC_N + 16 * lane, at = key / page;
-        int id = key < k1 ? c.b.pages[(size_t)table * c.b.table_stride + at] : 0;
-        if (id < 0 || id >= c.g.num_pages) { if (pw == 0) wv_paged_report(c.err, WV_PAGED_PAGE); id = -1; }
-        blk = id < 0 || key >= k1 ? -1LL : ((long long)id * c.g.kvh + kvh) * c.g.block;
-        slots = key - at * page;
-      }
-    };
-    float4 ks = make_float4(0.f, 0.f, 0.f, 0.f), vs = ks;                // the first of the warps: four keys a lane of the next tile
-    bool there = true;
-    auto scales = [&](int j) {
-      const int g = 8 * (j & 3) + (lane >> 2);
-      const long long at = __shfl_sync(0xffffffffu, blk, g);
-      const int slot = __shfl_sync(0xffffffffu, slots, g) + 4 * (lane & 3);
-      there = at >= 0 || k0 + j * PC_N + 16 * (lane >> 2) >= k1;         // what lies beyond the keys is not missing
-      ks = vs = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (at >= 0) {
-        ks = *reinterpret_cast<const float4*>(c.g.pool + at + c.g.kscale + 4 * slot);
-        vs = *reinterpret_cast<const float4*>(c.g.pool + at + c.g.vscale + 4 * slot);
-      }
-    };
-    // the copies of element e: into its stage (16 bits), or as they are
-    auto copy = [&](int e) {
-      const int j = e >> 1;
-      const bool is_v = e & 1;
-      const unsigned stage = smem_u32(s_kv) + (e % STAGES) * STAGE, raw = smem_u32(s_raw) + (e & 1) * S::RAW;
-      for (int g = pw; g < 8; g += PC_PRODUCERS) {
-        const long long at = __shfl_sync(0xffffffffu, blk, 8 * (j & 3) + g);
-        const int slot = __shfl_sync(0xffffffffu, slots, 8 * (j & 3) + g) + lr;
-        const int left = at < 0 ? 0 : k1 - (k0 + j * PC_N + 16 * g) - lr;          // the lane's rows 0, STEP, .. below this exist
-        const unsigned char* block = c.g.pool + (at < 0 ? 0 : at);
-        const unsigned char* src = block + (is_v ? page * code : 0) + slot * code + (BITS == 4 ? 8 : 16) * x;
-#pragma unroll
-        for (int i = 0; i < PER; i++) {
-          const bool on = mine && STEP * i < left;
-          const unsigned char* s = on ? src + STEP * i * code : block;
-          if constexpr (BITS == 16) {
-            const int r = 16 * g + lr + STEP * i;
-            const unsigned to = stage + (x >> 3) * PC_N * 128 + r * 128 + (((x & 7) ^ (r & 7)) << 4);
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(s), "r"(on ? 16 : 0) : "memory");
-          } else if constexpr (BITS == 8) {
-            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(raw + ((g * PER + i) * 32 + lane) * 16), "l"(s), "r"(on ? 16 : 0) : "memory");
-          } else {
-            asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(raw + ((g * PER + i) * 32 + lane) * 8), "l"(s), "r"(on ? 8 : 0) : "memory");
-          }
-        }
-        // the group's sub-scales, 16 n16 bytes; the warp shares them
-        if (BITS == 4 && lane < n16)
-          asm volatile("cp.async.ca.shared.global [%0], [%1], 16, %2;" ::"r"(raw + 8 * PER * 256 + g * 128 + 16 * lane),
-                       "l"(block + (at < 0 ? 0 : (is_v ? c.g.vsub : c.g.ksub) + (slot - lr) * n16 + 16 * lane)), "r"(at < 0 ? 0 : 16) : "memory");
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    };
     // Element e out of its copies into its stage. A lane stores two neighbouring 16-byte pieces; those of the upper half of a row start
     // with the second, so that eight lanes reach all banks.
     auto convert = [&](int e) {
@@ -775,16 +812,8 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
       return ok;
     };
     auto room = [&](int e) { return e < STAGES || wait(empty(e % STAGES), e / STAGES - 1, 720); };
-    // the tile's page numbers and scales, then its copies, are asked for two elements (one tile) ahead
-    auto ahead = [&](int e) {
-      if (e >= 2 * n) { asm volatile("cp.async.commit_group;" ::: "memory"); return; }
-      if (!(e & 1)) { places(e >> 1); if (pw == 0) scales(e >> 1); }
-      copy(e);
-    };
     if constexpr (BITS == 16) {
-      ahead(0);
       if (pw == 0) meta(0);
-      ahead(1);
       for (int e = 0; e < 2 * n && ok; e++) {
         asm volatile("cp.async.wait_group 1;" ::: "memory");
         arrive(e);
@@ -793,9 +822,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
         ahead(e + 2);
       }
     } else {
-      ahead(0);
       if (pw == 0) meta(0);
-      ahead(1);
       for (int e = 0; e < 2 * n && ok; e++) {
         asm volatile("cp.async.wait_group 1;" ::: "memory");
         __syncwarp();

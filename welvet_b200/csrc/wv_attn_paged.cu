@@ -124,17 +124,22 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  const unsigned flat = c.first + blockIdx.x, of_head = flat / (unsigned)c.g.kvh;
-  const int kvh = flat - of_head * c.g.kvh, sp = blockIdx.y;
+  // SHARED: blocks in one row, a part's splits one after the other
+  const bool own = SHARED && blockIdx.x >= c.split;
+  const int nsplit = SHARED && own ? c.own_nsplit : c.nsplit, slot0 = SHARED && own ? c.own_slot0 : c.slot0;
+  const unsigned mine = SHARED ? (own ? gridDim.x - c.split : c.split) / (unsigned)nsplit : 0u, at = SHARED ? blockIdx.x - (own ? c.split : 0u) : 0u;
+  const int sp = SHARED ? (int)(at / mine) : blockIdx.y;
+  const unsigned flat = SHARED ? at - sp * mine : c.first + blockIdx.x, of_head = flat / (unsigned)c.g.kvh;
+  const int kvh = flat - of_head * c.g.kvh;
   int seq, tile, table, shared = 0;                                      // table: the sequence whose pages are read
   WvSeq sq;
-  if (SHARED && c.part == 1) {                                           // the rows of a group's sequences, all behind its shared keys
-    pa_find_group(c, of_head, NROW, flat == 0 && sp == 0 && warp == 0 ? c.err : nullptr, seq, tile);
-    if (seq < 0) return;
-    const PaGroup g = pa_group(c, seq, nullptr);
-    shared = pa_shared_keys(c, seq, g, table);
+  if (SHARED && !own) {                                                  // the rows of a group's sequences, all behind its shared keys
+    PaGroup g;
+    int q0, q1;
+    if (!pa_find_group(c, of_head, NROW, flat == 0 && sp == 0 && warp == 0 ? c.err : nullptr, g, q0, q1, tile)) return;
+    shared = pa_shared_keys(c, g, table);
     if (shared == 0) return;
-    sq = WvSeq{g.q0, g.q1, shared, shared};
+    sq = WvSeq{q0, q1, shared, shared};
   } else {
     if (DP == 256 && !SHARED && c.tiles == 0) {                          // see wv_launch_attn_paged
       __shared__ int s_at[2];
@@ -146,7 +151,8 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
       seq = s_at[0]; tile = s_at[1];
       if (seq < 0) return;
     } else {
-      seq = of_head / c.tiles; tile = of_head - seq * c.tiles;
+      const unsigned tiles = SHARED ? c.own_tiles : c.tiles;
+      seq = of_head / tiles; tile = of_head - seq * tiles;
     }
     sq = wv_seq(c.b, c.g.page, seq, sp == 0 && kvh == 0 && tile == 0 ? c.err : nullptr);
     table = seq;
@@ -154,22 +160,22 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
   const int nrows = (sq.q1 - sq.q0) * c.group, r0 = tile * NROW;
   if (r0 >= nrows || nrows > c.rows_most) return;
   const int rn = min(NROW, nrows - r0);
-  if (SHARED && c.part == 2) shared = pa_shared_of(c, seq);
-  int lo, hi, per = c.per;
+  if (SHARED && own) shared = pa_shared_of(c, seq);
+  int lo, hi, per = SHARED && own ? c.own_per : c.per;
   pa_range(sq, r0 / c.group, (r0 + rn - 1) / c.group, c.window, lo, hi);
   auto rec = [&](int r) {                                                // a row's split result
-    if (SHARED) return ((size_t)(sq.q0 + (r0 + r) / c.group) * (c.group * c.g.kvh) + kvh * c.group + (r0 + r) % c.group) * c.nslots + c.slot0 + sp;
+    if (SHARED) return ((size_t)(sq.q0 + (r0 + r) / c.group) * (c.group * c.g.kvh) + kvh * c.group + (r0 + r) % c.group) * c.nslots + slot0 + sp;
     return ((size_t)blockIdx.x * c.kept + r) * c.nsplit + sp;
   };
   if (SHARED) {
-    if (c.part == 1) {
+    if (!own) {
       hi = min(hi, shared);
     } else {
       lo = max(lo, shared);
       // planned for what lies behind the longest prefix; where less is shared the splits are longer
-      if (hi > lo) per = max(per, ((hi - lo + c.nsplit - 1) / c.nsplit + 63) & ~63);
+      if (hi > lo) per = max(per, ((hi - lo + nsplit - 1) / nsplit + 63) & ~63);
       if (shared == 0 && sp == 0)                                        // nobody else writes these rows' results of part 1
-        for (int i = tid; i < rn * c.slot0; i += 32 * PR_WARPS) c.ml[rec(i / c.slot0) - c.slot0 + i % c.slot0] = make_float2(-INFINITY, 0.f);
+        for (int i = tid; i < rn * slot0; i += 32 * PR_WARPS) c.ml[rec(i / slot0) - slot0 + i % slot0] = make_float2(-INFINITY, 0.f);
     }
   }
   const unsigned first = (unsigned)lo + (unsigned)sp * (unsigned)per;
@@ -702,22 +708,34 @@ __global__ void __launch_bounds__(128) rows_join_kernel(const __grid_constant__ 
   pa_join_sums(c, blockIdx.x, c.nsplit, sq.q0 + r / c.group, kvh * c.group + r % c.group, pr_w, inv, threadIdx.x, 128);
 }
 
-// The same for the rows of wv_attn_shared_dev: a block for eight heads of a token, a warp each.
+// The same for the rows of wv_attn_shared_dev: a block for eight heads of a token, a warp each, four values a lane.
 __global__ void __launch_bounds__(256) shared_join_kernel(const __grid_constant__ PaCall c) {
   extern __shared__ float pr_w[];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int token = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, head = blockIdx.y * 8 + warp, heads = c.group * c.g.kvh;
   if (head >= heads) return;
+  const size_t rec = (size_t)token * heads + head;
+  float* w = pr_w + warp * c.nslots;
+  const float inv = pa_join_weights(c, rec, c.nslots, w);                // of a row that belongs to nobody, too: its results are not used
   const int s = wv_seq_of_row(c.b, token);
   if (s >= c.b.num_seqs) return;
   const WvSeq q = wv_seq(c.b, c.g.page, s, nullptr);
-  if (token < q.q0 || token >= q.q1) return;                             // a row that belongs to nobody
-  const size_t rec = (size_t)token * heads + head;
-  float* w = pr_w + warp * c.nslots;
-  const float inv = pa_join_weights(c, rec, c.nslots, w);
+  if (token < q.q0 || token >= q.q1) return;
   __syncwarp();
-  pa_join_sums(c, rec, c.nslots, token, head, w, inv, lane, 32);
+  const float* acc = c.acc + rec * c.nslots * c.g.hd;
+  float* out = c.out + (size_t)token * c.ldo + (size_t)head * c.g.hd;
+  for (int d = 4 * lane; d < c.g.hd; d += 128) {
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s0 = 0; s0 < c.nslots; s0 += 8) {
+      float4 v[8];
+#pragma unroll
+      for (int u = 0; u < 8; u++) v[u] = s0 + u < c.nslots && w[s0 + u] != 0.f ? *reinterpret_cast<const float4*>(acc + (size_t)(s0 + u) * c.g.hd + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int u = 0; u < 8; u++) if (s0 + u < c.nslots) { const float f = w[s0 + u]; a.x += v[u].x * f; a.y += v[u].y * f; a.z += v[u].z * f; a.w += v[u].w * f; }
+    }
+    *reinterpret_cast<float4*>(out + d) = make_float4(a.x * inv, a.y * inv, a.z * inv, a.w * inv);
+  }
 }
 
 template <int BITS, int DP, bool R16, bool EXACT, bool SHARED>
@@ -736,7 +754,7 @@ static cudaError_t rows_go(const PaCall& c, int blocks, cudaStream_t st) {
   }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[1];
-  cfg.gridDim = dim3((unsigned)blocks, (unsigned)c.nsplit); cfg.blockDim = dim3(32 * PR_WARPS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+  cfg.gridDim = SHARED ? dim3((unsigned)blocks) : dim3((unsigned)blocks, (unsigned)c.nsplit); cfg.blockDim = dim3(32 * PR_WARPS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at; cfg.numAttrs = 1;
@@ -869,15 +887,16 @@ int wv_launch_attn_shared(const WvKvPages& kv, const WvKvBatch& b, const WvKvGro
   if (rows > INT_MAX || (long long)b.num_seqs * ((long long)b.max_q * c.group / 8 + 1) * c.g.kvh > INT_MAX) {
     wv_set_error("wv_attn_shared_dev: %d rows of %d heads, %d sequences of %d tokens are too many", b.total_q, heads, b.num_seqs, b.max_q); return WV_ESHAPE;
   }
+  const long long top[2] = {each * c.group, (long long)b.max_q * c.group};                   // rows of a kv head: of a group on average, of a sequence at most
   struct Part { bool chunk, r16; long long grid, per, n; } part[2];
+  for (int i = 0; i < 2; i++) { part[i].chunk = c.g.hd <= 128 && top[i] > 32; part[i].r16 = top[i] > 8; }
+  const bool both = !part[0].chunk && !part[1].chunk;                    // one launch
+  if (both) part[0].r16 = part[1].r16 = part[0].r16 || part[1].r16;
   for (int i = 0; i < 2; i++) {
     Part& p = part[i];
-    const long long top = i ? (long long)b.max_q * c.group : each * c.group;      // rows of a kv head: of a sequence at most, of a group on average
     const long long keys = i ? std::max((long long)b.max_kv - front, 1LL) : front;
-    p.chunk = c.g.hd <= 128 && top > 32;
-    p.r16 = top > 8;
     const int size = p.chunk ? 256 : p.r16 ? 16 : 8;
-    const long long upto = (long long)b.total_q * c.group / size + (i ? b.num_seqs : share.num_groups), sure = (top + size - 1) / size;
+    const long long upto = (long long)b.total_q * c.group / size + (i ? b.num_seqs : share.num_groups), sure = (top[i] + size - 1) / size;
     const long long likely = i && p.chunk ? std::min(b.num_seqs * sure, upto) : (i ? b.num_seqs : share.num_groups) * sure;
     p.grid = i ? likely : upto;
     if (p.chunk) {
@@ -907,18 +926,26 @@ int wv_launch_attn_shared(const WvKvPages& kv, const WvKvBatch& b, const WvKvGro
   c.ml = reinterpret_cast<float2*>(lease.p);
   c.acc = lease.p + sums;
   cudaError_t e = cudaSuccess;
-  for (int i = 0; i < 2 && e == cudaSuccess; i++) {
-    PaCall r = c;
-    r.part = i + 1;
-    r.slot0 = i ? (int)part[0].n : 0;
-    r.per = (int)part[i].per; r.nsplit = (int)part[i].n;
-    if (part[i].chunk) {
-      r.rows_most = 0;
-      e = wv_launch_chunk_part(r, kv.bits, part[i].grid, st);
-    } else {
-      const int size = part[i].r16 ? 16 : 8;
-      r.tiles = i ? (unsigned)(((long long)b.max_q * c.group + size - 1) / size) : 1u;
-      e = rows_any<true>(r, kv.bits, part[i].r16, (int)(part[i].grid * c.g.kvh), st);
+  const long long blocks[2] = {part[0].grid * c.g.kvh * part[0].n, part[1].grid * c.g.kvh * part[1].n};
+  c.slot0 = 0; c.per = (int)part[0].per; c.nsplit = (int)part[0].n;
+  c.own_slot0 = (int)part[0].n; c.own_per = (int)part[1].per; c.own_nsplit = (int)part[1].n;
+  c.own_tiles = (unsigned)(((long long)b.max_q * c.group + (part[1].r16 ? 15 : 7)) / (part[1].r16 ? 16 : 8));
+  if (blocks[0] + blocks[1] > INT_MAX) { wv_set_error("wv_attn_shared_dev: %lld blocks are too many", blocks[0] + blocks[1]); return WV_ESHAPE; }
+  if (both) {
+    c.split = (unsigned)blocks[0];
+    e = rows_any<true>(c, kv.bits, part[0].r16, (int)(blocks[0] + blocks[1]), st);
+  } else {
+    for (int i = 0; i < 2 && e == cudaSuccess; i++) {
+      PaCall r = c;
+      if (part[i].chunk) {
+        r.part = i + 1;
+        r.rows_most = 0;
+        if (i) { r.slot0 = c.own_slot0; r.per = c.own_per; r.nsplit = c.own_nsplit; }
+        e = wv_launch_chunk_part(r, kv.bits, part[i].grid, st);
+      } else {
+        r.split = i ? 0u : (unsigned)blocks[0];
+        e = rows_any<true>(r, kv.bits, part[i].r16, (int)blocks[i], st);
+      }
     }
   }
   if (e == cudaSuccess) {

@@ -27,9 +27,12 @@ struct PaCall {
   float* acc;                      // [row][nsplit][head_dim]
   int* err;
   // wv_attn_shared_dev alone: groups of sequences whose first keys are the same pages. A launch takes those of all groups (part 1) or every
-  // sequence's own behind them (part 2); a row, token * heads + head, has nslots results, the launch's from slot0 on.
+  // sequence's own behind them (part 2); a row, token * heads + head, has nslots results, the launch's from slot0 on. Where the same kernel takes
+  // both they are one launch: its first `split` blocks are part 1, the others part 2 with what own_ says.
   WvKvGroups share;
   int part, slot0, nslots;
+  unsigned split, own_tiles;
+  int own_per, own_nsplit, own_slot0;
 };
 
 __device__ __forceinline__ float pa_ex2(float x) { float y; asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x)); return y; }
@@ -102,74 +105,79 @@ __device__ __forceinline__ void pa_find(const PaCall& c, int flat, int size, int
 }
 
 // ------------------------------------------------------------------ shared prefixes
-// The sequences [s0, s1) of group g, cut to the batch, and the rows [q0, q1) of their new tokens.
-struct PaGroup { int s0, s1, q0, q1; };
+// The sequences [s0, s1) of group g, cut to the batch, and how many tokens they are said to share.
+struct PaGroup { int s0, s1, n; };
 __device__ __forceinline__ PaGroup pa_group(const PaCall& c, int g, int* err) {
   PaGroup r;
-  const int a = c.share.start[g], e = c.share.start[g + 1];
+  const int a = c.share.start[g], e = c.share.start[g + 1], n = c.share.shared[g];
   r.s0 = min(max(a, 0), c.b.num_seqs);
   r.s1 = min(max(e, r.s0), c.b.num_seqs);
-  const int q0 = c.b.q_start[r.s0], q1 = c.b.q_start[r.s1], n = c.share.shared[g];
-  r.q0 = min(max(q0, 0), c.b.total_q);
-  r.q1 = min(max(q1, r.q0), c.b.total_q);
-  if (r.s0 != a || r.s1 != e || n < 0 || n > c.share.max_shared) wv_paged_report(err, WV_PAGED_LENGTH);
+  r.n = min(max(n, 0), c.share.max_shared);
+  if (r.s0 != a || r.s1 != e || r.n != n) wv_paged_report(err, WV_PAGED_LENGTH);
   return r;
 }
 // By a whole warp: the keys that the group's rows all see and that lie in whole pages, which is what they share, and the first of its sequences
-// with new tokens, whose row of the table says where they are.
-__device__ __forceinline__ int pa_shared_keys(const PaCall& c, int g, const PaGroup& r, int& table) {
+// with new tokens, whose row of the table says where they are. 128 sequences are loaded at once.
+__device__ __forceinline__ int pa_shared_keys(const PaCall& c, const PaGroup& r, int& table) {
   const int lane = threadIdx.x & 31;
-  int n = min(max(c.share.shared[g], 0), c.share.max_shared), first = INT_MAX;
-  for (int s0 = r.s0; s0 < r.s1; s0 += 32) {
-    const int s = s0 + lane;
-    if (s < r.s1) {
-      const WvSeq q = wv_seq(c.b, c.g.page, s, nullptr);
-      if (q.q1 > q.q0) { n = min(n, max(q.p0 + 1, 0)); first = min(first, s); }
-    }
+  int n = r.n, first = INT_MAX;
+  for (int s0 = r.s0; s0 < r.s1; s0 += 128) {
+    WvSeq q[4];
+#pragma unroll
+    for (int u = 0; u < 4; u++) q[u] = wv_seq(c.b, c.g.page, min(s0 + 32 * u + lane, r.s1 - 1), nullptr);
+#pragma unroll
+    for (int u = 0; u < 4; u++)
+      if (q[u].q1 > q[u].q0) { n = min(n, max(q[u].p0 + 1, 0)); first = min(first, min(s0 + 32 * u + lane, r.s1 - 1)); }
   }
   n = __reduce_min_sync(0xffffffffu, n);
   first = __reduce_min_sync(0xffffffffu, first);
   table = first == INT_MAX ? 0 : first;
   return first == INT_MAX ? 0 : n / c.g.page * c.g.page;
 }
-// The group that holds sequence seq (-1: none), found by a whole warp.
-__device__ __forceinline__ int pa_group_of(const PaCall& c, int seq) {
+// What sequence seq shares with its group (0: it has none), by a whole warp.
+__device__ __forceinline__ int pa_shared_of(const PaCall& c, int seq) {
   const int lane = threadIdx.x & 31;
   for (int g0 = 0; g0 < c.share.num_groups; g0 += 32) {
-    const int g = g0 + lane;
-    const unsigned m = __ballot_sync(0xffffffffu, g < c.share.num_groups && c.share.start[g] <= seq && seq < c.share.start[g + 1]);
-    if (m) return g0 + __ffs(m) - 1;
+    PaGroup r{0, 0, 0};
+    if (g0 + lane < c.share.num_groups) r = pa_group(c, g0 + lane, nullptr);
+    const unsigned m = __ballot_sync(0xffffffffu, r.s0 <= seq && seq < r.s1);
+    if (!m) continue;
+    const int at = __ffs(m) - 1;
+    r = PaGroup{__shfl_sync(0xffffffffu, r.s0, at), __shfl_sync(0xffffffffu, r.s1, at), __shfl_sync(0xffffffffu, r.n, at)};
+    int table;
+    return pa_shared_keys(c, r, table);
   }
-  return -1;
+  return 0;
 }
-// What sequence seq shares with its group, by a whole warp.
-__device__ __forceinline__ int pa_shared_of(const PaCall& c, int seq) {
-  const int g = pa_group_of(c, seq);
-  int table;
-  return g < 0 ? 0 : pa_shared_keys(c, g, pa_group(c, g, nullptr), table);
-}
-// The flat-th tile of `size` rows (tokens x group) of the groups: its group (-1: none) and its place in it. As pa_find.
-__device__ __forceinline__ void pa_find_group(const PaCall& c, int flat, int size, int* err, int& group, int& tile) {
+// The flat-th tile of `size` rows (tokens x group) of the groups, as pa_find: false if there is none, else its place in its group, the group, the
+// rows [q0, q1) of its sequences' new tokens.
+__device__ __forceinline__ bool pa_find_group(const PaCall& c, int flat, int size, int* err, PaGroup& group, int& q0, int& q1, int& tile) {
   const int lane = threadIdx.x & 31;
   int before = 0;
-  group = -1; tile = 0;
-  for (int g0 = 0; g0 < c.share.num_groups && (group < 0 || err); g0 += 32) {
-    int n = 0;
+  bool found = false;
+  for (int g0 = 0; g0 < c.share.num_groups && (!found || err); g0 += 32) {
+    PaGroup r{0, 0, 0};
+    int a = 0, e = 0;
     if (g0 + lane < c.share.num_groups) {
-      const PaGroup r = pa_group(c, g0 + lane, err);
-      n = (int)(((long long)(r.q1 - r.q0) * c.group + size - 1) / size);
+      r = pa_group(c, g0 + lane, err);
+      a = min(max(c.b.q_start[r.s0], 0), c.b.total_q);
+      e = min(max(c.b.q_start[r.s1], a), c.b.total_q);
     }
+    const int n = (int)(((long long)(e - a) * c.group + size - 1) / size);
     int upto = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) { const int v = __shfl_up_sync(0xffffffffu, upto, o); if (lane >= o) upto += v; }
     const unsigned hit = __ballot_sync(0xffffffffu, before + upto > flat);
-    if (hit && group < 0) {
+    if (hit && !found) {
       const int at = __ffs(hit) - 1;
-      group = g0 + at;
+      found = true;
+      group = PaGroup{__shfl_sync(0xffffffffu, r.s0, at), __shfl_sync(0xffffffffu, r.s1, at), __shfl_sync(0xffffffffu, r.n, at)};
+      q0 = __shfl_sync(0xffffffffu, a, at); q1 = __shfl_sync(0xffffffffu, e, at);
       tile = flat - before - __shfl_sync(0xffffffffu, upto - n, at);
     }
     before += __shfl_sync(0xffffffffu, upto, 31);
   }
+  return found;
 }
 
 // A row out of its splits' results, in two steps. By a whole warp (each of a block's may do it): the splits' weights into w[nsplit];
