@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes as C
 
+from . import adapters as _adapters
 from ._lib import WvKvBatch, WvKvGroups, WvKvPages, WvKvTable, check, lib
 
 
@@ -102,10 +103,12 @@ class PagedBlockDecoder:
     `cfg` is a decode.BlockConfig (MaxSeqLen is not used: the pages bound the lengths), `keys` maps q, k, v, o, gate, up, down to resident
     blob keys, `bufs` maps the working matrices of up to `max_tokens` rows (norm and proj [DModel], q and attn [NumHeads * HeadDim], k and v
     [NumKVHeads * HeadDim], gate and up [IntermediateDim]) and the weights attn_norm / ffn_norm to device pointers. A block has pages of its
-    own; the blocks of a stack share the working matrices and the batch."""
+    own; the blocks of a stack share the working matrices and the batch. `adapters` maps projections (q, k, v, o, gate, up, down, or some of
+    them) to adapters.Adapters of one set of slots and one type."""
 
-    def __init__(self, cfg, keys: dict, bufs: dict, pages: WvKvPages, max_tokens: int, window: int = 0):
+    def __init__(self, cfg, keys: dict, bufs: dict, pages: WvKvPages, max_tokens: int, window: int = 0, adapters: dict | None = None):
         self.cfg, self.keys, self.bufs, self.pages, self.max_tokens, self.window = cfg, keys, bufs, pages, max_tokens, window
+        self.adapters = adapters or {}
         qd, kd = cfg.NumHeads * cfg.HeadDim, cfg.NumKVHeads * cfg.HeadDim
 
         def group(names, outs):
@@ -113,22 +116,41 @@ class PagedBlockDecoder:
             return (C.c_uint64 * n)(*[keys[m] for m in names]), (C.c_void_p * n)(*[bufs[m] for m in names]), (C.c_int * n)(*outs)
         self._qkv, self._gu = group(("q", "k", "v"), (qd, kd, kd)), group(("gate", "up"), (cfg.IntermediateDim,) * 2)
 
-    def step(self, dh: int, batch: WvKvBatch, stream: int = 0) -> None:
-        """The rows of the hidden state [batch.total_q, DModel] at device address dh are updated in place."""
+    def step(self, dh: int, batch: WvKvBatch, stream: int = 0, groups: WvKvGroups | None = None, plan: int = 0) -> None:
+        """The rows of the hidden state [batch.total_q, DModel] at device address dh are updated in place. `groups` says which of the
+        batch's sequences share a prefix: attention reads it once for all of them. `plan` (adapters.PlanCUDA over the batch's rows) adds the
+        block's adapters to its projections."""
         c, b, k, n, L = self.cfg, self.bufs, self.keys, batch.total_q, lib()
         if n > self.max_tokens:
             raise ValueError(f"{n} new tokens, but the working matrices have {self.max_tokens} rows")
+        if groups is not None and self.window:
+            raise ValueError("a window and a shared prefix")
+        if plan and not self.adapters:
+            raise ValueError("a plan of adapters, but the block has none")
         if n == 0:
             return
+
+        def adapt(names, x, outs):
+            # the adapters of projections on the same x, added to their outputs in place
+            have = [m for m in names if m in self.adapters] if plan else []
+            if have:
+                _adapters.ApplyCUDA(_adapters.Group([self.adapters[m] for m in have]), plan, n, x, [outs[m] for m in have], stream=stream)
         qd = c.NumHeads * c.HeadDim
         check(L.wv_rmsnorm_dev(dh, b["attn_norm"], b["norm"], n, c.DModel, c.Eps, stream))
         check(L.wv_matvec_dev_multi(self._qkv[0], 3, b["norm"], self._qkv[1], n, c.DModel, self._qkv[2], stream))
+        adapt(("q", "k", "v"), b["norm"], b)
         KVWriteCUDA(self.pages, batch, b["k"], b["v"], b["q"], b["q"], c.NumHeads, c.RoPETheta, stream=stream)
-        AttnPagedCUDA(self.pages, batch, b["q"], b["attn"], c.NumHeads, 1.0 / (c.HeadDim ** 0.5), window=self.window, stream=stream)
+        if groups is not None:
+            AttnSharedCUDA(self.pages, batch, groups, b["q"], b["attn"], c.NumHeads, 1.0 / (c.HeadDim ** 0.5), stream=stream)
+        else:
+            AttnPagedCUDA(self.pages, batch, b["q"], b["attn"], c.NumHeads, 1.0 / (c.HeadDim ** 0.5), window=self.window, stream=stream)
         check(L.wv_matvec_dev(k["o"], b["attn"], b["proj"], n, qd, c.DModel, stream))
+        adapt(("o",), b["attn"], {"o": b["proj"]})
         check(L.wv_residual_add_dev(dh, b["proj"], n * c.DModel, stream))
         check(L.wv_rmsnorm_dev(dh, b["ffn_norm"], b["norm"], n, c.DModel, c.Eps, stream))
         check(L.wv_matvec_dev_multi(self._gu[0], 2, b["norm"], self._gu[1], n, c.DModel, self._gu[2], stream))
+        adapt(("gate", "up"), b["norm"], b)
         check(L.wv_silu_mul_dev(b["gate"], b["up"], b["gate"], n * c.IntermediateDim, stream))
         check(L.wv_matvec_dev(k["down"], b["gate"], b["proj"], n, c.IntermediateDim, c.DModel, stream))
+        adapt(("down",), b["gate"], {"down": b["proj"]})
         check(L.wv_residual_add_dev(dh, b["proj"], n * c.DModel, stream))
