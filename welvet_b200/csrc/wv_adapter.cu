@@ -222,17 +222,16 @@ template <int DT, int NR, int MR> struct AdShape {
   static __host__ __device__ constexpr int prow(int ranks) { return ((ranks < RP ? ranks : RP) * W::SIZE / 16 | 1) * 16; }
   static __host__ __device__ constexpr int unit(int ranks) { return 16 * Z * prow(ranks) + NR * PB * 4; }
   static __host__ __device__ constexpr int slab(int ranks) { return STEPS * STEP > 2 * unit(ranks) ? STEPS * STEP : 2 * unit(ranks); }
-  // the warps' sums of a pass, a few warps at a time; later t's fragments
+  // the warps' sums of a pass, a few warps at a time
   static constexpr int PP = RP + 4;                                      // floats of a row: rows 2 q of a warp's stores meet no bank twice
   static constexpr int ROUND = NR * RP * 4 * AD_WARPS <= 16384 ? AD_WARPS : 16384 / (NR * RP * 4);
   static constexpr size_t PART = (size_t)ROUND * NR * PP * 4;
   static __host__ __device__ constexpr int row(int ranks) { return (ranks + 15) / 16 * 16 + 4; }      // of t
   static __host__ __device__ constexpr size_t frags(int ranks) { return (size_t)((ranks + 15) / 16) * NB * 3 * 256; }
-  static __host__ __device__ constexpr size_t front(int ranks) {
-    const size_t frag = frags(ranks) + (DT == 2 ? (size_t)NR * row(ranks) * 4 : 0);        // float16: and t whole
-    return PART > frag ? PART : frag;
-  }
-  static __host__ __device__ constexpr size_t smem(int ranks, int slab_) { return (size_t)AD_WARPS * slab_ + front(ranks) + (size_t)NR * row(ranks) * 4; }
+  // [front: the warps' sums, later the whole t][back: this CTA's t, later t's fragments]
+  static __host__ __device__ constexpr size_t front(int ranks) { return PART > (size_t)NR * row(ranks) * 4 ? PART : (size_t)NR * row(ranks) * 4; }
+  static __host__ __device__ constexpr size_t back(int ranks) { return frags(ranks) > (size_t)NR * row(ranks) * 4 ? frags(ranks) : (size_t)NR * row(ranks) * 4; }
+  static __host__ __device__ constexpr size_t smem(int ranks, int slab_) { return (size_t)AD_WARPS * slab_ + front(ranks) + back(ranks); }
 };
 template <int N> __device__ __forceinline__ void ad_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 __device__ __forceinline__ void ad_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -472,10 +471,13 @@ __global__ void __launch_bounds__(AD_THREADS, AdShape<DT, NR, MR>::WIDE ? 1 : 2)
   asm volatile("barrier.cluster.arrive.release;" ::: "memory");
   asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
 
-  // ---------------------------------------------------------------- the CTAs' sums of t, scaled, as fragments [16 ranks][8 rows][piece][lane]
-  uint2* frag = reinterpret_cast<uint2*>(front);
-  float* whole = reinterpret_cast<float*>(front + S::frags(T.max_rank));      // float16: t [NR][tr], whose rows' largest are wanted first
-  for (int e = tid; e < nk * NB * 32; e += AD_THREADS) {
+  // ---------------------------------------------------------------- the CTAs' sums of t, scaled: each CTA adds up its share of it and hands that to all
+  // (with every CTA reading all of the others' sums, distributed shared memory took 3 us with 8 CTAs and 12 with 16). An item is what a lane has of a
+  // fragment: four ranks of a row.
+  float4* whole = reinterpret_cast<float4*>(front);      // [16 ranks][8 rows][lane]
+  uint2* frag = reinterpret_cast<uint2*>(t);             // [16 ranks][8 rows][piece][lane]
+  const int all = nk * NB * 32, share = (all + ctas - 1) / ctas;
+  for (int e = me * share + tid; e < min((me + 1) * share, all); e += AD_THREADS) {
     const int l = e & 31, n = e / 32 % NB, k = e / 32 / NB, at = (8 * n + (l >> 2)) * tr + 16 * k, j = 16 * k + 2 * (l & 3);
     float4 a[8], v = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int r0 = 0; r0 < ctas; r0 += 8) {               // eight under way at once
@@ -485,38 +487,39 @@ __global__ void __launch_bounds__(AD_THREADS, AdShape<DT, NR, MR>::WIDE ? 1 : 2)
       for (int r = 0; r < 8; r++) if (r0 + r < ctas) { v.x += a[r].x; v.y += a[r].y; v.z += a[r].z; v.w += a[r].w; }
     }
     v.x = j < rank ? v.x * scale : 0.f; v.y = j + 1 < rank ? v.y * scale : 0.f; v.z = j + 8 < rank ? v.z * scale : 0.f; v.w = j + 9 < rank ? v.w * scale : 0.f;
-    if constexpr (DT == 2) {
-      float* to = whole + at + 2 * (l & 3);
-      *reinterpret_cast<float2*>(to) = make_float2(v.x, v.y);
-      *reinterpret_cast<float2*>(to + 8) = make_float2(v.z, v.w);
-    } else {
-      unsigned f[3][2];
-      W::values(v, f);
-#pragma unroll
-      for (int s = 0; s < 3; s++) frag[((k * NB + n) * 3 + s) * 32 + l] = make_uint2(f[s][0], f[s][1]);
-    }
+    for (int r = 0; r < ctas; r++) cluster.map_shared_rank(whole, r)[e] = v;
   }
+  asm volatile("barrier.cluster.arrive.release;" ::: "memory");          // from here on nobody touches another CTA's shared memory
+  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
   if constexpr (DT == 2) {
-    __syncthreads();
-    for (int r = warp; r < NR; r += AD_WARPS) {
+    for (int r = warp; r < NR; r += AD_WARPS) {          // a power of two for each row
       unsigned top = 0u;
-      for (int j = lane; j < rank; j += 32) top = max(top, __float_as_uint(whole[r * tr + j]) & 0x7fffffffu);
+      for (int e = lane; e < nk * 4; e += 32) {
+        const float4 v = whole[((e >> 2) * NB + (r >> 3)) * 32 + (r & 7) * 4 + (e & 3)];
+        top = max(top, max(max(__float_as_uint(v.x) & 0x7fffffffu, __float_as_uint(v.y) & 0x7fffffffu), max(__float_as_uint(v.z) & 0x7fffffffu, __float_as_uint(v.w) & 0x7fffffffu)));
+      }
       top = __reduce_max_sync(0xffffffffu, top);
       float down;
       const float up = ad_up(top, down);
       if (lane == 0) s_down[r] = down;
       for (int e = lane; e < nk * 4; e += 32) {          // the row's fragments: eight steps at a time
-        const int k = e >> 2;
-        float4 v = ad_four(whole + r * tr + 16 * k, e & 3);
+        const int at = ((e >> 2) * NB + (r >> 3)) * 32 + (r & 7) * 4 + (e & 3);
+        float4 v = whole[at];
         v.x *= up; v.y *= up; v.z *= up; v.w *= up;
         unsigned f[3][2];
         W::values(v, f);
 #pragma unroll
-        for (int s = 0; s < 3; s++) frag[((k * NB + (r >> 3)) * 3 + s) * 32 + (r & 7) * 4 + (e & 3)] = make_uint2(f[s][0], f[s][1]);
+        for (int s = 0; s < 3; s++) frag[(at / 32 * 3 + s) * 32 + at % 32] = make_uint2(f[s][0], f[s][1]);
       }
     }
+  } else {
+    for (int e = tid; e < all; e += AD_THREADS) {
+      unsigned f[3][2];
+      W::values(whole[e], f);
+#pragma unroll
+      for (int s = 0; s < 3; s++) frag[(e / 32 * 3 + s) * 32 + e % 32] = make_uint2(f[s][0], f[s][1]);
+    }
   }
-  asm volatile("barrier.cluster.arrive.release;" ::: "memory");          // this CTA has read the others' sums
   __syncthreads();
 
   // ---------------------------------------------------------------- y = base + B t
@@ -531,7 +534,7 @@ __global__ void __launch_bounds__(AD_THREADS, AdShape<DT, NR, MR>::WIDE ? 1 : 2)
       to[n][h] = r < 0 ? nullptr : T.y + (size_t)r * T.ldy + 16 * Z * u0 + 2 * Z * g;
       down[n][h] = DT == 2 ? s_down[8 * n + 2 * q + h] : 1.f;
     }
-  const unsigned fr = smem_u32(front) + 8 * lane, wl = sl + W::place(prow);
+  const unsigned fr = smem_u32(frag) + 8 * lane, wl = sl + W::place(prow);
   const float* bl = reinterpret_cast<const float*>(slab + bo) + 2 * q * S::PB + 2 * Z * g;
   // t's fragments of a warp's one block of rows stay in registers where they are one piece
   constexpr int HELD = NB == 1 ? MR : 1;
@@ -615,7 +618,6 @@ __global__ void __launch_bounds__(AD_THREADS, AdShape<DT, NR, MR>::WIDE ? 1 : 2)
     v += last;
   }
   ad_wait<0>();
-  asm volatile("barrier.cluster.wait.acquire;" ::: "memory");            // nobody leaves while another reads its sums
 }
 
 // ------------------------------------------------------------------ host
@@ -730,13 +732,12 @@ extern "C" int wv_adapter_apply_dev(const WvAdapters* targets, int n, const void
   c.err = wv_paged_err_ptr();
   if (c.tiles * AD_CTAS > INT_MAX) { wv_set_error("%s: %d rows are too many", who, rows); return WV_ESHAPE; }
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  // CTAs of a cluster: as many as let the tiles that are expected (half of the adapters' last ones beside the full ones) run at once, two CTAs an SM; 64 rows of 32
-  // adapters beside Q, K and V take 17 us with 4 and 22 with 8, 2048 rows of six 54 and 96. 16 where that leaves the chip empty (a row: 7.7 us, 8.0 with 8). Where
-  // sums are one chain (32 rows, ranks beyond 32), no more than 1792 columns each.
+  // CTAs of a cluster: as many as let the tiles that are expected (half of the adapters' last ones beside the full ones) run at once, two CTAs an SM: a row
+  // beside Q, K and V takes 10.0, 8.0 and 7.5 us with 4, 8 and 16, 64 rows of 32 adapters 17 with 4 and 22 with 8, 2048 rows of six 53 and 69. Where sums are
+  // one chain (32 rows, ranks beyond 32), no more than 1792 columns each.
   const long long likely = n * std::max(1LL, (long long)rows / c.size + (std::min(rows, f.slots) + 1) / 2), room = 2LL * wv_sm_count();
   int ctas = 2;
-  while (ctas < 8 && likely * ctas * 2 <= room) ctas *= 2;
-  if (likely * 32 <= room / 2) ctas = AD_CTAS;
+  while (ctas < AD_CTAS && likely * ctas * 2 <= room) ctas *= 2;
   while (c.size == 32 && ranks > 32 && f.in > 1792 * ctas && ctas < AD_CTAS) ctas *= 2;
   const cudaError_t e = f.dtype == 1 ? ad_any<1>(c, n, ranks, ctas, st) : f.dtype == 2 ? ad_any<2>(c, n, ranks, ctas, st) : ad_any<3>(c, n, ranks, ctas, st);
   if (e != cudaSuccess) { cudaGetLastError(); wv_set_error("%s: launch: %s", who, cudaGetErrorString(e)); return WV_ECUDA; }
