@@ -11,6 +11,14 @@ from test_gpu_paged import Cache, attn64, bound
 pytestmark = pytest.mark.gpu
 
 
+@pytest.fixture(autouse=True)
+def always(hooks):
+    """The tests' sizes are too small for sharing to pay: take the shared keys apart all the same."""
+    hooks.wv_set_attn_sharing(1)
+    yield hooks.wv_set_attn_sharing
+    hooks.wv_set_attn_sharing(0)
+
+
 class Shared(Cache):
     """A cache whose sequences start[g] .. start[g + 1] - 1 name the same pages for their first shared[g] tokens."""
 
@@ -206,6 +214,23 @@ def test_same_as_the_paged_attention_when_rows_are_many(wv):
     wv.paged.AttnPagedCUDA(c.pages, b, q.data_ptr(), ref.data_ptr(), 16, 0.09)
     torch.cuda.synchronize()
     assert torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("seqs,shared,pays", [(2, 512, False), (8, 512, False), (8, 4480, True)])
+def test_shared_where_it_pays(wv, always, seqs, shared, pays):
+    """By itself the call takes the shared keys apart for seven passes saved over 4480 keys of eight heads, and is wv_attn_paged_dev below that."""
+    c = Shared(wv, 8, 64, 8, 128, [(1, shared + 30 + i) for i in range(seqs)], [0, seqs], [shared])
+    q = torch.randn(seqs, 8 * 128, device="cuda")
+    apart = c.attend(q, 8, 0.09)
+    always(0)
+    got, ref = c.attend(q, 8, 0.09), torch.empty_like(q)
+    wv.paged.AttnPagedCUDA(c.pages, c.batch, q.data_ptr(), ref.data_ptr(), 8, 0.09)
+    torch.cuda.synchronize()
+    assert torch.equal(got, apart if pays else ref) and wv._lib.lib().wv_device_status() == 0
+    c.share([0, seqs + 1], [shared])                                      # a group out of bounds is met only where groups are looked at
+    c.attend(q, 8, 0.09)
+    torch.cuda.synchronize()
+    assert wv._lib.lib().wv_device_status() == (wv._lib.WV_ESHAPE if pays else 0)
 
 
 def test_captured_and_replayed(wv):

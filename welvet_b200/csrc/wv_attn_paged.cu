@@ -25,6 +25,7 @@
 #include "wv_attn_paged.cuh"
 #include "wv_tma_common.cuh"
 #include "wv_lease.h"
+#include "wv_dev_hooks.h"
 #include <algorithm>
 #include <type_traits>
 
@@ -865,6 +866,23 @@ int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* d
 
 // The shared keys of every group for all rows of its sequences (part 1), every sequence's own keys (part 2), and the two joined. Part 1
 // runs on tcgen05 where a group has more than 32 rows of a kv head on average, part 2 where a sequence can have; otherwise 8 or 16 rows a pass.
+#ifdef WV_DEV_HOOKS
+static int g_sharing = 0;
+extern "C" void wv_set_attn_sharing(int always) { g_sharing = always; }
+#endif
+// Does it pay to take the front keys apart? It saves num_seqs - num_groups passes over them: 0.2 ps for each key, value of a kv head and eight
+// query rows, 0.28 for sixteen. It costs two results a row written and joined (at 2 TB/s of their bytes: the join is short) and 6 us, or 12 where the
+// front keys go to the chunk kernel, which takes that long to start. Of 186 shapes (2 to 48 sequences a group, 1 or 4 groups, 256 to 16384 shared
+// tokens, 1 or 4 new ones, three layouts) this takes the faster one or one within 5 % in all but 5, and loses 21 % at most; e.g. us apart / not, 32 heads over 8 of 128 in 8
+// bits: 2 sequences x 16384 tokens 23.3 / 22.8, 48 x 1024 42.5 / 29.7, 48 x 4096 48.1 / 94.8, 48 x 16384 75 / 298.
+static bool sharing_pays(const WvKvBatch& b, int num_groups, long long front, const WvKvGeom& g, int group, bool chunk) {
+#ifdef WV_DEV_HOOKS
+  if (g_sharing) return true;
+#endif
+  const long long rows = (long long)b.max_q * group;
+  const double saved = (double)(b.num_seqs - num_groups) * front * g.kvh * g.hd * (rows <= 8 ? 0.2e-6 : 0.28e-6 * ((rows + 15) / 16));
+  return saved > (chunk ? 12.0 : 6.0) + (double)b.total_q * group * g.kvh * (g.hd + 2) * 2 * 4 / 2e6;
+}
 int wv_launch_attn_shared(const WvKvPages& kv, const WvKvBatch& b, const WvKvGroups& share, const float* dq, int ldq, float* dout, int ldo, int heads, float scale,
                           cudaStream_t st) {
   PaCall c = {};
@@ -882,7 +900,8 @@ int wv_launch_attn_shared(const WvKvPages& kv, const WvKvBatch& b, const WvKvGro
   const long long front = (long long)c.share.max_shared / c.g.page * c.g.page;
   // two results a row at least
   const long long most_slots = std::min(PA_SCRATCH / std::max(rows * (c.g.hd + 2) * 4, 1LL), 1024LL);
-  if (share.num_groups == 0 || front == 0 || most_slots < 2)            // nothing is shared, or there are so many rows that it gains nothing
+  // nothing is shared, so little that it gains nothing, or there are so many rows
+  if (share.num_groups == 0 || front == 0 || most_slots < 2 || !sharing_pays(b, share.num_groups, front, c.g, c.group, c.g.hd <= 128 && each * c.group > 32))
     return wv_launch_attn_paged(kv, b, dq, ldq, dout, ldo, heads, scale, 0, st);
   if (rows > INT_MAX || (long long)b.num_seqs * ((long long)b.max_q * c.group / 8 + 1) * c.g.kvh > INT_MAX) {
     wv_set_error("wv_attn_shared_dev: %d rows of %d heads, %d sequences of %d tokens are too many", b.total_q, heads, b.num_seqs, b.max_q); return WV_ESHAPE;

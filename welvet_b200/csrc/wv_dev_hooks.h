@@ -20,6 +20,8 @@ void wv_set_tcg_stall(int slice, int spin);
 // FormatNone ring kernel: the first warp of every CTA never requests its `row`-th row (1, 2, ...; 0 = off) and the waits give up after
 // `spin` polls (0 = built-in limit).
 void wv_set_ring_stall(int row, int spin);
+// Attention over a shared prefix: always apart from the sequences' own keys where anything is shared (0 = only where it pays).
+void wv_set_attn_sharing(int always);
 #ifdef __cplusplus
 }
 #endif
