@@ -23,7 +23,7 @@
 // at a time (0 4 1 5 2 6 3 7); Q follows, and the outputs are put back.
 //
 // The running maximum is raised only where a logit may lie 2^10 above it, which a bound tells (the row's largest product times the
-// tile's largest scale), so that most tiles are read once; a row's two threads agree on that, and exchange their maxima through tensor
+// tile's largest scale), so that most tiles are read once; a row's threads agree on that, and exchange their maxima through tensor
 // memory that the next tile's sums will overwrite.
 //
 // A logit is S times its key's scale, in one fused step with the subtraction of the reference. The reference is a rounded product, so from
@@ -34,6 +34,14 @@
 // of two goes into the sum over tiles. Where the scales in a tile lie further apart than the pieces' range holds (2^8), the tile's
 // weighted sum is taken value by value in float32 instead.
 //
+// The parts of wv_attn_shared_dev take one tile of 128 rows a block (ONE): a step's two places in tensor memory go to every second step, so that
+// the next scores are made while this step's weights are, and its sums are added a step later; four threads a row (32 keys and a quarter of the
+// values each) and seven warps for the ring of four stages, of which another one takes the eighth group of rows each time. One tile in the form
+// above, with half of its warps idle, was one chain of S, weights, P V and sums of 7000 cycles a key tile behind three warps of conversions; this is 4500 at 0.6
+// instructions a cycle and scheduler, 2048 of them the tensor pipe's. Two groups of 16 sequences behind 65000 tokens, 64 heads in 4 bits: 243 -> 202 us (eight warps of
+// weights instead of 16: 231; three stages instead of four: 205; five of the idle warps as more converters alone: 270). 64 sequences behind 16384
+// tokens in 8 bits, 256 rows of 32 heads: 106 us in blocks of two tiles, 96 in blocks of one.
+//
 // Every wait is bounded: when one runs out the block records a code, all roles leave their loops, and tensor memory is released
 // after the MMAs in flight (waited for, bounded again).
 #include "wv_attn_paged.cuh"
@@ -42,11 +50,8 @@
 #include <stddef.h>
 #include <type_traits>
 
-#define PC_THREADS 640
-#define PC_MMA_WARP 19
 #define PC_M 128                    // rows of a tile
 #define PC_N 128                    // keys of a tile
-#define PC_PRODUCERS 3              // warps 16 - 18
 #define PC_LIFT 4.f                 // weights carry 2^4 and are at most 2^15 (2^10 over the reference, scales below 2)
 #define PC_SLACK 10.f
 #define PC_JOIN 4.f                 // 2^6 / 2^4: results that are joined with those of few rows carry the same factor
@@ -111,19 +116,24 @@ struct PcMeta {
   float beta[2], kmax[2];                   // 2^e, the largest kk
   unsigned flags[2];                        // 1: some key of the tile is not there, 2: value scales too far apart
   unsigned valid[2][4];                     // which keys are there
-  unsigned long long bar[21];
-  unsigned vote[2][2];
+  unsigned long long bar[23];
+  unsigned vote[2][4];
   unsigned tmem, qmax;
   unsigned char qexp[2 * PC_M], lift[2 * PC_M];      // of a row: exponent field of its largest |q|, and what it is lifted by
   int abort;
   int seq, tile, shared, table, q0, q1;
 };
-template <int BITS, int DP> struct PcShape {
-  static constexpr int STAGES = BITS == 16 ? 3 : 2, STAGE = DP / 64 * PC_N * 128, QPIECE = DP / 64 * PC_M * 128;
+// ONE: blocks of one tile of rows.
+template <int BITS, int DP, bool ONE> struct PcShape {
+  static constexpr int ROWS = ONE ? PC_M : 2 * PC_M;
+  // the warps: of rows, then those that fill the ring, then the one that issues the MMAs
+  static constexpr int PARTS = ONE ? 4 : 2, TILE_WARPS = 16, FEED = ONE ? 7 : 3, MMA_WARP = TILE_WARPS + FEED, THREADS = 32 * (MMA_WARP + 1);
+  static constexpr int STAGES = ONE ? 4 : BITS == 16 ? 3 : 2, STAGE = DP / 64 * PC_N * 128, QPIECE = DP / 64 * PC_M * 128;
   static constexpr int PIECES = BITS == 16 ? DP / 8 : DP / 16;                    // of a row: 16 bytes, or 16 codes
   static constexpr int PER = PIECES / 2;                                          // of 16 rows, a lane
   static constexpr int RAW = BITS == 16 ? 0 : PIECES * PC_N * (BITS == 8 ? 16 : 8) + (BITS == 4 ? 1024 : 0);      // 4 bits: codes, then sub-scales
-  static constexpr size_t SMEM = (size_t)4 * QPIECE + STAGES * STAGE + 2 * RAW + sizeof(PcMeta);
+  static constexpr int QBYTES = ROWS / PC_M * 2 * QPIECE;
+  static constexpr size_t SMEM = (size_t)QBYTES + STAGES * STAGE + 2 * RAW + sizeof(PcMeta);
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
@@ -132,29 +142,31 @@ template <int BITS> __device__ __forceinline__ int pc_dim(int p) {      // the v
   return p;
 }
 
-// SHARED: a part of wv_attn_shared_dev.
+// SHARED: a part of wv_attn_shared_dev, in blocks of one tile of rows.
 template <int BITS, int DP, bool SHARED>
-__global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_constant__ PaCall c) {
-  using S = PcShape<BITS, DP>;
+__global__ void __launch_bounds__(PcShape<BITS, DP, SHARED>::THREADS, 1) attn_chunk_kernel(const __grid_constant__ PaCall c) {
+  constexpr bool ONE = SHARED;
+  using S = PcShape<BITS, DP, ONE>;
+  constexpr int ROWS = S::ROWS, TW = S::TILE_WARPS, FEED = S::FEED;
   constexpr int STAGES = S::STAGES, STAGE = S::STAGE, QPIECE = S::QPIECE;
   constexpr unsigned IDESC_S = (1u << 4) | (PC_N / 8 << 17) | (PC_M / 16 << 24);                   // f32 sums, f16 operands, both K-major
   constexpr unsigned IDESC_O = (1u << 4) | (1u << 16) | (DP / 8 << 17) | (PC_M / 16 << 24);        // B with its columns innermost
   extern __shared__ __align__(1024) unsigned char pc_smem[];
   unsigned char* s_q = pc_smem;
-  unsigned char* s_kv = pc_smem + 4 * QPIECE;
+  unsigned char* s_kv = pc_smem + S::QBYTES;
   unsigned char* s_raw = s_kv + STAGES * STAGE;
   PcMeta& M = *reinterpret_cast<PcMeta*>(s_raw + 2 * S::RAW);
   const int tid = threadIdx.x, lane = tid & 31, warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
   auto full = [&](int s) { return smem_u32(&M.bar[s]); };
-  auto empty = [&](int s) { return smem_u32(&M.bar[3 + s]); };
-  auto s_full = [&](int t) { return smem_u32(&M.bar[6 + t]); };
-  auto p_full = [&](int t) { return smem_u32(&M.bar[8 + t]); };
-  auto o_full = [&](int t) { return smem_u32(&M.bar[10 + t]); };
-  auto m_full = [&](int s) { return smem_u32(&M.bar[12 + s]); };
-  auto m_empty = [&](int s) { return smem_u32(&M.bar[14 + s]); };
-  const unsigned done = smem_u32(&M.bar[16]);
-  auto v_bar = [&](int t) { return smem_u32(&M.bar[17 + t]); };
-  auto x_bar = [&](int t) { return smem_u32(&M.bar[19 + t]); };
+  auto empty = [&](int s) { return smem_u32(&M.bar[4 + s]); };
+  auto s_full = [&](int t) { return smem_u32(&M.bar[8 + t]); };
+  auto p_full = [&](int t) { return smem_u32(&M.bar[10 + t]); };
+  auto o_full = [&](int t) { return smem_u32(&M.bar[12 + t]); };
+  auto m_full = [&](int s) { return smem_u32(&M.bar[14 + s]); };
+  auto m_empty = [&](int s) { return smem_u32(&M.bar[16 + s]); };
+  const unsigned done = smem_u32(&M.bar[18]);
+  auto v_bar = [&](int t) { return smem_u32(&M.bar[19 + t]); };
+  auto x_bar = [&](int t) { return smem_u32(&M.bar[21 + t]); };
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (smem_u32(pc_smem) & 1023u) { if (tid == 0) atomicCAS_system(c.err - 1, 0, 799); return; }    // the swizzle counts from 1024-byte boundaries
@@ -167,11 +179,11 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
     if (SHARED && c.part == 1) {
       PaGroup g;
       int q0 = 0, q1 = 0;
-      if (pa_find_group(c, flat, 256, err, g, q0, q1, tile)) shared = pa_shared_keys(c, g, table);
+      if (pa_find_group(c, flat, ROWS, err, g, q0, q1, tile)) shared = pa_shared_keys(c, g, table);
       seq = shared == 0 ? -1 : 0;
       if (lane == 0) { M.q0 = q0; M.q1 = q1; }
     } else {
-      pa_find(c, flat, 256, c.rows_most, err, seq, tile);
+      pa_find(c, flat, ROWS, c.rows_most, err, seq, tile);
       table = seq;
       if (SHARED && seq >= 0) shared = pa_shared_of(c, seq);
     }
@@ -187,10 +199,10 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
   } else {
     sq = wv_seq(c.b, c.g.page, seq, sp == 0 && kvh == 0 ? c.err : nullptr);
   }
-  const int nrows = (sq.q1 - sq.q0) * c.group, r0 = M.tile * 256, rn = min(256, nrows - r0);
+  const int nrows = (sq.q1 - sq.q0) * c.group, r0 = M.tile * ROWS, rn = min(ROWS, nrows - r0);
   int lo, hi, per = c.per;
   pa_range(sq, r0 / c.group, (r0 + rn - 1) / c.group, c.window, lo, hi);
-  const size_t rec0 = ((size_t)flat * c.g.kvh + kvh) * 256;               // this block's rows in the split results
+  const size_t rec0 = ((size_t)flat * c.g.kvh + kvh) * ROWS;              // this block's rows in the split results
   auto rec = [&](int r) {
     if (SHARED) return ((size_t)(sq.q0 + (r0 + r) / c.group) * (c.group * c.g.kvh) + kvh * c.group + (r0 + r) % c.group) * c.nslots + c.slot0 + sp;
     return (rec0 + r) * c.nsplit + sp;
@@ -202,7 +214,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
       lo = max(lo, M.shared);
       if (hi > lo) per = max(per, ((hi - lo + c.nsplit - 1) / c.nsplit + PC_N - 1) & ~(PC_N - 1));      // planned for less where little is shared
       if (M.shared == 0 && sp == 0)                                      // nobody else writes these rows' results of part 1
-        for (int i = tid; i < rn * c.slot0; i += PC_THREADS) c.ml[rec(i / c.slot0) - c.slot0 + i % c.slot0] = make_float2(-INFINITY, 0.f);
+        for (int i = tid; i < rn * c.slot0; i += S::THREADS) c.ml[rec(i / c.slot0) - c.slot0 + i % c.slot0] = make_float2(-INFINITY, 0.f);
     }
   }
   const unsigned first = (unsigned)lo + (unsigned)sp * (unsigned)per;
@@ -210,37 +222,39 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
   const int hd = c.g.hd, pos0 = sq.p0;
   if (k0 >= k1) {
     if (SHARED || c.nsplit > 1) { if (tid < rn) c.ml[rec(tid)] = make_float2(-INFINITY, 0.f); }
-    else for (int i = tid; i < rn * hd; i += PC_THREADS) {
+    else for (int i = tid; i < rn * hd; i += S::THREADS) {
       const int r = r0 + i / hd;
       c.out[(size_t)(sq.q0 + r / c.group) * c.ldo + (size_t)(kvh * c.group + r % c.group) * hd + i % hd] = 0.f;
     }
     return;
   }
   const int n = (k1 - k0 + PC_N - 1) / PC_N;
-  const bool two = rn > PC_M;
+  const bool two = !ONE && rn > PC_M;
 
   if (tid == 0) {
-    for (int s = 0; s < STAGES; s++) { mbar_init(full(s), PC_PRODUCERS); mbar_init(empty(s), 1); }
+    for (int s = 0; s < STAGES; s++) { mbar_init(full(s), FEED); mbar_init(empty(s), 1); }
     for (int t = 0; t < 2; t++) {
-      mbar_init(s_full(t), 1); mbar_init(p_full(t), 8); mbar_init(o_full(t), 1);
-      mbar_init(m_full(t), 1); mbar_init(m_empty(t), two ? 16 : 8);
-      mbar_init(v_bar(t), 8); mbar_init(x_bar(t), 8);
-      M.vote[t][0] = M.vote[t][1] = 0;
+      mbar_init(s_full(t), 1); mbar_init(p_full(t), 4 * S::PARTS); mbar_init(o_full(t), 1);
+      mbar_init(m_full(t), 1); mbar_init(m_empty(t), ONE || two ? 16 : 8);
+      mbar_init(v_bar(t), 4 * S::PARTS); mbar_init(x_bar(t), 4 * S::PARTS);
+      M.vote[t][0] = M.vote[t][1] = M.vote[t][2] = M.vote[t][3] = 0;
     }
     mbar_init(done, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == PC_MMA_WARP) {
+  if (warp == S::MMA_WARP) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&M.tmem)), "n"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   // ---------------------------------------------------------------- K and V tiles: what their warps know of the pages, and the copies
-  const int pw = warp - 16, code = c.g.code, page = c.g.page;
-  // A warp takes the groups pw, pw + 3, .. of a tile's eight groups of 16 rows; a lane's piece (16 bytes of 16-bit rows, else 16 codes) is
+  const int pw = warp - TW, code = c.g.code, page = c.g.page;
+  // A warp takes the groups pw, pw + FEED, .. of a tile's eight groups of 16 rows; a lane's piece (16 bytes of 16-bit rows, else 16 codes) is
   // number x of rows lr, lr + STEP, ..
   constexpr int STEP = 32 / S::PIECES, PER = S::PER;
   const int x = lane % S::PIECES, lr = lane / S::PIECES, n16 = hd / 16;
   const bool mine = BITS == 16 ? 8 * x < hd : 16 * x < hd;
+  // (of seven warps another one takes the eighth group each time)
+  auto more = [&](int g, int e) { return !ONE ? g + FEED : g < FEED && e % FEED == pw ? FEED : 8; };
   // page numbers of 32 groups of 16 keys (four tiles) at a time, a lane each, as offsets in the pool (-1: not there)
   long long blk = 0;
   int slots = 0;
@@ -271,7 +285,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
     const int j = e >> 1;
     const bool is_v = e & 1;
     const unsigned stage = smem_u32(s_kv) + (e % STAGES) * STAGE, raw = smem_u32(s_raw) + (e & 1) * S::RAW;
-    for (int g = pw; g < 8; g += PC_PRODUCERS) {
+    for (int g = pw; g < 8; g = more(g, e)) {
       const long long at = __shfl_sync(0xffffffffu, blk, 8 * (j & 3) + g);
       const int slot = __shfl_sync(0xffffffffu, slots, 8 * (j & 3) + g) + lr;
       const int left = at < 0 ? 0 : k1 - (k0 + j * PC_N + 16 * g) - lr;          // the lane's rows 0, STEP, .. below this exist
@@ -311,9 +325,9 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
   // The warps of K and V ask for the first tile meanwhile; the others have eight rows under way at a time (one by one they were a chain of 13
   // round trips). Where the rows are is worked out once and kept in the room of the keys' scales: what runs once costs what its instructions
   // take to arrive, and a division for every row of an unrolled loop was 11 us of them.
-  constexpr int QW = PC_THREADS / 32 - PC_PRODUCERS;
-  const bool feeds = warp >= 16 && warp < 16 + PC_PRODUCERS;
-  const int qw = warp < 16 ? warp : 16, qt = 32 * qw + lane;
+  constexpr int QW = ONE ? S::MMA_WARP + 1 : TW + 1;
+  const bool feeds = warp >= TW && warp < TW + FEED, reads = ONE || !feeds;
+  const int qw = ONE || warp < TW ? warp : TW, qt = 32 * qw + lane;
   long long* q_at = reinterpret_cast<long long*>(M.kk);                  // of a row, as an offset; inverted if the row stands before position 0
   static_assert(sizeof(M.kk) + sizeof(M.fv) >= 256 * sizeof(long long) && offsetof(PcMeta, fv) == sizeof(M.kk), "room for the rows' offsets");
   if (tid < rn) {
@@ -325,7 +339,8 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
   if (feeds) {
     ahead(0);
     ahead(1);
-  } else {
+  }
+  if (reads) {
     unsigned top = 0;
 #pragma unroll 1
     for (int r0_ = qw; r0_ < rn; r0_ += 8 * QW) {
@@ -366,7 +381,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
     return own && up > 15 ? min(up, 100) : 0;
   };
   if (tid < 2 * PC_M) M.lift[tid] = (unsigned char)(tid < rn ? lift(tid) : 0);
-  for (int i = feeds ? 256 * (DP / 8) : qt; i < (two ? 256 : PC_M) * (DP / 8); i += 32 * QW) {      // 8 places of a row at a time
+  for (int i = reads ? qt : 256 * (DP / 8); i < (two ? 256 : PC_M) * (DP / 8); i += 32 * QW) {      // 8 places of a row at a time
     const int r = i / (DP / 8), j = i % (DP / 8);
     unsigned h[4] = {0u, 0u, 0u, 0u}, l[4] = {0u, 0u, 0u, 0u};
     const long long at = r < rn ? q_at[r] : -1;
@@ -396,18 +411,21 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
   auto fail = [&](int code) { atomicCAS_system(c.err - 1, 0, code); *(volatile int*)&M.abort = 1; };      // the word before is the waits'
   auto dead = [&]() { return *(volatile int*)&M.abort != 0; };
 
-  if (warp < 16) {
+  if (warp < TW) {
     // ============================================================== half a tile: weights of 64 keys, sums of half of the values
-    pc_regs_up<104>();
-    constexpr int HD = DP / 2, HK = PC_N / 2;
-    const int t = warp >> 3, hf = (warp >> 2) & 1, row = tid & (PC_M - 1), r = t * PC_M + row;
+    if (!ONE) pc_regs_up<104>();
+    constexpr int HD = DP / S::PARTS, HK = PC_N / S::PARTS;
+    const int t = warp / (4 * S::PARTS), hf = (warp >> 2) % S::PARTS, row = tid & (PC_M - 1), r = t * PC_M + row;
     if (t == 0 || two) {
       const unsigned lanes = (unsigned)((warp & 3) * 32) << 16;
-      const unsigned ts = tmem + lanes + t * PC_N + hf * HK, to = tmem + lanes + 256 + t * 128 + hf * HD, tx = to + HD - 2 * hf * HD;
+      unsigned ts, to, at_o;                                             // of a step; a single tile has the other's room for every second one
+      auto turn = [&](int b) { ts = tmem + lanes + b * PC_N + hf * HK; to = tmem + lanes + 256 + b * 128 + hf * HD; at_o = b; };
+      turn(t);
       const int prow = pos0 + (r0 + min(r, rn - 1)) / c.group;
       const int pmin = pos0 + (r0 + t * PC_M) / c.group, pmax = pos0 + (r0 + min(t * PC_M + PC_M, rn) - 1) / c.group;
       float o[HD], m = -INFINITY;
       float2 l2 = make_float2(0.f, 0.f);
+      float owed = 0.f;                                                  // the factor of the last step's sums, not yet added
 #pragma unroll
       for (int d = 0; d < HD; d++) o[d] = 0.f;
       bool ok = true;
@@ -418,19 +436,39 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
         ok = !__any_sync(0xffffffffu, !ok);
         return ok;
       };
-      // the tile's eight warps meet
+      // the tile's warps meet
       auto meet = [&](unsigned bar, int use, int why) {
         __syncwarp();
         if (lane == 0) mbar_arrive(bar);
         return wait(bar, use, why);
       };
+      // the sums of step j into o, by `f`
+      auto add = [&](int j, float f) {
+        const int b = ONE ? j & 1 : t;
+        const unsigned from = tmem + lanes + 256 + b * 128 + hf * HD;
+        if (!wait(o_full(b), ONE ? j >> 1 : j, 710 + b)) return false;
+        pc_fence_after();
+#pragma unroll
+        for (int q = 0; q < HD / 16; q++) {
+          unsigned a[16];
+          pc_ld16(from + 16 * q, a);
+          pc_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            const float2 v = __ffma2_rn(make_float2(__uint_as_float(a[i]), __uint_as_float(a[i + 1])), make_float2(f, f), make_float2(o[16 * q + i], o[16 * q + i + 1]));
+            o[16 * q + i] = v.x; o[16 * q + i + 1] = v.y;
+          }
+        }
+        return true;
+      };
       for (int j = 0; j < n; j++) {
+        if (ONE) turn(j & 1);
         const int ms = j & 1, key0 = k0 + j * PC_N;
         // rows that are lifted or have a reference of 2^20 or more: the warp rounds its logits first
         const unsigned lifted = M.lift[r];
         auto apart = [&]() { return __any_sync(0xffffffffu, lifted || (__float_as_uint(m) & 0x7fffffffu) - __float_as_uint(1048576.f) < 0x7f800000u - __float_as_uint(1048576.f)); };
         bool slow = apart();
-        if (!wait(m_full(ms), j >> 1, 700 + t) || !wait(s_full(t), j, 702 + t)) break;
+        if (!wait(m_full(ms), j >> 1, 700 + t) || !wait(s_full(ONE ? ms : t), ONE ? j >> 1 : j, 702 + t)) break;
         pc_fence_after();
         const unsigned kk = smem_u32(M.kk[ms]) + 4 * HK * hf, fv = smem_u32(M.fv[ms]) + 4 * HK * hf;
         float beta = M.beta[ms], alpha = 1.f;
@@ -444,31 +482,32 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
           if (first > 0) w &= first > 31 ? 0u : ~0u << first;
           return w & M.valid[ms][word];
         };
-        unsigned see[2] = {~0u, ~0u};
-        if (masked) { see[0] = sees(2 * hf, 2 * hf); see[1] = sees(2 * hf + 1, 2 * hf + 1); }
+        unsigned see[HK / 32];
+#pragma unroll
+        for (int i = 0; i < HK / 32; i++) see[i] = masked ? sees(HK / 32 * hf + i, HK / 32 * hf + i) : ~0u;
         // ---- the reference: may a logit lie too far above it?
         bool raise = masked;
         if (!masked) {
           float top = 0.f;
 #pragma unroll
-          for (int q = 0; q < 4; q++) {
+          for (int q = 0; q < HK / 16; q++) {
             unsigned a[16];
             pc_ld16(ts + 16 * q, a);
             pc_wait_ld();
 #pragma unroll
             for (int i = 0; i < 16; i += 2) top = fmaxf(top, fmaxf(__uint_as_float(a[i]), __uint_as_float(a[i + 1])));
           }
-          if (__any_sync(0xffffffffu, !(top * down * M.kmax[ms] <= m + PC_SLACK)) && lane == 0) atomicOr(&M.vote[t][nv & 1], 1u);
+          if (__any_sync(0xffffffffu, !(top * down * M.kmax[ms] <= m + PC_SLACK)) && lane == 0) atomicOr(&M.vote[t][nv & 3], 1u);
           if (!meet(v_bar(t), nv, 704 + t)) break;
-          raise = *(volatile unsigned*)&M.vote[t][nv & 1] != 0;
-          if ((warp & 7) == 0 && lane == 0) M.vote[t][(nv + 1) & 1] = 0; // nobody comes to the next vote before this warp's weights are there
+          raise = *(volatile unsigned*)&M.vote[t][nv & 3] != 0;
+          if (warp == 4 * S::PARTS * t && lane == 0) M.vote[t][(nv + 2) & 3] = 0; // nobody comes to that vote before this warp has come to the next
           nv++;
         }
         if (raise) {
           float mx = m;
 #pragma unroll 1
-          for (int q = 0; q < 4; q++) {
-            const unsigned bits = ((q < 2 ? see[0] : see[1]) >> (16 * (q & 1))) & 0xffffu;
+          for (int q = 0; q < HK / 16; q++) {
+            const unsigned bits = ((q < 2 ? see[0] : see[HK / 32 - 1]) >> (16 * (q & 1))) & 0xffffu;
             if (!__any_sync(0xffffffffu, bits)) continue;                // keys that none of the warp's rows sees
             unsigned a[16];
             pc_ld16(ts + 16 * q, a);
@@ -493,7 +532,8 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
           pc_fence_before();
           if (!meet(x_bar(t), nx++, 706 + t)) break;
           pc_fence_after();
-          mx = fmaxf(mx, __uint_as_float(pc_ld1(tx)));
+#pragma unroll
+          for (int i = 1; i < S::PARTS; i++) mx = fmaxf(mx, __uint_as_float(pc_ld1(to + ((hf + i) % S::PARTS - hf) * HD)));
           alpha = mx > m ? pa_ex2(m - mx) : 1.f;                         // 0 while there was nothing
           m = mx;
           slow = apart();
@@ -501,11 +541,12 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
         }
         const float2 off = m == -INFINITY ? make_float2(0.f, 0.f) : make_float2(PC_LIFT - m, PC_LIFT - m);
         if (flags & 2u) {
-          // ---- value by value in float32: both threads of a row go through all 128 keys; then P is zero
+          // ---- value by value in float32: all threads of a row go through all 128 keys; then P is zero
           const int e = 2 * j + 1;
           if (!wait(full(e % STAGES), e / STAGES, 708)) break;
           const unsigned char* v = s_kv + (e % STAGES) * STAGE;
-          const unsigned tt = tmem + lanes + t * PC_N;
+          const unsigned tt = tmem + lanes + at_o * PC_N;
+          if (ONE && j && owed != 0.f) { if (!add(j - 1, owed)) break; owed = 0.f; }
 #pragma unroll
           for (int d = 0; d < HD; d++) o[d] *= alpha;
           alpha = 1.f;
@@ -526,13 +567,13 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
           }
           beta = 0.f;
           pc_fence_before();
-          if (!meet(x_bar(t), nx++, 706 + t)) break;                     // the row's other thread has read S
+          if (!meet(x_bar(t), nx++, 706 + t)) break;                     // the row's other threads have read S
           pc_fence_after();
           unsigned z[16];
 #pragma unroll
           for (int i = 0; i < 16; i++) z[i] = 0u;
 #pragma unroll
-          for (int q = 0; q < 4; q++) pc_st16(ts + 16 * q, z);
+          for (int q = 0; q < HK / 16; q++) pc_st16(ts + 16 * q, z);
         } else {
           // ---- weights: 16 keys of S become 8 columns of their hi pieces and 8 of their lo pieces
           auto weights = [&](auto some, int q, unsigned bits) {
@@ -568,11 +609,11 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
           };
           if (!masked && !slow) {
 #pragma unroll
-            for (int q = 0; q < 4; q++) weights(std::false_type(), q, 0u);
+            for (int q = 0; q < HK / 16; q++) weights(std::false_type(), q, 0u);
           } else {
 #pragma unroll 1
-            for (int q = 0; q < 4; q++) {
-              const unsigned bits = ((q < 2 ? see[0] : see[1]) >> (16 * (q & 1))) & 0xffffu;
+            for (int q = 0; q < HK / 16; q++) {
+              const unsigned bits = ((q < 2 ? see[0] : see[HK / 32 - 1]) >> (16 * (q & 1))) & 0xffffu;
               if (!__any_sync(0xffffffffu, bits)) {
                 unsigned z[16];
 #pragma unroll
@@ -587,27 +628,18 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
         asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         pc_fence_before();
         __syncwarp();
-        if (lane == 0) { mbar_arrive(p_full(t)); mbar_arrive(m_empty(ms)); }
-        // ---- this tile's part of the sum
+        if (lane == 0) { mbar_arrive(p_full(ONE ? ms : t)); mbar_arrive(m_empty(ms)); }
+        // ---- this tile's part of the sum; with one tile of rows that of the step before, while the tensor pipe is at this one's
+        if (ONE && owed != 0.f && !add(j - 1, owed)) break;
         if (__any_sync(0xffffffffu, alpha != 1.f)) {
 #pragma unroll
           for (int d = 0; d < HD; d += 2) { const float2 v = __fmul2_rn(make_float2(o[d], o[d + 1]), make_float2(alpha, alpha)); o[d] = v.x; o[d + 1] = v.y; }
         }
-        if (!wait(o_full(t), j, 710 + t)) break;
-        pc_fence_after();
-#pragma unroll
-        for (int q = 0; q < HD / 16; q++) {
-          unsigned a[16];
-          pc_ld16(to + 16 * q, a);
-          pc_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            const float2 v = __ffma2_rn(make_float2(__uint_as_float(a[i]), __uint_as_float(a[i + 1])), make_float2(beta, beta), make_float2(o[16 * q + i], o[16 * q + i + 1]));
-            o[16 * q + i] = v.x; o[16 * q + i + 1] = v.y;
-          }
-        }
+        if (ONE) owed = beta;
+        else if (!add(j, beta)) break;
       }
-      // the row's divisor: the two halves' sums
+      if (ONE && ok) add(n - 1, owed);
+      // the row's divisor: its parts' sums
       float l = l2.x + l2.y;
       if (ok) {
         asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(to), "r"(__float_as_uint(l)) : "memory");
@@ -615,7 +647,10 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
         pc_fence_before();
         if (meet(x_bar(t), nx++, 706 + t)) {
           pc_fence_after();
-          l += __uint_as_float(pc_ld1(tx));
+          // in one order for all of a row's threads
+          l = __uint_as_float(pc_ld1(to - hf * HD));
+#pragma unroll
+          for (int i = 1; i < S::PARTS; i++) l += __uint_as_float(pc_ld1(to + (i - hf) * HD));
         }
       }
       if (r < rn) {
@@ -643,8 +678,8 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
       }
     }
   } else {
-    pc_regs_down<64>();
-    if (warp == PC_MMA_WARP) {
+    if (!ONE) pc_regs_down<64>();
+    if (warp == S::MMA_WARP) {
       // ============================================================ MMAs
       const bool leader = pc_elect();
       const unsigned qa = smem_u32(s_q), kv = smem_u32(s_kv);
@@ -655,7 +690,8 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
         ok = !__any_sync(0xffffffffu, !ok || dead());
         return ok;
       };
-      auto scores = [&](int t, int e) {                                  // S of tile t with the K tile that is element e of the ring
+      // S of tile t, at b, with the K tile that is element e of the ring
+      auto scores = [&](int t, int b, int e) {
         if (leader) {
           const unsigned kb = kv + (e % STAGES) * STAGE;
 #pragma unroll
@@ -663,28 +699,47 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
             const unsigned qb = qa + (2 * t + p) * QPIECE;
 #pragma unroll
             for (int k = 0; k < DP / 16; k++)
-              pc_mma_ss(tmem + t * PC_N, pc_desc(qb + (k >> 2) * PC_M * 128 + (k & 3) * 32, 16), pc_desc(kb + (k >> 2) * PC_N * 128 + (k & 3) * 32, 16), IDESC_S, !(p == 1 && k == 0));
+              pc_mma_ss(tmem + b * PC_N, pc_desc(qb + (k >> 2) * PC_M * 128 + (k & 3) * 32, 16), pc_desc(kb + (k >> 2) * PC_N * 128 + (k & 3) * 32, 16), IDESC_S, !(p == 1 && k == 0));
           }
-          pc_commit(s_full(t));
+          pc_commit(s_full(b));
         }
         __syncwarp();
       };
-      auto values = [&](int t, int e) {
+      auto values = [&](int b, int e) {
         if (leader) {
           const unsigned vb = kv + (e % STAGES) * STAGE;
 #pragma unroll
           for (int p = 1; p >= 0; p--)
 #pragma unroll
             for (int k = 0; k < PC_N / 16; k++)
-              pc_mma_ts(tmem + 256 + t * 128, tmem + t * PC_N + 16 * k + 8 * p, pc_desc(vb + k * 2048, PC_N * 128), IDESC_O, !(p == 1 && k == 0));
-          pc_commit(o_full(t));
+              pc_mma_ts(tmem + 256 + b * 128, tmem + b * PC_N + 16 * k + 8 * p, pc_desc(vb + k * 2048, PC_N * 128), IDESC_O, !(p == 1 && k == 0));
+          pc_commit(o_full(b));
         }
         __syncwarp();
       };
       auto release = [&](int e) { if (leader) pc_commit(empty(e % STAGES)); __syncwarp(); };
+      if constexpr (ONE) {
+        // A tile's steps take turns at two places in tensor memory: the next scores are on their way while the weights of this step are made.
+        for (int j = -1; j < n && ok; j++) {
+          if (j + 1 < n) {
+            const int e = 2 * (j + 1);
+            if (!wait(full(e % STAGES), e / STAGES, 712)) break;
+            pc_fence_after();
+            scores(0, (j + 1) & 1, e);
+            release(e);
+          }
+          if (j >= 0) {
+            const int e = 2 * j + 1;
+            if (!wait(full(e % STAGES), e / STAGES, 712) || !wait(p_full(j & 1), j >> 1, 713)) break;
+            pc_fence_after();
+            values(j & 1, e);
+            release(e);
+          }
+        }
+      } else {
       if (wait(full(0), 0, 712)) {
         pc_fence_after();
-        for (int t = 0; t < nt; t++) scores(t, 0);
+        for (int t = 0; t < nt; t++) scores(t, t, 0);
         release(0);
       }
       // From then on whatever is ready first: a tile's values of step pv[t] when its weights and V are there, its scores of the next
@@ -700,7 +755,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
       while (ok && (pv[0] < n || (nt == 2 && pv[1] < n))) {
         bool did = false;
         for (int t = 0; t < nt; t++) {
-          if (pv[t] < n && pv[t] < qk[t] && ready(full((2 * pv[t] + 1) % STAGES), (2 * pv[t] + 1) / STAGES) && ready(p_full(t), pv[t])) {
+                    if (pv[t] < n && pv[t] < qk[t] && ready(full((2 * pv[t] + 1) % STAGES), (2 * pv[t] + 1) / STAGES) && ready(p_full(t), pv[t])) {
             pc_fence_after();
             const int e = 2 * pv[t] + 1;
             values(t, e);
@@ -711,7 +766,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
           if (qk[t] < n && pv[t] >= qk[t] && ready(full(2 * qk[t] % STAGES), 2 * qk[t] / STAGES)) {
             pc_fence_after();
             const int e = 2 * qk[t];
-            scores(t, e);
+            scores(t, t, e);
             qk[t]++;
             if (nt == 1 || qk[t ^ 1] >= qk[t]) release(e);
             did = true;
@@ -720,6 +775,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
         idle = did ? 0 : idle + 1;
         if (idle > PC_SPIN) { if (leader) fail(713); ok = false; }
         if ((idle & 255) == 255 && __any_sync(0xffffffffu, dead())) ok = false;
+      }
       }
       if (!ok) {                                                         // what was issued has to end before tensor memory is given back
         if (leader) pc_commit(done);
@@ -733,7 +789,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
     auto convert = [&](int e) {
       const unsigned stage = smem_u32(s_kv) + (e % STAGES) * STAGE, raw = smem_u32(s_raw) + (e & 1) * S::RAW;
       const bool turned = (x >> 2) & 1;
-      for (int g = pw; g < 8; g += PC_PRODUCERS) {
+      for (int g = pw; g < 8; g = more(g, e)) {
         // all of a group's loads before the first store: the compiler may not move them past it
         unsigned c4[PER][BITS == 8 ? 4 : 2], sc[PER];
 #pragma unroll
@@ -838,7 +894,7 @@ __global__ void __launch_bounds__(PC_THREADS, 1) attn_chunk_kernel(const __grid_
   }
   pc_fence_before();
   __syncthreads();
-  if (warp == PC_MMA_WARP) {
+  if (warp == S::MMA_WARP) {
     pc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
   }
@@ -873,7 +929,7 @@ __global__ void __launch_bounds__(256) chunk_join_kernel(const __grid_constant__
 
 template <int BITS, int DP, bool SHARED>
 static cudaError_t chunk_go(const PaCall& c, long long flat, cudaStream_t st) {
-  constexpr size_t smem = PcShape<BITS, DP>::SMEM;
+  constexpr size_t smem = PcShape<BITS, DP, SHARED>::SMEM;
   auto kern = attn_chunk_kernel<BITS, DP, SHARED>;
   static unsigned long long attr_mask = 0;
   int dev = 0;
@@ -885,7 +941,7 @@ static cudaError_t chunk_go(const PaCall& c, long long flat, cudaStream_t st) {
   }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute at[1];
-  cfg.gridDim = dim3((unsigned)(flat * c.g.kvh), (unsigned)c.nsplit); cfg.blockDim = dim3(PC_THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
+  cfg.gridDim = dim3((unsigned)(flat * c.g.kvh), (unsigned)c.nsplit); cfg.blockDim = dim3(PcShape<BITS, DP, SHARED>::THREADS); cfg.dynamicSmemBytes = smem; cfg.stream = st;
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at; cfg.numAttrs = 1;

@@ -914,7 +914,7 @@ int wv_launch_attn_shared(const WvKvPages& kv, const WvKvBatch& b, const WvKvGro
   for (int i = 0; i < 2; i++) {
     Part& p = part[i];
     const long long keys = i ? std::max((long long)b.max_kv - front, 1LL) : front;
-    const int size = p.chunk ? 256 : p.r16 ? 16 : 8;
+    const int size = p.chunk ? 128 : p.r16 ? 16 : 8;
     const long long upto = (long long)b.total_q * c.group / size + (i ? b.num_seqs : share.num_groups), sure = (top[i] + size - 1) / size;
     const long long likely = i && p.chunk ? std::min(b.num_seqs * sure, upto) : (i ? b.num_seqs : share.num_groups) * sure;
     p.grid = i ? likely : upto;
