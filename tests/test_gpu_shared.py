@@ -100,6 +100,32 @@ def test_chunks_behind_a_prefix(wv, bits):
     Shared(wv, bits, 32, 2, 128, lens, [0, 4], [640]).check(8)
 
 
+@pytest.mark.parametrize("bits", [16, 8, 4])
+def test_many_tiles_a_block(wv, bits):
+    """40 sequences of the same 16384 tokens: blocks go through several tiles of keys, the stages of their rings many times around. Three runs."""
+    kvh, hd, heads, n, rows = 8, 128, 16, 16384, 40
+    c = Cache(wv, bits, 64, kvh, hd, [(1, n)])
+    rng = np.random.default_rng(bits)
+    c.fill(*(torch.from_numpy(rng.normal(0, 1, (n, kvh * hd)).astype(np.float32)).cuda() for _ in range(2)))
+    table = c.d_table[:1].repeat(rows, 1).contiguous()
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    start, kv, at, shared = ints(*range(rows + 1)), ints(*[n] * rows), ints(0, rows), ints(n, 0)
+    batch = wv.paged.Batch(start.data_ptr(), kv.data_ptr(), table.data_ptr(), rows, table.shape[1], rows, 1, n)
+    groups = wv.paged.Groups(at.data_ptr(), shared.data_ptr(), 1, n)
+    q = torch.from_numpy(rng.normal(0, 1, (rows, heads * hd)).astype(np.float32)).cuda()
+    want, mag, reach = attn64(q.cpu().numpy().reshape(rows, heads, hd), c.rows("k"), c.rows("v"), hd ** -0.5, 0, n - 1)
+    tol = bound(mag, reach, hd, n)
+    first = None
+    for _ in range(3):
+        out = torch.full_like(q, 77.0)
+        wv.paged.AttnSharedCUDA(c.pages, batch, groups, q.data_ptr(), out.data_ptr(), heads, hd ** -0.5)
+        torch.cuda.synchronize()
+        assert wv._lib.lib().wv_device_status() == 0
+        assert (np.abs(out.double().cpu().numpy().reshape(want.shape) - want) <= tol).all()
+        first = out if first is None else first
+        assert torch.equal(out, first)
+
+
 def test_chunks_of_wide_heads(wv):
     lens = [(40, 340), (9, 309), (1, 301)]
     Shared(wv, 8, 16, 1, 192, lens, [0, 3], [300]).check(4)

@@ -6,8 +6,7 @@
 //
 // Bound: HBM and latency for few rows (a tile reads all of A_s and B_s, 256 KB at rank 16 of 4096 x 4096, and a row of x has 16 KB), the
 // reading of x and y for prompts. A warp works alone: 16 columns of A and x, or 16 or 32 outputs' rows of B and their values of base, at a time through a
-// ring of its own (cp.async, no barrier but its own), and the first outputs' copies are under way while t is being added up. Copies by warps of their own for all
-// others, behind mbarriers, were slower: with two stages a CTA everyone waited for someone (2048 rows below: 55 us). The products run on mma.sync m16n8k16 with
+// ring of its own (cp.async, no barrier but its own), and the first outputs' copies are under way while t is being added up. The products run on mma.sync m16n8k16 with
 // the weights as the side of 16 and the rows of x as the side of 8: of a step of decoding an adapter has a row or two, and a tcgen05 tile of 128 would be nearly
 // all padding.
 //
@@ -18,6 +17,11 @@
 //
 // 16-bit weights come out of shared memory by ldmatrix, which puts a fragment's words where the product wants them (put together from
 // vector loads they took a move each).
+//
+// Measured, plan and targets, us from a graph (floor): a row, rank 16 of 4096 beside 4096 + 1024 + 1024 in bf16 7.2 (0.1); 64 rows of 32 such adapters 17 (3.4); 48
+// rows of 16, rank 64 of 4096 beside 2 x 14336 in f16 36 (13); 2048 rows of 6, rank 64 of 4096 beside 4096 in bf16 53 (16); 333 rows of 9, rank 24 of 14336
+// beside 4096 in f32 50 (7). What bounds them is a cluster's chain: its ring fills, t is made, added up and spread, and only then
+// do the outputs run; clusters of up to 16 CTAs shorten both parts (with 8 at most the last one took 54), and are kept from running in turns by the rule below.
 #include "wv_paged.cuh"
 #include "wv_tma_common.cuh"      // lds64, smem_u32
 #include <algorithm>

@@ -886,6 +886,8 @@ __global__ void __launch_bounds__(PcShape<BITS, DP, SHARED>::THREADS, 1) attn_ch
         convert(e);
         arrive(e);
         if ((e & 1) && e + 1 < 2 * n && pw == 0) { const int j = (e + 1) >> 1; if (j >= 2 && !wait(m_empty(j & 1), (j >> 1) - 1, 721)) break; meta(j); }
+        // the eighth group's codes come to where another warp's were
+        if (ONE && (e + 2) % FEED == pw && !wait(full(e % STAGES), e / STAGES, 722)) break;
         ahead(e + 2);
       }
     }

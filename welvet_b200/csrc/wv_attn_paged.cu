@@ -870,17 +870,17 @@ int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* d
 static int g_sharing = 0;
 extern "C" void wv_set_attn_sharing(int always) { g_sharing = always; }
 #endif
-// Does it pay to take the front keys apart? It saves num_seqs - num_groups passes over them: 0.2 ps for each key, value of a kv head and eight
-// query rows, 0.28 for sixteen. It costs two results a row written and joined (at 2 TB/s of their bytes: the join is short) and 6 us, or 12 where the
+// Does it pay to take the front keys apart? It saves num_seqs - num_groups passes over them: 0.25 ps for each key, value of a kv head and eight
+// query rows, 0.35 for sixteen. It costs two results a row written and joined (at 2 TB/s of their bytes: the join is short) and 6 us, or 12 where the
 // front keys go to the chunk kernel, which takes that long to start. Of 186 shapes (2 to 48 sequences a group, 1 or 4 groups, 256 to 16384 shared
-// tokens, 1 or 4 new ones, three layouts) this takes the faster one or one within 5 % in all but 5, and loses 21 % at most; e.g. us apart / not, 32 heads over 8 of 128 in 8
-// bits: 2 sequences x 16384 tokens 23.3 / 22.8, 48 x 1024 42.5 / 29.7, 48 x 4096 48.1 / 94.8, 48 x 16384 75 / 298.
+// tokens, 1 or 4 new ones, three layouts) this takes the faster way, or one within 5 %, in all but 6, and loses 27 % at most; e.g. us apart / not, 32 heads over 8 of
+// 128 in 8 bits: 2 sequences x 16384 tokens 23.1 / 22.6, 48 x 1024 34.6 / 29.5, 48 x 4096 41.6 / 94.9, 48 x 16384 72 / 298.
 static bool sharing_pays(const WvKvBatch& b, int num_groups, long long front, const WvKvGeom& g, int group, bool chunk) {
 #ifdef WV_DEV_HOOKS
   if (g_sharing) return true;
 #endif
   const long long rows = (long long)b.max_q * group;
-  const double saved = (double)(b.num_seqs - num_groups) * front * g.kvh * g.hd * (rows <= 8 ? 0.2e-6 : 0.28e-6 * ((rows + 15) / 16));
+  const double saved = (double)(b.num_seqs - num_groups) * front * g.kvh * g.hd * (rows <= 8 ? 0.25e-6 : 0.35e-6 * ((rows + 15) / 16));
   return saved > (chunk ? 12.0 : 6.0) + (double)b.total_q * group * g.kvh * (g.hd + 2) * 2 * 4 / 2e6;
 }
 int wv_launch_attn_shared(const WvKvPages& kv, const WvKvBatch& b, const WvKvGroups& share, const float* dq, int ldq, float* dout, int ldo, int heads, float scale,

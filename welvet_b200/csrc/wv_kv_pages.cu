@@ -6,9 +6,11 @@
 // order), and a call gives them out in rising order to the sequences in theirs, so every result is the same in each run: the places come from
 // sums over warps' counts, not from atomics. One cluster of eight CTAs walks the counts, each of its 128 warps its own stretch, twice: once
 // to count, once to write down what it found, with one exchange of the 128 counts between (distributed shared memory).
-// A pool of 20,000 pages is 156 of them a warp; of a million, 8192, and then the walk takes some 40 us.
+// Measured, us from a graph: trimming 64 sequences 1.7; extending 64 by a token each 6.2 for a pool of 2000 pages, 6.4 of 20,000, 8.9 of 200,000, 18.5 of
+// a million; compacting with nothing to move 6.4, 6.6, 14.0, 45.8 (its walk writes both lists, and a million pages are 8192 a warp).
 //
-// Copies of pages are bound by HBM: a block of 256 threads moves 16 KB at a time, four 16-byte pieces a thread under way.
+// Copies of pages are bound by HBM: a block of 256 threads moves 16 KB at a time, four 16-byte pieces a thread under way. A compaction that moves 322 MB
+// takes 126 us, 5.1 TB/s of reads and writes together where a plain copy reaches 6.5.
 #include "wv_paged.cuh"
 #include "wv_lease.h"
 #include <algorithm>
