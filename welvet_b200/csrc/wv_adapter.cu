@@ -20,7 +20,7 @@
 //
 // Measured, plan and targets, us from a graph (floor): a row, rank 16 of 4096 beside 4096 + 1024 + 1024 in bf16 7.2 (0.1); 64 rows of 32 such adapters 17 (3.4); 48
 // rows of 16, rank 64 of 4096 beside 2 x 14336 in f16 36 (13); 2048 rows of 6, rank 64 of 4096 beside 4096 in bf16 53 (16); 333 rows of 9, rank 24 of 14336
-// beside 4096 in f32 50 (7). What bounds them is a cluster's chain: its ring fills, t is made, added up and spread, and only then
+// beside 4096 in f32 50 (7). The plan is 2 of them, 4 for 2048 rows. What bounds the rest is a cluster's chain: its ring fills, t is made, added up and spread, and only then
 // do the outputs run; clusters of up to 16 CTAs shorten both parts (with 8 at most the last one took 54), and are kept from running in turns by the rule below.
 #include "wv_paged.cuh"
 #include "wv_tma_common.cuh"      // lds64, smem_u32

@@ -38,9 +38,9 @@
 // the next scores are made while this step's weights are, and its sums are added a step later; four threads a row (32 keys and a quarter of the
 // values each) and seven warps for the ring of four stages, of which another one takes the eighth group of rows each time. One tile in the form
 // above, with half of its warps idle, was one chain of S, weights, P V and sums of 7000 cycles a key tile behind three warps of conversions; this is 4500 at 0.6
-// instructions a cycle and scheduler, 2048 of them the tensor pipe's. Two groups of 16 sequences behind 65000 tokens, 64 heads in 4 bits: 243 -> 202 us (eight warps of
+// instructions a cycle and scheduler, 2048 of them the tensor pipe's. Two groups of 16 sequences behind 65000 tokens, 64 heads in 4 bits: 243 -> 203 us (eight warps of
 // weights instead of 16: 231; three stages instead of four: 205; five of the idle warps as more converters alone: 270). 64 sequences behind 16384
-// tokens in 8 bits, 256 rows of 32 heads: 106 us in blocks of two tiles, 96 in blocks of one.
+// tokens in 8 bits, 256 rows of 32 heads: 106 us in blocks of two tiles, 97 in blocks of one.
 //
 // Every wait is bounded: when one runs out the block records a code, all roles leave their loops, and tensor memory is released
 // after the MMAs in flight (waited for, bounded again).
