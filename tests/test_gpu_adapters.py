@@ -248,6 +248,12 @@ def test_refusals(wv):
         call("WV_ESHAPE", **k)
     call("WV_EFORMAT", dtype=4)
     call("WV_EFORMAT", dtype=0)
+    # outputs that another target, or x, stands in: targets run side by side
+    call("WV_EARG")
+    other = (C.c_void_p * 2)(p + 4096, p + 8192)
+    call("WV_EARG", n=2, y=(C.c_void_p * 2)(p + 4096, p + 4096))
+    call("WV_EARG", n=2, y=other, base=(C.c_void_p * 2)(p + 8192, p + 8192))
+    call("WV_EARG", n=2, y=(C.c_void_p * 2)(p + 4096, p))
     assert L.wv_adapter_plan_dev(None, 2, 2, p, None) == E.WV_EARG
     assert L.wv_adapter_plan_dev(p, 2, 2, None, None) == E.WV_EARG
     assert L.wv_adapter_plan_dev(p, 2, 2, p + 4, None) == E.WV_EARG

@@ -729,6 +729,12 @@ extern "C" int wv_adapter_apply_dev(const WvAdapters* targets, int n, const void
     ranks = std::max(ranks, w.max_rank);
   }
   if (rows == 0) return WV_OK;
+  // targets run side by side, and all of them read x
+  for (int i = 0; i < n; i++)
+    for (int j = 0; j < n; j++)
+      if (c.t[i].y == dx || (i != j && (c.t[i].y == c.t[j].y || c.t[i].y == c.t[j].base))) {
+        wv_set_error("%s: target %d writes what another one reads or writes", who, i); return WV_EARG;
+      }
   c.x = dx; c.ldx = ldx; c.in = f.in; c.rows = rows; c.slots = f.slots;
   c.size = ad_tile(rows, f.slots); c.tiles = ad_tiles(rows, f.slots);
   c.plan = static_cast<const int4*>(d_plan);
