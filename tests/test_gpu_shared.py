@@ -242,6 +242,20 @@ def test_same_as_the_paged_attention_when_rows_are_many(wv):
     assert torch.equal(got, ref)
 
 
+def test_loose_bounds_of_wide_heads(wv):
+    """Three sequences of one token under bounds that allow 400 million tiles of sixteen rows: the call is wv_attn_paged_dev."""
+    lens = [(1, 200), (1, 190), (1, 195)]
+    c = Shared(wv, 8, 16, 1, 256, lens, [0, 3], [176])
+    b, keep = c.batch_of(lens, max_q=1 << 28)
+    q = torch.randn(3, 8 * 256, device="cuda")
+    got, ref = c.attend(q, 8, 0.06, b), torch.empty_like(q)
+    wv.paged.AttnPagedCUDA(c.pages, b, q.data_ptr(), ref.data_ptr(), 8, 0.06)
+    torch.cuda.synchronize()
+    assert torch.equal(got, ref) and wv._lib.lib().wv_device_status() == 0
+    want, tol = c.want(q, 8, 0.06)
+    assert (np.abs(got.double().cpu().numpy() - want) <= tol).all()
+
+
 @pytest.mark.parametrize("seqs,shared,pays", [(2, 512, False), (8, 512, False), (8, 4480, True)])
 def test_shared_where_it_pays(wv, always, seqs, shared, pays):
     """By itself the call takes the shared keys apart for seven passes saved over 4480 keys of eight heads, and is wv_attn_paged_dev below that."""

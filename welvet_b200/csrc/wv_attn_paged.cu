@@ -903,9 +903,6 @@ int wv_launch_attn_shared(const WvKvPages& kv, const WvKvBatch& b, const WvKvGro
   // nothing is shared, so little that it gains nothing, or there are so many rows
   if (share.num_groups == 0 || front == 0 || most_slots < 2 || !sharing_pays(b, share.num_groups, front, c.g, c.group, c.g.hd <= 128 && each * c.group > 32))
     return wv_launch_attn_paged(kv, b, dq, ldq, dout, ldo, heads, scale, 0, st);
-  if (rows > INT_MAX || (long long)b.num_seqs * ((long long)b.max_q * c.group / 8 + 1) * c.g.kvh > INT_MAX) {
-    wv_set_error("wv_attn_shared_dev: %d rows of %d heads, %d sequences of %d tokens are too many", b.total_q, heads, b.num_seqs, b.max_q); return WV_ESHAPE;
-  }
   const long long top[2] = {each * c.group, (long long)b.max_q * c.group};                   // rows of a kv head: of a group on average, of a sequence at most
   struct Part { bool chunk, r16; long long grid, per, n; } part[2];
   for (int i = 0; i < 2; i++) { part[i].chunk = c.g.hd <= 128 && top[i] > 32; part[i].r16 = top[i] > 8; }
@@ -938,6 +935,10 @@ int wv_launch_attn_shared(const WvKvPages& kv, const WvKvBatch& b, const WvKvGro
       part[i].n = (keys + part[i].per - 1) / part[i].per;
     }
   }
+  // Bounds so loose that most of the tiles which they allow are empty (wide heads alone: the chunk kernel's follow total_q), or that a grid cannot hold them: the
+  // other call looks its sequences up.
+  if (!part[1].chunk && part[1].grid / 4 > (long long)b.total_q * c.group / (part[1].r16 ? 16 : 8) + b.num_seqs) return wv_launch_attn_paged(kv, b, dq, ldq, dout, ldo, heads, scale, 0, st);
+  if ((part[0].grid * part[0].n + part[1].grid * part[1].n) * c.g.kvh > INT_MAX) return wv_launch_attn_paged(kv, b, dq, ldq, dout, ldo, heads, scale, 0, st);
   c.nslots = (int)(part[0].n + part[1].n);
   WvLease lease;
   const size_t n = (size_t)rows * c.nslots, sums = (2 * n + 3) & ~(size_t)3;
@@ -949,7 +950,6 @@ int wv_launch_attn_shared(const WvKvPages& kv, const WvKvBatch& b, const WvKvGro
   c.slot0 = 0; c.per = (int)part[0].per; c.nsplit = (int)part[0].n;
   c.own_slot0 = (int)part[0].n; c.own_per = (int)part[1].per; c.own_nsplit = (int)part[1].n;
   c.own_tiles = (unsigned)(((long long)b.max_q * c.group + (part[1].r16 ? 15 : 7)) / (part[1].r16 ? 16 : 8));
-  if (blocks[0] + blocks[1] > INT_MAX) { wv_set_error("wv_attn_shared_dev: %lld blocks are too many", blocks[0] + blocks[1]); return WV_ESHAPE; }
   if (both) {
     c.split = (unsigned)blocks[0];
     e = rows_any<true>(c, kv.bits, part[0].r16, (int)(blocks[0] + blocks[1]), st);
