@@ -101,12 +101,22 @@ def test_chunks_behind_a_prefix(wv, bits):
 
 
 @pytest.mark.parametrize("bits", [16, 8, 4])
-def test_many_tiles_a_block(wv, bits):
-    """40 sequences of the same 16384 tokens: blocks go through several tiles of keys, the stages of their rings many times around. Three runs."""
+def test_long_chunks_behind_a_prefix(wv, bits):
+    """Pieces of prompts whose own keys are several tiles a block, the last ones masked, of ten blocks of rows a sequence."""
+    Shared(wv, bits, 64, 2, 128, [(300, 2012), (290, 1800), (2, 900)], [0, 3], [512]).check(8)
+
+
+@pytest.mark.parametrize("bits,spread", [(16, 0), (8, 0), (4, 0), (8, 15), (4, 15)])
+def test_many_tiles_a_block(wv, bits, spread):
+    """40 sequences of the same 16384 tokens: blocks go through several tiles of keys, the stages of their rings many times around. Three runs. With
+    `spread` every fifth tile of 128 value rows has scales up to 2^30 apart, more than float16 pieces of the weights hold, between tiles that have not."""
     kvh, hd, heads, n, rows = 8, 128, 16, 16384, 40
     c = Cache(wv, bits, 64, kvh, hd, [(1, n)])
     rng = np.random.default_rng(bits)
-    c.fill(*(torch.from_numpy(rng.normal(0, 1, (n, kvh * hd)).astype(np.float32)).cuda() for _ in range(2)))
+    k, v = (rng.normal(0, 1, (n, kvh * hd)).astype(np.float32) for _ in range(2))
+    if spread:
+        v *= np.exp2(np.where(np.arange(n) // 128 % 5 == 3, rng.integers(-spread, spread + 1, n), 0)).astype(np.float32)[:, None]
+    c.fill(torch.from_numpy(k).cuda(), torch.from_numpy(v).cuda())
     table = c.d_table[:1].repeat(rows, 1).contiguous()
     ints = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
     start, kv, at, shared = ints(*range(rows + 1)), ints(*[n] * rows), ints(0, rows), ints(n, 0)
