@@ -547,7 +547,7 @@ __global__ void __launch_bounds__(AD_THREADS, AdShape<DT, NR, MR>::WIDE ? 1 : 2)
 #pragma unroll
     for (int s = 0; s < 3; s++) { const uint2 v = lds64(at + s * 256); x[s][0] = v.x; x[s][1] = v.y; }
   };
-  if (NB == 1) {
+  if (NB == 1 && pieces == 1) {
 #pragma unroll
     for (int k = 0; k < HELD; k++) if (k < nk) fetch(fr + k * 768, xh[k]);
   }
@@ -564,7 +564,8 @@ __global__ void __launch_bounds__(AD_THREADS, AdShape<DT, NR, MR>::WIDE ? 1 : 2)
       for (int z = 0; z < Z; z++)
 #pragma unroll
         for (int n = 0; n < NB; n++) d[z][n][0] = d[z][n][1] = d[z][n][2] = d[z][n][3] = 0.f;
-    } else if (NB == 1) {
+    }
+    if (NB == 1 && pieces > 1) {                         // each unit goes through all pieces anew
 #pragma unroll
       for (int k = 0; k < HELD; k++) if (p * MR + k < nk) fetch(fr + (p * MR + k) * 768, xh[k]);
     }
