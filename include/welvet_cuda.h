@@ -213,7 +213,8 @@ int wv_attn_paged_dev(const WvKvPages* kv, const WvKvBatch* batch, const float* 
  * sequences are read and multiplied once, for all rows of the group. Group g is the sequences start[g] .. start[g + 1] - 1 (start[num_groups + 1]
  * rising, on the device; sequences before start[0] and behind the last are on their own), whose tables name the same pages for their first
  * shared[g] tokens. Only whole pages count, and only as far as every new token of the group sees them: whatever the lengths are, the
- * result is that of wv_attn_paged_dev, to its accuracy. max_shared and max_kv - max_shared plan the call's splits. Where the sizes given here
+ * result is that of wv_attn_paged_dev, to its accuracy. max_shared and max_kv - max_shared plan the call's splits: where far less is shared than max_shared
+ * says, few blocks do the work, and wv_attn_paged_dev is the faster call. Where the sizes given here
  * (num_seqs, num_groups, max_shared, max_q) say that it gains nothing, too few keys or too many rows, the call is wv_attn_paged_dev. Where it is
  * not, a start or shared[g] outside its bounds is cut and reported as a batch's lengths are; the rows of its sequences are then undefined, as they
  * are where the tables differ. Scratch as wv_attn_paged_dev. */

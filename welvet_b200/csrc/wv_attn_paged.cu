@@ -32,7 +32,7 @@
 int wv_sm_count();
 
 #define PR_WARPS 4
-#define PR_CHAIN 40           // products that a warp adds to its sums at most, see wv_launch_attn_paged
+#define PR_CHAIN 40           // products that a warp adds to its sums at most, see rows_per_split
 // The running maximum is raised only when a logit is 2^7 above it (the sums, 64 registers a lane, are multiplied each time), so weights
 // reach 2^7 and carry 2^6 instead of 2^13: at most 2^14, and 2^-30 of that is still there.
 #define PR_LIFT 6.f
@@ -50,6 +50,8 @@ template <int BITS, int DP> struct PrShape {
 __host__ __device__ constexpr int pr_blocks(int bits, int dp, bool r16) {
   return dp == 256 && (bits == 16 || r16) ? 1 : !r16 && (dp == 64 || (dp == 128 && bits < 16)) ? 3 : 2;
 }
+// The keys that make a warp's chains of products PR_CHAIN long.
+__host__ __device__ constexpr int pr_stretch(bool r16) { return 16 * PR_WARPS * (r16 ? PR_CHAIN / 2 : PR_CHAIN); }
 // And the stages of a warp's ring in what they leave.
 template <int BITS, int DP, bool R16> struct PrFit {
   static constexpr int STAGE = PrShape<BITS, DP>::STAGE;
@@ -173,14 +175,14 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
       hi = min(hi, shared);
     } else {
       lo = max(lo, shared);
-      // planned for what lies behind the longest prefix; where less is shared the splits are longer
+      // planned for what lies behind the longest prefix; where less is shared the splits are longer (and go in stretches, below)
       if (hi > lo) per = max(per, ((hi - lo + nsplit - 1) / nsplit + 63) & ~63);
       if (shared == 0 && sp == 0)                                        // nobody else writes these rows' results of part 1
         for (int i = tid; i < rn * slot0; i += 32 * PR_WARPS) c.ml[rec(i / slot0) - slot0 + i % slot0] = make_float2(-INFINITY, 0.f);
     }
   }
   const unsigned first = (unsigned)lo + (unsigned)sp * (unsigned)per;
-  const int k0 = (int)min(first, (unsigned)hi), k1 = min(hi, k0 + per);        // this block's keys; k0 is a multiple of 16 if there are any
+  int k0 = (int)min(first, (unsigned)hi), k1 = min(hi, k0 + per);              // this block's keys; k0 is a multiple of 16 if there are any
   if (k0 >= k1) {
     if (SHARED || c.nsplit > 1) { if (tid < rn) c.ml[rec(tid)] = make_float2(-INFINITY, 0.f); }
     else for (int i = tid; i < rn * hd; i += 32 * PR_WARPS) {            // rows that see nothing
@@ -190,8 +192,13 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
     return;
   }
 
+  // SHARED: a split that is longer than was planned, or that the scratch made long, goes in stretches, whose sums are joined in float32: its chains of products
+  // are as short as any other's. 16 sequences of 131072 keys (64 heads over 8 of 128, 8 bits) of which all could be shared and nothing is take 2350 us so, 2010 in one
+  // chain, whose sums were off by up to 7 times as much; a second set of sums beside the first would take 64 registers.
+  const int kfirst = k0, kend = k1;
+  if (SHARED) k1 = min(k1, k0 + pr_stretch(R16));
   // ---------------------------------------------------------------- the warp's groups of 16 keys: k0 / 16 + warp, + PR_WARPS, ...
-  const int g0 = k0 / 16 + warp, ng = ((k1 + 15) / 16 - g0 + PR_WARPS - 1) / PR_WARPS;
+  int g0 = k0 / 16 + warp, ng = ((k1 + 15) / 16 - g0 + PR_WARPS - 1) / PR_WARPS;
   // A lane's copies of a group's K (or V) rows: the source is contiguous, the place in the ring the same in every stage.
   unsigned dst[S::NCP];
 #pragma unroll
@@ -335,14 +342,18 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
     }
   }
   __syncthreads();
+  const int pmin = sq.p0 + r0 / c.group, pmax = sq.p0 + (r0 + rn - 1) / c.group;
+  float all_m[NR], all_l[NR];                                            // of the stretches before
+#pragma unroll
+  for (int i = 0; i < NR; i++) { all_m[i] = -INFINITY; all_l[i] = 0.f; }
+
+  for (;;) {
   uint4 qr[QREG ? (R16 ? 2 : 1) * KS : 1];
   if constexpr (QREG) {
 #pragma unroll
     for (int i = 0; i < (R16 ? 2 : 1) * KS; i++) qr[i] = s_qf[i * 32 + lane];
   }
   auto qfrag = [&](int i) -> uint4 { if constexpr (QREG) return qr[i]; else return s_qf[i * 32 + lane]; };
-
-  const int pmin = sq.p0 + r0 / c.group, pmax = sq.p0 + (r0 + rn - 1) / c.group;
 
   float o[NT][4], m[NR], l[NR];
 #pragma unroll
@@ -657,9 +668,18 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
       L += x.y * fw[w];
     }
     float* to;
-    float scale = 1.f;
+    float scale = 1.f, before = 0.f;
+    const bool more = SHARED && k0 != kfirst;
     if (SHARED || c.nsplit > 1) {
       to = c.acc + rec(r) * hd;
+      if (more) {                                                        // a lane's values of the stretches before are its own
+        const float top = fmaxf(M, all_m[i]), t0 = top == -INFINITY ? 0.f : top;
+        before = all_m[i] == -INFINITY ? (all_l[i] == all_l[i] ? 0.f : 1.f) : pa_ex2(all_m[i] - t0);
+        scale = M == -INFINITY ? (L == L ? 0.f : 1.f) : pa_ex2(M - t0);
+        L = all_l[i] * before + L * scale;
+        M = top;
+      }
+      if (SHARED) { all_m[i] = M; all_l[i] = L; }
       if (warp == 0 && cl == 0) c.ml[rec(r)] = make_float2(M, L);
     } else {
       to = c.out + (size_t)(sq.q0 + plast[i] - sq.p0) * c.ldo + where[i];
@@ -680,9 +700,28 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
 #pragma unroll
       for (int j = 0; j < 2; j++) {
         const int d = pr_vdim<BITS, DP>(4 * t4, 2 * cl + j);
-        if (d < hd) *reinterpret_cast<float4*>(to + d) = make_float4(v[j][0], v[j][1], v[j][2], v[j][3]);
+        if (d < hd) {
+          float4 y = make_float4(v[j][0], v[j][1], v[j][2], v[j][3]);
+          if (more) {
+            const float4 x = *reinterpret_cast<const float4*>(to + d);
+            y.x += x.x * before; y.y += x.y * before; y.z += x.z * before; y.w += x.w * before;
+          }
+          *reinterpret_cast<float4*>(to + d) = y;
+        }
       }
     }
+  }
+  if (!SHARED || k1 == kend) break;
+  k0 = k1; k1 = min(kend, k0 + pr_stretch(R16));
+  g0 = k0 / 16 + warp; ng = ((k1 + 15) / 16 - g0 + PR_WARPS - 1) / PR_WARPS;
+  stage_in = 0;
+  __syncthreads();                                                       // every warp has read the sums: the rings again
+  if (!EXACT) {
+    for (int i = tid * 16; i < PR_WARPS * NST * S::STAGE; i += 32 * PR_WARPS * 16) *reinterpret_cast<uint4*>(pr_smem + i) = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < NST - 1; i++) start(i);
   }
 }
 
@@ -782,7 +821,7 @@ template <bool SHARED> static cudaError_t rows_any(const PaCall& c, int bits, bo
 // 7e-7; 131000 keys in chains of 38 by 9e-7. So no more than 40, at 2 us of 26 for the drafted tokens and 4 of 126 for the batch above.
 static long long rows_per_split(long long keys, long long blocks, const WvKvGeom& g, int bits, bool r16) {
   const long long slots = (long long)wv_sm_count() * pr_blocks(bits, g.hd <= 64 ? 64 : g.hd <= 128 ? 128 : 256, r16);
-  const long long longest = 64 * (r16 ? PR_CHAIN / 2 : PR_CHAIN);
+  const long long longest = pr_stretch(r16);
   long long per = 64, cost = -1;
   for (long long w = 1; w <= 8; w++) {
     long long n = w * slots / blocks;
@@ -928,7 +967,7 @@ int wv_launch_attn_shared(const WvKvPages& kv, const WvKvBatch& b, const WvKvGro
     }
     p.n = (keys + p.per - 1) / p.per;
   }
-  if (part[0].n + part[1].n > most_slots) {                              // fewer and longer splits
+  if (part[0].n + part[1].n > most_slots) {                              // fewer and longer splits, which the kernel for few rows takes in stretches
     for (int i = 1; i >= 0; i--) {
       const long long n = std::min(part[i].n, i ? std::max(most_slots / 2, 1LL) : most_slots - part[1].n), keys = i ? std::max((long long)b.max_kv - front, 1LL) : front;
       part[i].per = ((keys + n - 1) / n + 127) & ~127LL;
