@@ -269,7 +269,8 @@ int wv_kv_copy_dev(const WvKvPages* pools, int num_pools, const int* d_src, cons
  *
  * wv_adapter_plan_dev sorts the rows of a step by adapter (d_slot[rows], -1: none) into a plan of wv_adapter_plan_bytes(), which the caller keeps while
  * the step's calls use it; it is 16-byte aligned. wv_adapter_apply_dev adds the adapters of up to four projections on the same x (of the same slots, in and dtype): dy[i]
- * [rows, out_i] = dbase[i] + ..., in place where dbase is NULL or names dy[i] (no dy is x, or of another target); rows without an adapter are copied. x and the sums are
+ * [rows, out_i] = dbase[i] + ..., in place where dbase is NULL or names dy[i]; otherwise no dy has a value in common with its dbase, and none ever
+ * with x or another target's matrices (columns beside one another in rows of one stride are fine); rows without an adapter are copied. x and the sums are
  * float32 (products carry 24 bits, but for values of x or A x below 2^-100, and of f16 weights for values of x or A x below 2^-31 of the largest of their row,
  * which may count as zero); a row of x that is not finite gives NaN where it has an adapter, and so does an
  * adapter's value. A slot or rank out of bounds is taken as none or cut, and a plan of other rows or slots does nothing; wv_device_status()

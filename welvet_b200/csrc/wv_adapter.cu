@@ -663,6 +663,23 @@ static int ad_counts(const char* who, int rows, int slots) {
   return WV_OK;
 }
 
+// Whether two matrices of `rows` rows, wp of each ldp values and wq of each ldq, have a value in common. Columns of one matrix with the same stride may lie
+// beside one another.
+static bool ad_meets(const float* p, int ldp, int wp, const float* q, int ldq, int wq, int rows) {
+  const long long d = (static_cast<long long>(reinterpret_cast<uintptr_t>(q)) - static_cast<long long>(reinterpret_cast<uintptr_t>(p))) / 4;      // both 16-byte aligned
+  const long long endp = (rows - 1LL) * ldp + wp, endq = (rows - 1LL) * ldq + wq;
+  if (d >= endp || -d >= endq) return false;
+  if (ldp == ldq) {
+    const long long o = (d % ldp + ldp) % ldp;           // q's columns begin o behind p's
+    return o < wp || o + wq > ldp;
+  }
+  for (long long r = 0; r < rows; r++) {                 // the first of q's rows that ends behind the beginning of p's
+    const long long a = r * ldp - d, j = a < wq ? 0 : (a - wq) / ldq + 1;
+    if (j < rows && j * ldq < a + wp) return true;
+  }
+  return false;
+}
+
 extern "C" int wv_adapter_plan_bytes(int rows, int slots, uint64_t* bytes) {
   const char* who = "wv_adapter_plan_bytes";
   if (!bytes) { wv_set_error("%s: null pointer", who); return WV_EARG; }
@@ -730,12 +747,17 @@ extern "C" int wv_adapter_apply_dev(const WvAdapters* targets, int n, const void
     ranks = std::max(ranks, w.max_rank);
   }
   if (rows == 0) return WV_OK;
-  // targets run side by side, and all of them read x
-  for (int i = 0; i < n; i++)
-    for (int j = 0; j < n; j++)
-      if (c.t[i].y == dx || (i != j && (c.t[i].y == c.t[j].y || c.t[i].y == c.t[j].base))) {
-        wv_set_error("%s: target %d writes what another one reads or writes", who, i); return WV_EARG;
+  // targets run side by side, all of them read x, and clusters read base while others write
+  for (int i = 0; i < n; i++) {
+    const AdTarget& t = c.t[i];
+    if (ad_meets(t.y, t.ldy, t.out, dx, ldx, f.in, rows)) { wv_set_error("%s: target %d writes into x", who, i); return WV_EARG; }
+    for (int j = 0; j < n; j++) {
+      const AdTarget& o = c.t[j];
+      if ((i != j && ad_meets(t.y, t.ldy, t.out, o.y, o.ldy, o.out, rows)) || ((i != j || t.y != t.base) && ad_meets(t.y, t.ldy, t.out, o.base, o.ldb, o.out, rows))) {
+        wv_set_error("%s: target %d writes what target %d reads or writes", who, i, j); return WV_EARG;
       }
+    }
+  }
   c.x = dx; c.ldx = ldx; c.in = f.in; c.rows = rows; c.slots = f.slots;
   c.size = ad_tile(rows, f.slots); c.tiles = ad_tiles(rows, f.slots);
   c.plan = static_cast<const int4*>(d_plan);
