@@ -228,7 +228,7 @@ int wv_attn_shared_dev(const WvKvPages* kv, const WvKvBatch* batch, const WvKvGr
 
 /* Page tables on the device. refs[num_pages] counts for every page the places of the tables that hold it (0: the page is free),
  * pages[num_seqs][table_stride] and kv_len[num_seqs] are a batch's: sequence s holds pages[s][0 .. ceil(kv_len[s] / page_size) - 1].
- * All-zero refs and kv_len are an empty cache. The calls below change all three and nothing else, but for the copies of pages that
+ * All-zero refs and kv_len are an empty cache; num_pages, num_seqs and table_stride are at most 2^30. The calls below change all three and nothing else, but for the copies of pages that
  * extend and compact make in `pools` (the caches of all blocks that use the table: pages of one size in tokens and number, of any width;
  * num_pools may be 0). They are asynchronous on `stream`, hold no state of their own and can be captured; calls that share a table are
  * ordered by the caller. An entry that breaks a rule is left out and wv_device_status() then reports WV_ESHAPE. Results are the same in

@@ -28,6 +28,7 @@ int wv_api_bind_device();
 #define KP_ENTRY 128            // threads of a trim's or a fork's entry
 #define KP_POOLS 128            // pools of a copy's launch
 #define KP_PIECES 1024u         // 16-byte pieces of a copy's item
+#define KP_MOST (1 << 30)       // pages, sequences and a row's places: the walks look up to 512 places ahead in 32 bits
 
 __device__ __forceinline__ void kp_start() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -329,6 +330,10 @@ static int kp_table(const char* who, const WvKvTable* t) {
   if (!t || !t->refs || !t->pages || !t->kv_len) { wv_set_error("%s: null pointer", who); return WV_EARG; }
   if (t->num_pages < 1 || t->num_seqs < 1 || t->table_stride < 1 || !wv_kv_shape_ok(16, t->page_size, 16)) {
     wv_set_error("%s: %d pages of %d, %d sequences of up to %d pages (a page holds a multiple of 16 tokens)", who, t->num_pages, t->page_size, t->num_seqs, t->table_stride);
+    return WV_ESHAPE;
+  }
+  if (std::max(t->num_pages, std::max(t->num_seqs, t->table_stride)) > KP_MOST) {
+    wv_set_error("%s: %d pages, %d sequences of up to %d pages (at most %d each)", who, t->num_pages, t->num_seqs, t->table_stride, KP_MOST);
     return WV_ESHAPE;
   }
   return WV_OK;
