@@ -265,7 +265,7 @@ int wv_kv_copy_dev(const WvKvPages* pools, int num_pools, const int* d_src, cons
  * WvAdapters are the adapters of one projection: `slots` of them (at most 8192), a[slots][max_rank][in] and b[slots][out][max_rank] of `dtype` (a core.DType value: 1 = f32,
  * 2 = f16, 3 = bf16), of which the first rank[s] ranks count (rank NULL: max_rank; what stands behind them is not used, whatever it is),
  * scale[s] (NULL: 1). rank and scale are device arrays, so that an adapter can be exchanged between the replays of a graph. max_rank is a multiple of 8 up to
- * 256, in a multiple of 8; the matrices are 16-byte aligned.
+ * 256, in a multiple of 8, in and out at most 2^30; the matrices are 16-byte aligned.
  *
  * wv_adapter_plan_dev sorts the rows of a step by adapter (d_slot[rows], -1: none) into a plan of wv_adapter_plan_bytes(), which the caller keeps while
  * the step's calls use it; it is 16-byte aligned. wv_adapter_apply_dev adds the adapters of up to four projections on the same x (of the same slots, in and dtype): dy[i]

@@ -40,6 +40,7 @@ int wv_sm_count();
 #define AD_TARGETS 4
 #define AD_RANK 256             // the largest max_rank
 #define AD_SLOTS 8192
+#define AD_WIDE (1 << 30)       // columns and outputs: a CTA's offsets, in bytes of at most half the columns, and the units' ends stay in 32 bits
 
 // A plan: {tiles, rows of a tile, rows, slots}, then a tile's {adapter (slots: none), first place, rows, 0}, then the rows in their places.
 // Tiles of 32 where an adapter has more than 8 rows on average.
@@ -719,6 +720,7 @@ extern "C" int wv_adapter_apply_dev(const WvAdapters* targets, int n, const void
   if ((rc = ad_counts(who, rows, f.slots))) return rc;
   if (f.dtype < 1 || f.dtype > 3) { wv_set_error("%s: dtype %d (1 float32, 2 float16, 3 bfloat16)", who, f.dtype); return WV_EFORMAT; }
   if (f.in < 8 || f.in % 8) { wv_set_error("%s: %d columns (a multiple of 8)", who, f.in); return WV_ESHAPE; }
+  if (f.in > AD_WIDE) { wv_set_error("%s: %d columns (at most %d)", who, f.in, AD_WIDE); return WV_ESHAPE; }
   if (ldx == 0) ldx = f.in;
   if (ldx < f.in || (ldx & 3)) { wv_set_error("%s: the row stride of x is %d for %d values (a multiple of 4)", who, ldx, f.in); return WV_ESHAPE; }
   if ((reinterpret_cast<uintptr_t>(dx) | reinterpret_cast<uintptr_t>(d_plan)) & 15) { wv_set_error("%s: x or the plan is not 16-byte aligned", who); return WV_EARG; }
@@ -729,8 +731,8 @@ extern "C" int wv_adapter_apply_dev(const WvAdapters* targets, int n, const void
     AdTarget& t = c.t[i];
     if (!w.a || !w.b || !dy[i]) { wv_set_error("%s: target %d: null pointer", who, i); return WV_EARG; }
     if (w.slots != f.slots || w.in != f.in || w.dtype != f.dtype) { wv_set_error("%s: target %d has other adapters, columns or another type than the first", who, i); return WV_ESHAPE; }
-    if (w.max_rank < 8 || w.max_rank % 8 || w.max_rank > AD_RANK || w.out < 1) {
-      wv_set_error("%s: target %d: %d outputs, rank %d (a multiple of 8, at most %d)", who, i, w.out, w.max_rank, AD_RANK); return WV_ESHAPE;
+    if (w.max_rank < 8 || w.max_rank % 8 || w.max_rank > AD_RANK || w.out < 1 || w.out > AD_WIDE) {
+      wv_set_error("%s: target %d: %d outputs (at most %d), rank %d (a multiple of 8, at most %d)", who, i, w.out, AD_WIDE, w.max_rank, AD_RANK); return WV_ESHAPE;
     }
     t.a = w.a; t.b = w.b; t.rank = w.rank; t.scale = w.scale; t.max_rank = w.max_rank; t.out = w.out;
     t.y = dy[i]; t.base = dbase ? dbase[i] : dy[i];
