@@ -271,8 +271,8 @@ int wv_kv_copy_dev(const WvKvPages* pools, int num_pools, const int* d_src, cons
  * the step's calls use it; it is 16-byte aligned. wv_adapter_apply_dev adds the adapters of up to four projections on the same x (of the same slots, in and dtype): dy[i]
  * [rows, out_i] = dbase[i] + ..., in place where dbase is NULL or names dy[i]; otherwise no dy has a value in common with its dbase, and none ever
  * with x or another target's matrices (columns beside one another in rows of one stride are fine); rows without an adapter are copied. x and the sums are
- * float32 (products carry 24 bits, but for values of x or A x below 2^-100, and of f16 weights for values of x or A x below 2^-31 of the largest of their row,
- * which may count as zero); a row of x that is not finite gives NaN where it has an adapter, and so does an
+ * float32; products carry 24 bits, but for values of x or A x below 2^-100, which may count as zero. Beside f16 weights a value of x or A x is off by up to 2^-32 of the
+ * largest of its row: it has 24 bits down to 2^-8 of that, 16 at 2^-16, and may count as zero from 2^-32 on. A row of x that is not finite gives NaN where it has an adapter, and so does an
  * adapter's value. A slot or rank out of bounds is taken as none or cut, and a plan of other rows or slots does nothing; wv_device_status()
  * then reports WV_ESHAPE. Row strides as above (ldb, ldy NULL: rows without a gap); asynchronous on `stream`. */
 typedef struct WvAdapters {

@@ -11,8 +11,9 @@
 // all padding.
 //
 // With 16-bit weights x and t go through as three pieces of the weights' type: of bfloat16 (8 bits each by truncation, exactly x), or of float16, behind a
-// power of two for each row, which holds 31 bits below the row's largest value so far. Float32 weights are split into three bfloat16 pieces themselves, and the
-// six products that matter are taken. So the products carry float32's 24 bits. The tensor core cuts instead of rounding as it adds, so chains of products are
+// power of two for each row: the third piece ends 2^-32 below the row's largest value so far, so a value 2^-8 of that keeps 24 bits and one 2^-16 of it 16. (float16 weights
+// as two bfloat16 pieces would keep them all, for five products in place of three.) Float32 weights are split into three bfloat16 pieces themselves, and the
+// six products that matter are taken. These products carry float32's 24 bits. The tensor core cuts instead of rounding as it adds, so chains of products are
 // short: what a warp has of the columns (3 in 128 of a CTA's, 24 to 42 in all), or 24 products where registers allow a second sum.
 //
 // 16-bit weights come out of shared memory by ldmatrix, which puts a fragment's words where the product wants them (put together from
