@@ -215,7 +215,8 @@ int wv_attn_paged_dev(const WvKvPages* kv, const WvKvBatch* batch, const float* 
  * shared[g] tokens. Only whole pages count, and only as far as every new token of the group sees them: whatever the lengths are, the
  * result is that of wv_attn_paged_dev, to its accuracy. max_shared and max_kv - max_shared plan the call's splits: where far less is shared than max_shared
  * says, few blocks do the work, and wv_attn_paged_dev is the faster call. Where the sizes given here
- * (num_seqs, num_groups, max_shared, max_q) say that it gains nothing, too few keys or too many rows, the call is wv_attn_paged_dev. Where it is
+ * (num_seqs, num_groups, max_shared, max_kv, max_q, total_q) say that it gains nothing, too few keys or so many new tokens that a sequence's rows fill tiles by
+ * themselves, the call is wv_attn_paged_dev. Where it is
  * not, a start or shared[g] outside its bounds is cut and reported as a batch's lengths are; the rows of its sequences are then undefined, as they
  * are where the tables differ. Scratch as wv_attn_paged_dev. */
 typedef struct WvKvGroups {

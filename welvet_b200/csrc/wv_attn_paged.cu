@@ -909,18 +909,73 @@ int wv_launch_attn_paged(const WvKvPages& kv, const WvKvBatch& b, const float* d
 static int g_sharing = 0;
 extern "C" void wv_set_attn_sharing(int always) { g_sharing = always; }
 #endif
-// Does it pay to take the front keys apart? It saves num_seqs - num_groups passes over them: 0.25 ps for each key, value of a kv head and eight
-// query rows, 0.35 for sixteen. It costs two results a row written and joined (at 2 TB/s of their bytes: the join is short) and 6 us, or 12 where the
-// front keys go to the chunk kernel, which takes that long to start. Of 186 shapes (2 to 48 sequences a group, 1 or 4 groups, 256 to 16384 shared
-// tokens, 1 or 4 new ones, three layouts) this takes the faster way, or one within 5 %, in all but 6, and loses 27 % at most; e.g. us apart / not, 32 heads over 8 of
-// 128 in 8 bits: 2 sequences x 16384 tokens 23.1 / 22.6, 48 x 1024 34.6 / 29.5, 48 x 4096 41.6 / 94.9, 48 x 16384 72 / 298.
-static bool sharing_pays(const WvKvBatch& b, int num_groups, long long front, const WvKvGeom& g, int group, bool chunk) {
+// Splits of `tiles` key tiles for blocks of the chunk kernel: the number (up to `most`) that costs least in waves of blocks, each worth its key tiles and
+// some four more of start and end.
+static long long chunk_waves(long long blocks, long long tiles, long long n) {
+  const long long sms = wv_sm_count();
+  return (blocks * n + sms - 1) / sms * ((tiles + n - 1) / n + 4);
+}
+static long long chunk_splits(long long blocks, long long tiles, long long most) {
+  long long best = 1, cost = -1;
+  for (long long n = 1; n <= most && n <= tiles; n++) {
+    const long long w = chunk_waves(blocks, tiles, n);
+    if (cost < 0 || w < cost) { cost = w; best = n; }
+  }
+  return best;
+}
+// Does it pay to take the front keys apart? A pass of the kernel for few rows over a key costs 0.25 ps for each value of a kv head and eight query rows, 0.35 for sixteen
+// (0.47 with heads beyond 128, which leave an SM half as many blocks).
+//
+// Up to 32 rows of a kv head a sequence, num_seqs - num_groups passes are saved. It costs two results a row written and joined (at 2 TB/s of their bytes: the
+// join is short) and 6 us, or 12 where the front keys go to the chunk kernel, which takes that long to start. Of 186 shapes (2 to 48 sequences a group, 1 or 4 groups,
+// 256 to 16384 shared tokens, 1 or 4 new ones, three layouts) this takes the faster way, or one within 5 %, in all but 6, and loses 27 % at most; e.g. us apart / not,
+// 32 heads over 8 of 128 in 8 bits: 2 sequences x 16384 tokens 23.1 / 22.6, 48 x 1024 34.6 / 29.5, 48 x 4096 41.6 / 94.9, 48 x 16384 72 / 298.
+//
+// More rows fill tiles of their own, and reading the front once saves what the tiles of the sequences leave empty, no more: beside that rule both ways are then
+// counted in waves of the chunk kernel's blocks, 4.5 us a key tile for 256 rows of a sequence (3.0 up to 128 of them) and 2.7 for 128 rows of a group or of one; a result
+// of all rows at 3 TB/s (many of them are still in L2). Of 203 shapes (9 to 1024 new tokens, even, ragged, and beside single ones; 4 to 64 sequences) this takes
+// the faster way, or one within 5 %, in all but 6, and loses 38 % at most; the rule above alone took the slower one in 82, by up to 2.2 times. Apart / not, as above: 16 x 16 tokens behind 16384
+// 213 / 417, 16 x 32 behind 4096 139 / 126, 16 x 65 behind 16384 789 / 1143, 16 x 128 behind 1024 287 / 134.
+// Wide heads likewise by tiles of sixteen rows: 64 x 1 token of 4 heads a kv head of 256 behind 8192 149 / 241, of 8 heads 253 / 244, 64 x 4 918 / 894; of 96 shapes none is
+// slower by more than 5 % (43 by the first rule).
+static bool sharing_pays(const WvKvBatch& b, int num_groups, long long front, const WvKvGeom& g, int group, long long each) {
 #ifdef WV_DEV_HOOKS
   if (g_sharing) return true;
 #endif
-  const long long rows = (long long)b.max_q * group;
-  const double saved = (double)(b.num_seqs - num_groups) * front * g.kvh * g.hd * (rows <= 8 ? 0.25e-6 : 0.35e-6 * ((rows + 15) / 16));
-  return saved > (chunk ? 12.0 : 6.0) + (double)b.total_q * group * g.kvh * (g.hd + 2) * 2 * 4 / 2e6;
+  const long long rows = (long long)b.max_q * group, first = each * group;           // of a sequence at most, of a group on average
+  const bool wide = g.hd > 128, chunk = !wide && first > 32;
+  const double result = (double)b.total_q * group * g.kvh * (g.hd + 2) * 2 * 4 / 2e6;  // of every row, written and read at 2 TB/s
+  if (!wide) {
+    const double saved = (double)(b.num_seqs - num_groups) * front * g.kvh * g.hd * (rows <= 8 ? 0.25e-6 : 0.35e-6 * ((rows + 15) / 16));
+    const bool pays = saved > (chunk ? 12.0 : 6.0) + result;
+    if (!pays || rows <= 32) return pays;
+  }
+  // as many sequences as total_q has room for have max_q new tokens, the others share what is left
+  const long long many = std::max(1LL, std::min<long long>(b.num_seqs, b.total_q / b.max_q)), others = b.num_seqs - many;
+  const long long rest = others > 0 ? (std::max(0LL, b.total_q - many * b.max_q) * group + others - 1) / others : 0;
+  if (wide) {
+    auto tiles = [](long long r) { return (double)((r + 15) / 16); };
+    const double alone = rows <= 8 ? 0.25 * b.num_seqs : 0.47 * (many * tiles(rows) + others * tiles(rest));
+    const double apart = rows <= 8 && first <= 8 ? 0.25 * num_groups : 0.47 * b.total_q * group / 16;
+    return (alone - apart) * front * g.kvh * g.hd * 1e-6 > 8.0 + result;
+  }
+  const double narrow = 0.6 + 0.4 * g.hd / 128;
+  auto few = [&](long long seqs, long long r, long long keys) { return (double)seqs * g.kvh * keys * g.hd * (r <= 8 ? 0.25e-6 : 0.35e-6 * ((r + 15) / 16)); };
+  // wv_attn_paged_dev: planned for blocks that the bounds allow, and those that there are
+  const bool alike = (long long)b.num_seqs * b.max_q == b.total_q;
+  const long long blocks = (rows + 255) / 256, upto = (long long)b.total_q * group / 256 + b.num_seqs, all = (b.max_kv + 127LL) / 128;
+  const long long n = chunk_splits((alike ? b.num_seqs * blocks : std::min(b.num_seqs * blocks, upto)) * g.kvh, all, 16);
+  const long long there = (many * blocks + (rest > 32 ? others * ((rest + 255) / 256) : 0)) * g.kvh;
+  double alone = 5 + chunk_waves(there, all, n) * (rows > 128 ? 4.5 : 3.0) * narrow;
+  if (n > 1) alone += 2 + 0.65 * n * there * 256 * (g.hd + 2) * 2 * 4 / 2e6;
+  if (others > 0 && rest <= 32) alone += 30 + few(others, rest, b.max_kv);
+  // the front keys, and every sequence's own in tiles of 128 rows
+  const long long fronts = (front + 127) / 128, owns = std::max((b.max_kv - front + 127) / 128, 1LL), sure = (rows + 127) / 128;
+  const long long groups = num_groups * ((first + 127) / 128) * g.kvh, m = chunk_splits(groups, fronts, 64);
+  const long long k = chunk_splits(std::min(b.num_seqs * sure, (long long)b.total_q * group / 128 + b.num_seqs) * g.kvh, owns, 64);
+  const double apart = 8 + (chunk ? chunk_waves(groups, fronts, m) * 2.7 * narrow : few(num_groups, first, front)) +
+                       chunk_waves((many * sure + others * ((rest + 127) / 128)) * g.kvh, owns, k) * 2.7 * narrow + 0.65 * result * ((chunk ? m : 1) + k);
+  return apart < alone;
 }
 int wv_launch_attn_shared(const WvKvPages& kv, const WvKvBatch& b, const WvKvGroups& share, const float* dq, int ldq, float* dout, int ldo, int heads, float scale,
                           cudaStream_t st) {
@@ -940,7 +995,7 @@ int wv_launch_attn_shared(const WvKvPages& kv, const WvKvBatch& b, const WvKvGro
   // two results a row at least
   const long long most_slots = std::min(PA_SCRATCH / std::max(rows * (c.g.hd + 2) * 4, 1LL), 1024LL);
   // nothing is shared, so little that it gains nothing, or there are so many rows
-  if (share.num_groups == 0 || front == 0 || most_slots < 2 || !sharing_pays(b, share.num_groups, front, c.g, c.group, c.g.hd <= 128 && each * c.group > 32))
+  if (share.num_groups == 0 || front == 0 || most_slots < 2 || !sharing_pays(b, share.num_groups, front, c.g, c.group, each))
     return wv_launch_attn_paged(kv, b, dq, ldq, dout, ldo, heads, scale, 0, st);
   const long long top[2] = {each * c.group, (long long)b.max_q * c.group};                   // rows of a kv head: of a group on average, of a sequence at most
   struct Part { bool chunk, r16; long long grid, per, n; } part[2];
@@ -955,13 +1010,8 @@ int wv_launch_attn_shared(const WvKvPages& kv, const WvKvBatch& b, const WvKvGro
     const long long likely = i && p.chunk ? std::min(b.num_seqs * sure, upto) : (i ? b.num_seqs : share.num_groups) * sure;
     p.grid = i ? likely : upto;
     if (p.chunk) {
-      const long long tiles = (keys + 127) / 128, sms = wv_sm_count(), blocks = likely * c.g.kvh;
-      long long best = 1, cost = -1;
-      for (long long n = 1; n <= 64 && n <= tiles; n++) {
-        const long long t = (tiles + n - 1) / n, w = (blocks * n + sms - 1) / sms * (t + 4);
-        if (cost < 0 || w < cost) { cost = w; best = n; }
-      }
-      p.per = (tiles + best - 1) / best * 128;
+      const long long tiles = (keys + 127) / 128, n = chunk_splits(likely * c.g.kvh, tiles, 64);
+      p.per = (tiles + n - 1) / n * 128;
     } else {
       p.per = rows_per_split(keys, likely * c.g.kvh, c.g, kv.bits, p.r16);
     }
