@@ -182,7 +182,8 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
     }
   }
   const unsigned first = (unsigned)lo + (unsigned)sp * (unsigned)per;
-  int k0 = (int)min(first, (unsigned)hi), k1 = min(hi, k0 + per);              // this block's keys; k0 is a multiple of 16 if there are any
+  const int k0 = (int)min(first, (unsigned)hi);
+  int k1 = min(hi, k0 + per);                                            // this block's keys; k0 is a multiple of 16 if there are any
   if (k0 >= k1) {
     if (SHARED || c.nsplit > 1) { if (tid < rn) c.ml[rec(tid)] = make_float2(-INFINITY, 0.f); }
     else for (int i = tid; i < rn * hd; i += 32 * PR_WARPS) {            // rows that see nothing
@@ -193,10 +194,15 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
   }
 
   // SHARED: a split that is longer than was planned, or that the scratch made long, goes in stretches, whose sums are joined in float32: its chains of products
-  // are as short as any other's. 16 sequences of 131072 keys (64 heads over 8 of 128, 8 bits) of which all could be shared and nothing is take 2350 us so, 2010 in one
+  // are as short as any other's. 16 sequences of 131072 keys (64 heads over 8 of 128, 8 bits) of which all could be shared and nothing is take 2180 us so, 2010 in one
   // chain, whose sums were off by up to 7 times as much; a second set of sums beside the first would take 64 registers.
-  const int kfirst = k0, kend = k1;
-  if (SHARED) k1 = min(k1, k0 + pr_stretch(R16));
+  __shared__ float2 s_all[SHARED ? 2 : 1][NROW];                         // {M, divisor} of the stretches before; read while the next turn's are written
+  __shared__ int s_end;
+  int turn = 0;
+  if (SHARED) {
+    if (tid == 0) s_end = k1;
+    k1 = min(k1, k0 + pr_stretch(R16));
+  }
   // ---------------------------------------------------------------- the warp's groups of 16 keys: k0 / 16 + warp, + PR_WARPS, ...
   int g0 = k0 / 16 + warp, ng = ((k1 + 15) / 16 - g0 + PR_WARPS - 1) / PR_WARPS;
   // A lane's copies of a group's K (or V) rows: the source is contiguous, the place in the ring the same in every stage.
@@ -343,10 +349,6 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
   }
   __syncthreads();
   const int pmin = sq.p0 + r0 / c.group, pmax = sq.p0 + (r0 + rn - 1) / c.group;
-  float all_m[NR], all_l[NR];                                            // of the stretches before
-#pragma unroll
-  for (int i = 0; i < NR; i++) { all_m[i] = -INFINITY; all_l[i] = 0.f; }
-
   for (;;) {
   uint4 qr[QREG ? (R16 ? 2 : 1) * KS : 1];
   if constexpr (QREG) {
@@ -669,18 +671,21 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
     }
     float* to;
     float scale = 1.f, before = 0.f;
-    const bool more = SHARED && k0 != kfirst;
+    const bool more = SHARED && turn > 0;
     if (SHARED || c.nsplit > 1) {
       to = c.acc + rec(r) * hd;
       if (more) {                                                        // a lane's values of the stretches before are its own
-        const float top = fmaxf(M, all_m[i]), t0 = top == -INFINITY ? 0.f : top;
-        before = all_m[i] == -INFINITY ? (all_l[i] == all_l[i] ? 0.f : 1.f) : pa_ex2(all_m[i] - t0);
+        const float2 all = s_all[turn & 1][r];
+        const float top = fmaxf(M, all.x), t0 = top == -INFINITY ? 0.f : top;
+        before = all.x == -INFINITY ? (all.y == all.y ? 0.f : 1.f) : pa_ex2(all.x - t0);
         scale = M == -INFINITY ? (L == L ? 0.f : 1.f) : pa_ex2(M - t0);
-        L = all_l[i] * before + L * scale;
+        L = all.y * before + L * scale;
         M = top;
       }
-      if (SHARED) { all_m[i] = M; all_l[i] = L; }
-      if (warp == 0 && cl == 0) c.ml[rec(r)] = make_float2(M, L);
+      if (warp == 0 && cl == 0) {
+        c.ml[rec(r)] = make_float2(M, L);
+        if (SHARED) s_all[(turn + 1) & 1][r] = make_float2(M, L);
+      }
     } else {
       to = c.out + (size_t)(sq.q0 + plast[i] - sq.p0) * c.ldo + where[i];
       scale = L == 0.f ? 0.f : 1.f / L;
@@ -711,9 +716,9 @@ __global__ void __launch_bounds__(32 * PR_WARPS, PrFit<BITS, DP, R16>::BLOCKS) a
       }
     }
   }
-  if (!SHARED || k1 == kend) break;
-  k0 = k1; k1 = min(kend, k0 + pr_stretch(R16));
-  g0 = k0 / 16 + warp; ng = ((k1 + 15) / 16 - g0 + PR_WARPS - 1) / PR_WARPS;
+  if (!SHARED || k1 == s_end) break;
+  turn++;
+  g0 = k1 / 16 + warp; k1 = min(s_end, k1 + pr_stretch(R16)); ng = ((k1 + 15) / 16 - g0 + PR_WARPS - 1) / PR_WARPS;
   stage_in = 0;
   __syncthreads();                                                       // every warp has read the sums: the rings again
   if (!EXACT) {
