@@ -755,7 +755,7 @@ __global__ void __launch_bounds__(PcShape<BITS, DP, SHARED>::THREADS, 1) attn_ch
       while (ok && (pv[0] < n || (nt == 2 && pv[1] < n))) {
         bool did = false;
         for (int t = 0; t < nt; t++) {
-                    if (pv[t] < n && pv[t] < qk[t] && ready(full((2 * pv[t] + 1) % STAGES), (2 * pv[t] + 1) / STAGES) && ready(p_full(t), pv[t])) {
+          if (pv[t] < n && pv[t] < qk[t] && ready(full((2 * pv[t] + 1) % STAGES), (2 * pv[t] + 1) / STAGES) && ready(p_full(t), pv[t])) {
             pc_fence_after();
             const int e = 2 * pv[t] + 1;
             values(t, e);
