@@ -14,15 +14,17 @@
 // power of two for each row: the third piece ends 2^-32 below the row's largest value so far, so a value 2^-8 of that keeps 24 bits and one 2^-16 of it 16. (float16 weights
 // as two bfloat16 pieces would keep them all, for five products in place of three.) Float32 weights are split into three bfloat16 pieces themselves, and the
 // six products that matter are taken. These products carry float32's 24 bits. The tensor core cuts instead of rounding as it adds, so chains of products are
-// short: what a warp has of the columns (3 in 128 of a CTA's, 24 to 42 in all), or 24 products where registers allow a second sum.
+// short: what a warp has of the columns (3 in 128 of a CTA's: 42 at most up to 28672 columns, and 3 in 2048 of wider matrices), or 24 products where registers allow
+// a second sum.
 //
 // 16-bit weights come out of shared memory by ldmatrix, which puts a fragment's words where the product wants them (put together from
 // vector loads they took a move each).
 //
 // Measured, plan and targets, us from a graph (floor): a row, rank 16 of 4096 beside 4096 + 1024 + 1024 in bf16 7.2 (0.1); 64 rows of 32 such adapters 17 (3.4); 48
 // rows of 16, rank 64 of 4096 beside 2 x 14336 in f16 36 (13); 2048 rows of 6, rank 64 of 4096 beside 4096 in bf16 53 (16); 333 rows of 9, rank 24 of 14336
-// beside 4096 in f32 50 (7). The plan is 2 of them, 4 for 2048 rows. What bounds the rest is a cluster's chain: its ring fills, t is made, added up and spread, and only then
-// do the outputs run; clusters of up to 16 CTAs shorten both parts (with 8 at most the last one took 54), and are kept from running in turns by the rule below.
+// beside 4096 in f32 50 (7). Ranks beyond 64 go in pieces; with rank 128 the first
+// takes 13 (0.4), the second 65 (13), the third 75 (22), the fourth 98 (17). The plan is 2 of them, 4 for 2048 rows. What bounds the rest is a cluster's chain: its ring
+// fills, t is made, added up and spread, and only then do the outputs run; clusters of up to 16 CTAs shorten both parts (with 8 at most the last one took 54), and are kept from running in turns by the rule below.
 #include "wv_paged.cuh"
 #include "wv_tma_common.cuh"      // lds64, smem_u32
 #include <algorithm>
@@ -770,7 +772,8 @@ extern "C" int wv_adapter_apply_dev(const WvAdapters* targets, int n, const void
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   // CTAs of a cluster: as many as let the tiles that are expected (half of the adapters' last ones beside the full ones) run at once, two CTAs an SM: a row
   // beside Q, K and V takes 10.0, 8.0 and 7.5 us with 4, 8 and 16, 64 rows of 32 adapters 17 with 4 and 22 with 8, 2048 rows of six 53 and 69. Where sums are
-  // one chain (32 rows, ranks beyond 32), no more than 1792 columns each.
+  // one chain (32 rows, ranks beyond 32), no more than 1792 columns each. Shared memory leaves an SM one CTA where ranks are wide (16-bit weights from some 80
+  // in tiles of 32 rows and 128 in tiles of 8, float32 ones beyond 32): such calls may run their clusters in two turns where one would do.
   const long long likely = n * std::max(1LL, (long long)rows / c.size + (std::min(rows, f.slots) + 1) / 2), room = 2LL * wv_sm_count();
   int ctas = 2;
   while (ctas < AD_CTAS && likely * ctas * 2 <= room) ctas *= 2;
